@@ -424,6 +424,118 @@ int q48_attn_prefill(q48_ctx *ctx, int64_t *out, const int64_t *QKV, int64_t *kc
 /* SwiGLU (llama_int.c:1549-1552) of every [gate | up] row: out[T][ffn]. */
 int q48_silu_mul_rows(q48_ctx *ctx, int64_t *out, const int64_t *GU, int T, int ffn);
 
+/* ---- quantised key/value cache -------------------------------------------- */
+/* The keys and values of a cache as 8- or 4-bit codes with one Q16.48 step per
+ * (position, KV head): 1.125 or 0.625 bytes a value of 64-wide heads instead
+ * of 8.  A head vector x of head_dim words becomes, with Q = 127 (8 bits) or 7
+ * (4 bits) and a = max |x_d|,
+ *   step   = min(ceil(a / Q), floor((2^63 - 1) / Q))
+ *   code_d = sign(x_d) min(Q, floor((|x_d| + floor(step / 2)) / step)), 0 where
+ *            step is 0,
+ * and is read as code_d * step (never past 63 bits), at most half a step from
+ * x_d (a word more than the step's half where |x_d| > 2^63 - 64).  Attention
+ * over the cache is exactly attention over those values.  The reference's own
+ * quantised caches (llama_int.c:129-179, 1197-1235) are other formats.
+ *
+ * The four arrays are device memory of the caller: k and v (16-byte aligned)
+ * [layers][max_seq][n_kv][head_dim * bits / 8] bytes, k_step and v_step
+ * [layers][max_seq][n_kv].  At 8 bits a code is a signed byte; at 4 bits byte b
+ * of a head holds dim b in its low and dim b + head_dim / 2 in its high half,
+ * two's complement.  head_dim 32, 64 or 128; max_seq at most 32767 (as
+ * q48_rope_init).  The struct itself is read during the call only. */
+typedef struct {
+    void *k, *v;
+    int64_t *k_step, *v_step;
+    int bits;
+    int layers, max_seq, n_kv, head_dim;
+} q48_qcache;
+/* bytes of k (or v) and of k_step (or v_step) for such a cache */
+int q48_qcache_bytes(int bits, int layers, int max_seq, int n_kv, int head_dim, size_t *codes,
+                     size_t *steps);
+/* Quantise rows p0 .. p0 + T - 1 of a layer from K and V, whose rows of n_kv *
+ * head_dim words lie ld words apart (so they may be parts of [q | k | v] rows);
+ * keys come rotated.  The counterpart of the KV store
+ * (llama_int.c:1414-1416). */
+int q48_qcache_store_rows(q48_ctx *ctx, const q48_qcache *cache, int layer, int p0, int T,
+                          const int64_t *K, const int64_t *V, int ld);
+/* The values rows p0 .. p0 + T - 1 stand for, into K and V (rows ld words apart;
+ * words between the rows are left as they are). */
+int q48_qcache_load_rows(q48_ctx *ctx, int64_t *K, int64_t *V, const q48_qcache *cache, int layer,
+                         int p0, int T, int ld);
+/* q48_rope_store_rows into a quantised cache: RoPE of the q and k heads of every
+ * [q | k | v] row in place, then the quantised store at p0 + t.  d_pos: the
+ * rows' RoPE positions (device, T ints; NULL: p0 + t), as drafted tokens of a
+ * tree have them.  A row whose position is outside the RoPE tables is neither
+ * rotated nor stored.  Needs q48_rope_init(head_dim, >= max_seq). */
+int q48_rope_store_rows_qcache(q48_ctx *ctx, int64_t *QKV, const q48_qcache *cache, int layer,
+                               int p0, int T, const int *d_pos, int n_heads);
+/* q48_attn_decode over a quantised cache: k_new and v_new are quantised into row
+ * pos, then rows 0 .. pos are attended to.  Same bits as q48_attn_decode over
+ * the values the cache stands for.  In step mode pos is read from the
+ * device-side state.  out shares no words with q, k_new or v_new. */
+int q48_attn_decode_qcache(q48_ctx *ctx, int64_t *out, const int64_t *q, const q48_qcache *cache,
+                           const int64_t *k_new, const int64_t *v_new, int layer, int pos,
+                           int n_heads);
+/* The same with the RoPE of q and k_new fused in (they come unrotated and stay
+ * so), as q48_attn_decode_rope.  Needs q48_rope_init(head_dim, >= max_seq). */
+int q48_attn_decode_rope_qcache(q48_ctx *ctx, int64_t *out, const int64_t *q,
+                                const q48_qcache *cache, const int64_t *k_new,
+                                const int64_t *v_new, int layer, int pos, int n_heads);
+
+/* ---- drafted tokens: attention of rows under a mask ------------------------- */
+/* Attention of T rotated rows [q | k | v] over a cache that already holds their
+ * keys and values at rows p0 .. p0 + T - 1.  Row t attends to every row before
+ * p0 and, among the T new rows, to those its mask names: mask is device memory
+ * of ceil(T / 64) 64-bit words a row, bit j % 64 of word j / 64 of row t for
+ * row p0 + j (bits from T on are ignored); NULL: rows p0 .. p0 + t, causal.  A
+ * row that attends to nothing (p0 = 0, no bit) gives zeros.  Each row's result
+ * is the reference's exact attention (llama_int.c:1502-1529) over the rows it
+ * attends to, in cache order, so a token of a tree gets the words that decoding
+ * its own path gives.  out [T][n_heads * head_dim] shares no words with QKV.
+ * head_dim 32, 64 or 128; p0 + T at most 32767. */
+int q48_attn_tree(q48_ctx *ctx, int64_t *out, const int64_t *QKV, const int64_t *kcache,
+                  const int64_t *vcache, int layer, int p0, int T, int n_heads, int n_kv,
+                  int head_dim, int max_seq, const uint64_t *mask);
+int q48_attn_rows_qcache(q48_ctx *ctx, int64_t *out, const int64_t *QKV, const q48_qcache *cache,
+                         int layer, int p0, int T, int n_heads, const uint64_t *mask);
+/* q48_rope_store_rows with the rows' RoPE positions given (device, T ints): row t
+ * is rotated at d_pos[t] and stored at cache row p0 + t.  A row whose position
+ * is outside the RoPE tables is neither rotated nor stored. */
+int q48_rope_store_rows_at(q48_ctx *ctx, int64_t *QKV, int64_t *kcache, int64_t *vcache,
+                           int layer, int p0, int T, const int *d_pos, int n_heads, int n_kv,
+                           int head_dim, int max_seq);
+/* Keep n of the rows stored from p0 on (the accepted path of a tree) in every
+ * layer: row p0 + d_rows[i] moves to p0 + i for i < n in turn, d_rows (device)
+ * strictly increasing from 0 on.  A d_rows[i] below i or past the cache moves
+ * nothing.  Other rows stay as they are. */
+int q48_cache_keep_rows(q48_ctx *ctx, int64_t *kcache, int64_t *vcache, int layers, int p0,
+                        const int *d_rows, int n, int n_kv, int head_dim, int max_seq);
+int q48_qcache_keep_rows(q48_ctx *ctx, const q48_qcache *cache, int p0, const int *d_rows, int n);
+
+/* ---- log probabilities -------------------------------------------------------- */
+/* For each of T rows of logits [T][vocab]: the log probability of token
+ * d_tokens[t] (0 where that is not an id of the vocabulary, as for a padded
+ * row), the entropy of the row's distribution, and its top_n (0 .. 32, at most
+ * vocab) most probable tokens, ties to the lowest id, with their log
+ * probabilities.  logp (with d_tokens) and entropy may be NULL, top_ids and
+ * top_logp [T][top_n] where top_n is 0, but not all of them.  vocab at most
+ * 2^22.  All in Q16.48: with m = max x, u_i = m - x_i (64 bits, unsigned),
+ *   e_i = floor(floor(T_j h 2^-48) 2^-n), u_i = n LN2 + j 2^42 + s, 0 <= s < 2^42,
+ *         j <= 44, LN2 = 195103586505167, T_j = round(2^48 e^(-j/64)),
+ *         h = C_0 - (s (C_1 - (s (... C_6) >> 48)) >> 48), C_k = round(2^48 / k!)
+ *   Z = sum e_i, b the largest with (Z >> b) >= 2^48, z = Z >> b, i = (z >> 42) - 64,
+ *   d = (z floor(2^54 / (64 + i)) >> 48) - 2^48,
+ *   logZ = b LN2 + round(2^48 log(1 + i/64)) + (d g >> 48),
+ *         g = D_1 - (d (D_2 - (... D_8) >> 48) >> 48), D_k = round(2^48 / k)
+ *   log probability of i = -(u_i + logZ), at least -2^63
+ *   entropy = logZ + floor(2^48 ((sum (e_i u_i >> 48)) >> b) / z).
+ * Unlike fp_safe_exp (fp_math.h:739-744), whose value is 0 below e^-10 and off by
+ * up to 0.3% above, e_i is within 4 units of 2^-48 of e^-u: the many improbable
+ * tokens of a vocabulary count.  No reference counterpart. */
+int q48_logprobs_rows(q48_ctx *ctx, const int64_t *logits, int T, int vocab, const int *d_tokens,
+                      int64_t *logp, int64_t *entropy, int top_n, int *top_ids,
+                      int64_t *top_logp);
+
 /* ---- sampling (sample_token, llama_int.c:2958-3039) --------------------- */
 /* rng_seed (llama_int.c:2909-2920): the xoroshiro128+ state of a seed
  * (SplitMix64), computed on the host.  Upload it to a device buffer of two

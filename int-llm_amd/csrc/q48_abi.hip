@@ -921,6 +921,22 @@ int q48_rope_store_rows(q48_ctx *c, int64_t *QKV, int64_t *kcache, int64_t *vcac
                                               n_kv, head_dim, max_seq));
 }
 
+int q48_rope_store_rows_at(q48_ctx *c, int64_t *QKV, int64_t *kcache, int64_t *vcache, int layer,
+                           int p0, int T, const int *d_pos, int n_heads, int n_kv, int head_dim,
+                           int max_seq)
+{
+    if (!c || !QKV || !kcache || !vcache || !d_pos || T <= 0 || layer < 0 || max_seq <= 0 ||
+        !heads_ok(n_heads, n_kv, head_dim))
+        return Q48_EINVAL;
+    if (!c->rope_cos || head_dim != c->rope_head_dim)
+        return Q48_ESTATE;
+    if (p0 < 0 || p0 >= max_seq || T > max_seq - p0)
+        return Q48_ERANGE;
+    q48_on_device on(c);
+    return launch_rc(q48_launch_pf_rope_store(c, QKV, kcache, vcache, layer, p0, T, n_heads,
+                                              n_kv, head_dim, max_seq, d_pos));
+}
+
 int q48_attn_prefill(q48_ctx *c, int64_t *out, const int64_t *QKV, int64_t *kcache,
                      int64_t *vcache, int layer, int p0, int T, int n_heads, int n_kv,
                      int head_dim, int max_seq)

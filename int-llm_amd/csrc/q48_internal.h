@@ -71,6 +71,26 @@ struct q48_graph {
     uint64_t attg[2];
 };
 
+// The context's device as the calling thread's current one, and the thread's own
+// device again at the end of the scope.
+struct q48_on_device {
+    int back = -1;
+    explicit q48_on_device(const q48_ctx *c)
+    {
+        int d = c->device;
+        if (hipGetDevice(&d) == hipSuccess && d != c->device &&
+            hipSetDevice(c->device) == hipSuccess)
+            back = d;
+    }
+    ~q48_on_device()
+    {
+        if (back >= 0)
+            (void)hipSetDevice(back);
+    }
+    q48_on_device(const q48_on_device &) = delete;
+    q48_on_device &operator=(const q48_on_device &) = delete;
+};
+
 // Grow the context workspace to at least `bytes` (stream-synchronising).
 int q48_ws_reserve(q48_ctx *c, size_t bytes);
 // Give back a device buffer the context owns (stream-synchronising): freed
@@ -195,9 +215,10 @@ int q48_launch_pf_embed(q48_ctx *c, int64_t *H, const int64_t *table, const int 
                         int dim);
 int q48_launch_pf_rmsnorm(q48_ctx *c, int64_t *out, const int64_t *X, const int64_t *w, int T,
                           int dim);
+// (d_pos: the rows' RoPE positions on the device, or null: p0 + t)
 int q48_launch_pf_rope_store(q48_ctx *c, int64_t *QKV, int64_t *kcache, int64_t *vcache,
                              int layer, int p0, int T, int n_heads, int n_kv, int hd,
-                             int max_seq);
+                             int max_seq, const int *d_pos = nullptr);
 // the same attention with both products on the int8 matrix cores
 // (q48_pfattn.hip): head_dim 32, 64 or 128 and at most
 // q48_pf_attn_mfma_max_pos() cache rows
@@ -209,6 +230,8 @@ int q48_launch_pf_attn_mfma(q48_ctx *c, int64_t *out, const int64_t *QKV, int64_
 int q48_launch_pf_attn(q48_ctx *c, int64_t *out, const int64_t *QKV, int64_t *kcache,
                        int64_t *vcache, int layer, int p0, int T, int n_heads, int n_kv, int hd,
                        int max_seq);
+// Whether a q48_qcache describes a cache the kernels can read (pointers, sizes).
+bool q48_qcache_ok(const q48_qcache *qc);
 int q48_launch_pf_silu(q48_ctx *c, int64_t *out, const int64_t *GU, int T, int ffn);
 // sample_token: the sampling workspace size in int64 words for n logits, and
 // the kernel chain (greedy temperatures are the caller's: argmax); with

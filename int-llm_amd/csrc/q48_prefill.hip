@@ -22,17 +22,20 @@ __global__ __launch_bounds__(256) void k_pf_embed(int64_t *__restrict__ H,
 }
 
 // rope_apply (llama_int.c:997-1008) of the q heads and k heads of row t at
-// position p0 + t, in place, then the KV store (1414-1416) of the rotated k
-// and of v.  Row layout [q (nh hd) | k (nkv hd) | v (nkv hd)].
+// position p0 + t, or d_pos[t] (a row whose position is outside the n_pos rows
+// of the tables is left alone), in place, then the KV store (1414-1416) at row
+// p0 + t of the rotated k and of v.  Row layout [q (nh hd) | k (nkv hd) | v (nkv hd)].
 __global__ __launch_bounds__(256) void k_pf_rope_store(
     int64_t *__restrict__ QKV, int64_t *__restrict__ kcache, int64_t *__restrict__ vcache,
     const int64_t *__restrict__ cos_t, const int64_t *__restrict__ sin_t, int layer, int p0,
-    int n_heads, int n_kv, int hd, int max_seq)
+    int n_heads, int n_kv, int hd, int max_seq, const int *__restrict__ d_pos, int n_pos)
 {
-    const int t = blockIdx.x, pos = p0 + t, half = hd / 2;
+    const int t = blockIdx.x, pos = d_pos ? d_pos[t] : p0 + t, half = hd / 2;
+    if (pos < 0 || pos >= n_pos)
+        return;
     const size_t kvd = (size_t)n_kv * hd, row = (size_t)(n_heads + 2 * n_kv) * hd;
     int64_t *q = QKV + (size_t)t * row, *k = q + (size_t)n_heads * hd, *v = k + kvd;
-    const size_t cr = ((size_t)layer * max_seq + pos) * kvd;
+    const size_t cr = ((size_t)layer * max_seq + p0 + t) * kvd;
     for (int idx = threadIdx.x; idx < (n_heads + n_kv) * half; idx += 256) {
         const int h = idx / half, i = idx % half;
         int64_t *vec = q + (size_t)h * hd;   // k heads follow the q heads
@@ -96,10 +99,11 @@ int q48_launch_pf_embed(q48_ctx *c, int64_t *H, const int64_t *table, const int 
 
 int q48_launch_pf_rope_store(q48_ctx *c, int64_t *QKV, int64_t *kcache, int64_t *vcache,
                              int layer, int p0, int T, int n_heads, int n_kv, int hd,
-                             int max_seq)
+                             int max_seq, const int *d_pos)
 {
     hipLaunchKernelGGL(k_pf_rope_store, dim3(T), dim3(256), 0, c->stream, QKV, kcache, vcache,
-                       c->rope_cos, c->rope_sin, layer, p0, n_heads, n_kv, hd, max_seq);
+                       c->rope_cos, c->rope_sin, layer, p0, n_heads, n_kv, hd, max_seq, d_pos,
+                       c->rope_max_seq);
     return (int)hipGetLastError();
 }
 

@@ -106,6 +106,18 @@ ABI_SIGNATURES = {
     "q48_graph_instantiate": [_P, C.POINTER(C.c_void_p)],
     "q48_graph_replay": [_P, _P, _I],
     "q48_graph_destroy": [_P, _P],
+    "q48_qcache_bytes": [_I, _I, _I, _I, _I, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)],
+    "q48_qcache_store_rows": [_P, _P, _I, _I, _I, _P, _P, _I],
+    "q48_qcache_load_rows": [_P, _P, _P, _P, _I, _I, _I, _I],
+    "q48_rope_store_rows_qcache": [_P, _P, _P, _I, _I, _I, _P, _I],
+    "q48_attn_decode_qcache": [_P, _P, _P, _P, _P, _P, _I, _I, _I],
+    "q48_attn_decode_rope_qcache": [_P, _P, _P, _P, _P, _P, _I, _I, _I],
+    "q48_attn_rows_qcache": [_P, _P, _P, _P, _I, _I, _I, _I, _P],
+    "q48_attn_tree": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P],
+    "q48_rope_store_rows_at": [_P, _P, _P, _P, _I, _I, _I, _P, _I, _I, _I, _I],
+    "q48_cache_keep_rows": [_P, _P, _P, _I, _I, _P, _I, _I, _I, _I],
+    "q48_qcache_keep_rows": [_P, _P, _I, _P, _I],
+    "q48_logprobs_rows": [_P, _P, _I, _I, _P, _P, _P, _I, _P, _P],
     "q48_set_attn_wait": [_P, C.c_int64],
     "q48_prof_enable": [_P, _I],
     "q48_timer_start": [_P],
@@ -117,6 +129,21 @@ ABI_SIGNATURES = {
 class Prof(C.Structure):
     """q48_prof: HIP-event timing of q48_gemv launches."""
     _fields_ = [("launches", C.c_int), ("ms", C.c_double), ("bytes", C.c_double)]
+
+
+class QCache(C.Structure):
+    """q48_qcache: a quantised key/value cache's device arrays and sizes."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_step", C.c_void_p),
+                ("v_step", C.c_void_p)] + [(n, C.c_int) for n in
+                                           ("bits", "layers", "max_seq", "n_kv", "head_dim")]
+
+
+def qcache_bytes(bits, layers, max_seq, n_kv, head_dim) -> tuple[int, int]:
+    """Bytes of a quantised cache's codes and steps (of its keys, and as many of its values)."""
+    c, s = C.c_size_t(), C.c_size_t()
+    check("q48_qcache_bytes", hip_lib().q48_qcache_bytes(bits, layers, max_seq, n_kv, head_dim,
+                                                         C.byref(c), C.byref(s)))
+    return c.value, s.value
 
 
 class Q48Error(RuntimeError):
@@ -440,6 +467,68 @@ class Context:
     def gemv_residual_stats(self, acc, W, x, M, K, stats):
         return check("q48_gemv_residual_stats",
                      hip_lib().q48_gemv_residual_stats(self.h, acc, W, x, M, K, stats))
+
+    # quantised cache, rows under a mask, log probabilities
+    @staticmethod
+    def qcache(k, v, k_step, v_step, bits, layers, max_seq, n_kv, head_dim) -> QCache:
+        """Describe a quantised cache in device memory the caller owns."""
+        return QCache(k, v, k_step, v_step, bits, layers, max_seq, n_kv, head_dim)
+
+    def new_qcache(self, bits, layers, max_seq, n_kv, head_dim) -> QCache:
+        """A zeroed quantised cache in buffers of this context."""
+        codes, steps = qcache_bytes(bits, layers, max_seq, n_kv, head_dim)
+        bufs = [self.buffer(n // 8) for n in (codes, codes, steps, steps)]
+        for b in bufs:
+            self.zero(b.ptr, b.nbytes)
+        return QCache(*(b.ptr for b in bufs), bits, layers, max_seq, n_kv, head_dim)
+
+    def qcache_store_rows(self, cache, layer, p0, T, K, V, ld):
+        """Quantise T rows of rotated keys K and values V (rows ld words apart) at row p0."""
+        return check("q48_qcache_store_rows", hip_lib().q48_qcache_store_rows(
+            self.h, C.byref(cache), layer, p0, T, K, V, ld))
+
+    def qcache_load_rows(self, K, V, cache, layer, p0, T, ld):
+        return check("q48_qcache_load_rows", hip_lib().q48_qcache_load_rows(
+            self.h, K, V, C.byref(cache), layer, p0, T, ld))
+
+    def rope_store_rows_qcache(self, qkv, cache, layer, p0, T, nh, d_pos=None):
+        return check("q48_rope_store_rows_qcache", hip_lib().q48_rope_store_rows_qcache(
+            self.h, qkv, C.byref(cache), layer, p0, T, d_pos, nh))
+
+    def attn_decode_qcache(self, out, q, cache, kn, vn, layer, pos, nh):
+        return check("q48_attn_decode_qcache", hip_lib().q48_attn_decode_qcache(
+            self.h, out, q, C.byref(cache), kn, vn, layer, pos, nh))
+
+    def attn_decode_rope_qcache(self, out, q, cache, kn, vn, layer, pos, nh):
+        return check("q48_attn_decode_rope_qcache", hip_lib().q48_attn_decode_rope_qcache(
+            self.h, out, q, C.byref(cache), kn, vn, layer, pos, nh))
+
+    def attn_rows_qcache(self, out, qkv, cache, layer, p0, T, nh, mask=None):
+        """Attention of T rotated [q | k | v] rows over a quantised cache that holds them."""
+        return check("q48_attn_rows_qcache", hip_lib().q48_attn_rows_qcache(
+            self.h, out, qkv, C.byref(cache), layer, p0, T, nh, mask))
+
+    def attn_tree(self, out, qkv, kc, vc, layer, p0, T, nh, nkv, hd, max_seq, mask=None):
+        """Attention of T rotated [q | k | v] rows over the int64 cache under a mask."""
+        return check("q48_attn_tree", hip_lib().q48_attn_tree(
+            self.h, out, qkv, kc, vc, layer, p0, T, nh, nkv, hd, max_seq, mask))
+
+    def rope_store_rows_at(self, qkv, kc, vc, layer, p0, T, d_pos, nh, nkv, hd, max_seq):
+        return check("q48_rope_store_rows_at", hip_lib().q48_rope_store_rows_at(
+            self.h, qkv, kc, vc, layer, p0, T, d_pos, nh, nkv, hd, max_seq))
+
+    def cache_keep_rows(self, kc, vc, layers, p0, d_rows, n, nkv, hd, max_seq):
+        return check("q48_cache_keep_rows", hip_lib().q48_cache_keep_rows(
+            self.h, kc, vc, layers, p0, d_rows, n, nkv, hd, max_seq))
+
+    def qcache_keep_rows(self, cache, p0, d_rows, n):
+        return check("q48_qcache_keep_rows", hip_lib().q48_qcache_keep_rows(
+            self.h, C.byref(cache), p0, d_rows, n))
+
+    def logprobs_rows(self, logits, T, vocab, tokens, logp, entropy, top_n=0, top_ids=None,
+                      top_logp=None):
+        return check("q48_logprobs_rows", hip_lib().q48_logprobs_rows(
+            self.h, logits, T, vocab, tokens, logp, entropy, top_n, top_ids, top_logp))
 
     def prof_enable(self, on: bool = True):
         check("q48_prof_enable", hip_lib().q48_prof_enable(self.h, int(on)))

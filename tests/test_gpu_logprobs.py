@@ -1,0 +1,143 @@
+"""q48_logprobs_rows on the GPU, word for word against the plain form in Python
+integers.
+"""
+import numpy as np
+import pytest
+
+import intllm
+import serve_plain as P
+
+pytestmark = pytest.mark.gpu
+I64 = np.iinfo(np.int64)
+
+
+def ints(ctx, a):
+    """An int32 array on the device (in a buffer of 8-byte words)."""
+    a = np.asarray(a, dtype=np.int32).ravel()
+    return ctx.to_device(np.concatenate([a, np.zeros(a.size % 2, np.int32)]).view(np.int64))
+
+
+def check_rows(ctx, x, tokens, top, ask=("logp", "entropy", "top")):
+    T, V = x.shape
+    d, tk = ctx.to_device(x), ints(ctx, tokens)
+    logp, ent = ctx.to_device(np.full(T, 5)), ctx.to_device(np.full(T, 5))
+    ids, tlp = ints(ctx, np.full(T * max(1, top), 5)), ctx.to_device(np.full(T * max(1, top), 5))
+    ctx.logprobs_rows(d.ptr, T, V, tk.ptr, logp.ptr if "logp" in ask else None,
+                      ent.ptr if "entropy" in ask else None, top if "top" in ask else 0, ids.ptr,
+                      tlp.ptr)
+    want = P.logprobs(x, tokens, top)
+    none = np.full(T, 5)
+    assert (logp.download() == (want[0] if "logp" in ask else none)).all()
+    assert (ent.download() == (want[1] if "entropy" in ask else none)).all()
+    if top and "top" in ask:
+        got = ids.download().view(np.int32)[:T * top].reshape(T, top)
+        assert (got == want[2]).all()
+        assert (tlp.download().reshape(T, top) == want[3]).all()
+    assert (d.download() == x.ravel()).all()
+
+
+def logits(rng, T, V, sigma=2.5):
+    return (rng.standard_normal((T, V)) * (sigma * P.ONE)).astype(np.int64)
+
+
+@pytest.mark.parametrize("V", [1, 2, 3, 63, 64, 65, 255, 257, 1000, 4095, 4097, 9001, 32000])
+@pytest.mark.parametrize("top", [0, 1, 5, 32])
+def test_sizes(ctx, V, top):
+    rng = np.random.default_rng(V)
+    T = 3 if V < 9000 else 1
+    x = logits(rng, T, V)
+    check_rows(ctx, x, rng.integers(0, V, T), min(top, V))
+
+
+@pytest.mark.parametrize("T", [1, 2, 7, 64, 300])
+def test_rows(ctx, T):
+    rng = np.random.default_rng(T)
+    x = logits(rng, T, 400)
+    tokens = rng.integers(0, 400, T)
+    tokens[T // 2] = -1
+    if T > 3:
+        tokens[1], tokens[2] = 400, I64.min >> 40   # past the vocabulary; far negative
+    check_rows(ctx, x, tokens, 20)
+
+
+def test_a_large_vocabulary(ctx):
+    rng = np.random.default_rng(1)
+    check_rows(ctx, logits(rng, 2, 151937), [151936, 0], 20)
+
+
+def edges():
+    rng = np.random.default_rng(0)
+    x = logits(rng, 12, 300)
+    x[0] = 0                                  # all the same: ties to the lowest id
+    x[1] = I64.min                            # the type's lowest value everywhere
+    x[2, ::2] = I64.min                       # and as a mask
+    x[3, 7], x[3, 8] = I64.max, I64.min       # u past 63 bits: the smallest log probability
+    x[4] = -1
+    x[4, 299] = 0                             # the last id alone
+    x[5] >>= 40
+    x[6, 3:9] = x[6].max() + 5                # ties at the top
+    x[7] = np.arange(300) * (P.LN2 // 3)      # u at multiples of LN2
+    x[8] = -np.arange(300) * (1 << 42)        # and of the table's step
+    x[9] = I64.max - np.arange(300)
+    x[10] = np.where(np.arange(300) == 40, 0, -(45 << 48))   # e below 2^-48 but one
+    x[11] *= 40
+    return x
+
+
+@pytest.mark.parametrize("top", [0, 3, 32])
+def test_edges(ctx, top):
+    x = edges()
+    tokens = np.arange(12) * 24 + 8
+    tokens[3] = 8
+    check_rows(ctx, x, tokens, top)
+
+
+@pytest.mark.parametrize("ask", [("logp",), ("entropy",), ("top",), ("logp", "top")])
+def test_parts(ctx, ask):
+    rng = np.random.default_rng(12)
+    check_rows(ctx, logits(rng, 5, 777), rng.integers(0, 777, 5), 6, ask)
+
+
+def test_probabilities_add_up(ctx):
+    """Every token's log probability: their exponentials add up to one (each e^logp is
+    within 2^-47 of its probability, 2000 of them within 2^-36)."""
+    rng = np.random.default_rng(2)
+    V = 2000
+    row = logits(rng, 1, V)
+    x = np.repeat(row, V, 0)
+    d, tk, logp = ctx.to_device(x), ints(ctx, np.arange(V)), ctx.buffer(V)
+    ctx.logprobs_rows(d.ptr, V, V, tk.ptr, logp.ptr, None)
+    lp = logp.download().astype(np.float64) / P.ONE
+    assert abs(np.exp(lp).sum() - 1) < 2.0 ** -36
+    f = row[0].astype(np.float64) / P.ONE
+    assert np.abs(lp - (f - np.log(np.exp(f - f.max()).sum()) - f.max())).max() < 2.0 ** -35
+
+
+def test_captured(ctx):
+    """Replays of a captured call, the logits changed between them."""
+    rng = np.random.default_rng(5)
+    lib = intllm.hip_lib()
+    T, V, top = 5, 5000, 7
+    with intllm.Context(0) as c:
+        d, tk = c.buffer(T * V), ints(c, rng.integers(0, V, T))
+        logp, ent, ids, tlp = c.buffer(T), c.buffer(T), c.buffer(T * top), c.buffer(T * top)
+
+        def call():
+            c.logprobs_rows(d.ptr, T, V, tk.ptr, logp.ptr, ent.ptr, top, ids.ptr, tlp.ptr)
+
+        d.upload(logits(rng, T, V))
+        call()
+        c.sync()
+        intllm.check("begin", lib.q48_graph_begin(c.h))
+        call()
+        intllm.check("end", lib.q48_graph_end(c.h))
+        for _ in range(4):
+            x = logits(rng, T, V)
+            d.upload(x)
+            intllm.check("launch", lib.q48_graph_launch(c.h, 1))
+            got = [b.download() for b in (logp, ent, ids, tlp)]
+            call()
+            assert all((b.download() == g).all() for b, g in zip((logp, ent, ids, tlp), got))
+        want = P.logprobs(x, tk.download().view(np.int32)[:T], top)
+        assert (got[0] == want[0]).all() and (got[1] == want[1]).all()
+        intllm.check("drop", lib.q48_graph_drop(c.h))

@@ -1,0 +1,460 @@
+"""The quantised key/value cache on the GPU: what is written and read back, and
+attention over it, word for word against the plain forms.
+"""
+import numpy as np
+import pytest
+
+import intllm
+import serve_plain as P
+
+pytestmark = pytest.mark.gpu
+I64 = np.iinfo(np.int64)
+
+
+def acts(rng, *shape, sigma=1.0):
+    return (rng.standard_normal(shape) * (sigma * P.ONE)).astype(np.int64)
+
+
+class Cache:
+    """A quantised cache on the device, its codes and steps for the tests to see."""
+
+    def __init__(self, ctx, bits, layers, max_seq, nkv, hd):
+        self.ctx, self.bits, self.shape = ctx, bits, (layers, max_seq, nkv)
+        codes, steps = intllm.qcache_bytes(bits, layers, max_seq, nkv, hd)
+        self.row = hd * bits // 8
+        self.bufs = [intllm.Buffer(ctx, n // 8) for n in (codes, codes, steps, steps)]
+        rng = np.random.default_rng(9)     # what a cache held before: any bytes
+        for b in self.bufs:
+            b.upload(rng.integers(I64.min, I64.max, b.n))
+        self.c = ctx.qcache(*(b.ptr for b in self.bufs), bits, layers, max_seq, nkv, hd)
+
+    def read(self):
+        """k, v bytes [layers][max_seq][nkv][row] and steps [layers][max_seq][nkv]"""
+        k, v, ks, vs = (b.download() for b in self.bufs)
+        s = self.shape
+        return (k.view(np.uint8).reshape(*s, self.row), v.view(np.uint8).reshape(*s, self.row),
+                ks.reshape(s), vs.reshape(s))
+
+    def fill(self, layer, K, V):
+        """Rows [0, n) of a layer from values, quantised by the plain form; their values."""
+        k, v, ks, vs = self.read()
+        out = []
+        for x, codes, steps in ((K, k, ks), (V, v, vs)):
+            c, st = P.quantise(x, self.bits)
+            codes[layer, :len(x)], steps[layer, :len(x)] = P.pack(c, self.bits), st
+            out.append(P.values(c, st))
+        for b, x in zip(self.bufs, (k, v, ks, vs)):
+            b.upload(np.ascontiguousarray(x).view(np.int64).ravel())
+        return out
+
+    def free(self):
+        for b in self.bufs:
+            b.free()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("nkv,hd,T,p0,pad", [(1, 32, 1, 0, 0), (4, 64, 1, 17, 0), (3, 64, 37, 5, 0),
+                                             (2, 128, 70, 0, 24), (8, 32, 129, 2, 1),
+                                             (7, 128, 5, 100, 640)])
+def test_store_and_load(ctx, bits, nkv, hd, T, p0, pad):
+    rng = np.random.default_rng(bits * 1000 + T)
+    max_seq, ld = p0 + T + 3, nkv * hd + pad
+    K, V = acts(rng, T, ld), acts(rng, T, ld, sigma=0.02)
+    K[0, 0], V[T // 2, 1] = I64.min, I64.max
+    if T > 4:
+        K[3], V[2] = 0, 0
+        K[4] = rng.integers(-20, 20, ld)
+    cache = Cache(ctx, bits, 2, max_seq, nkv, hd)
+    before = cache.read()
+    dk, dv = ctx.to_device(K), ctx.to_device(V)
+    ctx.qcache_store_rows(cache.c, 1, p0, T, dk.ptr, dv.ptr, ld)
+    after = cache.read()
+    back = [ctx.to_device(np.full(T * ld, 77, np.int64)) for _ in range(2)]
+    ctx.qcache_load_rows(back[0].ptr, back[1].ptr, cache.c, 1, p0, T, ld)
+    for i, x in enumerate((K, V)):
+        c, st = P.quantise(x[:, :nkv * hd].reshape(T, nkv, hd), bits)
+        for got, old, want in ((after[i], before[i], P.pack(c, bits)),
+                               (after[i + 2], before[i + 2], st)):
+            exp = old.copy()
+            exp[1, p0:p0 + T] = want           # and no other row
+            assert (got == exp).all()
+        got = back[i].download().reshape(T, ld)
+        assert (got[:, :nkv * hd].reshape(T, nkv, hd) == P.values(c, st)).all()
+        assert (got[:, nkv * hd:] == 77).all()
+    cache.free()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 32), (4, 4, 64), (6, 2, 128)])
+def test_rope_store(ctx, bits, nh, nkv, hd):
+    rng = np.random.default_rng(11)
+    T, p0, max_seq = 9, 4, 32
+    ctx.rope_init(hd, max_seq, 10000)
+    cos_t, sin_t = P.rope_tables(hd, max_seq)
+    x = acts(rng, T, nh + 2 * nkv, hd)
+    where = np.array([4, 5, 5, 6, -1, 31, 32, 0, 7], dtype=np.int32)
+    d_where = ctx.to_device(np.concatenate([where, [0]]).astype(np.int32).view(np.int64))
+    for at, ptr in ((range(p0, p0 + T), None), (where, d_where.ptr)):
+        cache = Cache(ctx, bits, 1, max_seq, nkv, hd)
+        before = cache.read()
+        d = ctx.to_device(x)
+        ctx.rope_store_rows_qcache(d.ptr, cache.c, 0, p0, T, nh, ptr)
+        got, after = d.download().reshape(x.shape), cache.read()
+        for t, pos in enumerate(at):
+            if not 0 <= pos < max_seq:
+                assert (got[t] == x[t]).all()
+                assert all((a[0, p0 + t] == b[0, p0 + t]).all() for a, b in zip(after, before))
+                continue
+            r = P.rope(x[t, :nh + nkv], cos_t, sin_t, int(pos))
+            assert (got[t, :nh + nkv] == r).all() and (got[t, nh + nkv:] == x[t, nh + nkv:]).all()
+            for i, y in enumerate((r[nh:], x[t, nh + nkv:])):
+                c, st = P.quantise(y, bits)
+                assert (after[i][0, p0 + t] == P.pack(c, bits)).all()
+                assert (after[i + 2][0, p0 + t] == st).all()
+        cache.free()
+
+
+SHAPES = [(1, 1, 64), (8, 2, 32), (32, 4, 64), (7, 1, 128), (8, 8, 64), (28, 4, 32), (6, 3, 128),
+          (16, 1, 64), (40, 2, 64)]
+
+
+def decode_case(ctx, bits, nh, nkv, hd, pos, max_seq, rng, rope=False, layer=0, layers=1,
+                sigma=1.0, edit=None):
+    """One decoded token against the plain form: its output and its row of the cache."""
+    cache = Cache(ctx, bits, layers, max_seq, nkv, hd)
+    K, V = acts(rng, pos + 1, nkv, hd, sigma=sigma), acts(rng, pos + 1, nkv, hd, sigma=sigma)
+    q = acts(rng, nh, hd, sigma=1.5)
+    if edit:
+        edit(q, K, V)
+    kv, vv = cache.fill(layer, K, V)
+    kn, vn = acts(rng, nkv, hd), acts(rng, nkv, hd)
+    qr, kr = q, kn
+    if rope:
+        ctx.rope_init(hd, max_seq, 10000)
+        cos_t, sin_t = P.rope_tables(hd, max_seq)
+        qr, kr = P.rope(q, cos_t, sin_t, pos), P.rope(kn, cos_t, sin_t, pos)
+    want_row = [P.quantise(kr, bits), P.quantise(vn, bits)]
+    kv[pos], vv[pos] = (P.values(*w) for w in want_row)
+    want = P.attend(qr[None], kv, vv, np.ones((1, pos + 1), bool))[0]
+    before = cache.read()
+    bufs = [ctx.to_device(a) for a in (q, kn, vn)]
+    out = ctx.to_device(np.full(nh * hd, 5, np.int64))
+    f = ctx.attn_decode_rope_qcache if rope else ctx.attn_decode_qcache
+    f(out.ptr, bufs[0].ptr, cache.c, bufs[1].ptr, bufs[2].ptr, layer, pos, nh)
+    got, after = out.download().reshape(nh, hd), cache.read()
+    assert (got == want).all(), np.argwhere(got != want)[:5]
+    for i, (c, st) in enumerate(want_row):
+        for b, a, w in ((before[i], after[i], P.pack(c, bits)), (before[i + 2], after[i + 2], st)):
+            b[layer, pos] = w
+            assert (a == b).all()
+    assert all((b.download() == a.ravel()).all() for b, a in zip(bufs, (q, kn, vn)))
+    cache.free()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("nh,nkv,hd", SHAPES)
+@pytest.mark.parametrize("pos", [0, 1, 15, 16, 63, 64, 130, 517])
+def test_decode(ctx, bits, nh, nkv, hd, pos):
+    decode_case(ctx, bits, nh, nkv, hd, pos, pos + 1 + pos % 3,
+                np.random.default_rng(pos * 10 + bits))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("nh,nkv,hd,pos", [(32, 4, 64, 2500), (8, 8, 128, 4100), (8, 1, 32, 9000),
+                                           (4, 2, 64, 20011), (2, 1, 64, 32766)])
+def test_decode_long(ctx, bits, nh, nkv, hd, pos):
+    decode_case(ctx, bits, nh, nkv, hd, pos, min(32767, pos + 40), np.random.default_rng(pos))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("pos", [3, 200, 5000])
+def test_decode_rope_in_a_later_layer(ctx, bits, pos):
+    decode_case(ctx, bits, 8, 2, 64, pos, pos + 5, np.random.default_rng(7), rope=True, layer=2,
+                layers=3)
+
+
+def big_values(q, K, V):
+    V[len(V) // 2] *= 300            # |v| past 2^51
+
+
+def huge_scores(q, K, V):
+    q[0] = I64.max                   # dot products that wrap
+    K[::3] = I64.min
+
+
+def tiny(q, K, V):
+    q[:] >>= 45
+    K[:] >>= 44
+    V[:] >>= 46
+
+
+def one_peak(q, K, V):
+    K[len(K) // 3] = np.sign(q[0]) * (8 * P.ONE)
+
+
+def zeros(q, K, V):
+    K[:], V[:] = 0, 0
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("edit", [big_values, huge_scores, tiny, one_peak, zeros])
+@pytest.mark.parametrize("pos", [40, 700, 4500])
+def test_decode_of_unusual_values(ctx, bits, edit, pos):
+    decode_case(ctx, bits, 8, 2, 64, pos, pos + 1, np.random.default_rng(pos), edit=edit)
+
+
+def rows_case(ctx, bits, nh, nkv, hd, T, p0, max_seq, sees, rng, edit=None, junk=False):
+    K, V = acts(rng, p0 + T, nkv, hd), acts(rng, p0 + T, nkv, hd)
+    qkv = acts(rng, T, nh + 2 * nkv, hd, sigma=1.5)
+    if edit:
+        edit(qkv[0], K, V)
+    mask = None
+    see = np.concatenate([np.ones((T, p0), bool), np.tri(T, dtype=bool) if sees is None else sees],
+                         1)
+    if sees is not None:
+        w = P.mask_words(sees)
+        if junk and T % 64:                  # bits from T on say nothing
+            w[:, -1] |= np.int64(-1) << np.int64(T % 64)
+        mask = ctx.to_device(w).ptr
+    out = ctx.to_device(np.full(T * nh * hd, 5, np.int64))
+    d = ctx.to_device(qkv)
+    if bits == 64:
+        kc, vc = np.zeros((2, max_seq, nkv, hd), np.int64), np.zeros((2, max_seq, nkv, hd), np.int64)
+        kc[:], vc[:] = I64.max // 3, I64.min // 3   # rows past the last, and the other layer
+        kc[1, :p0 + T], vc[1, :p0 + T] = K, V
+        dk, dv = ctx.to_device(kc), ctx.to_device(vc)
+        ctx.attn_tree(out.ptr, d.ptr, dk.ptr, dv.ptr, 1, p0, T, nh, nkv, hd, max_seq, mask)
+        want = P.attend(qkv[:, :nh], K, V, see)
+    else:
+        cache = Cache(ctx, bits, 2, max_seq, nkv, hd)
+        kv, vv = cache.fill(1, K, V)
+        ctx.attn_rows_qcache(out.ptr, d.ptr, cache.c, 1, p0, T, nh, mask)
+        want = P.attend(qkv[:, :nh], kv, vv, see)
+    got = out.download().reshape(T, nh, hd)
+    assert (got == want).all(), np.argwhere(got != want)[:5]
+    assert (d.download() == qkv.ravel()).all()
+    if bits != 64:
+        cache.free()
+
+
+@pytest.mark.parametrize("bits", [8, 4, 64])
+@pytest.mark.parametrize("nh,nkv,hd", SHAPES)
+@pytest.mark.parametrize("T,p0", [(1, 0), (3, 0), (17, 30), (5, 700)])
+def test_rows_causal(ctx, bits, nh, nkv, hd, T, p0):
+    rows_case(ctx, bits, nh, nkv, hd, T, p0, p0 + T + 2, None, np.random.default_rng(T + p0))
+
+
+@pytest.mark.parametrize("bits", [8, 4, 64])
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 32), (32, 4, 64), (7, 1, 128), (4, 4, 64)])
+@pytest.mark.parametrize("T,p0,pad", [(2, 0, 1), (16, 0, 3), (33, 100, 2), (65, 7, 1), (130, 0, 5)])
+def test_rows_tree(ctx, bits, nh, nkv, hd, T, p0, pad):
+    rng = np.random.default_rng(T)
+    sees, _ = P.tree(rng, T, pad)
+    rows_case(ctx, bits, nh, nkv, hd, T, p0, p0 + T, sees, rng, junk=True)
+
+
+@pytest.mark.parametrize("bits", [8, 4, 64])
+def test_rows_under_any_mask(ctx, bits):
+    """Masks that no tree has: later rows seen, nothing seen at all, one row seen."""
+    rng = np.random.default_rng(5)
+    sees = rng.random((70, 70)) < 0.3
+    sees[11] = False
+    sees[12] = False
+    sees[12, 69] = True
+    sees[69] = True
+    rows_case(ctx, bits, 8, 2, 64, 70, 0, 70, sees, rng)
+    rows_case(ctx, bits, 8, 2, 64, 70, 33, 111, sees, rng)
+    rows_case(ctx, bits, 8, 2, 64, 70, 0, 70, np.zeros((70, 70), bool), rng)
+
+
+@pytest.mark.parametrize("bits", [8, 4, 64])
+@pytest.mark.parametrize("T,p0", [(40, 1500), (300, 0), (9, 5000), (2, 20000)])
+def test_rows_long(ctx, bits, T, p0):
+    rows_case(ctx, bits, 8, 2, 64, T, p0, p0 + T + 1, None, np.random.default_rng(T))
+
+
+@pytest.mark.parametrize("bits", [8, 4, 64])
+@pytest.mark.parametrize("edit", [big_values, huge_scores, tiny, one_peak, zeros])
+@pytest.mark.parametrize("T,p0", [(20, 0), (5, 300), (6, 3000)])
+def test_rows_of_unusual_values(ctx, bits, edit, T, p0):
+    rng = np.random.default_rng(T)
+    sees, _ = P.tree(rng, T, 1)
+    rows_case(ctx, bits, 8, 2, 64, T, p0, p0 + T, sees, rng, edit=edit)
+
+
+def test_step_mode_and_graph(ctx):
+    """Decode replayed from a graph, the position on the device: every replay
+    against the eager form, across the positions where kernels change."""
+    rng = np.random.default_rng(21)
+    nh, nkv, hd, max_seq, n = 8, 2, 64, 3000, 5
+    for start in (2, 2040, 2990):
+        with intllm.Context(0) as c:
+            c.rope_init(hd, max_seq, 10000)
+            cache = Cache(c, 8, 1, max_seq, nkv, hd)
+            cache.fill(0, acts(rng, start, nkv, hd), acts(rng, start, nkv, hd))
+            other = Cache(c, 8, 1, max_seq, nkv, hd)
+            for a, b in zip(other.bufs, cache.bufs):
+                a.upload(b.download())
+            q, kn, vn = (c.to_device(acts(rng, m, hd)) for m in (nh, nkv, nkv))
+            out, want = c.buffer(nh * hd), c.buffer(nh * hd)
+            logits = c.to_device(np.arange(8))
+            toks = c.buffer(8)
+
+            def step():
+                c.attn_decode_rope_qcache(out.ptr, q.ptr, cache.c, kn.ptr, vn.ptr, 0, start, nh)
+                intllm.check("q48_argmax_step", intllm.hip_lib().q48_argmax_step(
+                    c.h, logits.ptr, 8, toks.ptr, 16))
+
+            lib = intllm.hip_lib()
+            intllm.check("step", lib.q48_step_set(c.h, 0, start))
+            intllm.check("step", lib.q48_step_mode(c.h, 1))
+            step()                                   # workspaces reach their size
+            c.sync()
+            intllm.check("step", lib.q48_step_set(c.h, 0, start))
+            intllm.check("begin", lib.q48_graph_begin(c.h))
+            step()
+            intllm.check("end", lib.q48_graph_end(c.h))
+            for i in range(n):
+                intllm.check("launch", lib.q48_graph_launch(c.h, 1))
+                got = out.download()
+                intllm.check("step", lib.q48_step_mode(c.h, 0))
+                c.attn_decode_rope_qcache(want.ptr, q.ptr, other.c, kn.ptr, vn.ptr, 0, start + i,
+                                          nh)
+                assert (want.download() == got).all(), (start, i)
+                intllm.check("step", lib.q48_step_mode(c.h, 1))
+            assert all((a.download() == b.download()).all()
+                       for a, b in zip(cache.bufs, other.bufs))
+            intllm.check("drop", lib.q48_graph_drop(c.h))
+            cache.free()
+            other.free()
+
+
+def test_step_position_outside_the_cache_changes_nothing(ctx):
+    lib = intllm.hip_lib()
+    rng = np.random.default_rng(4)
+    with intllm.Context(0) as c:
+        cache = Cache(c, 4, 1, 50, 2, 64)
+        before = cache.read()
+        q, kn, vn = (c.to_device(acts(rng, m, 64)) for m in (4, 2, 2))
+        out = c.to_device(np.full(256, 5, np.int64))
+        intllm.check("mode", lib.q48_step_mode(c.h, 1))
+        for pos in (50, 4000):       # (q48_step_set itself refuses a negative one)
+            intllm.check("set", lib.q48_step_set(c.h, 0, pos))
+            c.attn_decode_qcache(out.ptr, q.ptr, cache.c, kn.ptr, vn.ptr, 0, 3, 4)
+        assert all((a == b).all() for a, b in zip(before, cache.read()))
+        cache.free()
+
+
+def test_two_contexts_at_once(ctx):
+    """Two programs' calls in flight together, each on its own stream and workspace."""
+    rng = np.random.default_rng(8)
+    K, V = acts(rng, 2100, 2, 64), acts(rng, 2100, 2, 64)
+    with intllm.Context(0) as a, intllm.Context(0) as b:
+        state = []
+        for c in (a, b):
+            cache = Cache(c, 8, 1, 2100, 2, 64)
+            cache.fill(0, K, V)
+            q = acts(rng, 6, 12, 64)
+            state.append((c, cache, q, c.to_device(q), c.buffer(6 * 8 * 64)))
+        for _ in range(5):
+            for c, cache, _, d, out in state:
+                c.attn_rows_qcache(out.ptr, d.ptr, cache.c, 0, 2090, 6, 8)
+        kv, vv = (P.values(*P.quantise(x, 8)) for x in (K, V))
+        see = np.concatenate([np.ones((6, 2090), bool), np.tri(6, dtype=bool)], 1)
+        for c, cache, q, _, out in state:
+            want = P.attend(q[:, :8], kv[:2096], vv[:2096], see)
+            assert (out.download().reshape(6, 8, 64) == want).all()
+            cache.free()
+
+
+def test_cache_past_four_gigabytes(ctx):
+    """The last layer of a cache whose offsets pass 32 bits."""
+    rng = np.random.default_rng(3)
+    layers, max_seq, nkv, hd, nh = 131, 32767, 8, 128, 16
+    codes, steps = intllm.qcache_bytes(8, layers, max_seq, nkv, hd)
+    assert codes > 1 << 32
+    bufs = [intllm.Buffer(ctx, n // 8) for n in (codes, codes, steps, steps)]
+    cache = ctx.qcache(*(b.ptr for b in bufs), 8, layers, max_seq, nkv, hd)
+    T, p0 = 40, 0
+    K, V, qkv = acts(rng, T, nkv, hd), acts(rng, T, nkv, hd), acts(rng, T, nh + 2 * nkv, hd)
+    dk, dv, dq = (ctx.to_device(x) for x in (K, V, qkv))
+    out = ctx.buffer(T * nh * hd)
+    ctx.qcache_store_rows(cache, layers - 1, p0, T, dk.ptr, dv.ptr, nkv * hd)
+    ctx.attn_rows_qcache(out.ptr, dq.ptr, cache, layers - 1, p0, T, nh)
+    kv, vv = (P.values(*P.quantise(x, 8)) for x in (K, V))
+    want = P.attend(qkv[:, :nh], kv, vv, np.tri(T, dtype=bool))
+    assert (out.download().reshape(T, nh, hd) == want).all()
+    for b in bufs:
+        b.free()
+
+
+def test_int64_rows_equal_the_decode_and_prefill_entry_points(ctx):
+    """attn_tree's causal form against q48_attn_prefill, and a tree's paths against
+    q48_attn_decode of their own tokens."""
+    rng = np.random.default_rng(6)
+    nh, nkv, hd, T, p0, max_seq = 8, 2, 64, 12, 40, 64
+    ctx.rope_init(hd, max_seq, 10000)
+    K, V = acts(rng, max_seq, nkv, hd), acts(rng, max_seq, nkv, hd)
+    qkv = acts(rng, T, nh + 2 * nkv, hd)
+    dk, dv, dq = (ctx.to_device(x) for x in (K, V, qkv))
+    a, b = ctx.buffer(T * nh * hd), ctx.buffer(T * nh * hd)
+    ctx.attn_tree(a.ptr, dq.ptr, dk.ptr, dv.ptr, 0, p0, T, nh, nkv, hd, max_seq)
+    ctx.attn_prefill(b.ptr, dq.ptr, dk.ptr, dv.ptr, 0, p0, T, nh, nkv, hd, max_seq)
+    assert (a.download() == b.download()).all()
+    sees, _ = P.tree(rng, T)
+    m = ctx.to_device(P.mask_words(sees))
+    ctx.attn_tree(a.ptr, dq.ptr, dk.ptr, dv.ptr, 0, p0, T, nh, nkv, hd, max_seq, m.ptr)
+    got = a.download().reshape(T, nh, hd)
+    for t in range(T):
+        path = [*range(p0), *(p0 + np.nonzero(sees[t])[0])]
+        k2, v2 = ctx.to_device(K[path]), ctx.to_device(V[path])
+        kn, vn = ctx.to_device(K[path[-1]]), ctx.to_device(V[path[-1]])
+        q, o = ctx.to_device(qkv[t, :nh]), ctx.buffer(nh * hd)
+        ctx.attn_decode(o.ptr, q.ptr, k2.ptr, v2.ptr, kn.ptr, vn.ptr, 0, len(path) - 1, nh, nkv,
+                        hd, len(path))
+        assert (o.download().reshape(nh, hd) == got[t]).all()
+
+
+def test_rope_store_rows_at(ctx):
+    rng = np.random.default_rng(13)
+    nh, nkv, hd, T, p0, max_seq, layers = 4, 2, 64, 6, 3, 16, 2
+    ctx.rope_init(hd, max_seq, 10000)
+    cos_t, sin_t = P.rope_tables(hd, max_seq)
+    x = acts(rng, T, nh + 2 * nkv, hd)
+    where = np.array([3, 4, 4, 16, -5, 15], dtype=np.int32)
+    old = acts(rng, layers, max_seq, nkv, hd)
+    dk, dv, d = ctx.to_device(old), ctx.to_device(old + 1), ctx.to_device(x)
+    dw = ctx.to_device(where.view(np.int64))
+    ctx.rope_store_rows_at(d.ptr, dk.ptr, dv.ptr, 1, p0, T, dw.ptr, nh, nkv, hd, max_seq)
+    k, v, got = old.copy(), old + 1, x.copy()
+    for t, pos in enumerate(where):
+        if 0 <= pos < max_seq:
+            got[t, :nh + nkv] = P.rope(x[t, :nh + nkv], cos_t, sin_t, int(pos))
+            k[1, p0 + t], v[1, p0 + t] = got[t, nh:nh + nkv], x[t, nh + nkv:]
+    assert (d.download() == got.ravel()).all()
+    assert (dk.download() == k.ravel()).all() and (dv.download() == v.ravel()).all()
+
+
+@pytest.mark.parametrize("rows", [[0], [2], [0, 1, 2], [1, 2, 3, 7], [0, 3, 4], [5, 6], [0, 99, -4]])
+def test_keep_rows(ctx, rows):
+    rng = np.random.default_rng(2)
+    layers, max_seq, nkv, hd, p0 = 3, 12, 3, 64, 4
+    d = ctx.to_device(np.array(rows + [0] * (len(rows) % 2), dtype=np.int32).view(np.int64))
+
+    def keep(x):   # [layers][max_seq][...]
+        y = x.copy()
+        for i, r in enumerate(rows):
+            if r > i and p0 + r < max_seq:
+                y[:, p0 + i] = x[:, p0 + r]
+        return y
+
+    k, v = acts(rng, layers, max_seq, nkv, hd), acts(rng, layers, max_seq, nkv, hd)
+    dk, dv = ctx.to_device(k), ctx.to_device(v)
+    ctx.cache_keep_rows(dk.ptr, dv.ptr, layers, p0, d.ptr, len(rows), nkv, hd, max_seq)
+    assert (dk.download() == keep(k).ravel()).all() and (dv.download() == keep(v).ravel()).all()
+    for bits in (8, 4):
+        cache = Cache(ctx, bits, layers, max_seq, nkv, hd)
+        before = cache.read()
+        ctx.qcache_keep_rows(cache.c, p0, d.ptr, len(rows))
+        assert all((a == keep(b)).all() for a, b in zip(cache.read(), before))
+        cache.free()
