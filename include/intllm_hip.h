@@ -472,7 +472,8 @@ int q48_rope_store_rows_qcache(q48_ctx *ctx, int64_t *QKV, const q48_qcache *cac
 /* q48_attn_decode over a quantised cache: k_new and v_new are quantised into row
  * pos, then rows 0 .. pos are attended to.  Same bits as q48_attn_decode over
  * the values the cache stands for.  In step mode pos is read from the
- * device-side state.  out shares no words with q, k_new or v_new. */
+ * device-side state.  out shares no words with q, k_new or v_new.  n_heads at most
+ * 1024. */
 int q48_attn_decode_qcache(q48_ctx *ctx, int64_t *out, const int64_t *q, const q48_qcache *cache,
                            const int64_t *k_new, const int64_t *v_new, int layer, int pos,
                            int n_heads);
@@ -492,7 +493,7 @@ int q48_attn_decode_rope_qcache(q48_ctx *ctx, int64_t *out, const int64_t *q,
  * is the reference's exact attention (llama_int.c:1502-1529) over the rows it
  * attends to, in cache order, so a token of a tree gets the words that decoding
  * its own path gives.  out [T][n_heads * head_dim] shares no words with QKV.
- * head_dim 32, 64 or 128; p0 + T at most 32767. */
+ * head_dim 32, 64 or 128; n_heads at most 1024; p0 + T at most 32767. */
 int q48_attn_tree(q48_ctx *ctx, int64_t *out, const int64_t *QKV, const int64_t *kcache,
                   const int64_t *vcache, int layer, int p0, int T, int n_heads, int n_kv,
                   int head_dim, int max_seq, const uint64_t *mask);

@@ -228,7 +228,7 @@ int q48_rope_store_rows_qcache(q48_ctx *c, int64_t *QKV, const q48_qcache *qc, i
                                int T, const int *d_pos, int n_heads)
 {
     if (!c || !QKV || !q48_qcache_ok(qc) || layer < 0 || layer >= qc->layers || T <= 0 ||
-        n_heads <= 0 || n_heads > 65535 || n_heads % qc->n_kv)
+        n_heads <= 0 || n_heads > 1024 || n_heads % qc->n_kv)
         return Q48_EINVAL;
     if (!c->rope_cos || qc->head_dim != c->rope_head_dim || qc->max_seq > c->rope_max_seq)
         return Q48_ESTATE;
