@@ -472,8 +472,9 @@ int q48_rope_store_rows_qcache(q48_ctx *ctx, int64_t *QKV, const q48_qcache *cac
 /* q48_attn_decode over a quantised cache: k_new and v_new are quantised into row
  * pos, then rows 0 .. pos are attended to.  Same bits as q48_attn_decode over
  * the values the cache stands for.  In step mode pos is read from the
- * device-side state.  out shares no words with q, k_new or v_new.  n_heads at most
- * 1024. */
+ * device-side state; the kernels are chosen from the pos argument also then, so a
+ * graph captured at a short position stays right, and gets slower, as replays move
+ * past it.  out shares no words with q, k_new or v_new.  n_heads at most 1024. */
 int q48_attn_decode_qcache(q48_ctx *ctx, int64_t *out, const int64_t *q, const q48_qcache *cache,
                            const int64_t *k_new, const int64_t *v_new, int layer, int pos,
                            int n_heads);

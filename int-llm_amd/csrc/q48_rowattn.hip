@@ -91,11 +91,15 @@ __device__ __forceinline__ int64_t row16_max64(int64_t v)
 }
 
 // A launch's query vectors are, per KV head, v = (t - t0) G + g (row t, query
-// head kh G + g), taken in tiles of 16 (one MFMA tile of rows); the cache rows in
-// chunks of ch.  Three kernels, each a grid of (chunk, tile, KV head) blocks: the
-// softmax of the exact path needs the row's maximum before the first exponential
-// and the whole sum before the first quotient, and its truncations leave no way
-// to rescale later, so each of the two is a launch boundary.
+// head kh G + g), taken in tiles of up to 16 (the rows of one MFMA tile).  Two
+// forms of the same phases:
+//  - one launch: a block takes a tile over all its rows, scores in LDS (k_ra_tile);
+//  - three launches over (chunk of ch rows, tile of 16, KV head) blocks with the
+//    scores in the workspace (k_ra_score, k_ra_exp, k_ra_value), for spans past
+//    LDS and where the tiles alone leave compute units idle.  The softmax of the
+//    exact path needs the row's maximum before the first exponential and the whole
+//    sum before the first quotient, and its truncations leave no way to rescale
+//    later, so each of the two is a launch boundary.
 struct RaPlan {
     int64_t *sc;     // [n_kv][16 tiles][spad]: scores, then exponentials
     int64_t *cm;     // [n_kv][16 tiles][nchunk]: a chunk's maximum
@@ -103,18 +107,26 @@ struct RaPlan {
     int *far;        // [n_kv][tiles][nchunk]: a visible score outside [-2^62, 2^62)
     int *odd;        // [n_kv][tiles][nchunk]: an exponential outside [0, ONE]
     int ch, nchunk, spad, tiles, t0, Tn;   // rows t0 .. t0 + Tn - 1 of the T
+    int vb;          // vectors a tile
 };
 
-// rows [0, span) hold all that a tile's vectors may see
+// rows [0, span) hold all that vectors up to vlast may see
 template <bool DEC>
-__device__ __forceinline__ int tile_span(const RaArgs &a, const RaPlan &p, int tile, int G, int p0)
+__device__ __forceinline__ int tile_span(const RaArgs &a, const RaPlan &p, int vlast, int G, int p0)
 {
     if (DEC)
         return p0 + 1;
     if (a.mask)
         return p0 + a.T;
-    const int last = (16 * tile + 15) / G;
+    const int last = vlast / G;
     return p0 + p.t0 + (last < p.Tn ? last + 1 : p.Tn);
+}
+
+// rows [0, clear) are seen by row t and every later row of its tile
+template <bool DEC>
+__device__ __forceinline__ int rows_clear(const RaArgs &a, int p0, int t)
+{
+    return DEC || (!a.mask) ? p0 + t + 1 : p0;
 }
 
 // whether row t sees cache row j (j < span)
@@ -141,123 +153,111 @@ __device__ __forceinline__ bool position(const RaArgs &a, int &p0)
     return true;
 }
 
-// 16 codes as int8 MFMA operands: dims d0 .. d0 + 15 of a head's row
+// ---- keys as MFMA operands -----------------------------------------------------
+// Lane (j = lane % 16, kq = lane / 16) holds dims 64 ks + 16 kq .. + 15 of its row,
+// as loaded: int64 words, or the bytes of the codes (4 bits, HD 128: one load
+// holds both ks, the low and the high halves).
 template <int BITS, int HD>
-__device__ __forceinline__ v4i codes16(const uint8_t *row, int d0)
-{
-    if constexpr (BITS == 8) {
-        return *reinterpret_cast<const v4i *>(row + d0);
-    } else {
-        v4i w = *reinterpret_cast<const v4i *>(row + (d0 & (HD / 2 - 1)));
-        const int sh = d0 < HD / 2 ? 0 : 4;
+struct KeyRow {
+    static constexpr int KS = HD < 64 ? 1 : HD / 64, NL = BITS == 8 ? KS : 1;
+    v4i w[NL];
+    uint64_t step;
+    __device__ __forceinline__ void load(const RaArgs &a, size_t row, int kq)
+    {
+        const uint8_t *k = a.k + row * (HD * BITS / 8);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            // a nibble n as a signed byte: (n ^ 8) - 8 without borrows
-            const uint32_t n = ((uint32_t)w[i] >> sh) & 0x0F0F0F0Fu;
-            w[i] = (int)(((n ^ 0x08080808u) + 0x78787878u) ^ 0x80808080u);
+        for (int n = 0; n < NL; ++n) {
+            const int d0 = min(64 * n + 16 * kq, HD - 16);
+            w[n] = *reinterpret_cast<const v4i *>(k + (BITS == 8 ? d0 : d0 & (HD / 2 - 1)));
         }
-        return w;
+        step = (uint64_t)a.ks[row];
     }
-}
+    __device__ __forceinline__ void fresh(const uint8_t *k, uint64_t st, int kq)
+    {
+#pragma unroll
+        for (int n = 0; n < NL; ++n) {
+            const int d0 = min(64 * n + 16 * kq, HD - 16);
+            w[n] = *reinterpret_cast<const v4i *>(k + (BITS == 8 ? d0 : d0 & (HD / 2 - 1)));
+        }
+        step = st;
+    }
+    __device__ __forceinline__ v4i operand(int ks, int kq) const
+    {
+        if constexpr (BITS == 8) {
+            return w[ks];
+        } else {
+            const int sh = min(64 * ks + 16 * kq, HD - 16) < HD / 2 ? 0 : 4;
+            v4i o;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                // a nibble n as a signed byte: (n ^ 8) - 8 without borrows
+                const uint32_t n = ((uint32_t)w[0][i] >> sh) & 0x0F0F0F0Fu;
+                o[i] = (int)(((n ^ 0x08080808u) + 0x78787878u) ^ 0x80808080u);
+            }
+            return o;
+        }
+    }
+};
 
 // bits 48 .. 111 of step * sum_d q_d c_d from the digit sums: with q = sum_a s_a
-// 256^a + C (q48_digits.hpp), sum_d q_d c_d = sum_a 256^a acc[a] + C cs, below 2^80
-__device__ __forceinline__ int64_t code_dot(const v4i (&acc)[8], int i, int cs, uint64_t step)
+// 256^a + C (q48_digits.hpp), sum_d q_d c_d = sum_a 256^a acc[a] + C cs, below
+// 2^80 (|acc| <= 128 127 128 < 2^21, so two digits join in 32 bits); c0 and c1 are
+// the low and high word of C times cs = sum_d c_d.
+__device__ __forceinline__ int64_t code_dot(const v4i (&acc)[8], int i, int64_t c0, int64_t c1,
+                                            uint64_t step)
 {
-    int64_t lo = (int64_t)(uint32_t)kDig * cs, hi = (int64_t)(kDig >> 32) * cs;
-    lo = mad_shl<0>(acc[0][i], lo);
-    lo = mad_shl<8>(acc[1][i], lo);
-    lo = mad_shl<16>(acc[2][i], lo);
-    lo = mad_shl<24>(acc[3][i], lo);
-    hi = mad_shl<0>(acc[4][i], hi);
-    hi = mad_shl<8>(acc[5][i], hi);
-    hi = mad_shl<16>(acc[6][i], hi);
-    hi = mad_shl<24>(acc[7][i], hi);
+    int64_t lo = c0 + (acc[0][i] + (acc[1][i] << 8));
+    int64_t hi = c1 + (acc[4][i] + (acc[5][i] << 8));
+    lo = mad_shl<16>(acc[2][i] + (acc[3][i] << 8), lo);
+    hi = mad_shl<16>(acc[6][i] + (acc[7][i] << 8), hi);
     hi += lo >> 32;
-    const uint64_t nl = ((uint64_t)hi << 32) | (uint32_t)lo;
-    const int64_t nh = hi >> 32;
-    const uint64_t ph = __umul64hi(nl, step) + (uint64_t)nh * step;
-    return (int64_t)((ph << 16) | ((nl * step) >> 48));
+    // words n0, n1 (unsigned) and n2 (signed) of the sum, s0 and s1 of the step
+    const uint32_t n0 = (uint32_t)lo, n1 = (uint32_t)hi, n2 = (uint32_t)(hi >> 32);
+    const uint32_t s0 = (uint32_t)step, s1 = (uint32_t)(step >> 32);
+    const uint64_t t = (uint64_t)n0 * s1 + __umulhi(n0, s0);
+    const uint64_t u = (uint64_t)n1 * s0 + (uint32_t)t;
+    const uint64_t v = (uint64_t)n1 * s1 + (t >> 32) + (u >> 32);   // words 2, 3
+    const uint32_t w3 = (uint32_t)(v >> 32) + n2 * s1 + __umulhi(n2, s0) -
+                        ((int32_t)n2 < 0 ? s0 : 0);
+    uint64_t top = ((uint64_t)w3 << 32) | (uint32_t)v;
+    top += (uint64_t)(n2 * s0);
+    return (int64_t)((top << 16) | ((uint32_t)u >> 16));
 }
 
-// The scores of TB tiles of vectors over one chunk, and each vector's maximum
-// over the rows it sees.  Wave w takes the 16-row tiles w, w + 4, ...: its lane
-// (j = lane % 16) holds row j's 16 dims of MFMA operand once for all TB tiles; a
-// query's digits come from LDS.  DEC: RoPE of the queries and the new key, and
-// the store of the new row (by the blocks that own it).
-template <int BITS, int HD, int TB, bool DEC>
-__global__ __launch_bounds__(256) void k_ra_score(RaArgs a, RaPlan p)
+// Digits of a tile's queries as the A operands of the score products, and C sum_d
+// q_d for int64 keys, by NT threads; qs: rotated queries in LDS, or null.
+template <int BITS, int HD, int NT>
+__device__ __forceinline__ void query_digits(const RaArgs &a, const RaPlan &p,
+                                             v4i (*dig)[8][64], q48_u128 *cq, int v0, int vlast,
+                                             int G, int kh, const int64_t *qs, int tid)
 {
-    q48_round_down();
     constexpr int KS = HD < 64 ? 1 : HD / 64;
-    __shared__ v4i dig[TB][KS][8][64];
-    __shared__ q48_u128 cq[TB * 16];
-    __shared__ int vt[TB * 16];
-    __shared__ int64_t mxs[4][TB * 16];
-    __shared__ int farw[TB];
-    __shared__ __align__(16) uint8_t nk[2][HD];
-    __shared__ int64_t nst[2];
-    __shared__ int64_t qs[DEC ? 16 : 1][DEC ? HD : 1];
-
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int rl = lane & 15, kq = lane >> 4;
-    const int kh = blockIdx.z, G = a.n_heads / a.n_kv, NV = p.Tn * G;
-    const int tile0 = blockIdx.y * TB, ntile = min(TB, p.tiles - tile0);
-    int p0;
-    if (!position<DEC>(a, p0))
-        return;
-    const int begin = (int)blockIdx.x * p.ch;
-    const int end = min(begin + p.ch, tile_span<DEC>(a, p, tile0 + ntile - 1, G, p0));
-    if (begin >= end)
-        return;
-
-    if (tid < TB * 16)
-        vt[tid] = p.t0 + min(16 * tile0 + tid, NV - 1) / G;
-    if (tid < TB)
-        farw[tid] = 0;
-    if constexpr (DEC) {
-        for (int it = tid; it < 16 * (HD / 2); it += 256) {
-            const int v = min(16 * tile0 + it / (HD / 2), NV - 1), i = it % (HD / 2);
-            const int64_t *q = a.q + (size_t)(kh * G + v) * HD;
-            int64_t x0 = q[i], x1 = q[i + HD / 2];
-            if (a.cos_t)
-                q48_rope_pair(x0, x1, a.cos_t[(size_t)p0 * (HD / 2) + i],
-                              a.sin_t[(size_t)p0 * (HD / 2) + i]);
-            qs[it / (HD / 2)][i] = x0;
-            qs[it / (HD / 2)][i + HD / 2] = x1;
-        }
-        if (p0 >= begin && p0 < end && tid < 32)
-            new_row<BITS, HD>(a, p0, kh, tid, nk, nst, blockIdx.y == 0);
-        __syncthreads();
-    }
-    // a.out of this tile's vectors, for the sums that the chunks add
-    if (p.nchunk > 1 && blockIdx.x == 0)
-        for (int i = tid; i < ntile * 16 * HD; i += 256) {
-            const int v = 16 * tile0 + i / HD;
-            if (v < NV)
-                a.out[((size_t)(p.t0 + v / G) * a.n_heads + kh * G + v % G) * HD + i % HD] = 0;
-        }
-    for (int it = tid; it < ntile * KS * 64; it += 256) {
-        const int tb = it / (KS * 64), ks = it / 64 % KS, l = it & 63;
-        const int v = min(16 * (tile0 + tb) + (l & 15), NV - 1), d0 = 64 * ks + 16 * (l >> 4);
+    for (int it = tid; it < KS * 64; it += NT) {
+        const int ks = it >> 6, l = it & 63;
+        const int v = min(v0 + (l & 15), vlast), d0 = 64 * ks + 16 * (l >> 4);
         uint64_t x[16];
-        q48_u128 sum = 0;
         if (d0 < HD) {
-            const int64_t *q;
-            if constexpr (DEC)
-                q = &qs[l & 15][d0];
-            else
-                q = a.q + (size_t)(p.t0 + v / G) * a.ldq + (size_t)(kh * G + v % G) * HD + d0;
+            const int64_t *q =
+                qs ? qs + (v - v0) * HD + d0
+                   : a.q + (size_t)(p.t0 + v / G) * a.ldq + (size_t)(kh * G + v % G) * HD + d0;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
+            for (int e = 0; e < 16; ++e)
                 x[e] = (uint64_t)q[e];
-                if (BITS == 64)
-                    sum += (q48_u128)(q48_i128)q[e];
-            }
         } else {
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 x[e] = kDig;   // digits of zero
+        }
+        if constexpr (BITS == 64) {
+            q48_u128 sum = 0;
+            if (d0 < HD)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    sum += (q48_u128)(q48_i128)(int64_t)x[e];
+            sum += shfl_xor128(sum, 16);   // the four lanes of a row are in one wave
+            sum += shfl_xor128(sum, 32);
+            if (l < 16)
+                cq[16 * ks + l] = sum * kDig;
         }
         v4i o[8];
 #pragma unroll
@@ -271,31 +271,680 @@ __global__ __launch_bounds__(256) void k_ra_score(RaArgs a, RaPlan p)
         }
 #pragma unroll
         for (int d = 0; d < 8; ++d)
-            dig[tb][ks][d][l] = o[d];
-        if constexpr (BITS == 64) {
-            // the four lanes of a row are in one wave; with KS = 2 its halves are
-            // in different waves, so the second adds what it reads back below
-            sum += shfl_xor128(sum, 16);
-            sum += shfl_xor128(sum, 32);
-            if (l < 16 && ks == 0)
-                cq[tb * 16 + l] = sum * kDig;
+            dig[ks][d][l] = o[d];
+    }
+}
+
+// A tile's scores before the scale: s[i] = (sum_d q_d k_d) >> 48 of row j's key and
+// the tile's vector 4 kq + i.
+template <int HD>
+__device__ __forceinline__ void code_scores(int64_t (&s)[4], const v4i (*dig)[8][64],
+                                            const v4i (&B)[HD < 64 ? 1 : HD / 64], int64_t c0,
+                                            int64_t c1, uint64_t step, int lane, int nrow)
+{
+    constexpr int KS = HD < 64 ? 1 : HD / 64;
+    v4i acc[8];
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+        acc[d] = (v4i){0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int d = 0; d < 8; ++d)
+            acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(dig[ks][d][lane], B[ks], acc[d], 0, 0,
+                                                          0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i == 0 || i < nrow)   // a short tile has no vector 4 kq + i
+            s[i] = code_dot(acc, i, c0, c1, step);
+}
+
+// C's low and high word times sum_d c_d of the operand's row, on every lane: a
+// product with a row of ones
+template <int HD>
+__device__ __forceinline__ void code_sum(int64_t &c0, int64_t &c1,
+                                         const v4i (&B)[HD < 64 ? 1 : HD / 64], int kq)
+{
+    v4i sum = {0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < (HD < 64 ? 1 : HD / 64); ++ks) {
+        const int o = 64 * ks + 16 * kq < HD ? 0x01010101 : 0;
+        sum = __builtin_amdgcn_mfma_i32_16x16x64_i8((v4i){o, o, o, o}, B[ks], sum, 0, 0, 0);
+    }
+    c0 = (int64_t)(uint32_t)kDig * sum[0];
+    c1 = (int64_t)(uint32_t)(kDig >> 32) * sum[0];
+    // the product's other three words are not reused while it may still write them
+    asm("" : : "v"(sum), "v"(c0), "v"(c1));
+}
+
+// Operands of 16 int64 key rows (eight digit planes), and C sum_d k_d - HD C^2
+template <int HD>
+__device__ __forceinline__ q48_u128 key_digits(v4i (&B)[HD < 64 ? 1 : HD / 64][8],
+                                               const int64_t *k, int kq)
+{
+    constexpr int KS = HD < 64 ? 1 : HD / 64;
+    q48_u128 ck = 0;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const int d0 = 64 * ks + 16 * kq;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            uint64_t x4[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x4[e] = d0 < HD ? (uint64_t)k[d0 + 4 * g + e] : kDig;
+                if (d0 < HD)
+                    ck += (q48_u128)(q48_i128)(int64_t)x4[e];
+            }
+            uint32_t wd[8];
+            digits4(x4, wd);
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+                B[ks][d][g] = (int)wd[d];
         }
     }
-    __syncthreads();
-    if constexpr (BITS == 64 && KS == 2) {
-        if (tid < ntile * 16) {
-            const int v = min(16 * tile0 + tid, NV - 1);
-            const int64_t *q =
-                a.q + (size_t)(p.t0 + v / G) * a.ldq + (size_t)(kh * G + v % G) * HD + 64;
-            q48_u128 sum = 0;
-            for (int e = 0; e < 64; ++e)
-                sum += (q48_u128)(q48_i128)q[e];
-            cq[tid] += sum * kDig;
+    ck += shfl_xor128(ck, 16);
+    ck += shfl_xor128(ck, 32);
+    return ck * kDig - (q48_u128)kDig * kDig * (q48_u128)HD;
+}
+
+template <int HD>
+__device__ __forceinline__ void word_scores(int64_t (&s)[4], const v4i (*dig)[8][64],
+                                            const v4i (&B)[HD < 64 ? 1 : HD / 64][8],
+                                            const q48_u128 *cq, q48_u128 ck, int lane, int nrow)
+{
+    constexpr int KS = HD < 64 ? 1 : HD / 64;
+    v4i acc[14];
+#pragma unroll
+    for (int d = 0; d < 14; ++d)
+        acc[d] = (v4i){0, 0, 0, 0};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            const v4i A = dig[ks][x][lane];
+#pragma unroll
+            for (int y = 0; y < 8; ++y)
+                if (x + y <= 13)
+                    acc[x + y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A, B[ks][y], acc[x + y], 0,
+                                                                      0, 0);
         }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (i == 0 || i < nrow) {
+            const int m = 4 * (lane >> 4) + i;
+            q48_u128 c = cq[m] + ck;
+            if (KS == 2)
+                c += cq[16 + m];
+            s[i] = digits_shr48(acc, i, c);
+        }
+}
+
+// Scores of TB tiles (vectors v0 .. of 16 each) over rows [begin, end), 16 rows a
+// wave at a time (wave w of NW); put(tb, m, j, s) takes vector m's score, and mx
+// and far gather each tile's maxima over the rows seen and far scores.
+template <int BITS, int HD, int TB, int NW, bool DEC, typename Put>
+__device__ __forceinline__ void score_rows(const RaArgs &a, const v4i (*dig)[HD < 64 ? 1 : HD / 64][8][64],
+                                           const q48_u128 (*cq)[HD < 64 ? 16 : HD / 4],
+                                           const int *vt, int ntile, int nrow, int kh, int p0,
+                                           int begin, int end, const uint8_t *nk, int64_t nst,
+                                           int clear, int w, int lane, int64_t (&mx)[TB][4],
+                                           uint32_t (&far)[TB], KeyRow<BITS == 64 ? 8 : BITS, HD> &next,
+                                           Put put)
+{
+    constexpr int KS = HD < 64 ? 1 : HD / 64;
+    const int rl = lane & 15, kq = lane >> 4;
+    for (int j0 = begin + 16 * w; j0 < end; j0 += 16 * NW) {
+        const int j = j0 + rl, jc = min(j, end - 1);
+        const bool all = j0 + 16 <= clear;   // (clear <= end)
+        const size_t row = (size_t)jc * a.n_kv + kh;
+        v4i B[KS][BITS == 64 ? 8 : 1];
+        q48_u128 ck = 0;
+        int64_t c0 = 0, c1 = 0;
+        uint64_t step = 0;
+        v4i C[KS];
+        if constexpr (BITS == 64) {
+            ck = key_digits<HD>(B, reinterpret_cast<const int64_t *>(a.k) + row * HD, kq);
+        } else {
+            KeyRow<BITS, HD> now = next;
+            if (j0 + 16 * NW < end)
+                next.load(a, (size_t)min(j + 16 * NW, end - 1) * a.n_kv + kh, kq);
+            if (DEC && jc == p0)
+                now.fresh(nk, (uint64_t)nst, kq);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+                C[ks] = now.operand(ks, kq);
+            step = now.step;
+            code_sum<HD>(c0, c1, C, kq);
+        }
+#pragma unroll
+        for (int tb = 0; tb < TB; ++tb) {
+            if (tb >= ntile)
+                break;
+            int64_t s[4];
+            if constexpr (BITS == 64)
+                word_scores<HD>(s, dig[tb], B, cq[tb], ck, lane, nrow);
+            else
+                code_scores<HD>(s, dig[tb], C, c0, c1, step, lane, nrow);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (i > 0 && i >= nrow)
+                    break;
+                const int m = 4 * kq + i;
+                // the scale of 64-wide heads is 2^45: a shift
+                s[i] = HD == 64 ? s[i] >> 3 : q48_mul(s[i], a.scale);
+                if (all || j < end)
+                    put(tb, m, j, s[i]);
+                if (all || (j < end && sees<DEC>(a, p0, vt[tb * 16 + m], j))) {
+                    far[tb] |= (uint32_t)((uint64_t)s[i] >> 32) + 0x40000000u;
+                    mx[tb][i] = s[i] > mx[tb][i] ? s[i] : mx[tb][i];
+                }
+            }
+        }
+    }
+}
+
+// ---- values as doubles ------------------------------------------------------------
+
+// v[n] = c[n] st of lane n of each row of 16 lanes (exact below 2^53), n < 16:
+// row_newbcast hands a row's steps to its lanes.  The four moves cover the wait
+// states between a vector write of st and its DPP read.
+__device__ __forceinline__ void scale16(double (&v)[16], const double (&c)[16], double st)
+{
+#define RA_MUL4(A, B, C, D)                                                                      \
+    asm("v_mov_b64_e32 %0, 0\n\t"                                                                \
+        "v_mov_b64_e32 %1, 0\n\t"                                                                \
+        "v_mov_b64_e32 %2, 0\n\t"                                                                \
+        "v_mov_b64_e32 %3, 0\n\t"                                                                \
+        "v_fmac_f64_dpp %0, %4, %5 row_newbcast:" #A " row_mask:0xf bank_mask:0xf\n\t"          \
+        "v_fmac_f64_dpp %1, %4, %6 row_newbcast:" #B " row_mask:0xf bank_mask:0xf\n\t"          \
+        "v_fmac_f64_dpp %2, %4, %7 row_newbcast:" #C " row_mask:0xf bank_mask:0xf\n\t"          \
+        "v_fmac_f64_dpp %3, %4, %8 row_newbcast:" #D " row_mask:0xf bank_mask:0xf"              \
+        : "=&v"(v[A]), "=&v"(v[B]), "=&v"(v[C]), "=&v"(v[D])                                     \
+        : "v"(st), "v"(c[A]), "v"(c[B]), "v"(c[C]), "v"(c[D]))
+    RA_MUL4(0, 1, 2, 3);
+    RA_MUL4(4, 5, 6, 7);
+    RA_MUL4(8, 9, 10, 11);
+    RA_MUL4(12, 13, 14, 15);
+#undef RA_MUL4
+}
+
+// Where a lane's values are: byte offsets from the first row of a group of CP rows,
+// for its 16 rows vp + n at dim vd (a byte of 4-bit codes holds dims b and b + HD /
+// 2), made once: the loads then take a scalar base and these.
+template <int BITS, int HD>
+struct ValueRows {
+    static constexpr int DL = HD == 128 ? 2 : 1, CP = HD == 32 ? 32 : 16, RB = HD * BITS / 8;
+    uint32_t off[16];
+    uint32_t at;
+    int vp, sh;
+    const uint8_t *base;
+    __device__ __forceinline__ ValueRows(const RaArgs &a, int kh, int lane)
+    {
+        const int vd = HD == 32 ? lane & 31 : lane;
+        vp = HD == 32 ? 16 * (lane >> 5) : 0;
+        sh = vd < HD / 2 ? 0 : 4;
+        at = BITS == 64 ? 8 * vd : BITS == 8 ? vd : vd & (HD / 2 - 1);
+        base = a.v + (size_t)kh * RB;
+#pragma unroll
+        for (int n = 0; n < 16; ++n)
+            off[n] = (uint32_t)(vp + n) * (uint32_t)(a.n_kv * RB) + at;
+    }
+    // The values of rows j + vp + n (past last: that row's); j is the wave's.  int64
+    // words gather their range in big.  rl: the lane's place in its row of 16.  fresh
+    // (or null): the codes and the step of row last, which the cache may not hold yet.
+    __device__ __forceinline__ void load(double (&v)[DL][16], const RaArgs &a, int kh, int j,
+                                         int last, int rl, uint32_t &big,
+                                         const uint8_t *fresh = nullptr, int64_t fresh_step = 0)
+    {
+        const uint8_t *g = base + (size_t)j * (size_t)(a.n_kv * RB);
+        const bool tail = j + CP - 1 > last;
+        if (tail)   // the wave's last group: the offsets are not used again
+#pragma unroll
+            for (int n = 0; n < 16; ++n)
+                off[n] = (uint32_t)min(vp + n, last - j) * (uint32_t)(a.n_kv * RB) + at;
+        if constexpr (BITS == 64) {
+            int64_t x[DL][16];
+#pragma unroll
+            for (int n = 0; n < 16; ++n)
+#pragma unroll
+                for (int l = 0; l < DL; ++l)
+                    x[l][n] = *reinterpret_cast<const int64_t *>(g + off[n] + 512 * l);
+#pragma unroll
+            for (int n = 0; n < 16; ++n)
+#pragma unroll
+                for (int l = 0; l < DL; ++l)
+                    v[l][n] = q48_f51(x[l][n], big);
+        } else {
+            int b[16], b2[16];
+#pragma unroll
+            for (int n = 0; n < 16; ++n) {
+                b[n] = (int8_t)g[off[n]];
+                if (BITS == 8 && HD == 128)
+                    b2[n] = (int8_t)g[off[n] + 64];
+            }
+            int64_t step = a.vs[(size_t)min(j + vp + rl, last) * a.n_kv + kh];
+            if (fresh && j + CP - 1 >= last) {
+                if (j + vp + rl >= last)
+                    step = fresh_step;
+#pragma unroll
+                for (int n = 0; n < 16; ++n)
+                    if (j + vp + n == last) {
+                        b[n] = (int8_t)fresh[at];
+                        if (BITS == 8 && HD == 128)
+                            b2[n] = (int8_t)fresh[at + 64];
+                    }
+            }
+            const double st = (double)step;
+            double c[16];
+#pragma unroll
+            for (int n = 0; n < 16; ++n)
+                c[n] = (double)(BITS == 8
+                                    ? b[n]
+                                    : (int)__builtin_amdgcn_sbfe(b[n], HD == 128 ? 0 : sh, 4));
+            scale16(v[0], c, st);
+            if constexpr (DL == 2) {
+#pragma unroll
+                for (int n = 0; n < 16; ++n)
+                    c[n] = (double)(BITS == 8 ? b2[n] : b[n] >> 4);
+                scale16(v[1], c, st);
+            }
+        }
+    }
+};
+
+// acc[l][r] += the 16 rows' values under vector r's weights (q(r): this lane's, row
+// rl's weight), four vectors at a time, rounding down (q48_fsum4x4): one FP64
+// operation a (vector, row, dim); absent vectors are skipped by fours.
+template <int HD, typename Weight>
+__device__ __forceinline__ void add_values(double (&acc)[HD == 128 ? 2 : 1][16],
+                                           const double (&v)[HD == 128 ? 2 : 1][16], int nrow,
+                                           Weight weight)
+{
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+        if (r >= nrow)
+            break;
+        double q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            q[i] = weight(r + i);
+#pragma unroll
+        for (int l = 0; l < (HD == 128 ? 2 : 1); ++l) {
+            auto f4 = [&](auto base) {
+                constexpr int B = decltype(base)::value;
+                const double x[4] = {v[l][B], v[l][B + 1], v[l][B + 2], v[l][B + 3]};
+                q48_fsum4x4<B>(acc[l][r], acc[l][r + 1], acc[l][r + 2], acc[l][r + 3], q, x);
+            };
+            f4(std::integral_constant<int, 0>{});
+            f4(std::integral_constant<int, 4>{});
+            f4(std::integral_constant<int, 8>{});
+            f4(std::integral_constant<int, 12>{});
+        }
+    }
+}
+
+// a step whose values all stay within [-2^51, 2^51)
+template <int BITS>
+__device__ __forceinline__ bool step_fits(int64_t step)
+{
+    return (uint64_t)step < ((uint64_t)1 << 51) / (BITS == 8 ? 127 : 7);
+}
+
+// q48_exp_neg with its constants where v_fma_f64 takes them (a multiply-add whose
+// addend is a constant otherwise copies it first: 24 moves in 95 instructions).
+__device__ __forceinline__ uint64_t exp_neg(uint64_t u)
+{
+    const uint64_t lim = (uint64_t)10 << 48;
+    const bool in = u <= lim;
+    double h = __builtin_bit_cast(double, 0x4330000000000000ull + (uint64_t)Q48_ONE +
+                                              ((in ? u : lim) >> 14));
+    const double k24 = 0x1p-24, k28 = -0x1p28, k52 = 0x1p52;
+#pragma unroll
+    for (int k = 0; k < 12; ++k) {
+        double y;
+        asm("v_fma_f64 %0, %1, %2, %3" : "=v"(y) : "v"(h), "s"(k24), "v"(k28));
+        asm("v_fma_f64 %0, %1, %1, %2" : "=v"(h) : "v"(y), "s"(k52));
+    }
+    const uint64_t r = (uint64_t)q48_usqr((uint64_t)q48_usqr(q48_word_m52(h)));
+    const double rd = (double)r;
+    double y = __builtin_amdgcn_rcp(rd);
+    y = __builtin_fma(y, __builtin_fma(-rd, y, 1.0), y);
+    y = __builtin_fma(y, __builtin_fma(-rd, y, 1.0), y);
+    const uint64_t q0 = q48_word_m52(__builtin_fma(y, 0x1p96, 0x1p52 - 0.5));
+    const uint64_t rem = (uint64_t)0 - q0 * r;
+    return in ? q0 + (rem >= r ? 1 : 0) : 0;
+}
+
+// The exponentials of vector t's scores row[j], j = begin + l, + L, ..., in place: 0
+// where it does not see j, up to `fill` >= end.  Two at a time where every row is
+// seen: a chain of 24 dependent operations each.  Returns their sum; odd: one is
+// outside [0, ONE] (far: scores whose differences may wrap).
+template <bool DEC>
+__device__ __forceinline__ uint64_t exp_rows(const RaArgs &a, int p0, int t, int64_t *row,
+                                             int64_t m, bool far, int begin, int end, int fill,
+                                             int l, int L, int &odd)
+{
+    uint64_t sum = 0;
+    int j = begin + l;
+    if (!far) {
+        const int clear = min(end, rows_clear<DEC>(a, p0, t));
+        for (; j + L < clear; j += 2 * L) {
+            const uint64_t e0 = exp_neg((uint64_t)m - (uint64_t)row[j]);
+            const uint64_t e1 = exp_neg((uint64_t)m - (uint64_t)row[j + L]);
+            row[j] = (int64_t)e0;
+            row[j + L] = (int64_t)e1;
+            sum += e0 + e1;
+        }
+    }
+    for (; j < fill; j += L) {
+        int64_t e = 0;
+        if (j < end && sees<DEC>(a, p0, t, j)) {
+            if (!far) {
+                e = (int64_t)exp_neg((uint64_t)m - (uint64_t)row[j]);
+            } else {
+                e = q48_safe_exp((int64_t)((uint64_t)row[j] - (uint64_t)m));
+                odd |= (uint64_t)e > (uint64_t)Q48_ONE;
+            }
+        }
+        row[j] = e;
+        sum += (uint64_t)e;
+    }
+    return sum;
+}
+
+// 2^48 / d for the quotients of a softmax row (1 <= d < 2^63; 0 for d = 0): as
+// q48_divisor_of, whose bound of 2^62 a row past 16384 positions may pass.  The
+// quotient's bound is the same there: e / d shrinks as d grows.
+__device__ __forceinline__ double quotient_factor(uint64_t d)
+{
+    const double dd = (double)d;
+    double y = __builtin_amdgcn_rcp(dd);
+    y = __builtin_fma(y, __builtin_fma(-dd, y, 1.0), y);
+    y = __builtin_fma(y, __builtin_fma(-dd, y, 1.0), y);
+    return d ? y * 0x1p48 : 0.0;
+}
+
+// fp_div(e, den) 2^-48 for 0 <= e <= ONE <= den, or 0 for e = den = 0
+__device__ __forceinline__ double quotient_scaled(uint64_t e, uint64_t den, double y48)
+{
+    const double ed = __builtin_bit_cast(double, e | 0x4330000000000000ull) - 0x1p52;
+    const uint64_t q0 = q48_word_m52(__builtin_fma(ed, y48, 0x1p52 - 0.5));
+    const uint64_t rem = (e << 48) - q0 * den;
+    return q48_pscaled((int64_t)(q0 + (rem >= den ? 1 : 0)));
+}
+
+// dim d of a vector's sum over rows [begin, end) in integers.  e: exponentials of
+// any kind, the weights fp_div(e, sum) where the sum is positive, else e; or
+// (scaled) the weights 2^-48 as doubles.
+template <int BITS, int HD>
+__device__ int64_t plain_sum(const RaArgs &a, const int64_t *e, int64_t sum, bool scaled, int kh,
+                             int d, int begin, int end, const uint8_t *fresh = nullptr,
+                             const int64_t *fresh_step = nullptr)
+{
+    const q48_divisor dv = q48_divisor_of(sum);
+    uint64_t o = 0;
+    for (int j = begin; j < end; ++j) {
+        int64_t x = e[j];
+        if (scaled)
+            x = (int64_t)(__builtin_bit_cast(double, x) * 0x1p48);
+        else if (sum > 0)
+            x = q48_div_by(x, dv);
+        o += (uint64_t)q48_mul(x, fresh && j == end - 1
+                                      ? value_at<BITS, HD>(fresh, fresh_step, 0, d)
+                                      : value_at<BITS, HD>(a.v, a.vs, (size_t)j * a.n_kv + kh, d));
+    }
+    return (int64_t)o;
+}
+
+template <int HD>
+__device__ __forceinline__ int64_t *out_at(const RaArgs &a, const RaPlan &p, int v, int G, int kh)
+{
+    return a.out + ((size_t)(p.t0 + v / G) * a.n_heads + kh * G + v % G) * HD;
+}
+
+// The tile's queries of a decoded token into LDS (vectors v0 .. v0 + n - 1), rotated
+// where the tables are given.
+template <int HD, int NT>
+__device__ __forceinline__ void decode_queries(const RaArgs &a, int64_t *qs, int v0, int n, int G,
+                                               int kh, int p0, int tid)
+{
+    for (int it = tid; it < n * (HD / 2); it += NT) {
+        const int m = it / (HD / 2), i = it % (HD / 2);
+        const int64_t *q = a.q + (size_t)(kh * G + v0 + m) * HD;
+        int64_t x0 = q[i], x1 = q[i + HD / 2];
+        if (a.cos_t)
+            q48_rope_pair(x0, x1, a.cos_t[(size_t)p0 * (HD / 2) + i],
+                          a.sin_t[(size_t)p0 * (HD / 2) + i]);
+        qs[m * HD + i] = x0;
+        qs[m * HD + i + HD / 2] = x1;
+    }
+}
+
+// ---- one launch ----------------------------------------------------------------------
+
+// k_ra_tile's arrays beside the scores (digits, sums, queries, maxima, row sums, the
+// rest rounded up), and what a compute unit's 160 KB of LDS leaves for the scores
+constexpr size_t rt_static(int hd, int nw)
+{
+    return (size_t)(hd < 64 ? 1 : hd / 64) * (8 * 1024 + 256) + 16 * hd * 8 + 2 * 16 * nw * 8 +
+           2 * hd + 512;
+}
+constexpr size_t rt_lds(int hd, int nw) { return 160 * 1024 - rt_static(hd, nw); }
+
+// A tile of up to vb vectors over all its rows, the scores in LDS: they become
+// exponentials, then weights in place.  8 waves; a wave takes 16 rows at a time for
+// the scores and the values.
+template <int BITS, int HD, bool DEC, int RT_NT>
+__global__ __launch_bounds__(RT_NT) void k_ra_tile(RaArgs a, RaPlan p)
+{
+    constexpr int RT_NW = RT_NT / 64;
+    q48_round_down();
+    constexpr int KS = HD < 64 ? 1 : HD / 64;
+    constexpr int PG = HD == 32 ? 2 : 1, CP = 16 * PG;
+    extern __shared__ __align__(16) int64_t sc[];   // [vb][stride]
+    __shared__ v4i dig[1][KS][8][64];
+    __shared__ q48_u128 cq[1][16 * KS];
+    __shared__ int vt[16];
+    __shared__ int64_t mxs[RT_NW][16];
+    __shared__ uint64_t psum[16][RT_NW];
+    __shared__ int flags;                           // 1: a far score, 2: no plain softmax
+    __shared__ __align__(16) uint8_t nk[2][HD];
+    __shared__ int64_t nst[2];
+    __shared__ uint64_t lam[16][HD];                // a decoded token's queries, then the sums
+
+    static_assert(sizeof(dig) + sizeof(cq) + sizeof(vt) + sizeof(mxs) + sizeof(psum) +
+                          sizeof(flags) + sizeof(nk) + sizeof(nst) + sizeof(lam) + 64 <=
+                      rt_static(HD, RT_NW),
+                  "k_ra_tile's LDS");
+
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rl = lane & 15, kq = lane >> 4;
+    const int kh = blockIdx.y, G = a.n_heads / a.n_kv, NV = p.Tn * G;
+    const int v0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * p.vb;   // the longest spans first
+    const int nrow = min(p.vb, NV - v0), stride = p.spad + 4;   // 4 rows on: the other half of the banks
+    int p0;
+    if (!position<DEC>(a, p0))
+        return;
+    const int S = tile_span<DEC>(a, p, v0 + nrow - 1, G, p0);
+
+    KeyRow<BITS == 64 ? 8 : BITS, HD> next;
+    if constexpr (BITS != 64)   // on its way while the queries are split
+        if (16 * w < S)
+            next.load(a, (size_t)min(16 * w + rl, S - 1) * a.n_kv + kh, kq);
+    if (tid < 16)
+        vt[tid] = p.t0 + min(v0 + tid, NV - 1) / G;
+    if (tid == 0)
+        flags = 0;
+    int64_t *qs = reinterpret_cast<int64_t *>(&lam[0][0]);
+    if constexpr (DEC) {
+        decode_queries<HD, RT_NT>(a, qs, v0, nrow, G, kh, p0, tid);
+        if (tid >= RT_NT - 64 && tid < RT_NT - 32)
+            new_row<BITS, HD>(a, p0, kh, tid - (RT_NT - 64), nk, nst, v0 == 0);
         __syncthreads();
     }
+    query_digits<BITS, HD, RT_NT>(a, p, dig[0], cq[0], v0, v0 + nrow - 1, G, kh,
+                                  DEC ? qs : nullptr, tid);
+    __syncthreads();
+    for (int i = tid; i < 16 * HD; i += RT_NT)
+        (&lam[0][0])[i] = 0;
 
-    const bool pow2 = HD == 64;   // the scale is 2^45: a shift
+    {
+        int64_t mx[1][4] = {{INT64_MIN, INT64_MIN, INT64_MIN, INT64_MIN}};
+        uint32_t far[1] = {0};
+        score_rows<BITS, HD, 1, RT_NW, DEC>(a, dig, cq, vt, 1, nrow, kh, p0, 0, S, nk[0],
+                                            DEC && BITS != 64 ? nst[0] : 0,
+                                            rows_clear<DEC>(a, p0, p.t0 + v0 / G), w, lane, mx,
+                                            far, next, [&](int, int m, int j, int64_t s) {
+                                                if (m < nrow)
+                                                    sc[m * stride + j] = s;
+                                            });
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t m = row16_max64(mx[0][i]);
+            if (rl == 0)
+                mxs[w][4 * kq + i] = m;
+        }
+        if (far[0] & 0x80000000u)
+            atomicOr(&flags, 1);
+    }
+    __syncthreads();
+
+    // exponentials: a wave takes whole vectors, or 8 / vb waves share one
+    const int wr = p.vb >= RT_NW ? 1 : RT_NW / p.vb;   // waves a vector (vb a power of two)
+    const int sub = w % wr;
+    const int fill = (S + 31) & ~31;
+    const bool far = flags & 1;
+    int odd = 0;
+    for (int r = w / wr; r < nrow; r += RT_NW / wr) {
+        int64_t m = mxs[0][r];
+#pragma unroll
+        for (int u = 1; u < RT_NW; ++u)
+            m = mxs[u][r] > m ? mxs[u][r] : m;
+        uint64_t sum = exp_rows<DEC>(a, p0, vt[r], sc + r * stride, m, far, 0, S, fill,
+                                     lane + 64 * sub, 64 * wr, odd);
+        sum = (uint64_t)q48_wave_sum64((int64_t)sum);
+        if (lane == 0)
+            psum[r][sub] = sum;
+    }
+    if constexpr (BITS != 64)
+        for (int j = tid; j < S; j += RT_NT) {
+            const int64_t st = DEC && j == p0 ? nst[1] : a.vs[(size_t)j * a.n_kv + kh];
+            odd |= !step_fits<BITS>(st);
+        }
+    const bool slow = __syncthreads_or(odd);
+    auto total = [&](int r) {
+        uint64_t s = 0;
+        for (int u = 0; u < wr; ++u)
+            s += psum[r][u];
+        return s;
+    };
+    uint32_t big = 0;
+    if (!slow) {
+        ValueRows<BITS, HD> rows(a, kh, lane);
+        const int vd = HD == 32 ? lane & 31 : lane, vp = rows.vp;
+        for (int r = w / wr; r < nrow; r += RT_NW / wr) {
+            const uint64_t den = total(r);
+            const double y48 = quotient_factor(den);
+            int64_t *row = sc + r * stride;
+#pragma unroll 2
+            for (int j = lane + 64 * sub; j < fill; j += 64 * wr)
+                row[j] = __builtin_bit_cast(int64_t,
+                                            quotient_scaled((uint64_t)row[j], den, y48));
+        }
+        __syncthreads();
+        double acc[HD == 128 ? 2 : 1][16];
+#pragma unroll
+        for (int l = 0; l < (HD == 128 ? 2 : 1); ++l)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                acc[l][r] = Q48_FSUM0;
+        for (int j0 = CP * w; j0 < S; j0 += RT_NW * CP) {
+            double v[HD == 128 ? 2 : 1][16];
+            rows.load(v, a, kh, j0, S - 1, rl, big, DEC && BITS != 64 ? nk[1] : nullptr,
+                      DEC && BITS != 64 ? nst[1] : 0);
+            add_values<HD>(acc, v, nrow, [&](int r) {
+                if (r >= nrow)
+                    return 0.0;
+                return __builtin_bit_cast(double, sc[r * stride + j0 + vp + rl]);
+            });
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            if (r < nrow)
+#pragma unroll
+                for (int l = 0; l < (HD == 128 ? 2 : 1); ++l)
+                    atomicAdd(reinterpret_cast<unsigned long long *>(&lam[r][vd + 64 * l]),
+                              (unsigned long long)q48_fsum_total(acc[l][r]));
+    }
+    const bool redo = __syncthreads_or(q48_f51_big(big)) || slow;
+    for (int i = tid; i < nrow * HD; i += RT_NT) {
+        const int r = i / HD, d = i % HD;
+        out_at<HD>(a, p, v0 + r, G, kh)[d] =
+            redo ? plain_sum<BITS, HD>(a, sc + r * stride, (int64_t)total(r), !slow, kh, d, 0, S,
+                                        DEC ? nk[1] : nullptr, nst + 1)
+                 : (int64_t)lam[r][d];
+    }
+}
+
+// ---- three launches ---------------------------------------------------------------------
+
+// The scores of TB tiles of 16 vectors over one chunk, and each vector's maximum
+// over the rows it sees: a row's operand is made once for all TB tiles.  DEC: the
+// store of the new row too (by the blocks that own it).
+template <int BITS, int HD, int TB, bool DEC>
+__global__ __launch_bounds__(256) void k_ra_score(RaArgs a, RaPlan p)
+{
+    q48_round_down();
+    constexpr int KS = HD < 64 ? 1 : HD / 64;
+    __shared__ v4i dig[TB][KS][8][64];
+    __shared__ q48_u128 cq[TB][16 * KS];
+    __shared__ int vt[TB * 16];
+    __shared__ int64_t mxs[4][TB * 16];
+    __shared__ int farw[TB];
+    __shared__ __align__(16) uint8_t nk[2][HD];
+    __shared__ int64_t nst[2];
+    __shared__ int64_t qs[DEC ? 16 * HD : 1];
+
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rl = lane & 15, kq = lane >> 4;
+    const int kh = blockIdx.z, G = a.n_heads / a.n_kv, NV = p.Tn * G;
+    const int tile0 = blockIdx.y * TB, ntile = min(TB, p.tiles - tile0);
+    int p0;
+    if (!position<DEC>(a, p0))
+        return;
+    const int begin = (int)blockIdx.x * p.ch;
+    const int end =
+        min(begin + p.ch, tile_span<DEC>(a, p, 16 * (tile0 + ntile) - 1, G, p0));
+    if (begin >= end)
+        return;
+
+    KeyRow<BITS == 64 ? 8 : BITS, HD> next;
+    if constexpr (BITS != 64)
+        if (begin + 16 * w < end)
+            next.load(a, (size_t)min(begin + 16 * w + rl, end - 1) * a.n_kv + kh, kq);
+    if (tid < TB * 16)
+        vt[tid] = p.t0 + min(16 * tile0 + tid, NV - 1) / G;
+    if (tid < TB)
+        farw[tid] = 0;
+    if constexpr (DEC) {
+        decode_queries<HD, 256>(a, qs, 16 * tile0, min(16, NV - 16 * tile0), G, kh, p0, tid);
+        if (p0 >= begin && p0 < end && tid >= 192 && tid < 224)
+            new_row<BITS, HD>(a, p0, kh, tid - 192, nk, nst, blockIdx.y == 0);
+        __syncthreads();
+    }
+    // a.out of these tiles' vectors, for the sums that the chunks add
+    if (p.nchunk > 1 && blockIdx.x == 0)
+        for (int i = tid; i < ntile * 16 * HD; i += 256) {
+            const int v = 16 * tile0 + i / HD;
+            if (v < NV)
+                out_at<HD>(a, p, v, G, kh)[i % HD] = 0;
+        }
+    for (int tb = 0; tb < ntile; ++tb)
+        query_digits<BITS, HD, 256>(a, p, dig[tb], cq[tb], 16 * (tile0 + tb), NV - 1, G, kh,
+                                    DEC ? qs : nullptr, (tid + 256 - 64 * (tb & 3)) & 255);
+    __syncthreads();
+
     int64_t mx[TB][4];
     uint32_t far[TB];
 #pragma unroll
@@ -305,107 +954,13 @@ __global__ __launch_bounds__(256) void k_ra_score(RaArgs a, RaPlan p)
         for (int i = 0; i < 4; ++i)
             mx[tb][i] = INT64_MIN;
     }
-    const v4i ones = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
-    for (int j0 = begin + 16 * w; j0 < end; j0 += 64) {
-        const int j = j0 + rl, jc = min(j, end - 1);
-        const size_t row = (size_t)jc * a.n_kv + kh;
-        v4i B[KS][BITS == 64 ? 8 : 1];
-        q48_u128 ck = 0;
-        int cs = 0;
-        uint64_t step = 0;
-        if constexpr (BITS == 64) {
-            const int64_t *k = reinterpret_cast<const int64_t *>(a.k) + row * HD;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const int d0 = 64 * ks + 16 * kq;
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    uint64_t x4[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x4[e] = d0 < HD ? (uint64_t)k[d0 + 4 * g + e] : kDig;
-                        if (d0 < HD)
-                            ck += (q48_u128)(q48_i128)(int64_t)x4[e];
-                    }
-                    uint32_t wd[8];
-                    digits4(x4, wd);
-#pragma unroll
-                    for (int d = 0; d < 8; ++d)
-                        B[ks][d][g] = (int)wd[d];
-                }
-            }
-            ck += shfl_xor128(ck, 16);
-            ck += shfl_xor128(ck, 32);
-            ck = ck * kDig - (q48_u128)kDig * kDig * (q48_u128)HD;
-        } else {
-            const bool fresh = DEC && jc == p0;
-            const uint8_t *k = a.k + row * (HD * BITS / 8);
-            v4i sum = {0, 0, 0, 0};
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const int d0 = min(64 * ks + 16 * kq, HD - 16);   // zero digits past HD
-                B[ks][0] = fresh ? codes16<BITS, HD>(nk[0], d0) : codes16<BITS, HD>(k, d0);
-                v4i one = ones;
-                if (64 * ks + 16 * kq >= HD)
-                    one = (v4i){0, 0, 0, 0};
-                sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(one, B[ks][0], sum, 0, 0, 0);
-            }
-            cs = sum[0];
-            step = (uint64_t)(fresh ? nst[0] : a.ks[row]);
-        }
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb) {
-            if (tb >= ntile)
-                break;
-            int64_t *sc = p.sc + (((size_t)kh * p.tiles + tile0 + tb) * 16) * p.spad;
-            int64_t s[4];
-            if constexpr (BITS == 64) {
-                v4i acc[14];
-#pragma unroll
-                for (int d = 0; d < 14; ++d)
-                    acc[d] = (v4i){0, 0, 0, 0};
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        const v4i A = dig[tb][ks][x][lane];
-#pragma unroll
-                        for (int y = 0; y < 8; ++y)
-                            if (x + y <= 13)
-                                acc[x + y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                                    A, B[ks][y], acc[x + y], 0, 0, 0);
-                    }
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    s[i] = digits_shr48(acc, i, cq[tb * 16 + 4 * kq + i] + ck);
-            } else {
-                v4i acc[8];
-#pragma unroll
-                for (int d = 0; d < 8; ++d)
-                    acc[d] = (v4i){0, 0, 0, 0};
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                    for (int d = 0; d < 8; ++d)
-                        acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
-                            dig[tb][ks][d][lane], B[ks][0], acc[d], 0, 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    s[i] = code_dot(acc, i, cs, step);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int m = 4 * kq + i;
-                s[i] = pow2 ? s[i] >> 3 : q48_mul(s[i], a.scale);
-                if (j < end)
-                    sc[(size_t)m * p.spad + j] = s[i];
-                if (j < end && sees<DEC>(a, p0, vt[tb * 16 + m], j)) {
-                    far[tb] |= (uint32_t)((uint64_t)s[i] >> 32) + 0x40000000u;
-                    mx[tb][i] = s[i] > mx[tb][i] ? s[i] : mx[tb][i];
-                }
-            }
-        }
-    }
+    int64_t *sc = p.sc + ((size_t)kh * p.tiles + tile0) * 16 * p.spad;
+    score_rows<BITS, HD, TB, 4, DEC>(a, dig, cq, vt, ntile, min(16, NV - 16 * tile0), kh, p0,
+                                     begin, end, nk[0], DEC && BITS != 64 ? nst[0] : 0,
+                                     rows_clear<DEC>(a, p0, p.t0 + 16 * tile0 / G), w, lane, mx,
+                                     far, next, [&](int tb, int m, int j, int64_t s) {
+                                         sc[(size_t)(16 * tb + m) * p.spad + j] = s;
+                                     });
 #pragma unroll
     for (int tb = 0; tb < TB; ++tb) {
 #pragma unroll
@@ -441,7 +996,7 @@ __global__ __launch_bounds__(256) void k_ra_exp(RaArgs a, RaPlan p)
     int p0;
     if (!position<DEC>(a, p0))
         return;
-    const int span = tile_span<DEC>(a, p, tile, G, p0);
+    const int span = tile_span<DEC>(a, p, 16 * tile + 15, G, p0);
     const int begin = (int)blockIdx.x * p.ch, end = min(begin + p.ch, span);
     if (begin >= end)
         return;
@@ -469,24 +1024,9 @@ __global__ __launch_bounds__(256) void k_ra_exp(RaArgs a, RaPlan p)
             m = x > m ? x : m;
         }
         const int t = p.t0 + (16 * tile + r) / G;
-        int64_t *sc = p.sc + vec * p.spad;
-        uint64_t sum = 0;
         int odd = 0;
-        const int fill = min(begin + p.ch, (end + 31) & ~31);
-        for (int j = begin + l; j < fill; j += L) {
-            int64_t e = 0;
-            if (j < end && sees<DEC>(a, p0, t, j)) {
-                const int64_t s = sc[j];
-                if (!far) {
-                    e = q48_exp_neg((uint64_t)m - (uint64_t)s);
-                } else {
-                    e = q48_safe_exp((int64_t)((uint64_t)s - (uint64_t)m));
-                    odd |= (uint64_t)e > (uint64_t)Q48_ONE;
-                }
-            }
-            sc[j] = e;
-            sum += (uint64_t)e;
-        }
+        uint64_t sum = exp_rows<DEC>(a, p0, t, p.sc + vec * p.spad, m, far, begin, end,
+                                     min(begin + p.ch, (end + 31) & ~31), l, L, odd);
         sum = group_sum64<16>(sum);
         for (int o = 16; o < L; o <<= 1)
             sum += __shfl_xor(sum, o);
@@ -500,35 +1040,12 @@ __global__ __launch_bounds__(256) void k_ra_exp(RaArgs a, RaPlan p)
         p.odd[((size_t)kh * p.tiles + tile) * p.nchunk + blockIdx.x] = odds;
 }
 
-// 2^48 / d for the quotients of a softmax row (1 <= d < 2^63; 0 for d = 0): as
-// q48_divisor_of, whose bound of 2^62 a row past 16384 positions may pass.  The
-// quotient's bound is the same there: e / d shrinks as d grows.
-__device__ __forceinline__ double quotient_factor(uint64_t d)
-{
-    const double dd = (double)d;
-    double y = __builtin_amdgcn_rcp(dd);
-    y = __builtin_fma(y, __builtin_fma(-dd, y, 1.0), y);
-    y = __builtin_fma(y, __builtin_fma(-dd, y, 1.0), y);
-    return d ? y * 0x1p48 : 0.0;
-}
-
-// fp_div(e, den) 2^-48 for 0 <= e <= ONE <= den, or 0 for e = den = 0
-__device__ __forceinline__ double quotient_scaled(uint64_t e, uint64_t den, double y48)
-{
-    const double ed = __builtin_bit_cast(double, e | 0x4330000000000000ull) - 0x1p52;
-    const uint64_t q0 = q48_word_m52(__builtin_fma(ed, y48, 0x1p52 - 0.5));
-    const uint64_t rem = (e << 48) - q0 * den;
-    return q48_pscaled((int64_t)(q0 + (rem >= den ? 1 : 0)));
-}
-
 // The values of a chunk under its weights, added to out.  Wave w takes the
-// 16-row groups w, w + 4, ... by itself: the quotients of 16 vectors (four a lane)
-// go through LDS so that lane l of every row of 16 lanes holds row l % 16's
-// weights, and row_newbcast hands them to the lanes, which hold one dim each
-// (head_dim 128: two; 32: two groups of rows) of the values as doubles: one FP64
-// operation a (vector, row, dim), rounding down (q48_fsum4x4).  Tiles of fewer
-// vectors skip the sums of four absent ones.  A chunk with a value outside
-// [-2^51, 2^51), or weights that are no plain softmax, multiplies in integers.
+// 16-row groups w, w + 4, ... by itself (head_dim 32: 32 rows, 16 for each half of
+// the wave): the quotients of its vectors (four a lane) go through LDS so that
+// lane l of every row of 16 lanes holds row l % 16's weights.  A chunk with a value
+// outside [-2^51, 2^51), or weights that are no plain softmax, multiplies in
+// integers.
 template <int BITS, int HD, bool DEC>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 1 : 2))) void
 k_ra_value(RaArgs a, RaPlan p)
@@ -545,7 +1062,7 @@ k_ra_value(RaArgs a, RaPlan p)
     int p0;
     if (!position<DEC>(a, p0))
         return;
-    const int span = tile_span<DEC>(a, p, tile, G, p0);
+    const int span = tile_span<DEC>(a, p, 16 * tile + 15, G, p0);
     const int begin = (int)blockIdx.x * p.ch, end = min(begin + p.ch, span);
     if (begin >= end)
         return;
@@ -567,11 +1084,9 @@ k_ra_value(RaArgs a, RaPlan p)
     int slow = 0;
     for (int c = tid; c < chunks; c += 256)
         slow |= p.odd[((size_t)kh * p.tiles + tile) * p.nchunk + c];
-    if constexpr (BITS != 64) {
-        constexpr uint64_t top = ((uint64_t)1 << 51) / (BITS == 8 ? 127 : 7);
+    if constexpr (BITS != 64)
         for (int j = begin + tid; j < end; j += 256)
-            slow |= (uint64_t)a.vs[(size_t)j * a.n_kv + kh] >= top;
-    }
+            slow |= !step_fits<BITS>(a.vs[(size_t)j * a.n_kv + kh]);
     slow = __syncthreads_or(slow);   // dens and lam too
     uint32_t big = 0;
     if (!slow) {
@@ -582,8 +1097,8 @@ k_ra_value(RaArgs a, RaPlan p)
             den[i] = dens[4 * i + g];
             y48[i] = quotient_factor(den[i]);
         }
-        const int vd = HD == 32 ? lane & 31 : lane;
-        const int vp = HD == 32 ? 16 * (lane >> 5) : 0;
+        ValueRows<BITS, HD> rows(a, kh, lane);
+        const int vd = HD == 32 ? lane & 31 : lane, vp = rows.vp;
         double acc[DL][16];
 #pragma unroll
         for (int l = 0; l < DL; ++l)
@@ -603,29 +1118,7 @@ k_ra_value(RaArgs a, RaPlan p)
             load_e(begin + CP * w);
         for (int j0 = begin + CP * w; j0 < end; j0 += 4 * CP) {
             double v[DL][16];
-            if constexpr (BITS == 64) {
-                const int64_t *vb = reinterpret_cast<const int64_t *>(a.v) + (size_t)kh * HD + vd;
-#pragma unroll
-                for (int n = 0; n < 16; ++n)
-#pragma unroll
-                    for (int l = 0; l < DL; ++l)
-                        v[l][n] = q48_f51(
-                            vb[(size_t)min(j0 + vp + n, end - 1) * a.n_kv * HD + 64 * l], big);
-            } else {
-                // a lane's own row's step, handed to the lanes of its row group
-                const double st =
-                    (double)a.vs[(size_t)min(j0 + vp + rl, end - 1) * a.n_kv + kh];
-                const uint8_t *vb = a.v + (size_t)kh * (HD * BITS / 8);
-#pragma unroll
-                for (int n = 0; n < 16; ++n) {
-                    const uint8_t *vr =
-                        vb + (size_t)min(j0 + vp + n, end - 1) * a.n_kv * (HD * BITS / 8);
-                    const double sn = __shfl(st, (lane & 48) | n);
-#pragma unroll
-                    for (int l = 0; l < DL; ++l)
-                        v[l][n] = (double)code_at<BITS, HD>(vr, vd + 64 * l) * sn;
-                }
-            }
+            rows.load(v, a, kh, j0, end - 1, rl, big);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (4 * i < nrow)
@@ -641,28 +1134,7 @@ k_ra_value(RaArgs a, RaPlan p)
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                if (r >= nrow)
-                    break;
-                double q[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    q[i] = pw[w][r + i][vp + rl];
-#pragma unroll
-                for (int l = 0; l < DL; ++l) {
-                    auto f4 = [&](auto base) {
-                        constexpr int B = decltype(base)::value;
-                        const double x[4] = {v[l][B], v[l][B + 1], v[l][B + 2], v[l][B + 3]};
-                        q48_fsum4x4<B>(acc[l][r], acc[l][r + 1], acc[l][r + 2], acc[l][r + 3], q,
-                                       x);
-                    };
-                    f4(std::integral_constant<int, 0>{});
-                    f4(std::integral_constant<int, 4>{});
-                    f4(std::integral_constant<int, 8>{});
-                    f4(std::integral_constant<int, 12>{});
-                }
-            }
+            add_values<HD>(acc, v, nrow, [&](int r) { return pw[w][r][vp + rl]; });
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -675,23 +1147,14 @@ k_ra_value(RaArgs a, RaPlan p)
                     atomicAdd(reinterpret_cast<unsigned long long *>(&lam[r][vd + 64 * l]),
                               (unsigned long long)q48_fsum_total(acc[l][r]));
     }
-    const bool redo = __syncthreads_or(q48_f51_big(big));
+    const bool redo = __syncthreads_or(q48_f51_big(big)) || slow;
     for (int i = tid; i < nrow * HD; i += 256) {
-        const int r = i / HD, d = i % HD, v = 16 * tile + r;
-        uint64_t o = lam[r][d];
-        if (slow || redo) {
-            const int64_t sum = (int64_t)dens[r];
-            const q48_divisor dv = q48_divisor_of(sum);
-            o = 0;
-            for (int j = begin; j < end; ++j) {
-                int64_t e = sc[(size_t)r * p.spad + j];
-                if (sum > 0)
-                    e = q48_div_by(e, dv);
-                o += (uint64_t)q48_mul(e, value_at<BITS, HD>(a.v, a.vs, (size_t)j * a.n_kv + kh, d));
-            }
-        }
-        int64_t *out =
-            a.out + ((size_t)(p.t0 + v / G) * a.n_heads + kh * G + v % G) * HD + d;
+        const int r = i / HD, d = i % HD;
+        const uint64_t o = redo ? (uint64_t)plain_sum<BITS, HD>(a, sc + (size_t)r * p.spad,
+                                                               (int64_t)dens[r], false, kh, d,
+                                                               begin, end)
+                                : lam[r][d];
+        int64_t *out = out_at<HD>(a, p, 16 * tile + r, G, kh) + d;
         if (p.nchunk > 1)
             atomicAdd(reinterpret_cast<unsigned long long *>(out), (unsigned long long)o);
         else
@@ -712,6 +1175,28 @@ bool overlap(const int64_t *a, size_t na, const int64_t *b, size_t nb)
     return (uintptr_t)a < (uintptr_t)(b + nb) && (uintptr_t)b < (uintptr_t)(a + na);
 }
 
+// Estimated times of the two forms, in us, for a span of S rows:
+//   one launch     8 + rounds of blocks * S * (c0 + c1 vb), at one block a compute unit
+//   three launches l + pairs of vectors and rows * c3
+// with (c0, c1, l, c3) measured from 250 to 3000 rows and 8 to 8192 vectors.  us, one
+// / three, 32 heads on 4 of 64, 8 bits: one token at 250 rows 10.1 / 16.0, at 1000
+// 18.0 / 15.0; 16 tokens at 1000 20.8 / 22.9; 64 at 900 30.7 / 42.4, at 2000 54.0 /
+// 74.1; 256 at 700 70.1 / 112.3.  int64: 4 tokens at 500 20.0 / 20.7, 16 at 1000 36.0
+// / 29.6, 64 at 900 44.5 / 62.6.  128-wide heads on 8, 8 bits: one token at 500 17.6 /
+// 16.1, 64 at 2000 114.0 / 91.3.
+template <int BITS, int HD>
+bool one_launch(int vb, int S, long vectors, long blocks, int cus)
+{
+    constexpr int h = HD == 32 ? 0 : HD == 64 ? 1 : 2;
+    constexpr double c0[2][3] = {{7.5e-3, 9e-3, 14e-3}, {33e-3, 22e-3, 43e-3}};
+    constexpr double c1[2][3] = {{1.4e-3, 1.3e-3, 2.4e-3}, {1e-3, 1.5e-3, 2e-3}};
+    constexpr double l[2] = {15, 20};
+    constexpr double c3[2][3] = {{19e-6, 13.7e-6, 17.5e-6}, {31e-6, 23e-6, 37e-6}};
+    constexpr int w = BITS == 64;
+    const double one = 8 + (double)((blocks + cus - 1) / cus) * S * (c0[w][h] + c1[w][h] * vb);
+    return one <= l[w] + (double)vectors * S * c3[w][h];
+}
+
 // Rows of one launch: their scores take at most this much workspace.
 constexpr size_t RA_WS_MAX = (size_t)1 << 30;
 
@@ -723,6 +1208,35 @@ int launch_hd(q48_ctx *c, RaArgs &a)
     const int S = DEC ? (a.d_pos ? a.max_seq : a.p0 + 1) : a.p0 + a.T;
     RaPlan p = {};
     p.spad = (S + 63) & ~63;
+    {
+        // Tiles of the fewest vectors (a power of two) that still leave about a block a
+        // compute unit, and whose scores fit LDS.  Full tiles of many rows take 16
+        // waves where those keep their registers (128 each; us, 16 / 8 waves: 384 rows
+        // at 512 94 / 104, 256 rows at 0 30.1 / 27.4).
+        int vb = 16;
+        while (vb > 1 && ((a.T * G + vb - 1) / vb) * a.n_kv < c->cu_count)
+            vb >>= 1;
+        while (vb > 1 && (size_t)vb * (p.spad + 4) * 8 > rt_lds(HD, 16))
+            vb >>= 1;
+        const long tiles = (a.T * G + vb - 1) / vb;
+        const size_t lds = (size_t)vb * (p.spad + 4) * 8;
+        // (in step mode the position given says what to expect)
+        if (lds <= rt_lds(HD, 16) &&
+            one_launch<BITS, HD>(vb, a.p0 + a.T, (long)a.T * a.n_heads, tiles * a.n_kv,
+                                 c->cu_count)) {
+            constexpr bool WIDE = HD == 64 && BITS != 64;
+            p.Tn = a.T;
+            p.vb = vb;
+            const dim3 grid(tiles, a.n_kv);
+            if (WIDE && vb == 16 && S >= 512)
+                hipLaunchKernelGGL((k_ra_tile<BITS, HD, DEC, WIDE ? 1024 : 512>), grid, dim3(1024),
+                                   lds, c->stream, a, p);
+            else
+                hipLaunchKernelGGL((k_ra_tile<BITS, HD, DEC, 512>), grid, dim3(512), lds,
+                                   c->stream, a, p);
+            return hipGetLastError() == hipSuccess ? Q48_OK : Q48_EHIP;
+        }
+    }
     const size_t row_bytes = (size_t)a.n_heads * p.spad * 8;
     int Tn = (int)(RA_WS_MAX / row_bytes);
     Tn = Tn < 1 ? 1 : Tn < a.T ? Tn : a.T;
