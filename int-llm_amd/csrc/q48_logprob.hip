@@ -24,7 +24,7 @@ static __constant__ int64_t kExp[45] = {
     176142539529353LL, 173411702571733LL, 170723203316912LL, 168076385379650LL, 165470602551013LL,
     162905218640611LL, 160379607321268LL, 157893151976115LL, 155445245548039LL, 153035290391475LL,
     150662698126495LL, 148326889495156LL, 146027294220076LL, 143763350865205LL, 141534506698753LL};
-static __constant__ int64_t kFact[7] = {
+constexpr int64_t kFactK[7] = {
     281474976710656LL, 281474976710656LL, 140737488355328LL, 46912496118443LL, 11728124029611LL,
     2345624805922LL, 390937467654LL};
 static __constant__ int64_t kRcp[64] = {
@@ -59,18 +59,49 @@ static __constant__ int64_t kInv[8] = {
     281474976710656LL, 140737488355328LL, 93824992236885LL, 70368744177664LL, 56294995342131LL,
     46912496118443LL, 40210710958665LL, 35184372088832LL};
 
-// e_i of u (include/intllm_hip.h)
-__device__ __forceinline__ int64_t lp_exp(uint64_t u)
+// T_j 2^-48 as doubles, into LDS
+__device__ __forceinline__ void lp_table(double *tab, int tid)
 {
-    const uint64_t n = u / LP_LN2;
-    if (n >= 49)
-        return 0;
-    const int64_t r = (int64_t)(u - n * LP_LN2), s = r & (((int64_t)1 << 42) - 1);
-    int64_t h = kFact[6];
+    if (tid < 45)
+        tab[tid] = (double)kExp[tid] * 0x1p-48;
+}
+
+// e of u (include/intllm_hip.h), and floor(e u 2^-48) added to w, e to z.  FP64 rounds
+// down, so with M = 2^52 a truncated product of integers below 2^49 is one fused
+// operation, fma(a, b 2^-48, M) = M + floor(a b 2^-48), and a Horner step two: the
+// next h = (C_k + M) - that, exact.  About 45 operations.
+__device__ __forceinline__ void lp_term(uint64_t u, bool in, const double *tab, uint64_t &z,
+                                        uint64_t &w)
+{
+    constexpr uint64_t lim = 49 * (uint64_t)LP_LN2;   // e = 0 from here on; 2^53.1
+    in = in && u < lim;
+    const uint64_t uc = in ? u : 0;
+    const double ud = __builtin_fma((double)(uint32_t)(uc >> 32), 0x1p32, (double)(uint32_t)uc);
+    // u / LN2 within one of the quotient, then the remainder settles it
+    uint32_t n = (uint32_t)q48_word_m52(__builtin_fma(ud, 1.0 / (double)LP_LN2, 0x1p52));
+    int64_t r = (int64_t)(uc - (uint64_t)n * LP_LN2);
+    n = r < 0 ? n - 1 : n;
+    r = r < 0 ? r + LP_LN2 : r;
+    n = r >= LP_LN2 ? n + 1 : n;
+    r = r >= LP_LN2 ? r - LP_LN2 : r;
+    const uint64_t sl = (uint64_t)r & (((uint64_t)1 << 42) - 1);
+    const double s = __builtin_fma(__builtin_bit_cast(double, sl | 0x4330000000000000ull), 0x1p-48,
+                                   -16.0);   // s 2^-48
+    double h = (double)kFactK[6];
 #pragma unroll
     for (int k = 5; k >= 0; --k)
-        h = kFact[k] - q48_mul(s, h);
-    return q48_mul(kExp[r >> 42], h) >> n;
+        h = ((double)kFactK[k] + 0x1p52) - __builtin_fma(s, h, 0x1p52);
+    const uint64_t e = q48_word_m52(__builtin_fma(tab[(uint32_t)(r >> 42)], h, 0x1p52)) >> n;
+    if (in) {
+        z += e;
+        if (uc < ((uint64_t)1 << 53)) {
+            const double ed =
+                __builtin_bit_cast(double, e | 0x4330000000000000ull) - 0x1p52;
+            w += q48_word_m52(__builtin_fma(ed, ud * 0x1p-48, 0x1p52));
+        } else {
+            w += (uint64_t)q48_mul((int64_t)e, (int64_t)uc);
+        }
+    }
 }
 
 // logZ of Z >= 2^48, and its b
@@ -94,49 +125,41 @@ __device__ __forceinline__ int64_t lp_value(uint64_t u, int64_t logz)
     return v < u || v > (uint64_t)INT64_MAX ? INT64_MIN : -(int64_t)v;
 }
 
-__global__ __launch_bounds__(256) void k_lp_simple(const int64_t *__restrict__ X, int V,
-                                                  const int *__restrict__ tokens,
-                                                  int64_t *__restrict__ logp,
-                                                  int64_t *__restrict__ entropy, int top,
-                                                  int *__restrict__ ids,
-                                                  int64_t *__restrict__ tlp)
+// A value's order as an unsigned word, and its high half: what the selection of
+// the most probable tokens compares first.
+__device__ __forceinline__ uint32_t lp_high(int64_t x)
 {
-    q48_round_down();
-    __shared__ int64_t red[4], bv[4];
-    __shared__ uint64_t sums[4][4];
-    __shared__ int bi[4];
-    const int t = blockIdx.x, tid = threadIdx.x;
-    const int64_t *x = X + (size_t)t * V;
-    int64_t m = INT64_MIN;
-    for (int i = tid; i < V; i += 256)
-        m = x[i] > m ? x[i] : m;
-    m = block_max64<256>(m, red);
-    q48_u128 z = 0, w = 0;
-    for (int i = tid; i < V; i += 256) {
-        const uint64_t u = (uint64_t)m - (uint64_t)x[i];
-        const int64_t e = lp_exp(u);
-        if (e) {
-            z += (uint64_t)e;
-            w += (uint64_t)q48_mul(e, (int64_t)u);
-        }
+    return (uint32_t)((uint64_t)x >> 32) ^ 0x80000000u;
+}
+
+// The n-th largest of the high halves that the lanes of a wave hold in g[0 .. N - 1]
+// (64 N >= n), from the top bit down: n of the groups whose maxima these are have a
+// value at least that large, so the n largest values of the row are among the values
+// whose high halves are not below it.
+template <int N>
+__device__ __forceinline__ uint32_t lp_threshold(const uint32_t (&g)[N], int n)
+{
+    uint32_t t = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t c = t | (1u << bit);
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            count += __popcll(__ballot(g[i] >= c));
+        if (count >= n)
+            t = c;
     }
-    z = q48_wave_sum128(z);
-    w = q48_wave_sum128(w);
-    if ((tid & 63) == 0) {
-        sums[tid >> 6][0] = (uint64_t)z;
-        sums[tid >> 6][1] = (uint64_t)(z >> 64);
-        sums[tid >> 6][2] = (uint64_t)w;
-        sums[tid >> 6][3] = (uint64_t)(w >> 64);
-    }
-    __syncthreads();
-    z = w = 0;
-    for (int i = 0; i < 4; ++i) {
-        z += ((q48_u128)sums[i][1] << 64) | sums[i][0];
-        w += ((q48_u128)sums[i][3] << 64) | sums[i][2];
-    }
+    return t;
+}
+
+// The row's results from its sums z and w.  Every thread returns logZ.
+__device__ __forceinline__ int64_t lp_finish(q48_u128 z, q48_u128 w, int64_t m, const int64_t *x,
+                                             int V, int t, const int *tokens, int64_t *logp,
+                                             int64_t *entropy, bool writer)
+{
     int b;
     const int64_t logz = lp_log(z, b);
-    if (tid == 0) {
+    if (writer) {
         if (logp) {
             const int id = tokens[t];
             logp[t] = id >= 0 && id < V ? lp_value((uint64_t)m - (uint64_t)x[id], logz) : 0;
@@ -144,14 +167,44 @@ __global__ __launch_bounds__(256) void k_lp_simple(const int64_t *__restrict__ X
         if (entropy)
             entropy[t] = logz + q48_div((int64_t)(w >> b), (int64_t)(z >> b));
     }
+    return logz;
+}
+
+constexpr int LP_CAP = 512;   // candidates of a row; past that (ties) the slow selection
+
+// The top values of a row from its candidates cv, ci [0, count): each counts those
+// before it.  count <= LP_CAP.
+template <int NT>
+__device__ __forceinline__ void lp_rank(const int64_t *cv, const int *ci, int count, int64_t m,
+                                        int64_t logz, int t, int top, int *ids, int64_t *tlp,
+                                        int tid)
+{
+    for (int i = tid; i < count; i += NT) {
+        const int64_t v = cv[i];
+        const int id = ci[i];
+        int rank = 0;
+        for (int k = 0; k < count; ++k)
+            rank += cv[k] > v || (cv[k] == v && ci[k] < id);
+        if (rank < top) {
+            ids[(size_t)t * top + rank] = id;
+            tlp[(size_t)t * top + rank] = lp_value((uint64_t)m - (uint64_t)v, logz);
+        }
+    }
+}
+
+// The same by top passes over the row, for rows with more candidates: the largest
+// value after the last one in the order (value, lowest id).
+template <int NT>
+__device__ void lp_select(const int64_t *x, int V, int64_t m, int64_t logz, int t, int top,
+                          int *ids, int64_t *tlp, int tid, int64_t *bv, int *bi)
+{
     int64_t lv = INT64_MAX;
     int li = -1;
     for (int n = 0; n < top; ++n) {
         int64_t v = INT64_MIN;
         int at = INT_MAX;
-        for (int i = tid; i < V; i += 256)
-            if ((x[i] < lv || (x[i] == lv && i > li)) &&
-                (at == INT_MAX || x[i] > v)) {
+        for (int i = tid; i < V; i += NT)
+            if ((x[i] < lv || (x[i] == lv && i > li)) && (at == INT_MAX || x[i] > v)) {
                 v = x[i];
                 at = i;
             }
@@ -171,7 +224,7 @@ __global__ __launch_bounds__(256) void k_lp_simple(const int64_t *__restrict__ X
         __syncthreads();
         v = bv[0];
         at = bi[0];
-        for (int i = 1; i < 4; ++i)
+        for (int i = 1; i < NT / 64; ++i)
             if (bi[i] != INT_MAX && (at == INT_MAX || bv[i] > v || (bv[i] == v && bi[i] < at))) {
                 v = bv[i];
                 at = bi[i];
@@ -183,6 +236,239 @@ __global__ __launch_bounds__(256) void k_lp_simple(const int64_t *__restrict__ X
             tlp[(size_t)t * top + n] = lp_value((uint64_t)m - (uint64_t)v, logz);
         }
     }
+}
+
+// Sums of z and w (64-bit words) over a block's waves, in exact 128 bits.
+template <int NW>
+__device__ __forceinline__ void lp_total(q48_u128 &z, q48_u128 &w, uint64_t (*sums)[4], int tid)
+{
+    z = q48_wave_sum128(z);
+    w = q48_wave_sum128(w);
+    if ((tid & 63) == 0) {
+        uint64_t *s = sums[tid >> 6];
+        s[0] = (uint64_t)z;
+        s[1] = (uint64_t)(z >> 64);
+        s[2] = (uint64_t)w;
+        s[3] = (uint64_t)(w >> 64);
+    }
+    __syncthreads();
+    z = w = 0;
+    for (int i = 0; i < NW; ++i) {
+        z += ((q48_u128)sums[i][1] << 64) | sums[i][0];
+        w += ((q48_u128)sums[i][3] << 64) | sums[i][2];
+    }
+}
+
+// One block a row of up to 1024 R logits, which stay in registers between the
+// maximum and the exponentials: the row is read once.  Groups of 8 threads keep
+// their maxima for the threshold, which wave 0 finds while the others start on the
+// exponentials.
+template <int R>
+__global__ __launch_bounds__(1024) void k_lp_row(const int64_t *__restrict__ X, int V,
+                                                const int *__restrict__ tokens,
+                                                int64_t *__restrict__ logp,
+                                                int64_t *__restrict__ entropy, int top,
+                                                int *__restrict__ ids, int64_t *__restrict__ tlp)
+{
+    q48_round_down();
+    __shared__ double tab[48];
+    __shared__ int64_t red[16];
+    __shared__ uint32_t gmax[128];
+    __shared__ uint64_t sums[16][4];
+    __shared__ int64_t cv[LP_CAP];
+    __shared__ int ci[LP_CAP];
+    __shared__ int count;
+    __shared__ uint32_t thr;
+    const int t = blockIdx.x, tid = threadIdx.x;
+    const int64_t *x = X + (size_t)t * V;
+    int64_t v[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k)
+        v[k] = 1024 * k + tid < V ? x[1024 * k + tid] : INT64_MIN;
+    lp_table(tab, tid);
+    if (tid == 0)
+        count = 0;
+    int64_t m = v[0];
+#pragma unroll
+    for (int k = 1; k < R; ++k)
+        m = v[k] > m ? v[k] : m;
+    const uint32_t mine = lp_high(m);
+    if (top) {
+        // the maximum of 8 lanes' high halves; 0 below every value where none has one
+        uint32_t g = tid < V ? mine : 0;
+        g = max(g, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)g, Q48_DPP_XOR1, 0xf, 0xf, false));
+        g = max(g, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)g, Q48_DPP_XOR2, 0xf, 0xf, false));
+        g = max(g, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)g, Q48_DPP_HALF_MIRROR, 0xf, 0xf,
+                                                         false));
+        if ((tid & 7) == 0)
+            gmax[tid >> 3] = g;
+    }
+    m = block_max64<1024>(m, red, false);
+    if (top && tid < 64) {
+        const uint32_t g[2] = {gmax[tid], gmax[tid + 64]};
+        const uint32_t h = lp_threshold<2>(g, top);
+        if (tid == 0)
+            thr = h;
+    }
+    uint64_t z64 = 0, w64 = 0;   // R terms below 2^49 each
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        lp_term((uint64_t)m - (uint64_t)v[k], 1024 * k + tid < V, tab, z64, w64);
+        if (k & 1)   // two terms at a time: more would not fit the registers
+            __builtin_amdgcn_sched_barrier(0);
+    }
+    q48_u128 z = z64, w = w64;
+    lp_total<16>(z, w, sums, tid);
+    const int64_t logz = lp_finish(z, w, m, x, V, t, tokens, logp, entropy, tid == 0);
+    if (!top)
+        return;
+    if (mine >= thr) {
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+            if (1024 * k + tid < V && lp_high(v[k]) >= thr) {
+                const int at = atomicAdd(&count, 1);
+                if (at < LP_CAP) {
+                    cv[at] = v[k];
+                    ci[at] = 1024 * k + tid;
+                }
+            }
+    }
+    __syncthreads();
+    if (count <= LP_CAP)
+        lp_rank<1024>(cv, ci, count, m, logz, t, top, ids, tlp, tid);
+    else
+        lp_select<1024>(x, V, m, logz, t, top, ids, tlp, tid, red, reinterpret_cast<int *>(sums));
+}
+
+// ---- a row over many blocks ------------------------------------------------------------
+// Three launches of (chunk, row) blocks, at most 64 chunks a row: the chunks' wave
+// maxima; sums and candidates; the row's results.
+
+struct LpWork {
+    int64_t *gmax;     // [T][4 chunks]: a wave's maximum
+    uint64_t *sums;    // [T][chunks][4]: z and w, 128 bits each
+    int *count;        // [T]
+    int64_t *cv;       // [T][LP_CAP]
+    int *ci;           // [T][LP_CAP]
+    int chunks, ch;    // ch: values a chunk, a multiple of 256
+};
+
+__global__ __launch_bounds__(256) void k_lp_max(const int64_t *__restrict__ X, int V, LpWork p)
+{
+    const int t = blockIdx.y, c = blockIdx.x, tid = threadIdx.x;
+    const int64_t *x = X + (size_t)t * V;
+    const int end = min(V, (c + 1) * p.ch);
+    int64_t m = INT64_MIN;
+#pragma unroll 4
+    for (int i = c * p.ch + tid; i < end; i += 256)
+        m = x[i] > m ? x[i] : m;
+    m = q48_wave_max64(m);
+    if ((tid & 63) == 0)
+        p.gmax[(size_t)t * 4 * p.chunks + 4 * c + (tid >> 6)] = m;
+    if (c == 0 && tid == 0)
+        p.count[t] = 0;
+}
+
+__global__ __launch_bounds__(256) void k_lp_sum(const int64_t *__restrict__ X, int V, int top,
+                                               LpWork p)
+{
+    q48_round_down();
+    __shared__ double tab[48];
+    __shared__ uint64_t sums[4][4];
+    __shared__ uint32_t thr;
+    const int t = blockIdx.y, c = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const int64_t *x = X + (size_t)t * V;
+    const int end = min(V, (c + 1) * p.ch);
+    int64_t g[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int k = lane + 64 * i;
+        g[i] = k < 4 * p.chunks ? p.gmax[(size_t)t * 4 * p.chunks + k] : INT64_MIN;
+    }
+    lp_table(tab, tid);
+    int64_t m = g[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i)
+        m = g[i] > m ? g[i] : m;
+    m = q48_wave_max64(m);
+    if (top && tid < 64) {
+        // waves past the row's end have no value: they count as below every other
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int k = lane + 64 * i;
+            h[i] = k < 4 * p.chunks && (k >> 2) * p.ch + 64 * (k & 3) < V ? lp_high(g[i]) : 0;
+        }
+        const uint32_t n = lp_threshold<4>(h, top);
+        if (tid == 0)
+            thr = n;
+    }
+    __syncthreads();
+    uint64_t z64 = 0, w64 = 0;
+#pragma unroll 2
+    for (int i = c * p.ch + tid; i < end; i += 256) {
+        const int64_t v = x[i];
+        lp_term((uint64_t)m - (uint64_t)v, true, tab, z64, w64);
+        if (top && lp_high(v) >= thr) {
+            const int at = atomicAdd(p.count + t, 1);
+            if (at < LP_CAP) {
+                p.cv[(size_t)t * LP_CAP + at] = v;
+                p.ci[(size_t)t * LP_CAP + at] = i;
+            }
+        }
+    }
+    q48_u128 z = z64, w = w64;
+    lp_total<4>(z, w, sums, tid);
+    if (tid == 0) {
+        uint64_t *s = p.sums + 4 * ((size_t)t * p.chunks + c);
+        s[0] = (uint64_t)z;
+        s[1] = (uint64_t)(z >> 64);
+        s[2] = (uint64_t)w;
+        s[3] = (uint64_t)(w >> 64);
+    }
+}
+
+__global__ __launch_bounds__(256) void k_lp_end(const int64_t *__restrict__ X, int V,
+                                               const int *__restrict__ tokens,
+                                               int64_t *__restrict__ logp,
+                                               int64_t *__restrict__ entropy, int top,
+                                               int *__restrict__ ids, int64_t *__restrict__ tlp,
+                                               LpWork p)
+{
+    q48_round_down();
+    __shared__ int64_t cv[LP_CAP], bv[4];
+    __shared__ int ci[LP_CAP], bi[4];
+    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+    const int64_t *x = X + (size_t)t * V;
+    int64_t m = INT64_MIN;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (lane + 64 * i < 4 * p.chunks) {
+            const int64_t g = p.gmax[(size_t)t * 4 * p.chunks + lane + 64 * i];
+            m = g > m ? g : m;
+        }
+    const int count = top ? p.count[t] : 0;
+    for (int i = tid; i < min(count, LP_CAP); i += 256) {
+        cv[i] = p.cv[(size_t)t * LP_CAP + i];
+        ci[i] = p.ci[(size_t)t * LP_CAP + i];
+    }
+    q48_u128 z = 0, w = 0;
+    if (lane < p.chunks) {
+        const uint64_t *s = p.sums + 4 * ((size_t)t * p.chunks + lane);
+        z = ((q48_u128)s[1] << 64) | s[0];
+        w = ((q48_u128)s[3] << 64) | s[2];
+    }
+    m = q48_wave_max64(m);
+    z = q48_wave_sum128(z);
+    w = q48_wave_sum128(w);
+    const int64_t logz = lp_finish(z, w, m, x, V, t, tokens, logp, entropy, tid == 0);
+    __syncthreads();
+    if (!top)
+        return;
+    if (count <= LP_CAP)
+        lp_rank<256>(cv, ci, count, m, logz, t, top, ids, tlp, tid);
+    else
+        lp_select<256>(x, V, m, logz, t, top, ids, tlp, tid, bv, bi);
 }
 
 } // namespace
@@ -197,8 +483,56 @@ int q48_logprobs_rows(q48_ctx *c, const int64_t *logits, int T, int vocab, const
         (top_n > 0 && (!top_ids || !top_logp)) || (!logp && !entropy && top_n == 0))
         return Q48_EINVAL;
     q48_on_device on(c);
-    hipLaunchKernelGGL(k_lp_simple, dim3(T), dim3(256), 0, c->stream, logits, vocab, d_tokens, logp,
-                       entropy, top_n, top_ids, top_logp);
+    if (vocab <= 32768 && (vocab <= 8192 || T >= 64)) {
+#define LP_ROW(R)                                                                              \
+    hipLaunchKernelGGL(k_lp_row<R>, dim3(T), dim3(1024), 0, c->stream, logits, vocab, d_tokens, \
+                       logp, entropy, top_n, top_ids, top_logp)
+        if (vocab <= 4096)
+            LP_ROW(4);
+        else if (vocab <= 8192)
+            LP_ROW(8);
+        else if (vocab <= 16384)
+            LP_ROW(16);
+        else
+            LP_ROW(32);
+#undef LP_ROW
+        return hipGetLastError() == hipSuccess ? Q48_OK : Q48_EHIP;
+    }
+    LpWork p = {};
+    p.ch = ((vocab + 63) / 64 + 255) & ~255;
+    p.chunks = (vocab + p.ch - 1) / p.ch;
+    size_t o = 0;
+    auto take = [&](size_t bytes) {
+        const size_t at = o;
+        o += (bytes + 255) & ~(size_t)255;
+        return at;
+    };
+    // rows of one launch: a grid's y, and a bounded workspace
+    const int rows = T < 32768 ? T : 32768;
+    const size_t o_g = take((size_t)rows * 4 * p.chunks * 8);
+    const size_t o_s = take((size_t)rows * p.chunks * 32), o_n = take((size_t)rows * 4);
+    const size_t o_v = take((size_t)rows * LP_CAP * 8), o_i = take((size_t)rows * LP_CAP * 4);
+    const int rc = q48_ws_reserve(c, o);
+    if (rc)
+        return rc;
+    uint8_t *ws = (uint8_t *)c->ws;
+    p.gmax = (int64_t *)(ws + o_g);
+    p.sums = (uint64_t *)(ws + o_s);
+    p.count = (int *)(ws + o_n);
+    p.cv = (int64_t *)(ws + o_v);
+    p.ci = (int *)(ws + o_i);
+    for (int t0 = 0; t0 < T; t0 += rows) {
+        const int n = rows < T - t0 ? rows : T - t0;
+        const int64_t *x = logits + (size_t)t0 * vocab;
+        hipLaunchKernelGGL(k_lp_max, dim3(p.chunks, n), dim3(256), 0, c->stream, x, vocab, p);
+        hipLaunchKernelGGL(k_lp_sum, dim3(p.chunks, n), dim3(256), 0, c->stream, x, vocab, top_n,
+                           p);
+        hipLaunchKernelGGL(k_lp_end, dim3(n), dim3(256), 0, c->stream, x, vocab,
+                           d_tokens ? d_tokens + t0 : nullptr, logp ? logp + t0 : nullptr,
+                           entropy ? entropy + t0 : nullptr, top_n,
+                           top_ids ? top_ids + (size_t)t0 * top_n : nullptr,
+                           top_logp ? top_logp + (size_t)t0 * top_n : nullptr, p);
+    }
     return hipGetLastError() == hipSuccess ? Q48_OK : Q48_EHIP;
 }
 
