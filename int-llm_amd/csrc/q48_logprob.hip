@@ -11,6 +11,7 @@ namespace {
 
 constexpr int64_t LP_LN2 = 195103586505167LL;   // fp_log's ln 2 (fp_math.h:752-773)
 constexpr int LP_MAX_TOP = 32;
+constexpr int LP_CAP = 512;   // candidates of a row; past that (ties) the slow selection
 
 // round(2^48 e^(-j/64)), round(2^48 / k!), floor(2^54 / (64 + j)),
 // round(2^48 log(1 + j/64)), round(2^48 / (k + 1))
@@ -66,42 +67,75 @@ __device__ __forceinline__ void lp_table(double *tab, int tid)
         tab[tid] = (double)kExp[tid] * 0x1p-48;
 }
 
-// e of u (include/intllm_hip.h), and floor(e u 2^-48) added to w, e to z.  FP64 rounds
-// down, so with M = 2^52 a truncated product of integers below 2^49 is one fused
-// operation, fma(a, b 2^-48, M) = M + floor(a b 2^-48), and a Horner step two: the
-// next h = (C_k + M) - that, exact.  About 45 operations.
-__device__ __forceinline__ void lp_term(uint64_t u, bool in, const double *tab, uint64_t &z,
-                                        uint64_t &w)
+// e of each u (include/intllm_hip.h; 0 from LP_LIM on), added to z, and floor(e u
+// 2^-48) added to w.  FP64 rounds down, so with M = 2^52 a truncated product of
+// integers below 2^49 is one fused operation, fma(a, b 2^-48, M) = M + floor(a b
+// 2^-48), and a Horner step two: the next h = (C_k + M) - that, exact.  u = q 2^52 +
+// u0 (q <= 2) keeps every double an exact integer where u passes 2^53: r = (q 2^52 -
+// n LN2) + u0.  1 / LN2 is rounded down, so n is the quotient or one less.  About 55
+// operations and no branch; N terms step by step, since one is a chain of them all.
+constexpr uint64_t LP_LIM = 49 * (uint64_t)LP_LN2;   // 2^53.1
+template <int N>
+__device__ __forceinline__ void lp_terms(const uint64_t (&u)[N], const double *tab, uint64_t &z,
+                                         uint64_t &w)
 {
-    constexpr uint64_t lim = 49 * (uint64_t)LP_LN2;   // e = 0 from here on; 2^53.1
-    in = in && u < lim;
-    const uint64_t uc = in ? u : 0;
-    const double ud = __builtin_fma((double)(uint32_t)(uc >> 32), 0x1p32, (double)(uint32_t)uc);
-    // u / LN2 within one of the quotient, then the remainder settles it
-    uint32_t n = (uint32_t)q48_word_m52(__builtin_fma(ud, 1.0 / (double)LP_LN2, 0x1p52));
-    int64_t r = (int64_t)(uc - (uint64_t)n * LP_LN2);
-    n = r < 0 ? n - 1 : n;
-    r = r < 0 ? r + LP_LN2 : r;
-    n = r >= LP_LN2 ? n + 1 : n;
-    r = r >= LP_LN2 ? r - LP_LN2 : r;
-    const uint64_t sl = (uint64_t)r & (((uint64_t)1 << 42) - 1);
-    const double s = __builtin_fma(__builtin_bit_cast(double, sl | 0x4330000000000000ull), 0x1p-48,
-                                   -16.0);   // s 2^-48
-    double h = (double)kFactK[6];
+    constexpr double ln2 = (double)LP_LN2, inv = 0x1.7154765200000p-48;
+    static_assert(inv * ln2 < 1.0 && inv * ln2 > 1.0 - 0x1p-24, "1 / LN2, rounded down");
+    bool in[N], more[N];
+    uint32_t q[N], n[N];
+    double u0[N], top[N], tn[N], r[N], tj[N], s[N], h[N], tt[N];
+#define LP_EACH for (int i = 0; i < N; ++i)
+#pragma unroll
+    LP_EACH
+    {
+        in[i] = u[i] < LP_LIM;
+        const uint32_t hi = in[i] ? (uint32_t)(u[i] >> 32) : 0;
+        q[i] = hi >> 20;
+        u0[i] = __builtin_bit_cast(double, ((uint64_t)((hi & 0xFFFFFu) | 0x43300000u) << 32) |
+                                               (uint32_t)u[i]) -
+                0x1p52;
+    }
+#pragma unroll
+    LP_EACH top[i] = __builtin_ldexp((double)q[i], 52);
+#pragma unroll
+    LP_EACH tn[i] = __builtin_fma(u0[i] + top[i], inv, 0x1p52);
+#pragma unroll
+    LP_EACH
+    {
+        n[i] = (uint32_t)__builtin_bit_cast(uint64_t, tn[i]);
+        r[i] = __builtin_fma(-(tn[i] - 0x1p52), ln2, top[i]) + u0[i];
+    }
+#pragma unroll
+    LP_EACH
+    {
+        more[i] = r[i] >= ln2;
+        n[i] += more[i];
+        r[i] = more[i] ? r[i] - ln2 : r[i];
+    }
+#pragma unroll
+    LP_EACH tj[i] = __builtin_fma(r[i], 0x1p-42, 0x1p52);
+#pragma unroll
+    LP_EACH
+    {
+        tt[i] = tab[(uint32_t)__builtin_bit_cast(uint64_t, tj[i]) & 63];
+        s[i] = __builtin_fma(tj[i] - 0x1p52, -0x1p-6, r[i] * 0x1p-48);   // s 2^-48
+        h[i] = (double)kFactK[6];
+    }
 #pragma unroll
     for (int k = 5; k >= 0; --k)
-        h = ((double)kFactK[k] + 0x1p52) - __builtin_fma(s, h, 0x1p52);
-    const uint64_t e = q48_word_m52(__builtin_fma(tab[(uint32_t)(r >> 42)], h, 0x1p52)) >> n;
-    if (in) {
+#pragma unroll
+        LP_EACH h[i] = ((double)kFactK[k] + 0x1p52) - __builtin_fma(s[i], h[i], 0x1p52);
+#pragma unroll
+    LP_EACH
+    {
+        const uint64_t e = q48_word_m52(__builtin_fma(tt[i], h[i], 0x1p52)) >> (in[i] ? n[i] : 63);
+        const double ed = __builtin_bit_cast(double, e | 0x4330000000000000ull) - 0x1p52;
         z += e;
-        if (uc < ((uint64_t)1 << 53)) {
-            const double ed =
-                __builtin_bit_cast(double, e | 0x4330000000000000ull) - 0x1p52;
-            w += q48_word_m52(__builtin_fma(ed, ud * 0x1p-48, 0x1p52));
-        } else {
-            w += (uint64_t)q48_mul((int64_t)e, (int64_t)uc);
-        }
+        // e 2^4 q: e is below 2^27 where q is not 0
+        w += q48_word_m52(__builtin_fma(ed, u0[i] * 0x1p-48, 0x1p52)) +
+             (uint64_t)(uint32_t)e * (16 * q[i]);
     }
+#undef LP_EACH
 }
 
 // logZ of Z >= 2^48, and its b
@@ -133,44 +167,70 @@ __device__ __forceinline__ uint32_t lp_high(int64_t x)
 }
 
 // The n-th largest of the high halves that the lanes of a wave hold in g[0 .. N - 1]
-// (64 N >= n), from the top bit down: n of the groups whose maxima these are have a
-// value at least that large, so the n largest values of the row are among the values
-// whose high halves are not below it.
+// (64 N >= n), two bits at a time from the top: n of the groups whose maxima these
+// are have a value at least that large, so the n largest values of the row are among
+// the values whose high halves are not below it.
 template <int N>
 __device__ __forceinline__ uint32_t lp_threshold(const uint32_t (&g)[N], int n)
 {
     uint32_t t = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t c = t | (1u << bit);
-        int count = 0;
+    for (int bit = 30; bit >= 0; bit -= 2) {
+        int count[3] = {0, 0, 0};
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            count += __popcll(__ballot(g[i] >= c));
-        if (count >= n)
-            t = c;
+#pragma unroll
+            for (int c = 0; c < 3; ++c)
+                count[c] += __popcll(__ballot(g[i] >= (t | ((uint32_t)(c + 1) << bit))));
+        t |= (uint32_t)((count[0] >= n) + (count[1] >= n) + (count[2] >= n)) << bit;
     }
     return t;
 }
 
-// The row's results from its sums z and w.  Every thread returns logZ.
+// The candidates (high half >= thr) among the values first + k stride < end of the
+// threads whose maximum is one, appended to cv and ci: the wave reads such a thread's
+// values together, 64 at a time.
+__device__ __forceinline__ void lp_collect(const int64_t *x, int first, int stride, int end,
+                                           bool some, uint32_t thr, int64_t *cv, int *ci,
+                                           int *count, int cap, int lane)
+{
+    uint64_t todo = __ballot(some);
+    while (todo) {
+        const int l = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        for (int i = __builtin_amdgcn_readlane(first, l) + lane * stride; i < end;
+             i += 64 * stride) {
+            const int64_t y = x[i];
+            if (lp_high(y) >= thr) {
+                const int at = atomicAdd(count, 1);
+                if (at < cap) {
+                    cv[at] = y;
+                    ci[at] = i;
+                }
+            }
+        }
+    }
+}
+
+// The row's log probability and entropy from its sums z and w; returns logZ.
 __device__ __forceinline__ int64_t lp_finish(q48_u128 z, q48_u128 w, int64_t m, const int64_t *x,
                                              int V, int t, const int *tokens, int64_t *logp,
                                              int64_t *entropy, bool writer)
 {
+    // the token's logit on its way during the logarithm
+    const int id = logp ? tokens[t] : -1;
+    const bool valid = id >= 0 && id < V;
+    const int64_t y = valid ? x[id] : m;
     int b;
     const int64_t logz = lp_log(z, b);
     if (writer) {
-        if (logp) {
-            const int id = tokens[t];
-            logp[t] = id >= 0 && id < V ? lp_value((uint64_t)m - (uint64_t)x[id], logz) : 0;
-        }
+        if (logp)
+            logp[t] = valid ? lp_value((uint64_t)m - (uint64_t)y, logz) : 0;
         if (entropy)
             entropy[t] = logz + q48_div((int64_t)(w >> b), (int64_t)(z >> b));
     }
     return logz;
 }
 
-constexpr int LP_CAP = 512;   // candidates of a row; past that (ties) the slow selection
 
 // The top values of a row from its candidates cv, ci [0, count): each counts those
 // before it.  count <= LP_CAP.
@@ -238,106 +298,141 @@ __device__ void lp_select(const int64_t *x, int V, int64_t m, int64_t logz, int 
     }
 }
 
-// Sums of z and w (64-bit words) over a block's waves, in exact 128 bits.
-template <int NW>
-__device__ __forceinline__ void lp_total(q48_u128 &z, q48_u128 &w, uint64_t (*sums)[4], int tid)
+// Sums of z and w over a wave, in exact 128 bits, as four words (lane 0).
+__device__ __forceinline__ void lp_wave_sums(uint64_t z64, uint64_t w64, uint64_t *s, int lane)
 {
-    z = q48_wave_sum128(z);
-    w = q48_wave_sum128(w);
-    if ((tid & 63) == 0) {
-        uint64_t *s = sums[tid >> 6];
+    const q48_u128 z = q48_wave_sum128(z64), w = q48_wave_sum128(w64);
+    if (lane == 0) {
         s[0] = (uint64_t)z;
         s[1] = (uint64_t)(z >> 64);
         s[2] = (uint64_t)w;
         s[3] = (uint64_t)(w >> 64);
     }
-    __syncthreads();
-    z = w = 0;
-    for (int i = 0; i < NW; ++i) {
-        z += ((q48_u128)sums[i][1] << 64) | sums[i][0];
-        w += ((q48_u128)sums[i][3] << 64) | sums[i][2];
-    }
 }
 
-// One block a row of up to 1024 R logits, which stay in registers between the
-// maximum and the exponentials: the row is read once.  Groups of 8 threads keep
-// their maxima for the threshold, which wave 0 finds while the others start on the
-// exponentials.
+// A row of logits through a buffer descriptor: loads past its end give 0 and need no
+// branch.  (The whole offset goes where the bounds check sees it: not into the scalar
+// offset, which it leaves out.)
+struct LpRow {
+    __amdgpu_buffer_rsrc_t d;
+    __device__ __forceinline__ LpRow(const int64_t *x, int V)
+        : d(__builtin_amdgcn_make_buffer_rsrc(const_cast<int64_t *>(x), 0, V * 8, 0x00027000))
+    {
+    }
+    __device__ __forceinline__ int64_t at(int i) const
+    {
+        return __builtin_bit_cast(int64_t, __builtin_amdgcn_raw_buffer_load_b64(d, 8 * i, 0, 0));
+    }
+};
+
+constexpr int LR_NT = 512;
+
+// Rows of up to 512 R logits, a block a row at a time (row blockIdx.x, + gridDim.x,
+// ...): a row stays in registers between the maximum and the exponentials, so it is
+// read once, and the next row's loads go out as its registers fall free, under the
+// remaining exponentials.  Groups of 4 threads keep their maxima for the threshold,
+// which wave 0 finds before its exponentials; the few threads with a candidate read
+// their logits again.
 template <int R>
-__global__ __launch_bounds__(1024) void k_lp_row(const int64_t *__restrict__ X, int V,
-                                                const int *__restrict__ tokens,
-                                                int64_t *__restrict__ logp,
-                                                int64_t *__restrict__ entropy, int top,
-                                                int *__restrict__ ids, int64_t *__restrict__ tlp)
+__global__ __launch_bounds__(LR_NT) void k_lp_row(const int64_t *__restrict__ X, int T, int V,
+                                                 const int *__restrict__ tokens,
+                                                 int64_t *__restrict__ logp,
+                                                 int64_t *__restrict__ entropy, int top,
+                                                 int *__restrict__ ids, int64_t *__restrict__ tlp)
 {
     q48_round_down();
-    __shared__ double tab[48];
-    __shared__ int64_t red[16];
-    __shared__ uint32_t gmax[128];
-    __shared__ uint64_t sums[16][4];
-    __shared__ int64_t cv[LP_CAP];
+    constexpr int NW = LR_NT / 64;
+    __shared__ double tab[64];
+    __shared__ int64_t red[2][NW];
+    __shared__ uint32_t gmax[LR_NT / 4];
+    __shared__ uint64_t sums[NW][4];
+    __shared__ int64_t cv[LP_CAP], slogz;
     __shared__ int ci[LP_CAP];
     __shared__ int count;
     __shared__ uint32_t thr;
-    const int t = blockIdx.x, tid = threadIdx.x;
-    const int64_t *x = X + (size_t)t * V;
-    int64_t v[R];
-#pragma unroll
-    for (int k = 0; k < R; ++k)
-        v[k] = 1024 * k + tid < V ? x[1024 * k + tid] : INT64_MIN;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int whole = V / LR_NT;   // tiles of 512 with every thread in the row
     lp_table(tab, tid);
-    if (tid == 0)
-        count = 0;
-    int64_t m = v[0];
-#pragma unroll
-    for (int k = 1; k < R; ++k)
-        m = v[k] > m ? v[k] : m;
-    const uint32_t mine = lp_high(m);
-    if (top) {
-        // the maximum of 8 lanes' high halves; 0 below every value where none has one
-        uint32_t g = tid < V ? mine : 0;
-        g = max(g, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)g, Q48_DPP_XOR1, 0xf, 0xf, false));
-        g = max(g, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)g, Q48_DPP_XOR2, 0xf, 0xf, false));
-        g = max(g, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)g, Q48_DPP_HALF_MIRROR, 0xf, 0xf,
-                                                         false));
-        if ((tid & 7) == 0)
-            gmax[tid >> 3] = g;
-    }
-    m = block_max64<1024>(m, red, false);
-    if (top && tid < 64) {
-        const uint32_t g[2] = {gmax[tid], gmax[tid + 64]};
-        const uint32_t h = lp_threshold<2>(g, top);
-        if (tid == 0)
-            thr = h;
-    }
-    uint64_t z64 = 0, w64 = 0;   // R terms below 2^49 each
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-        lp_term((uint64_t)m - (uint64_t)v[k], 1024 * k + tid < V, tab, z64, w64);
-        if (k & 1)   // two terms at a time: more would not fit the registers
-            __builtin_amdgcn_sched_barrier(0);
-    }
-    q48_u128 z = z64, w = w64;
-    lp_total<16>(z, w, sums, tid);
-    const int64_t logz = lp_finish(z, w, m, x, V, t, tokens, logp, entropy, tid == 0);
-    if (!top)
-        return;
-    if (mine >= thr) {
+    int64_t v[R];
+    {
+        const LpRow row(X + (size_t)blockIdx.x * V, V);
 #pragma unroll
         for (int k = 0; k < R; ++k)
-            if (1024 * k + tid < V && lp_high(v[k]) >= thr) {
-                const int at = atomicAdd(&count, 1);
-                if (at < LP_CAP) {
-                    cv[at] = v[k];
-                    ci[at] = 1024 * k + tid;
-                }
-            }
+            v[k] = row.at(k * LR_NT + tid);
     }
-    __syncthreads();
-    if (count <= LP_CAP)
-        lp_rank<1024>(cv, ci, count, m, logz, t, top, ids, tlp, tid);
-    else
-        lp_select<1024>(x, V, m, logz, t, top, ids, tlp, tid, red, reinterpret_cast<int *>(sums));
+    int par = 0;
+    for (int t = blockIdx.x; t < T; t += gridDim.x, par ^= 1) {
+        const int64_t *x = X + (size_t)t * V;
+        int64_t m = INT64_MIN;
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            int64_t y = v[k];
+            if (k >= whole)
+                y = k * LR_NT + tid < V ? y : INT64_MIN;
+            m = y > m ? y : m;
+        }
+        const uint32_t mine = lp_high(m);
+        if (top) {
+            // the maximum of 4 lanes' high halves; 0, below every value, where none has one
+            uint32_t g = tid < V ? mine : 0;
+            g = max(g, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)g, Q48_DPP_XOR1, 0xf, 0xf,
+                                                             false));
+            g = max(g, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)g, Q48_DPP_XOR2, 0xf, 0xf,
+                                                             false));
+            if ((tid & 3) == 0)
+                gmax[tid >> 2] = g;
+        }
+        if (tid == 0)
+            count = 0;
+        m = block_max64<LR_NT>(m, red[par], false);
+        if (top && tid < 64) {
+            const uint32_t g[2] = {gmax[tid], gmax[tid + 64]};
+            const uint32_t h = lp_threshold<2>(g, top);
+            if (tid == 0)
+                thr = h;
+        }
+        // (a block's last row: a row of no logits, nothing is read)
+        const bool again = t + gridDim.x < (unsigned)T;
+        const LpRow next(again ? x + (size_t)gridDim.x * V : x, again ? V : 0);
+        uint64_t z64 = 0, w64 = 0;   // R terms below 2^49 each
+#pragma unroll
+        for (int k = 0; k < R; k += 4) {
+            uint64_t u[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                u[i] = (uint64_t)m - (uint64_t)v[k + i];
+                if (k + i >= whole)
+                    u[i] = (k + i) * LR_NT + tid < V ? u[i] : LP_LIM;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                v[k + i] = next.at((k + i) * LR_NT + tid);
+            lp_terms<4>(u, tab, z64, w64);
+            __builtin_amdgcn_sched_barrier(0);   // more terms would not fit the registers
+        }
+        lp_wave_sums(z64, w64, sums[tid >> 6], lane);
+        __syncthreads();
+        if (tid < 64) {
+            q48_u128 z = 0, w = 0;
+            for (int i = 0; i < NW; ++i) {
+                z += ((q48_u128)sums[i][1] << 64) | sums[i][0];
+                w += ((q48_u128)sums[i][3] << 64) | sums[i][2];
+            }
+            const int64_t logz = lp_finish(z, w, m, x, V, t, tokens, logp, entropy, tid == 0);
+            if (tid == 0)
+                slogz = logz;
+        }
+        if (!top)
+            continue;   // (the next row's first barrier is behind its reads of v alone)
+        lp_collect(x, tid, LR_NT, V, tid < V && mine >= thr, thr, cv, ci, &count, LP_CAP, lane);
+        __syncthreads();
+        if (count <= LP_CAP)
+            lp_rank<LR_NT>(cv, ci, count, m, slogz, t, top, ids, tlp, tid);
+        else
+            lp_select<LR_NT>(x, V, m, slogz, t, top, ids, tlp, tid, red[par],
+                             reinterpret_cast<int *>(sums));
+        __syncthreads();
+    }
 }
 
 // ---- a row over many blocks ------------------------------------------------------------
@@ -346,7 +441,7 @@ __global__ __launch_bounds__(1024) void k_lp_row(const int64_t *__restrict__ X, 
 
 struct LpWork {
     int64_t *gmax;     // [T][4 chunks]: a wave's maximum
-    uint64_t *sums;    // [T][chunks][4]: z and w, 128 bits each
+    uint64_t *sums;    // [T][4 chunks][4]: a wave's z and w, 128 bits each
     int *count;        // [T]
     int64_t *cv;       // [T][LP_CAP]
     int *ci;           // [T][LP_CAP]
@@ -373,8 +468,7 @@ __global__ __launch_bounds__(256) void k_lp_sum(const int64_t *__restrict__ X, i
                                                LpWork p)
 {
     q48_round_down();
-    __shared__ double tab[48];
-    __shared__ uint64_t sums[4][4];
+    __shared__ double tab[64];
     __shared__ uint32_t thr;
     const int t = blockIdx.y, c = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const int64_t *x = X + (size_t)t * V;
@@ -391,6 +485,7 @@ __global__ __launch_bounds__(256) void k_lp_sum(const int64_t *__restrict__ X, i
     for (int i = 1; i < 4; ++i)
         m = g[i] > m ? g[i] : m;
     m = q48_wave_max64(m);
+    __syncthreads();   // the table
     if (top && tid < 64) {
         // waves past the row's end have no value: they count as below every other
         uint32_t h[4];
@@ -403,29 +498,28 @@ __global__ __launch_bounds__(256) void k_lp_sum(const int64_t *__restrict__ X, i
         if (tid == 0)
             thr = n;
     }
-    __syncthreads();
     uint64_t z64 = 0, w64 = 0;
-#pragma unroll 2
-    for (int i = c * p.ch + tid; i < end; i += 256) {
-        const int64_t v = x[i];
-        lp_term((uint64_t)m - (uint64_t)v, true, tab, z64, w64);
-        if (top && lp_high(v) >= thr) {
-            const int at = atomicAdd(p.count + t, 1);
-            if (at < LP_CAP) {
-                p.cv[(size_t)t * LP_CAP + at] = v;
-                p.ci[(size_t)t * LP_CAP + at] = i;
-            }
-        }
+    int64_t mine = INT64_MIN;
+    int i = c * p.ch + tid;
+    for (; i + 256 < end; i += 512) {
+        const int64_t v[2] = {x[i], x[i + 256]};
+        mine = v[0] > mine ? v[0] : mine;
+        mine = v[1] > mine ? v[1] : mine;
+        const uint64_t u[2] = {(uint64_t)m - (uint64_t)v[0], (uint64_t)m - (uint64_t)v[1]};
+        lp_terms<2>(u, tab, z64, w64);
     }
-    q48_u128 z = z64, w = w64;
-    lp_total<4>(z, w, sums, tid);
-    if (tid == 0) {
-        uint64_t *s = p.sums + 4 * ((size_t)t * p.chunks + c);
-        s[0] = (uint64_t)z;
-        s[1] = (uint64_t)(z >> 64);
-        s[2] = (uint64_t)w;
-        s[3] = (uint64_t)(w >> 64);
+    if (i < end) {
+        mine = x[i] > mine ? x[i] : mine;
+        const uint64_t u[1] = {(uint64_t)m - (uint64_t)x[i]};
+        lp_terms<1>(u, tab, z64, w64);
     }
+    lp_wave_sums(z64, w64, p.sums + 4 * (4 * ((size_t)t * p.chunks + c) + (tid >> 6)), lane);
+    if (!top)
+        return;
+    __syncthreads();   // the threshold
+    const int first = c * p.ch + tid;
+    lp_collect(x, first, 256, end, first < end && lp_high(mine) >= thr, thr,
+               p.cv + (size_t)t * LP_CAP, p.ci + (size_t)t * LP_CAP, p.count + t, LP_CAP, lane);
 }
 
 __global__ __launch_bounds__(256) void k_lp_end(const int64_t *__restrict__ X, int V,
@@ -436,7 +530,7 @@ __global__ __launch_bounds__(256) void k_lp_end(const int64_t *__restrict__ X, i
                                                LpWork p)
 {
     q48_round_down();
-    __shared__ int64_t cv[LP_CAP], bv[4];
+    __shared__ int64_t cv[LP_CAP], bv[4], slogz;
     __shared__ int ci[LP_CAP], bi[4];
     const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const int64_t *x = X + (size_t)t * V;
@@ -447,28 +541,37 @@ __global__ __launch_bounds__(256) void k_lp_end(const int64_t *__restrict__ X, i
             const int64_t g = p.gmax[(size_t)t * 4 * p.chunks + lane + 64 * i];
             m = g > m ? g : m;
         }
+    // wave 0: the row's sums; the others: its candidates
     const int count = top ? p.count[t] : 0;
-    for (int i = tid; i < min(count, LP_CAP); i += 256) {
-        cv[i] = p.cv[(size_t)t * LP_CAP + i];
-        ci[i] = p.ci[(size_t)t * LP_CAP + i];
+    if (tid < 64) {
+        q48_u128 z = 0, w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lane + 64 * i < 4 * p.chunks) {
+                const uint64_t *s = p.sums + 4 * ((size_t)t * 4 * p.chunks + lane + 64 * i);
+                z += ((q48_u128)s[1] << 64) | s[0];
+                w += ((q48_u128)s[3] << 64) | s[2];
+            }
+        m = q48_wave_max64(m);
+        z = q48_wave_sum128(z);
+        w = q48_wave_sum128(w);
+        const int64_t logz = lp_finish(z, w, m, x, V, t, tokens, logp, entropy, tid == 0);
+        if (tid == 0)
+            slogz = logz;
+    } else {
+        m = q48_wave_max64(m);
+        for (int i = tid - 64; i < min(count, LP_CAP); i += 192) {
+            cv[i] = p.cv[(size_t)t * LP_CAP + i];
+            ci[i] = p.ci[(size_t)t * LP_CAP + i];
+        }
     }
-    q48_u128 z = 0, w = 0;
-    if (lane < p.chunks) {
-        const uint64_t *s = p.sums + 4 * ((size_t)t * p.chunks + lane);
-        z = ((q48_u128)s[1] << 64) | s[0];
-        w = ((q48_u128)s[3] << 64) | s[2];
-    }
-    m = q48_wave_max64(m);
-    z = q48_wave_sum128(z);
-    w = q48_wave_sum128(w);
-    const int64_t logz = lp_finish(z, w, m, x, V, t, tokens, logp, entropy, tid == 0);
-    __syncthreads();
     if (!top)
         return;
+    __syncthreads();
     if (count <= LP_CAP)
-        lp_rank<256>(cv, ci, count, m, logz, t, top, ids, tlp, tid);
+        lp_rank<256>(cv, ci, count, m, slogz, t, top, ids, tlp, tid);
     else
-        lp_select<256>(x, V, m, logz, t, top, ids, tlp, tid, bv, bi);
+        lp_select<256>(x, V, m, slogz, t, top, ids, tlp, tid, bv, bi);
 }
 
 } // namespace
@@ -484,17 +587,19 @@ int q48_logprobs_rows(q48_ctx *c, const int64_t *logits, int T, int vocab, const
         return Q48_EINVAL;
     q48_on_device on(c);
     if (vocab <= 32768 && (vocab <= 8192 || T >= 64)) {
-#define LP_ROW(R)                                                                              \
-    hipLaunchKernelGGL(k_lp_row<R>, dim3(T), dim3(1024), 0, c->stream, logits, vocab, d_tokens, \
-                       logp, entropy, top_n, top_ids, top_logp)
+#define LP_ROW(R, PER)                                                                         \
+    hipLaunchKernelGGL(k_lp_row<R>, dim3(T < PER * c->cu_count ? T : PER * c->cu_count),       \
+                       dim3(LR_NT), 0, c->stream, logits, T, vocab, d_tokens, logp, entropy,   \
+                       top_n, top_ids, top_logp)
+        // (the second number: blocks a compute unit's registers hold)
         if (vocab <= 4096)
-            LP_ROW(4);
+            LP_ROW(8, 2);
         else if (vocab <= 8192)
-            LP_ROW(8);
+            LP_ROW(16, 2);
         else if (vocab <= 16384)
-            LP_ROW(16);
+            LP_ROW(32, 1);
         else
-            LP_ROW(32);
+            LP_ROW(64, 1);
 #undef LP_ROW
         return hipGetLastError() == hipSuccess ? Q48_OK : Q48_EHIP;
     }
@@ -510,7 +615,7 @@ int q48_logprobs_rows(q48_ctx *c, const int64_t *logits, int T, int vocab, const
     // rows of one launch: a grid's y, and a bounded workspace
     const int rows = T < 32768 ? T : 32768;
     const size_t o_g = take((size_t)rows * 4 * p.chunks * 8);
-    const size_t o_s = take((size_t)rows * p.chunks * 32), o_n = take((size_t)rows * 4);
+    const size_t o_s = take((size_t)rows * 4 * p.chunks * 32), o_n = take((size_t)rows * 4);
     const size_t o_v = take((size_t)rows * LP_CAP * 8), o_i = take((size_t)rows * LP_CAP * 4);
     const int rc = q48_ws_reserve(c, o);
     if (rc)
