@@ -56,7 +56,7 @@ static __constant__ int64_t kLog[64] = {
     164958141293684LL, 167395169302662LL, 169811278358287LL, 172206824534353LL, 174582154889912LL,
     176937607771029LL, 179273513100022LL, 181590192652790LL, 183887960324830LL, 186167122386477LL,
     188427977727901LL, 190670818094329LL, 192895928311988LL};
-static __constant__ int64_t kInv[8] = {
+constexpr int64_t kInvK[8] = {
     281474976710656LL, 140737488355328LL, 93824992236885LL, 70368744177664LL, 56294995342131LL,
     46912496118443LL, 40210710958665LL, 35184372088832LL};
 
@@ -138,19 +138,23 @@ __device__ __forceinline__ void lp_terms(const uint64_t (&u)[N], const double *t
 #undef LP_EACH
 }
 
-// logZ of Z >= 2^48, and its b
-__device__ int64_t lp_log(q48_u128 Z, int &b)
+// logZ of Z >= 2^48, and its b; the Horner steps as in lp_terms, around 1.5 2^52 since
+// d may be a unit or two below 0
+__device__ __forceinline__ int64_t lp_log(q48_u128 Z, int &b)
 {
     const uint64_t zh = (uint64_t)(Z >> 64), zl = (uint64_t)Z;
     b = (zh ? 128 - __builtin_clzll(zh) : 64 - __builtin_clzll(zl)) - 49;
     const int64_t z = (int64_t)(Z >> b);
     const int j = (int)(z >> 42) - 64;
-    const int64_t d = q48_mul(z, kRcp[j]) - Q48_ONE;
-    int64_t g = kInv[7];
+    const int64_t rcp = kRcp[j], l = kLog[j];
+    const double M = 0x1.8p52, d = (double)(q48_mul(z, rcp) - Q48_ONE) * 0x1p-48;
+    double g = (double)kInvK[7];
 #pragma unroll
     for (int k = 6; k >= 0; --k)
-        g = kInv[k] - q48_mul(d, g);
-    return b * LP_LN2 + kLog[j] + q48_mul(d, g);
+        g = ((double)kInvK[k] + M) - __builtin_fma(d, g, M);
+    const int64_t log1p = __builtin_bit_cast(int64_t, __builtin_fma(d, g, M)) -
+                          __builtin_bit_cast(int64_t, M);
+    return b * LP_LN2 + l + log1p;
 }
 
 __device__ __forceinline__ int64_t lp_value(uint64_t u, int64_t logz)
@@ -186,9 +190,22 @@ __device__ __forceinline__ uint32_t lp_threshold(const uint32_t (&g)[N], int n)
     return t;
 }
 
+template <bool AGENT>
+__device__ __forceinline__ void lp_put(int64_t *cv, int *ci, int at, int64_t y, int i)
+{
+    if (AGENT) {
+        __hip_atomic_store(cv + at, y, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(ci + at, i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    } else {
+        cv[at] = y;
+        ci[at] = i;
+    }
+}
+
 // The candidates (high half >= thr) among the values first + k stride < end of the
 // threads whose maximum is one, appended to cv and ci: the wave reads such a thread's
 // values together, 64 at a time.
+template <bool AGENT>
 __device__ __forceinline__ void lp_collect(const int64_t *x, int first, int stride, int end,
                                            bool some, uint32_t thr, int64_t *cv, int *ci,
                                            int *count, int cap, int lane)
@@ -202,10 +219,8 @@ __device__ __forceinline__ void lp_collect(const int64_t *x, int first, int stri
             const int64_t y = x[i];
             if (lp_high(y) >= thr) {
                 const int at = atomicAdd(count, 1);
-                if (at < cap) {
-                    cv[at] = y;
-                    ci[at] = i;
-                }
+                if (at < cap)
+                    lp_put<AGENT>(cv, ci, at, y, i);
             }
         }
     }
@@ -298,15 +313,28 @@ __device__ void lp_select(const int64_t *x, int V, int64_t m, int64_t logz, int 
     }
 }
 
-// Sums of z and w over a wave, in exact 128 bits, as four words (lane 0).
+__device__ __forceinline__ void agent_store(uint64_t *p, uint64_t v)
+{
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename T>
+__device__ __forceinline__ T agent_load(const T *p)
+{
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Sums of z and w over a wave, in exact 128 bits, as four words (lanes 0 to 3).
+template <bool AGENT>
 __device__ __forceinline__ void lp_wave_sums(uint64_t z64, uint64_t w64, uint64_t *s, int lane)
 {
     const q48_u128 z = q48_wave_sum128(z64), w = q48_wave_sum128(w64);
-    if (lane == 0) {
-        s[0] = (uint64_t)z;
-        s[1] = (uint64_t)(z >> 64);
-        s[2] = (uint64_t)w;
-        s[3] = (uint64_t)(w >> 64);
+    const q48_u128 v = lane & 2 ? w : z;
+    const uint64_t word = (uint64_t)(lane & 1 ? v >> 64 : v);
+    if (lane < 4) {
+        if (AGENT)
+            agent_store(s + lane, word);
+        else
+            s[lane] = word;
     }
 }
 
@@ -410,7 +438,7 @@ __global__ __launch_bounds__(LR_NT) void k_lp_row(const int64_t *__restrict__ X,
             lp_terms<4>(u, tab, z64, w64);
             __builtin_amdgcn_sched_barrier(0);   // more terms would not fit the registers
         }
-        lp_wave_sums(z64, w64, sums[tid >> 6], lane);
+        lp_wave_sums<false>(z64, w64, sums[tid >> 6], lane);
         __syncthreads();
         if (tid < 64) {
             q48_u128 z = 0, w = 0;
@@ -424,7 +452,7 @@ __global__ __launch_bounds__(LR_NT) void k_lp_row(const int64_t *__restrict__ X,
         }
         if (!top)
             continue;   // (the next row's first barrier is behind its reads of v alone)
-        lp_collect(x, tid, LR_NT, V, tid < V && mine >= thr, thr, cv, ci, &count, LP_CAP, lane);
+        lp_collect<false>(x, tid, LR_NT, V, tid < V && mine >= thr, thr, cv, ci, &count, LP_CAP, lane);
         __syncthreads();
         if (count <= LP_CAP)
             lp_rank<LR_NT>(cv, ci, count, m, slogz, t, top, ids, tlp, tid);
@@ -436,13 +464,14 @@ __global__ __launch_bounds__(LR_NT) void k_lp_row(const int64_t *__restrict__ X,
 }
 
 // ---- a row over many blocks ------------------------------------------------------------
-// Three launches of (chunk, row) blocks, at most 64 chunks a row: the chunks' wave
-// maxima; sums and candidates; the row's results.
+// Two launches of (chunk, row) blocks, at most 64 chunks a row: the chunks' wave
+// maxima; then sums and candidates, which go out with agent-coherent stores ahead of
+// a ticket, and the row's last block makes its results (no block waits on another).
 
 struct LpWork {
     int64_t *gmax;     // [T][4 chunks]: a wave's maximum
     uint64_t *sums;    // [T][4 chunks][4]: a wave's z and w, 128 bits each
-    int *count;        // [T]
+    int *count;        // [T][2]: candidates, tickets
     int64_t *cv;       // [T][LP_CAP]
     int *ci;           // [T][LP_CAP]
     int chunks, ch;    // ch: values a chunk, a multiple of 256
@@ -460,24 +489,31 @@ __global__ __launch_bounds__(256) void k_lp_max(const int64_t *__restrict__ X, i
     m = q48_wave_max64(m);
     if ((tid & 63) == 0)
         p.gmax[(size_t)t * 4 * p.chunks + 4 * c + (tid >> 6)] = m;
-    if (c == 0 && tid == 0)
-        p.count[t] = 0;
+    if (c == 0 && tid < 2)
+        p.count[2 * t + tid] = 0;
 }
 
-__global__ __launch_bounds__(256) void k_lp_sum(const int64_t *__restrict__ X, int V, int top,
+__global__ __launch_bounds__(256) void k_lp_sum(const int64_t *__restrict__ X, int V,
+                                               const int *__restrict__ tokens,
+                                               int64_t *__restrict__ logp,
+                                               int64_t *__restrict__ entropy, int top,
+                                               int *__restrict__ ids, int64_t *__restrict__ tlp,
                                                LpWork p)
 {
     q48_round_down();
     __shared__ double tab[64];
+    __shared__ int64_t cv[LP_CAP], bv[4], slogz;
+    __shared__ int ci[LP_CAP], bi[4];
     __shared__ uint32_t thr;
+    __shared__ int last;
     const int t = blockIdx.y, c = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
     const int64_t *x = X + (size_t)t * V;
-    const int end = min(V, (c + 1) * p.ch);
+    const int end = min(V, (c + 1) * p.ch), groups = 4 * p.chunks;
     int64_t g[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int k = lane + 64 * i;
-        g[i] = k < 4 * p.chunks ? p.gmax[(size_t)t * 4 * p.chunks + k] : INT64_MIN;
+        g[i] = k < groups ? p.gmax[(size_t)t * groups + k] : INT64_MIN;
     }
     lp_table(tab, tid);
     int64_t m = g[0];
@@ -492,7 +528,7 @@ __global__ __launch_bounds__(256) void k_lp_sum(const int64_t *__restrict__ X, i
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int k = lane + 64 * i;
-            h[i] = k < 4 * p.chunks && (k >> 2) * p.ch + 64 * (k & 3) < V ? lp_high(g[i]) : 0;
+            h[i] = k < groups && (k >> 2) * p.ch + 64 * (k & 3) < V ? lp_high(g[i]) : 0;
         }
         const uint32_t n = lp_threshold<4>(h, top);
         if (tid == 0)
@@ -513,56 +549,45 @@ __global__ __launch_bounds__(256) void k_lp_sum(const int64_t *__restrict__ X, i
         const uint64_t u[1] = {(uint64_t)m - (uint64_t)x[i]};
         lp_terms<1>(u, tab, z64, w64);
     }
-    lp_wave_sums(z64, w64, p.sums + 4 * (4 * ((size_t)t * p.chunks + c) + (tid >> 6)), lane);
-    if (!top)
+    uint64_t *sums = p.sums + (size_t)t * groups * 4;
+    lp_wave_sums<true>(z64, w64, sums + 4 * (4 * c + (tid >> 6)), lane);
+    if (top) {
+        __syncthreads();   // the threshold
+        const int first = c * p.ch + tid;
+        lp_collect<true>(x, first, 256, end, first < end && lp_high(mine) >= thr, thr,
+                         p.cv + (size_t)t * LP_CAP, p.ci + (size_t)t * LP_CAP, p.count + 2 * t,
+                         LP_CAP, lane);
+    }
+    // every wave's stores are out before the block's ticket
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0)
+        last = __hip_atomic_fetch_add(p.count + 2 * t + 1, 1, __ATOMIC_RELAXED,
+                                      __HIP_MEMORY_SCOPE_AGENT) == p.chunks - 1;
+    __syncthreads();
+    if (!last)
         return;
-    __syncthreads();   // the threshold
-    const int first = c * p.ch + tid;
-    lp_collect(x, first, 256, end, first < end && lp_high(mine) >= thr, thr,
-               p.cv + (size_t)t * LP_CAP, p.ci + (size_t)t * LP_CAP, p.count + t, LP_CAP, lane);
-}
 
-__global__ __launch_bounds__(256) void k_lp_end(const int64_t *__restrict__ X, int V,
-                                               const int *__restrict__ tokens,
-                                               int64_t *__restrict__ logp,
-                                               int64_t *__restrict__ entropy, int top,
-                                               int *__restrict__ ids, int64_t *__restrict__ tlp,
-                                               LpWork p)
-{
-    q48_round_down();
-    __shared__ int64_t cv[LP_CAP], bv[4], slogz;
-    __shared__ int ci[LP_CAP], bi[4];
-    const int t = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-    const int64_t *x = X + (size_t)t * V;
-    int64_t m = INT64_MIN;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < 4 * p.chunks) {
-            const int64_t g = p.gmax[(size_t)t * 4 * p.chunks + lane + 64 * i];
-            m = g > m ? g : m;
-        }
-    // wave 0: the row's sums; the others: its candidates
-    const int count = top ? p.count[t] : 0;
+    // the row's last block.  Wave 0: the row's sums; the others: its candidates
+    const int count = top ? agent_load(p.count + 2 * t) : 0;
     if (tid < 64) {
         q48_u128 z = 0, w = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 64 * i < 4 * p.chunks) {
-                const uint64_t *s = p.sums + 4 * ((size_t)t * 4 * p.chunks + lane + 64 * i);
-                z += ((q48_u128)s[1] << 64) | s[0];
-                w += ((q48_u128)s[3] << 64) | s[2];
+        for (int k = 0; k < 4; ++k)
+            if (lane + 64 * k < groups) {
+                const uint64_t *s = sums + 4 * (lane + 64 * k);
+                z += ((q48_u128)agent_load(s + 1) << 64) | agent_load(s);
+                w += ((q48_u128)agent_load(s + 3) << 64) | agent_load(s + 2);
             }
-        m = q48_wave_max64(m);
         z = q48_wave_sum128(z);
         w = q48_wave_sum128(w);
         const int64_t logz = lp_finish(z, w, m, x, V, t, tokens, logp, entropy, tid == 0);
         if (tid == 0)
             slogz = logz;
     } else {
-        m = q48_wave_max64(m);
-        for (int i = tid - 64; i < min(count, LP_CAP); i += 192) {
-            cv[i] = p.cv[(size_t)t * LP_CAP + i];
-            ci[i] = p.ci[(size_t)t * LP_CAP + i];
+        for (int k = tid - 64; k < min(count, LP_CAP); k += 192) {
+            cv[k] = agent_load(p.cv + (size_t)t * LP_CAP + k);
+            ci[k] = agent_load(p.ci + (size_t)t * LP_CAP + k);
         }
     }
     if (!top)
@@ -586,7 +611,11 @@ int q48_logprobs_rows(q48_ctx *c, const int64_t *logits, int T, int vocab, const
         (top_n > 0 && (!top_ids || !top_logp)) || (!logp && !entropy && top_n == 0))
         return Q48_EINVAL;
     q48_on_device on(c);
-    if (vocab <= 32768 && (vocab <= 8192 || T >= 64)) {
+    // A block a row where the row fits its registers and there are rows for most compute
+    // units; else a row over many blocks.  us, a block a row / many: one row of 8000 10.2
+    // / 11.4; 64 rows of 16000 16.2 / 17, of 32000 26.1 / 19.4; 128 of 32000 27.5 / 26.8,
+    // 256 32.4 / 40.4.
+    if (vocab <= 8192 || (vocab <= 16384 && T >= 64) || (vocab <= 32768 && T >= 128)) {
 #define LP_ROW(R, PER)                                                                         \
     hipLaunchKernelGGL(k_lp_row<R>, dim3(T < PER * c->cu_count ? T : PER * c->cu_count),       \
                        dim3(LR_NT), 0, c->stream, logits, T, vocab, d_tokens, logp, entropy,   \
@@ -604,7 +633,12 @@ int q48_logprobs_rows(q48_ctx *c, const int64_t *logits, int T, int vocab, const
         return hipGetLastError() == hipSuccess ? Q48_OK : Q48_EHIP;
     }
     LpWork p = {};
-    p.ch = ((vocab + 63) / 64 + 255) & ~255;
+    // about a block a compute unit (two for long rows), 8 to 64 a row: the blocks of a
+    // row take turns at its ticket (us at 16 rows of 32000: 16 chunks a row 14.2, 32
+    // 16.4, 64 21.9; of 130000: 16 22.7, 32 21.4)
+    int want = (vocab > 65536 ? 2 : 1) * c->cu_count / T;
+    want = want < 8 ? 8 : want > 64 ? 64 : want;
+    p.ch = ((vocab + want - 1) / want + 255) & ~255;
     p.chunks = (vocab + p.ch - 1) / p.ch;
     size_t o = 0;
     auto take = [&](size_t bytes) {
@@ -615,7 +649,7 @@ int q48_logprobs_rows(q48_ctx *c, const int64_t *logits, int T, int vocab, const
     // rows of one launch: a grid's y, and a bounded workspace
     const int rows = T < 32768 ? T : 32768;
     const size_t o_g = take((size_t)rows * 4 * p.chunks * 8);
-    const size_t o_s = take((size_t)rows * 4 * p.chunks * 32), o_n = take((size_t)rows * 4);
+    const size_t o_s = take((size_t)rows * 4 * p.chunks * 32), o_n = take((size_t)rows * 8);
     const size_t o_v = take((size_t)rows * LP_CAP * 8), o_i = take((size_t)rows * LP_CAP * 4);
     const int rc = q48_ws_reserve(c, o);
     if (rc)
@@ -630,9 +664,7 @@ int q48_logprobs_rows(q48_ctx *c, const int64_t *logits, int T, int vocab, const
         const int n = rows < T - t0 ? rows : T - t0;
         const int64_t *x = logits + (size_t)t0 * vocab;
         hipLaunchKernelGGL(k_lp_max, dim3(p.chunks, n), dim3(256), 0, c->stream, x, vocab, p);
-        hipLaunchKernelGGL(k_lp_sum, dim3(p.chunks, n), dim3(256), 0, c->stream, x, vocab, top_n,
-                           p);
-        hipLaunchKernelGGL(k_lp_end, dim3(n), dim3(256), 0, c->stream, x, vocab,
+        hipLaunchKernelGGL(k_lp_sum, dim3(p.chunks, n), dim3(256), 0, c->stream, x, vocab,
                            d_tokens ? d_tokens + t0 : nullptr, logp ? logp + t0 : nullptr,
                            entropy ? entropy + t0 : nullptr, top_n,
                            top_ids ? top_ids + (size_t)t0 * top_n : nullptr,

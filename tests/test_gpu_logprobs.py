@@ -65,28 +65,55 @@ def test_a_large_vocabulary(ctx):
     check_rows(ctx, logits(rng, 2, 151937), [151936, 0], 20)
 
 
-def edges():
+def batch(rng, T, V):
+    """T rows of V logits that are eight rows over and over, and what they give."""
+    x = logits(rng, 8, V)
+    return np.tile(x, (T // 8 + 1, 1))[:T], lambda tokens, top: [
+        np.tile(w, (T // 8 + 1,) + (1,) * (w.ndim - 1))[:T] for w in P.logprobs(x, tokens, top)]
+
+
+@pytest.mark.parametrize("T,V", [(600, 3000), (300, 8192), (70, 12000), (300, 16384), (20, 12000),
+                                 (140, 20000), (600, 32768), (130, 32767), (40, 32769),
+                                 (9, 70001)])
+def test_many_rows(ctx, T, V):
+    """More rows than a launch's blocks, and every form's largest row."""
+    rng = np.random.default_rng(T + V)
+    x, want = batch(rng, T, V)
+    tokens = rng.integers(0, V, 8)
+    d, tk = ctx.to_device(x), ints(ctx, np.tile(tokens, T // 8 + 1)[:T])
+    logp, ent, ids, tlp = ctx.buffer(T), ctx.buffer(T), ctx.buffer(T * 9), ctx.buffer(T * 9)
+    ctx.logprobs_rows(d.ptr, T, V, tk.ptr, logp.ptr, ent.ptr, 9, ids.ptr, tlp.ptr)
+    w = want(tokens, 9)
+    assert (logp.download() == w[0]).all() and (ent.download() == w[1]).all()
+    assert (ids.download().view(np.int32)[:T * 9].reshape(T, 9) == w[2]).all()
+    assert (tlp.download().reshape(T, 9) == w[3]).all()
+    for b in (d, tk, logp, ent, ids, tlp):
+        b.free()
+
+
+def edges(width=300):
     rng = np.random.default_rng(0)
-    x = logits(rng, 12, 300)
+    x = logits(rng, 12, width)
     x[0] = 0                                  # all the same: ties to the lowest id
     x[1] = I64.min                            # the type's lowest value everywhere
     x[2, ::2] = I64.min                       # and as a mask
     x[3, 7], x[3, 8] = I64.max, I64.min       # u past 63 bits: the smallest log probability
     x[4] = -1
-    x[4, 299] = 0                             # the last id alone
+    x[4, -1] = 0                             # the last id alone
     x[5] >>= 40
     x[6, 3:9] = x[6].max() + 5                # ties at the top
-    x[7] = np.arange(300) * (P.LN2 // 3)      # u at multiples of LN2
-    x[8] = -np.arange(300) * (1 << 42)        # and of the table's step
-    x[9] = I64.max - np.arange(300)
-    x[10] = np.where(np.arange(300) == 40, 0, -(45 << 48))   # e below 2^-48 but one
+    x[7] = np.arange(width) % 400 * (P.LN2 // 3)      # u at multiples of LN2
+    x[8] = -(np.arange(width) % 4000) * (1 << 42)     # and of the table's step
+    x[9] = I64.max - np.arange(width)
+    x[10] = np.where(np.arange(width) == 40, 0, -(45 << 48))   # e below 2^-48 but one
     x[11] *= 40
     return x
 
 
 @pytest.mark.parametrize("top", [0, 3, 32])
-def test_edges(ctx, top):
-    x = edges()
+@pytest.mark.parametrize("width", [300, 9000])
+def test_edges(ctx, top, width):
+    x = edges(width)
     tokens = np.arange(12) * 24 + 8
     tokens[3] = 8
     check_rows(ctx, x, tokens, top)
