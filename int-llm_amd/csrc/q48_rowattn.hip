@@ -94,7 +94,7 @@ __device__ __forceinline__ int64_t row16_max64(int64_t v)
 // head kh G + g), taken in tiles of up to 16 (the rows of one MFMA tile).  Two
 // forms of the same phases:
 //  - one launch: a block takes a tile over all its rows, scores in LDS (k_ra_tile);
-//  - three launches over (chunk of ch rows, tile of 16, KV head) blocks with the
+//  - three launches over (chunk of rows, tile of 16, KV head) blocks with the
 //    scores in the workspace (k_ra_score, k_ra_exp, k_ra_value), for spans past
 //    LDS and where the tiles alone leave compute units idle.  The softmax of the
 //    exact path needs the row's maximum before the first exponential and the whole
@@ -102,12 +102,13 @@ __device__ __forceinline__ int64_t row16_max64(int64_t v)
 //    later, so each of the two is a launch boundary.
 struct RaPlan {
     int64_t *sc;     // [n_kv][16 tiles][spad]: scores, then exponentials
-    int64_t *cm;     // [n_kv][16 tiles][nchunk]: a chunk's maximum
-    uint64_t *cs;    // [n_kv][16 tiles][nchunk]: a chunk's sum of exponentials
-    int *far;        // [n_kv][tiles][nchunk]: a visible score outside [-2^62, 2^62)
-    int *odd;        // [n_kv][tiles][nchunk]: an exponential outside [0, ONE]
-    int ch, nchunk, spad, tiles, t0, Tn;   // rows t0 .. t0 + Tn - 1 of the T
-    int vb;          // vectors a tile
+    int64_t *cm;     // [n_kv][16 tiles][n1]: a chunk's maximum
+    uint64_t *cs;    // [n_kv][16 tiles][n2]: a chunk's sum of exponentials
+    int *far;        // [n_kv][tiles][n1]: a visible score outside [-2^62, 2^62)
+    int *odd;        // [n_kv][tiles][n2]: an exponential outside [0, ONE]
+    int ch1, n1, ch2, n2, ch3, n3;   // rows a chunk, and chunks, of each launch
+    int spad, tiles, t0, Tn;         // rows t0 .. t0 + Tn - 1 of the T
+    int vb;                          // vectors a tile
 };
 
 // rows [0, span) hold all that vectors up to vlast may see
@@ -348,36 +349,77 @@ __device__ __forceinline__ q48_u128 key_digits(v4i (&B)[HD < 64 ? 1 : HD / 64][8
     return ck * kDig - (q48_u128)kDig * kDig * (q48_u128)HD;
 }
 
+// The 63 digit products by the weight of their sum, 256^d: two chains at a time, and
+// each sum joins the score as soon as it is whole, so that two of the 14 are live
+// instead of all (206 -> 140 registers with HD 64: three waves a SIMD).
 template <int HD>
 __device__ __forceinline__ void word_scores(int64_t (&s)[4], const v4i (*dig)[8][64],
                                             const v4i (&B)[HD < 64 ? 1 : HD / 64][8],
                                             const q48_u128 *cq, q48_u128 ck, int lane, int nrow)
 {
     constexpr int KS = HD < 64 ? 1 : HD / 64;
-    v4i acc[14];
-#pragma unroll
-    for (int d = 0; d < 14; ++d)
-        acc[d] = (v4i){0, 0, 0, 0};
+    v4i A[KS][8];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-            const v4i A = dig[ks][x][lane];
+        for (int x = 0; x < 8; ++x)
+            A[ks][x] = dig[ks][x][lane];
+    uint32_t c[4][4], w1[4], w2[4];
+    int64_t cur[4];
 #pragma unroll
-            for (int y = 0; y < 8; ++y)
-                if (x + y <= 13)
-                    acc[x + y] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A, B[ks][y], acc[x + y], 0,
-                                                                      0, 0);
+    for (int i = 0; i < 4; ++i) {
+        const int m = 4 * (lane >> 4) + i;
+        q48_u128 t = cq[m] + ck;
+        if (KS == 2)
+            t += cq[16 + m];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            c[i][k] = (uint32_t)(t >> (32 * k));
+        cur[i] = (int64_t)c[i][0];
+    }
+    v4i acc[2][2];
+#pragma unroll
+    for (int d = 0; d < 16; d += 2) {
+        // the products of this pair of weights, under the last pair's sums
+        v4i(&now)[2] = acc[d / 2 & 1];
+        if (d < 14) {
+            now[0] = now[1] = (v4i){0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if (d + e - x >= 0 && d + e - x < 8)
+                            now[e] = __builtin_amdgcn_mfma_i32_16x16x64_i8(
+                                A[ks][x], B[ks][d + e - x], now[e], 0, 0, 0);
         }
+        if (d > 0) {
+            const v4i(&was)[2] = acc[d / 2 - 1 & 1];
+            const int k = d - 2;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (k == 4 || k == 8 || k == 12) {   // bits 8 k on, with the carry
+                    if (k == 8)
+                        w1[i] = (uint32_t)cur[i];
+                    if (k == 12)
+                        w2[i] = (uint32_t)cur[i];
+                    cur[i] = (cur[i] >> 32) + (int64_t)c[i][k / 4];
+                }
+                // |was| <= 8 KS 64 128 128 = 2^24: two join in 64 bits first
+                const int64_t two = mad_shl<8>(was[1][i], (int64_t)was[0][i]);
+                cur[i] = (k & 2) ? (int64_t)((uint64_t)cur[i] + ((uint64_t)two << 16))
+                                 : cur[i] + two;
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (i == 0 || i < nrow) {
-            const int m = 4 * (lane >> 4) + i;
-            q48_u128 c = cq[m] + ck;
-            if (KS == 2)
-                c += cq[16 + m];
-            s[i] = digits_shr48(acc, i, c);
-        }
+        if (i == 0 || i < nrow)
+            s[i] = (int64_t)(((uint64_t)__builtin_amdgcn_alignbit((uint32_t)cur[i], w2[i], 16)
+                              << 32) |
+                             __builtin_amdgcn_alignbit(w2[i], w1[i], 16));
 }
 
 // Scores of TB tiles (vectors v0 .. of 16 each) over rows [begin, end), 16 rows a
@@ -422,9 +464,9 @@ __device__ __forceinline__ void score_rows(const RaArgs &a, const v4i (*dig)[HD 
             if (tb >= ntile)
                 break;
             int64_t s[4];
-            if constexpr (BITS == 64)
+            if constexpr (BITS == 64) {
                 word_scores<HD>(s, dig[tb], B, cq[tb], ck, lane, nrow);
-            else
+            } else
                 code_scores<HD>(s, dig[tb], C, c0, c1, step, lane, nrow);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -490,40 +532,47 @@ struct ValueRows {
         for (int n = 0; n < 16; ++n)
             off[n] = (uint32_t)(vp + n) * (uint32_t)(a.n_kv * RB) + at;
     }
-    // The values of rows j + vp + n (past last: that row's); j is the wave's.  int64
-    // words gather their range in big.  rl: the lane's place in its row of 16.  fresh
-    // (or null): the codes and the step of row last, which the cache may not hold yet.
-    __device__ __forceinline__ void load(double (&v)[DL][16], const RaArgs &a, int kh, int j,
-                                         int last, int rl, uint32_t &big,
-                                         const uint8_t *fresh = nullptr, int64_t fresh_step = 0)
+    // The values of rows j + vp + n (past last: that row's), on their way; j is the
+    // wave's.  rl: the lane's place in its row of 16.
+    int64_t x[BITS == 64 ? DL : 1][BITS == 64 ? 16 : 1];
+    int b[BITS == 64 ? 1 : 16], b2[BITS == 8 && HD == 128 ? 16 : 1];
+    int64_t step;
+    __device__ __forceinline__ void fetch(const RaArgs &a, int kh, int j, int last, int rl)
     {
         const uint8_t *g = base + (size_t)j * (size_t)(a.n_kv * RB);
-        const bool tail = j + CP - 1 > last;
-        if (tail)   // the wave's last group: the offsets are not used again
+        if (j + CP - 1 > last)   // the wave's last group: the offsets are not used again
 #pragma unroll
             for (int n = 0; n < 16; ++n)
                 off[n] = (uint32_t)min(vp + n, last - j) * (uint32_t)(a.n_kv * RB) + at;
         if constexpr (BITS == 64) {
-            int64_t x[DL][16];
 #pragma unroll
             for (int n = 0; n < 16; ++n)
 #pragma unroll
                 for (int l = 0; l < DL; ++l)
                     x[l][n] = *reinterpret_cast<const int64_t *>(g + off[n] + 512 * l);
+        } else {
+#pragma unroll
+            for (int n = 0; n < 16; ++n) {
+                b[n] = (int8_t)g[off[n]];
+                if constexpr (BITS == 8 && HD == 128)
+                    b2[n] = (int8_t)g[off[n] + 64];
+            }
+            step = a.vs[(size_t)min(j + vp + rl, last) * a.n_kv + kh];
+        }
+    }
+    // What was fetched, as doubles; int64 words gather their range in big.  fresh (or
+    // null): the codes and the step of row last, which the cache may not hold yet.
+    __device__ __forceinline__ void take(double (&v)[DL][16], int j, int last, int rl,
+                                         uint32_t &big, const uint8_t *fresh = nullptr,
+                                         int64_t fresh_step = 0)
+    {
+        if constexpr (BITS == 64) {
 #pragma unroll
             for (int n = 0; n < 16; ++n)
 #pragma unroll
                 for (int l = 0; l < DL; ++l)
                     v[l][n] = q48_f51(x[l][n], big);
         } else {
-            int b[16], b2[16];
-#pragma unroll
-            for (int n = 0; n < 16; ++n) {
-                b[n] = (int8_t)g[off[n]];
-                if (BITS == 8 && HD == 128)
-                    b2[n] = (int8_t)g[off[n] + 64];
-            }
-            int64_t step = a.vs[(size_t)min(j + vp + rl, last) * a.n_kv + kh];
             if (fresh && j + CP - 1 >= last) {
                 if (j + vp + rl >= last)
                     step = fresh_step;
@@ -531,7 +580,7 @@ struct ValueRows {
                 for (int n = 0; n < 16; ++n)
                     if (j + vp + n == last) {
                         b[n] = (int8_t)fresh[at];
-                        if (BITS == 8 && HD == 128)
+                        if constexpr (BITS == 8 && HD == 128)
                             b2[n] = (int8_t)fresh[at + 64];
                     }
             }
@@ -545,8 +594,12 @@ struct ValueRows {
             scale16(v[0], c, st);
             if constexpr (DL == 2) {
 #pragma unroll
-                for (int n = 0; n < 16; ++n)
-                    c[n] = (double)(BITS == 8 ? b2[n] : b[n] >> 4);
+                for (int n = 0; n < 16; ++n) {
+                    if constexpr (BITS == 8)
+                        c[n] = (double)b2[n];
+                    else
+                        c[n] = (double)(b[n] >> 4);
+                }
                 scale16(v[1], c, st);
             }
         }
@@ -859,10 +912,18 @@ __global__ __launch_bounds__(RT_NT) void k_ra_tile(RaArgs a, RaPlan p)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
                 acc[l][r] = Q48_FSUM0;
+        // the next rows' values on their way under the sums, where the registers allow
+        constexpr bool AHEAD = BITS != 64 && RT_NT == 512;
+        if (AHEAD && CP * w < S)
+            rows.fetch(a, kh, CP * w, S - 1, rl);
         for (int j0 = CP * w; j0 < S; j0 += RT_NW * CP) {
             double v[HD == 128 ? 2 : 1][16];
-            rows.load(v, a, kh, j0, S - 1, rl, big, DEC && BITS != 64 ? nk[1] : nullptr,
+            if (!AHEAD)
+                rows.fetch(a, kh, j0, S - 1, rl);
+            rows.take(v, j0, S - 1, rl, big, DEC && BITS != 64 ? nk[1] : nullptr,
                       DEC && BITS != 64 ? nst[1] : 0);
+            if (AHEAD && j0 + RT_NW * CP < S)
+                rows.fetch(a, kh, j0 + RT_NW * CP, S - 1, rl);
             add_values<HD>(acc, v, nrow, [&](int r) {
                 if (r >= nrow)
                     return 0.0;
@@ -893,7 +954,8 @@ __global__ __launch_bounds__(RT_NT) void k_ra_tile(RaArgs a, RaPlan p)
 // over the rows it sees: a row's operand is made once for all TB tiles.  DEC: the
 // store of the new row too (by the blocks that own it).
 template <int BITS, int HD, int TB, bool DEC>
-__global__ __launch_bounds__(256) void k_ra_score(RaArgs a, RaPlan p)
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void
+k_ra_score(RaArgs a, RaPlan p)
 {
     q48_round_down();
     constexpr int KS = HD < 64 ? 1 : HD / 64;
@@ -913,9 +975,9 @@ __global__ __launch_bounds__(256) void k_ra_score(RaArgs a, RaPlan p)
     int p0;
     if (!position<DEC>(a, p0))
         return;
-    const int begin = (int)blockIdx.x * p.ch;
+    const int begin = (int)blockIdx.x * p.ch1;
     const int end =
-        min(begin + p.ch, tile_span<DEC>(a, p, 16 * (tile0 + ntile) - 1, G, p0));
+        min(begin + p.ch1, tile_span<DEC>(a, p, 16 * (tile0 + ntile) - 1, G, p0));
     if (begin >= end)
         return;
 
@@ -934,7 +996,7 @@ __global__ __launch_bounds__(256) void k_ra_score(RaArgs a, RaPlan p)
         __syncthreads();
     }
     // a.out of these tiles' vectors, for the sums that the chunks add
-    if (p.nchunk > 1 && blockIdx.x == 0)
+    if (p.n3 > 1 && blockIdx.x == 0)
         for (int i = tid; i < ntile * 16 * HD; i += 256) {
             const int v = 16 * tile0 + i / HD;
             if (v < NV)
@@ -978,10 +1040,10 @@ __global__ __launch_bounds__(256) void k_ra_score(RaArgs a, RaPlan p)
 #pragma unroll
         for (int u = 1; u < 4; ++u)
             m = mxs[u][tid] > m ? mxs[u][tid] : m;
-        p.cm[(((size_t)kh * p.tiles + tile0) * 16 + tid) * p.nchunk + blockIdx.x] = m;
+        p.cm[(((size_t)kh * p.tiles + tile0) * 16 + tid) * p.n1 + blockIdx.x] = m;
     }
     if (tid < ntile)
-        p.far[((size_t)kh * p.tiles + tile0 + tid) * p.nchunk + blockIdx.x] = farw[tid];
+        p.far[((size_t)kh * p.tiles + tile0 + tid) * p.n1 + blockIdx.x] = farw[tid];
 }
 
 // Exponentials in place of a chunk's scores (0 for rows a vector does not see,
@@ -997,24 +1059,24 @@ __global__ __launch_bounds__(256) void k_ra_exp(RaArgs a, RaPlan p)
     if (!position<DEC>(a, p0))
         return;
     const int span = tile_span<DEC>(a, p, 16 * tile + 15, G, p0);
-    const int begin = (int)blockIdx.x * p.ch, end = min(begin + p.ch, span);
+    const int begin = (int)blockIdx.x * p.ch2, end = min(begin + p.ch2, span);
     if (begin >= end)
         return;
     if (tid == 0)
         odds = 0;
     __syncthreads();
-    const int chunks = (span + p.ch - 1) / p.ch;
+    const int chunks = (span + p.ch1 - 1) / p.ch1;
     // lanes of a vector: 16, or 32 or 64 where the tile has few vectors
     const int lg = nrow > 8 ? 4 : nrow > 4 ? 5 : 6, L = 1 << lg;
     const int r = tid >> lg, l = tid & (L - 1);
-    const int *farp = p.far + ((size_t)kh * p.tiles + tile) * p.nchunk;
+    const int *farp = p.far + ((size_t)kh * p.tiles + tile) * p.n1;
     int far = 0;
     for (int c = l; c < chunks; c += L)
         far |= farp[c];
     far = __any(far);
     if (r < nrow) {
         const size_t vec = ((size_t)kh * p.tiles + tile) * 16 + r;
-        const int64_t *cm = p.cm + vec * p.nchunk;
+        const int64_t *cm = p.cm + vec * p.n1;
         int64_t m = INT64_MIN;
         for (int c = l; c < chunks; c += L)
             m = cm[c] > m ? cm[c] : m;
@@ -1026,18 +1088,18 @@ __global__ __launch_bounds__(256) void k_ra_exp(RaArgs a, RaPlan p)
         const int t = p.t0 + (16 * tile + r) / G;
         int odd = 0;
         uint64_t sum = exp_rows<DEC>(a, p0, t, p.sc + vec * p.spad, m, far, begin, end,
-                                     min(begin + p.ch, (end + 31) & ~31), l, L, odd);
+                                     min(begin + p.ch2, (end + 31) & ~31), l, L, odd);
         sum = group_sum64<16>(sum);
         for (int o = 16; o < L; o <<= 1)
             sum += __shfl_xor(sum, o);
         if (l == 0)
-            p.cs[vec * p.nchunk + blockIdx.x] = sum;
+            p.cs[vec * p.n2 + blockIdx.x] = sum;
         if (odd)
             atomicOr(&odds, 1);
     }
     __syncthreads();
     if (tid == 0)
-        p.odd[((size_t)kh * p.tiles + tile) * p.nchunk + blockIdx.x] = odds;
+        p.odd[((size_t)kh * p.tiles + tile) * p.n2 + blockIdx.x] = odds;
 }
 
 // The values of a chunk under its weights, added to out.  Wave w takes the
@@ -1063,10 +1125,10 @@ k_ra_value(RaArgs a, RaPlan p)
     if (!position<DEC>(a, p0))
         return;
     const int span = tile_span<DEC>(a, p, 16 * tile + 15, G, p0);
-    const int begin = (int)blockIdx.x * p.ch, end = min(begin + p.ch, span);
+    const int begin = (int)blockIdx.x * p.ch3, end = min(begin + p.ch3, span);
     if (begin >= end)
         return;
-    const int chunks = (span + p.ch - 1) / p.ch;
+    const int chunks = (span + p.ch2 - 1) / p.ch2;
     const size_t vec0 = ((size_t)kh * p.tiles + tile) * 16;
     const int64_t *sc = p.sc + vec0 * p.spad;
     {
@@ -1074,7 +1136,7 @@ k_ra_value(RaArgs a, RaPlan p)
         uint64_t s = 0;
         if (r < nrow)
             for (int c = l; c < chunks; c += 16)
-                s += p.cs[(vec0 + r) * p.nchunk + c];
+                s += p.cs[(vec0 + r) * p.n2 + c];
         s = group_sum64<16>(s);
         if (l == 0)
             dens[r] = s;
@@ -1083,7 +1145,7 @@ k_ra_value(RaArgs a, RaPlan p)
         (&lam[0][0])[i] = 0;
     int slow = 0;
     for (int c = tid; c < chunks; c += 256)
-        slow |= p.odd[((size_t)kh * p.tiles + tile) * p.nchunk + c];
+        slow |= p.odd[((size_t)kh * p.tiles + tile) * p.n2 + c];
     if constexpr (BITS != 64)
         for (int j = begin + tid; j < end; j += 256)
             slow |= !step_fits<BITS>(a.vs[(size_t)j * a.n_kv + kh]);
@@ -1114,11 +1176,19 @@ k_ra_value(RaArgs a, RaPlan p)
                     for (int u = 0; u < PG; ++u)
                         er[PG * i + u] = (uint64_t)sc[(size_t)(4 * i + g) * p.spad + j0 + 16 * u + rl];
         };
-        if (begin + CP * w < end)
+        constexpr bool AHEAD = BITS != 64;   // (registers)
+        if (begin + CP * w < end) {
             load_e(begin + CP * w);
+            if (AHEAD)
+                rows.fetch(a, kh, begin + CP * w, end - 1, rl);
+        }
         for (int j0 = begin + CP * w; j0 < end; j0 += 4 * CP) {
             double v[DL][16];
-            rows.load(v, a, kh, j0, end - 1, rl, big);
+            if (!AHEAD)
+                rows.fetch(a, kh, j0, end - 1, rl);
+            rows.take(v, j0, end - 1, rl, big);
+            if (AHEAD && j0 + 4 * CP < end)
+                rows.fetch(a, kh, j0 + 4 * CP, end - 1, rl);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (4 * i < nrow)
@@ -1155,7 +1225,7 @@ k_ra_value(RaArgs a, RaPlan p)
                                                                begin, end)
                                 : lam[r][d];
         int64_t *out = out_at<HD>(a, p, 16 * tile + r, G, kh) + d;
-        if (p.nchunk > 1)
+        if (p.n3 > 1)
             atomicAdd(reinterpret_cast<unsigned long long *>(out), (unsigned long long)o);
         else
             *out = (int64_t)o;
@@ -1241,21 +1311,35 @@ int launch_hd(q48_ctx *c, RaArgs &a)
     int Tn = (int)(RA_WS_MAX / row_bytes);
     Tn = Tn < 1 ? 1 : Tn < a.T ? Tn : a.T;
     p.tiles = (Tn * G + 15) / 16;
-    // chunks for about 512 blocks, of 64 rows at least
-    const long blocks = (long)p.tiles * a.n_kv;
-    int n = (int)(blocks >= 512 ? 1 : (512 + blocks - 1) / blocks);
-    n = n < p.spad / 64 ? n : p.spad / 64;
-    p.ch = ((S + n - 1) / n + 63) & ~63;
-    p.nchunk = (S + p.ch - 1) / p.ch;
+    const long tiles = (long)p.tiles * a.n_kv;
+    constexpr int TB = DEC ? 1 : BITS == 64 && HD < 128 ? 4 : 2;
+    // Chunks for about `want` blocks, of 64 rows at least, 128 past 4096: a later launch's
+    // blocks read every chunk's maximum or sum, and the values' sums of all chunks meet in
+    // atomics.
+    // us of 48 tokens at 4000 (int64) with 512 / 1024 score blocks 146 / 132, with 512 /
+    // 2048 exponential blocks 146 / 137, with 512 / 1024 value blocks 146 / 147; of 26 at
+    // 2047 (8 bits) 45 / 46, 45 / 43, 45 / 51; of one at 16000 with chunks of 128 / 64
+    // rows 27 / 30 (any of the three).
+    auto chunk = [&](long blocks, long want, int &ch, int &n) {
+        long k = want / blocks, most = p.spad / (S > 4096 ? 128 : 64);
+        k = k < most ? k : most;
+        k = k < 1 ? 1 : k;
+        ch = (int)(((S + k - 1) / k + 63) & ~63);
+        n = (S + ch - 1) / ch;
+    };
+    chunk((tiles + TB - 1) / TB, BITS == 64 ? 1024 : 512, p.ch1, p.n1);
+    chunk(tiles, 2048, p.ch2, p.n2);
+    chunk(tiles, 512, p.ch3, p.n3);
     size_t o = 0;
     auto take = [&](size_t bytes) {
         const size_t at = o;
         o += (bytes + 255) & ~(size_t)255;
         return at;
     };
-    const size_t vecs = (size_t)a.n_kv * p.tiles * 16, ft = (size_t)a.n_kv * p.tiles * p.nchunk;
-    const size_t o_sc = take(vecs * p.spad * 8), o_cm = take(vecs * p.nchunk * 8);
-    const size_t o_cs = take(vecs * p.nchunk * 8), o_far = take(ft * 4), o_odd = take(ft * 4);
+    const size_t vecs = (size_t)a.n_kv * p.tiles * 16;
+    const size_t o_sc = take(vecs * p.spad * 8), o_cm = take(vecs * p.n1 * 8);
+    const size_t o_cs = take(vecs * p.n2 * 8);
+    const size_t o_far = take(tiles * p.n1 * 4), o_odd = take(tiles * p.n2 * 4);
     int rc = q48_ws_reserve(c, o);
     if (rc)
         return rc;
@@ -1265,16 +1349,14 @@ int launch_hd(q48_ctx *c, RaArgs &a)
     p.cs = (uint64_t *)(ws + o_cs);
     p.far = (int *)(ws + o_far);
     p.odd = (int *)(ws + o_odd);
-    constexpr int TB = DEC ? 1 : BITS == 64 ? 4 : 2;
     for (p.t0 = 0; p.t0 < a.T; p.t0 += Tn) {
         p.Tn = Tn < a.T - p.t0 ? Tn : a.T - p.t0;
-        const int tiles = (p.Tn * G + 15) / 16;
-        const dim3 grid(p.nchunk, tiles, a.n_kv);
+        const int nt = (p.Tn * G + 15) / 16;
         hipLaunchKernelGGL((k_ra_score<BITS, HD, TB, DEC>),
-                           dim3(p.nchunk, (tiles + TB - 1) / TB, a.n_kv), dim3(256), 0, c->stream,
-                           a, p);
-        hipLaunchKernelGGL((k_ra_exp<DEC>), grid, dim3(256), 0, c->stream, a, p);
-        hipLaunchKernelGGL((k_ra_value<BITS, HD, DEC>), grid, dim3(256), 0, c->stream, a, p);
+                           dim3(p.n1, (nt + TB - 1) / TB, a.n_kv), dim3(256), 0, c->stream, a, p);
+        hipLaunchKernelGGL((k_ra_exp<DEC>), dim3(p.n2, nt, a.n_kv), dim3(256), 0, c->stream, a, p);
+        hipLaunchKernelGGL((k_ra_value<BITS, HD, DEC>), dim3(p.n3, nt, a.n_kv), dim3(256), 0,
+                           c->stream, a, p);
     }
     return hipGetLastError() == hipSuccess ? Q48_OK : Q48_EHIP;
 }
