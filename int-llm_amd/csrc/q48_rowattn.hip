@@ -142,6 +142,19 @@ __device__ __forceinline__ bool sees(const RaArgs &a, int p0, int t, int j)
     return j - p0 <= t;
 }
 
+// whether any of the rows t0 .. t1 sees cache row j: a row that none sees (padding
+// that was never stored) may hold anything
+template <bool DEC>
+__device__ __forceinline__ bool seen(const RaArgs &a, int p0, int t0, int t1, int j)
+{
+    if (DEC || j < p0 || !a.mask)
+        return true;
+    bool any = false;
+    for (int t = t0; t <= t1; ++t)
+        any |= sees<DEC>(a, p0, t, j);
+    return any;
+}
+
 template <bool DEC>
 __device__ __forceinline__ bool position(const RaArgs &a, int &p0)
 {
@@ -883,7 +896,7 @@ __global__ __launch_bounds__(RT_NT) void k_ra_tile(RaArgs a, RaPlan p)
     if constexpr (BITS != 64)
         for (int j = tid; j < S; j += RT_NT) {
             const int64_t st = DEC && j == p0 ? nst[1] : a.vs[(size_t)j * a.n_kv + kh];
-            odd |= !step_fits<BITS>(st);
+            odd |= !step_fits<BITS>(st) && seen<DEC>(a, p0, vt[0], vt[nrow - 1], j);
         }
     const bool slow = __syncthreads_or(odd);
     auto total = [&](int r) {
@@ -1064,31 +1077,51 @@ __global__ __launch_bounds__(256) void k_ra_exp(RaArgs a, RaPlan p)
         return;
     if (tid == 0)
         odds = 0;
-    __syncthreads();
     const int chunks = (span + p.ch1 - 1) / p.ch1;
     // lanes of a vector: 16, or 32 or 64 where the tile has few vectors
     const int lg = nrow > 8 ? 4 : nrow > 4 ? 5 : 6, L = 1 << lg;
     const int r = tid >> lg, l = tid & (L - 1);
+    const size_t vec = ((size_t)kh * p.tiles + tile) * 16 + min(r, nrow - 1);
     const int *farp = p.far + ((size_t)kh * p.tiles + tile) * p.n1;
+    const int64_t *cm = p.cm + vec * p.n1;
+    int64_t *sc = p.sc + vec * p.spad;
+    // the lane's first scores on their way while the maximum is found
+    int64_t ahead[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        ahead[i] = sc[min(begin + l + i * L, end - 1)];
     int far = 0;
-    for (int c = l; c < chunks; c += L)
+    int64_t m = INT64_MIN;
+    for (int c = l; c < chunks; c += L) {
         far |= farp[c];
+        m = cm[c] > m ? cm[c] : m;
+    }
     far = __any(far);
+    m = row16_max64(m);
+    for (int o = 16; o < L; o <<= 1) {
+        const int64_t x = __shfl_xor(m, o);
+        m = x > m ? x : m;
+    }
+    __syncthreads();   // odds
     if (r < nrow) {
-        const size_t vec = ((size_t)kh * p.tiles + tile) * 16 + r;
-        const int64_t *cm = p.cm + vec * p.n1;
-        int64_t m = INT64_MIN;
-        for (int c = l; c < chunks; c += L)
-            m = cm[c] > m ? cm[c] : m;
-        m = row16_max64(m);
-        for (int o = 16; o < L; o <<= 1) {
-            const int64_t x = __shfl_xor(m, o);
-            m = x > m ? x : m;
-        }
         const int t = p.t0 + (16 * tile + r) / G;
+        const int fill = min(begin + p.ch2, (end + 31) & ~31);
+        const int clear = far ? begin : min(end, rows_clear<DEC>(a, p0, t));
         int odd = 0;
-        uint64_t sum = exp_rows<DEC>(a, p0, t, p.sc + vec * p.spad, m, far, begin, end,
-                                     min(begin + p.ch2, (end + 31) & ~31), l, L, odd);
+        uint64_t sum = 0;
+        int from = begin;
+        if (begin + 4 * L <= clear) {
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                const uint64_t e0 = exp_neg((uint64_t)m - (uint64_t)ahead[i]);
+                const uint64_t e1 = exp_neg((uint64_t)m - (uint64_t)ahead[i + 1]);
+                sc[begin + l + i * L] = (int64_t)e0;
+                sc[begin + l + (i + 1) * L] = (int64_t)e1;
+                sum += e0 + e1;
+            }
+            from = begin + 4 * L;
+        }
+        sum += exp_rows<DEC>(a, p0, t, sc, m, far, from, end, fill, l, L, odd);
         sum = group_sum64<16>(sum);
         for (int o = 16; o < L; o <<= 1)
             sum += __shfl_xor(sum, o);
@@ -1131,6 +1164,23 @@ k_ra_value(RaArgs a, RaPlan p)
     const int chunks = (span + p.ch2 - 1) / p.ch2;
     const size_t vec0 = ((size_t)kh * p.tiles + tile) * 16;
     const int64_t *sc = p.sc + vec0 * p.spad;
+    // the wave's first exponentials and values on their way while the sums are joined
+    ValueRows<BITS, HD> rows(a, kh, lane);
+    uint64_t er[4 * PG];
+    auto load_e = [&](int j0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (4 * i < nrow)
+#pragma unroll
+                for (int u = 0; u < PG; ++u)
+                    er[PG * i + u] = (uint64_t)sc[(size_t)(4 * i + g) * p.spad + j0 + 16 * u + rl];
+    };
+    constexpr bool AHEAD = BITS != 64;   // (registers)
+    if (begin + CP * w < end) {
+        load_e(begin + CP * w);
+        if (AHEAD)
+            rows.fetch(a, kh, begin + CP * w, end - 1, rl);
+    }
     {
         const int r = tid >> 4, l = tid & 15;
         uint64_t s = 0;
@@ -1148,7 +1198,8 @@ k_ra_value(RaArgs a, RaPlan p)
         slow |= p.odd[((size_t)kh * p.tiles + tile) * p.n2 + c];
     if constexpr (BITS != 64)
         for (int j = begin + tid; j < end; j += 256)
-            slow |= !step_fits<BITS>(a.vs[(size_t)j * a.n_kv + kh]);
+            slow |= !step_fits<BITS>(a.vs[(size_t)j * a.n_kv + kh]) &&
+                    seen<DEC>(a, p0, p.t0 + 16 * tile / G, p.t0 + (16 * tile + nrow - 1) / G, j);
     slow = __syncthreads_or(slow);   // dens and lam too
     uint32_t big = 0;
     if (!slow) {
@@ -1159,7 +1210,6 @@ k_ra_value(RaArgs a, RaPlan p)
             den[i] = dens[4 * i + g];
             y48[i] = quotient_factor(den[i]);
         }
-        ValueRows<BITS, HD> rows(a, kh, lane);
         const int vd = HD == 32 ? lane & 31 : lane, vp = rows.vp;
         double acc[DL][16];
 #pragma unroll
@@ -1167,21 +1217,6 @@ k_ra_value(RaArgs a, RaPlan p)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
                 acc[l][r] = Q48_FSUM0;
-        uint64_t er[4 * PG];
-        auto load_e = [&](int j0) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (4 * i < nrow)
-#pragma unroll
-                    for (int u = 0; u < PG; ++u)
-                        er[PG * i + u] = (uint64_t)sc[(size_t)(4 * i + g) * p.spad + j0 + 16 * u + rl];
-        };
-        constexpr bool AHEAD = BITS != 64;   // (registers)
-        if (begin + CP * w < end) {
-            load_e(begin + CP * w);
-            if (AHEAD)
-                rows.fetch(a, kh, begin + CP * w, end - 1, rl);
-        }
         for (int j0 = begin + CP * w; j0 < end; j0 += 4 * CP) {
             double v[DL][16];
             if (!AHEAD)

@@ -458,3 +458,62 @@ def test_keep_rows(ctx, rows):
         ctx.qcache_keep_rows(cache.c, p0, d.ptr, len(rows))
         assert all((a == keep(b)).all() for a, b in zip(cache.read(), before))
         cache.free()
+
+
+@pytest.mark.parametrize("bits", [8, 4, 64])
+@pytest.mark.parametrize("p0", [0, 50, 2500])
+def test_rows_never_stored_may_hold_anything(ctx, bits, p0):
+    """A padded batch: the last rows are masked everywhere and their cache rows hold
+    what memory held."""
+    rng = np.random.default_rng(p0 + bits)
+    nh, nkv, hd, T, pad = 8, 2, 64, 20, 3
+    max_seq = p0 + T
+    sees, _ = P.tree(rng, T, pad)
+    sees[:, T - pad:] = False
+    K, V = acts(rng, max_seq, nkv, hd), acts(rng, max_seq, nkv, hd)
+    K[max_seq - pad:] = I64.min
+    V[max_seq - pad:] = rng.integers(I64.min, I64.max, (pad, nkv, hd))
+    qkv = acts(rng, T, nh + 2 * nkv, hd)
+    mask = ctx.to_device(P.mask_words(sees))
+    d, out = ctx.to_device(qkv), ctx.buffer(T * nh * hd)
+    see = np.concatenate([np.ones((T, p0), bool), sees], 1)
+    if bits == 64:
+        dk, dv = ctx.to_device(K), ctx.to_device(V)
+        ctx.attn_tree(out.ptr, d.ptr, dk.ptr, dv.ptr, 0, p0, T, nh, nkv, hd, max_seq, mask.ptr)
+    else:
+        cache = Cache(ctx, bits, 1, max_seq, nkv, hd)      # any bytes, steps too
+        kv, vv = cache.fill(0, K[:-pad], V[:-pad])
+        K[:-pad], V[:-pad] = kv, vv
+        ctx.attn_rows_qcache(out.ptr, d.ptr, cache.c, 0, p0, T, nh, mask.ptr)
+        cache.free()
+    want = P.attend(qkv[:, :nh], K, V, see)
+    assert (out.download().reshape(T, nh, hd) == want).all()
+
+
+def test_more_rows_than_one_workspace(ctx):
+    """Rows in several launches (a GiB of scores each): against q48_attn_prefill, and
+    the quantised cache against the int64 cache of the values it stands for."""
+    rng = np.random.default_rng(17)
+    nh, nkv, hd, T, p0, max_seq = 64, 8, 32, 150, 16000, 16160
+    ctx.rope_init(hd, max_seq, 10000)
+    K, V = acts(rng, max_seq, nkv, hd), acts(rng, max_seq, nkv, hd)
+    qkv = acts(rng, T, nh + 2 * nkv, hd)
+    bufs = [ctx.to_device(x) for x in (K, V, qkv)]
+    dk, dv, dq = bufs
+    a, b = intllm.Buffer(ctx, T * nh * hd), intllm.Buffer(ctx, T * nh * hd)
+    ctx.attn_tree(a.ptr, dq.ptr, dk.ptr, dv.ptr, 0, p0, T, nh, nkv, hd, max_seq)
+    ctx.attn_prefill(b.ptr, dq.ptr, dk.ptr, dv.ptr, 0, p0, T, nh, nkv, hd, max_seq)
+    assert (a.download() == b.download()).all()
+    for bits in (8, 4):
+        cache = Cache(ctx, bits, 1, max_seq, nkv, hd)
+        ctx.qcache_store_rows(cache.c, 0, 0, max_seq, dk.ptr, dv.ptr, nkv * hd)
+        back = [intllm.Buffer(ctx, K.size) for _ in range(2)]
+        ctx.qcache_load_rows(back[0].ptr, back[1].ptr, cache.c, 0, 0, max_seq, nkv * hd)
+        ctx.attn_rows_qcache(a.ptr, dq.ptr, cache.c, 0, p0, T, nh)
+        ctx.attn_tree(b.ptr, dq.ptr, back[0].ptr, back[1].ptr, 0, p0, T, nh, nkv, hd, max_seq)
+        assert (a.download() == b.download()).all()
+        for x in back:
+            x.free()
+        cache.free()
+    for x in (*bufs, a, b):
+        x.free()

@@ -112,6 +112,7 @@ def test_refusals():
     assert dec(c, 64, far, x, far, far, 2, 0, 4) == EINVAL
     assert dec(c, 64, far, x, far, far, 0, 0, 3) == EINVAL
     assert dec(c, 64, far, x, far, far, 0, 0, 0) == EINVAL
+    assert dec(c, 64, far, x, far, far, 0, 0, 1026) == EINVAL
     assert dec(c, far, far, x, 64, 64, 0, 0, 4) == EINVAL          # out over q
     assert dec(c, far, 64, x, far + 8, 64, 0, 0, 4) == EINVAL      # out over k_new
     assert dec(c, far, 64, x, 64, far + 2040, 0, 0, 4) == EINVAL   # out's last word in v_new
@@ -122,6 +123,7 @@ def test_refusals():
     assert rows(c, 64, far, x, 0, 99, 2, 4, None) == ERANGE
     assert rows(c, 64, far, x, 0, 0, 0, 4, None) == EINVAL
     assert rows(c, 64, far, x, 0, 0, 1, 5, None) == EINVAL
+    assert rows(c, 64, far, x, 0, 0, 1, 1026, None) == EINVAL
     assert rows(c, far + 64, far, x, 0, 0, 1, 4, None) == EINVAL
     t = lib.q48_attn_tree
     assert t(c, 64, far, far, far, 0, 0, 1, 4, 2, 48, 100, None) == EINVAL
