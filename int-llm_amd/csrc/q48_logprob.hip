@@ -633,11 +633,12 @@ int q48_logprobs_rows(q48_ctx *c, const int64_t *logits, int T, int vocab, const
         return hipGetLastError() == hipSuccess ? Q48_OK : Q48_EHIP;
     }
     LpWork p = {};
-    // about a block a compute unit (two for long rows), 8 to 64 a row: the blocks of a
+    // about a block a compute unit (two for long rows), 9 to 64 a row: the blocks of a
     // row take turns at its ticket (us at 16 rows of 32000: 16 chunks a row 14.2, 32
-    // 16.4, 64 21.9; of 130000: 16 22.7, 32 21.4)
+    // 16.4, 64 21.9; of 130000: 16 22.7, 32 21.4).  9 leave 8 whole ones, with chunks of
+    // whole 256s, past 8192 logits: 32 wave maxima, which a threshold for 32 tokens needs.
     int want = (vocab > 65536 ? 2 : 1) * c->cu_count / T;
-    want = want < 8 ? 8 : want > 64 ? 64 : want;
+    want = want < 9 ? 9 : want > 64 ? 64 : want;
     p.ch = ((vocab + want - 1) / want + 255) & ~255;
     p.chunks = (vocab + p.ch - 1) / p.ch;
     size_t o = 0;

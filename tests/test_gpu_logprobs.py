@@ -73,7 +73,7 @@ def batch(rng, T, V):
 
 
 @pytest.mark.parametrize("T,V", [(600, 3000), (300, 8192), (70, 12000), (300, 16384), (20, 12000),
-                                 (140, 20000), (600, 32768), (130, 32767), (40, 32769),
+                                 (140, 20000), (600, 32768), (130, 32767), (40, 32769), (40, 8200),
                                  (9, 70001)])
 def test_many_rows(ctx, T, V):
     """More rows than a launch's blocks, and every form's largest row."""
@@ -167,4 +167,33 @@ def test_captured(ctx):
             assert all((b.download() == g).all() for b, g in zip((logp, ent, ids, tlp), got))
         want = P.logprobs(x, tk.download().view(np.int32)[:T], top)
         assert (got[0] == want[0]).all() and (got[1] == want[1]).all()
+        intllm.check("drop", lib.q48_graph_drop(c.h))
+
+
+def test_captured_over_many_blocks(ctx):
+    """The same where a row's blocks meet at a ticket, other calls between the replays."""
+    rng = np.random.default_rng(6)
+    lib = intllm.hip_lib()
+    T, V, top = 3, 40000, 7
+    with intllm.Context(0) as c:
+        d, tk = c.buffer(T * V), ints(c, rng.integers(0, V, T))
+        outs = [c.buffer(n) for n in (T, T, T * top, T * top)]
+
+        def call(rows):
+            logp, ent, ids, tlp = (b.ptr for b in outs)
+            c.logprobs_rows(d.ptr, rows, V, tk.ptr, logp, ent, top, ids, tlp)
+
+        d.upload(logits(rng, T, V))
+        call(T)
+        c.sync()
+        intllm.check("begin", lib.q48_graph_begin(c.h))
+        call(T)
+        intllm.check("end", lib.q48_graph_end(c.h))
+        for _ in range(4):
+            d.upload(logits(rng, T, V))
+            intllm.check("launch", lib.q48_graph_launch(c.h, 1))
+            got = [b.download() for b in outs]
+            call(1)                       # other chunks in the same workspace
+            call(T)
+            assert all((b.download() == g).all() for b, g in zip(outs, got))
         intllm.check("drop", lib.q48_graph_drop(c.h))
