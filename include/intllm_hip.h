@@ -442,7 +442,8 @@ int q48_silu_mul_rows(q48_ctx *ctx, int64_t *out, const int64_t *GU, int T, int 
  * [layers][max_seq][n_kv].  At 8 bits a code is a signed byte; at 4 bits byte b
  * of a head holds dim b in its low and dim b + head_dim / 2 in its high half,
  * two's complement.  head_dim 32, 64 or 128; max_seq at most 32767 (as
- * q48_rope_init).  The struct itself is read during the call only. */
+ * q48_rope_init), layers and n_kv at most 65535.  The struct itself is read during
+ * the call only. */
 typedef struct {
     void *k, *v;
     int64_t *k_step, *v_step;

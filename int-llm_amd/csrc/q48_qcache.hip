@@ -128,7 +128,7 @@ bool q48_qcache_ok(const q48_qcache *qc)
     return qc && qc->k && qc->v && qc->k_step && qc->v_step && (qc->bits == 8 || qc->bits == 4) &&
            ((uintptr_t)qc->k & 15) == 0 && ((uintptr_t)qc->v & 15) == 0 &&
            ((uintptr_t)qc->k_step & 7) == 0 && ((uintptr_t)qc->v_step & 7) == 0 &&
-           qc->layers > 0 && qc->max_seq > 0 && qc->max_seq <= 32767 && qc->n_kv > 0 &&
+           qc->layers > 0 && qc->layers <= 65535 && qc->max_seq > 0 && qc->max_seq <= 32767 && qc->n_kv > 0 &&
            qc->n_kv <= 65535 &&
            (qc->head_dim == 32 || qc->head_dim == 64 || qc->head_dim == 128);
 }
@@ -260,7 +260,7 @@ int q48_cache_keep_rows(q48_ctx *c, int64_t *kcache, int64_t *vcache, int layers
 
 int q48_qcache_keep_rows(q48_ctx *c, const q48_qcache *qc, int p0, const int *d_rows, int n)
 {
-    if (!c || !d_rows || !q48_qcache_ok(qc) || qc->layers > 65535 || n <= 0)
+    if (!c || !d_rows || !q48_qcache_ok(qc) || n <= 0)
         return Q48_EINVAL;
     if (p0 < 0 || p0 >= qc->max_seq || n > qc->max_seq - p0)
         return Q48_ERANGE;

@@ -650,11 +650,12 @@ __device__ __forceinline__ void add_values(double (&acc)[HD == 128 ? 2 : 1][16],
     }
 }
 
-// a step whose values all stay within [-2^51, 2^51)
+// a step whose values all stay within [-2^51, 2^51), the lowest code's too, which a
+// cache that was not quantised here may hold
 template <int BITS>
 __device__ __forceinline__ bool step_fits(int64_t step)
 {
-    return (uint64_t)step < ((uint64_t)1 << 51) / (BITS == 8 ? 127 : 7);
+    return (uint64_t)step <= (uint64_t)1 << (52 - BITS);
 }
 
 // q48_exp_neg with its constants where v_fma_f64 takes them (a multiply-add whose

@@ -517,3 +517,91 @@ def test_more_rows_than_one_workspace(ctx):
         cache.free()
     for x in (*bufs, a, b):
         x.free()
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("p0", [20, 2500])
+@pytest.mark.parametrize("top", [2 ** 51, 2 ** 52])
+def test_codes_below_the_quantiser_s_lowest(ctx, bits, p0, top):
+    """A cache may hold -128 (-8) too, which quantising never writes; around the largest
+    steps whose values are summed in FP64."""
+    rng = np.random.default_rng(p0 + bits)
+    nh, nkv, hd, T = 8, 2, 64, 3
+    cache = Cache(ctx, bits, 1, p0 + T, nkv, hd)
+    low, Q = -(1 << (bits - 1)), P.LEVELS[bits]
+    codes = rng.integers(low, low + 2, (2, p0 + T, nkv, hd))
+    steps = np.stack([rng.integers(1, P.ONE >> 10, (p0 + T, nkv)),
+                      top // Q - rng.integers(-1, 2, (p0 + T, nkv))])
+    codes[0, p0 // 2] = -1                    # the only near key: nearly all the weight
+    k, v, ks, vs = cache.read()
+    k[0], v[0] = (P.pack(c, bits) for c in codes)
+    ks[0], vs[0] = steps
+    for b, x in zip(cache.bufs, (k, v, ks, vs)):
+        b.upload(np.ascontiguousarray(x).view(np.int64).ravel())
+    qkv = np.abs(acts(rng, T, nh + 2 * nkv, hd, sigma=4.0))
+    d, out = ctx.to_device(qkv), ctx.buffer(T * nh * hd)
+    ctx.attn_rows_qcache(out.ptr, d.ptr, cache.c, 0, p0, T, nh)
+    kv, vv = (P.values(c, s) for c, s in zip(codes, steps))
+    see = np.concatenate([np.ones((T, p0), bool), np.tri(T, dtype=bool)], 1)
+    assert (out.download().reshape(T, nh, hd) == P.attend(qkv[:, :nh], kv, vv, see)).all()
+    cache.free()
+
+
+@pytest.mark.parametrize("bits", [8, 4, 64])
+@pytest.mark.parametrize("p0", [40, 2500])
+def test_verifying_captured(ctx, bits, p0):
+    """Store, attend, keep as one graph, the rows, positions, mask and path changed
+    between replays: against the same calls made eagerly on a twin."""
+    rng = np.random.default_rng(p0 + bits)
+    lib = intllm.hip_lib()
+    nh, nkv, hd, T, n, max_seq = 8, 2, 64, 13, 4, p0 + 20
+    with intllm.Context(0) as c:
+        c.rope_init(hd, max_seq, 10000)
+        words = T * (nh + 2 * nkv) * hd
+        src, pos, mask, path = (c.buffer(m) for m in (words, 8, T, 2))
+        K, V = acts(rng, max_seq, nkv, hd), acts(rng, max_seq, nkv, hd)
+        sides = []
+        for _ in range(2):
+            qkv, out = c.buffer(words), c.buffer(T * nh * hd)
+            if bits == 64:
+                sides.append((qkv, out, [c.to_device(K), c.to_device(V)], None))
+            else:
+                q = Cache(c, bits, 1, max_seq, nkv, hd)
+                q.fill(0, K, V)
+                sides.append((qkv, out, q.bufs, q.c))
+
+        def verify(qkv, out, bufs, cache):
+            if bits == 64:
+                k, v = (b.ptr for b in bufs)
+                c.rope_store_rows_at(qkv.ptr, k, v, 0, p0, T, pos.ptr, nh, nkv, hd, max_seq)
+                c.attn_tree(out.ptr, qkv.ptr, k, v, 0, p0, T, nh, nkv, hd, max_seq, mask.ptr)
+                c.cache_keep_rows(k, v, 1, p0, path.ptr, n, nkv, hd, max_seq)
+            else:
+                c.rope_store_rows_qcache(qkv.ptr, cache, 0, p0, T, nh, pos.ptr)
+                c.attn_rows_qcache(out.ptr, qkv.ptr, cache, 0, p0, T, nh, mask.ptr)
+                c.qcache_keep_rows(cache, p0, path.ptr, n)
+
+        def fresh():
+            sees, parent = P.tree(rng, T, 0)
+            x = acts(rng, words)
+            for side in sides:
+                side[0].upload(x)
+            pos.upload(np.concatenate([p0 + sees.sum(1) - 1, np.zeros(16 - T)])
+                       .astype(np.int32).view(np.int64))
+            mask.upload(P.mask_words(sees).ravel())
+            path.upload(np.sort(rng.choice(T, n, False)).astype(np.int32).view(np.int64))
+
+        fresh()
+        for side in sides:
+            verify(*side)
+        c.sync()
+        intllm.check("begin", lib.q48_graph_begin(c.h))
+        verify(*sides[0])
+        intllm.check("end", lib.q48_graph_end(c.h))
+        for _ in range(4):
+            fresh()
+            intllm.check("launch", lib.q48_graph_launch(c.h, 1))
+            verify(*sides[1])
+            for a, b in zip((*sides[0][:2], *sides[0][2]), (*sides[1][:2], *sides[1][2])):
+                assert (a.download() == b.download()).all()
+        intllm.check("drop", lib.q48_graph_drop(c.h))

@@ -74,6 +74,7 @@ def cache(**kw):
 
 BAD_CACHES = [dict(k=None), dict(v=None), dict(k_step=None), dict(v_step=None), dict(k=4104),
               dict(v=8193), dict(k_step=68), dict(bits=6), dict(bits=0), dict(layers=0),
+              dict(layers=65536), dict(n_kv=65536),
               dict(max_seq=0), dict(max_seq=32768), dict(n_kv=0), dict(head_dim=48),
               dict(head_dim=256)]
 
