@@ -60,11 +60,15 @@ constexpr int64_t kInvK[8] = {
     281474976710656LL, 140737488355328LL, 93824992236885LL, 70368744177664LL, 56294995342131LL,
     46912496118443LL, 40210710958665LL, 35184372088832LL};
 
-// T_j 2^-48 as doubles, into LDS
-__device__ __forceinline__ void lp_table(double *tab, int tid)
+// T_j 2^-48 as doubles, and the logarithm's tables, into LDS
+__device__ __forceinline__ void lp_table(double *tab, int64_t *rcps, int64_t *logs, int tid)
 {
     if (tid < 45)
         tab[tid] = (double)kExp[tid] * 0x1p-48;
+    if (tid < 64) {
+        rcps[tid] = kRcp[tid];
+        logs[tid] = kLog[tid];
+    }
 }
 
 // e of each u (include/intllm_hip.h; 0 from LP_LIM on), added to z, and floor(e u
@@ -140,13 +144,14 @@ __device__ __forceinline__ void lp_terms(const uint64_t (&u)[N], const double *t
 
 // logZ of Z >= 2^48, and its b; the Horner steps as in lp_terms, around 1.5 2^52 since
 // d may be a unit or two below 0
-__device__ __forceinline__ int64_t lp_log(q48_u128 Z, int &b)
+__device__ __forceinline__ int64_t lp_log(q48_u128 Z, int &b, const int64_t *rcps,
+                                          const int64_t *logs)
 {
     const uint64_t zh = (uint64_t)(Z >> 64), zl = (uint64_t)Z;
     b = (zh ? 128 - __builtin_clzll(zh) : 64 - __builtin_clzll(zl)) - 49;
     const int64_t z = (int64_t)(Z >> b);
     const int j = (int)(z >> 42) - 64;
-    const int64_t rcp = kRcp[j], l = kLog[j];
+    const int64_t rcp = rcps[j], l = logs[j];
     const double M = 0x1.8p52, d = (double)(q48_mul(z, rcp) - Q48_ONE) * 0x1p-48;
     double g = (double)kInvK[7];
 #pragma unroll
@@ -170,22 +175,53 @@ __device__ __forceinline__ uint32_t lp_high(int64_t x)
     return (uint32_t)((uint64_t)x >> 32) ^ 0x80000000u;
 }
 
-// The n-th largest of the high halves that the lanes of a wave hold in g[0 .. N - 1]
-// (64 N >= n), two bits at a time from the top: n of the groups whose maxima these
-// are have a value at least that large, so the n largest values of the row are among
-// the values whose high halves are not below it.
+// A threshold that n of the high halves g[0 .. N - 1] of a wave's lanes (64 N >= n)
+// reach, most often no more: from the top, two bits at a time, until n are left.  n of
+// the groups whose maxima these are have a value at least that large, so the n largest
+// values of the row are among the values whose high halves are not below it.  high: the
+// largest of all; the bits above the first in which a maximum but 0 (no value) differs
+// from it are taken as they are.  A step is 3 N compares and counts, 140 ns for N = 4:
+// all 16 took 2.3 us of a single row's 12.
 template <int N>
-__device__ __forceinline__ uint32_t lp_threshold(const uint32_t (&g)[N], int n)
+__device__ __forceinline__ uint32_t lp_threshold(const uint32_t (&g)[N], uint32_t high, int n)
 {
-    uint32_t t = 0;
-    for (int bit = 30; bit >= 0; bit -= 2) {
-        int count[3] = {0, 0, 0};
+    uint32_t low = high;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        low = min(low, g[i] ? g[i] : high);
+    low = min(low, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)low, Q48_DPP_XOR1, 0xf, 0xf, false));
+    low = min(low, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)low, Q48_DPP_XOR2, 0xf, 0xf, false));
+    low = min(low, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)low, Q48_DPP_HALF_MIRROR, 0xf, 0xf,
+                                                         false));
+    low = min(low, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)low, Q48_DPP_MIRROR, 0xf, 0xf,
+                                                         false));
+    uint32_t differ = 0;
+#pragma unroll
+    for (int row = 0; row < 64; row += 16)
+        differ |= (uint32_t)__builtin_amdgcn_readlane((int)low, row) ^ high;
+    int bit = differ ? 31 - __builtin_clz(differ) : 0;
+    bit &= ~1;
+    auto reach = [&](uint32_t t) {
+        int c = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i)
+            c += __popcll(__ballot(g[i] >= t));
+        return c;
+    };
+    uint32_t t = (high >> bit >> 2) << bit << 2;
+    int have = reach(t);
+    if (have < n) {   // some of the n groups have no value
+        t = 0;
+        bit = 30;
+    }
+    for (; bit >= 0 && have != n; bit -= 2) {
+        int count[3];
 #pragma unroll
-            for (int c = 0; c < 3; ++c)
-                count[c] += __popcll(__ballot(g[i] >= (t | ((uint32_t)(c + 1) << bit))));
-        t |= (uint32_t)((count[0] >= n) + (count[1] >= n) + (count[2] >= n)) << bit;
+        for (int c = 0; c < 3; ++c)
+            count[c] = reach(t | ((uint32_t)(c + 1) << bit));
+        const int d = (count[0] >= n) + (count[1] >= n) + (count[2] >= n);
+        t |= (uint32_t)d << bit;
+        have = d == 3 ? count[2] : d == 2 ? count[1] : d == 1 ? count[0] : have;
     }
     return t;
 }
@@ -226,20 +262,29 @@ __device__ __forceinline__ void lp_collect(const int64_t *x, int first, int stri
     }
 }
 
-// The row's log probability and entropy from its sums z and w; returns logZ.
-__device__ __forceinline__ int64_t lp_finish(q48_u128 z, q48_u128 w, int64_t m, const int64_t *x,
-                                             int V, int t, const int *tokens, int64_t *logp,
-                                             int64_t *entropy, bool writer)
+// The token of a row and its logit, loaded ahead of the sums they are used with.
+struct LpToken {
+    bool valid;
+    int64_t y;
+    __device__ __forceinline__ LpToken(const int64_t *x, int V, const int *tokens, bool wanted, int t)
+    {
+        const int id = wanted ? tokens[t] : -1;
+        valid = id >= 0 && id < V;
+        y = valid ? x[id] : 0;
+    }
+};
+
+// The row's log probability and entropy from its sums z and w; returns logZ.  rcps, logs:
+// the logarithm's tables.
+__device__ __forceinline__ int64_t lp_finish(q48_u128 z, q48_u128 w, int64_t m, LpToken k, int t,
+                                             const int64_t *rcps, const int64_t *logs,
+                                             int64_t *logp, int64_t *entropy, bool writer)
 {
-    // the token's logit on its way during the logarithm
-    const int id = logp ? tokens[t] : -1;
-    const bool valid = id >= 0 && id < V;
-    const int64_t y = valid ? x[id] : m;
     int b;
-    const int64_t logz = lp_log(z, b);
+    const int64_t logz = lp_log(z, b, rcps, logs);
     if (writer) {
         if (logp)
-            logp[t] = valid ? lp_value((uint64_t)m - (uint64_t)y, logz) : 0;
+            logp[t] = k.valid ? lp_value((uint64_t)m - (uint64_t)k.y, logz) : 0;
         if (entropy)
             entropy[t] = logz + q48_div((int64_t)(w >> b), (int64_t)(z >> b));
     }
@@ -247,24 +292,36 @@ __device__ __forceinline__ int64_t lp_finish(q48_u128 z, q48_u128 w, int64_t m, 
 }
 
 
-// The top values of a row from its candidates cv, ci [0, count): each counts those
-// before it.  count <= LP_CAP.
+// How many of the candidates cv, ci [0, count) come before the candidate v, id, eight
+// at a time (the arrays hold LP_CAP + 8: what lies past count is not counted).
+__device__ __forceinline__ int lp_before(const int64_t *cv, const int *ci, int count, int64_t v,
+                                         int id)
+{
+    int rank = 0;
+    for (int k = 0; k < count; k += 8)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            rank += (k + i < count) & ((cv[k + i] > v) | ((cv[k + i] == v) & (ci[k + i] < id)));
+    return rank;
+}
+
+__device__ __forceinline__ void lp_place(int rank, int64_t v, int id, int64_t m, int64_t logz, int t,
+                                         int top, int *ids, int64_t *tlp)
+{
+    if (rank < top) {
+        ids[(size_t)t * top + rank] = id;
+        tlp[(size_t)t * top + rank] = lp_value((uint64_t)m - (uint64_t)v, logz);
+    }
+}
+
+// The top values of a row from its candidates.  count <= LP_CAP.
 template <int NT>
 __device__ __forceinline__ void lp_rank(const int64_t *cv, const int *ci, int count, int64_t m,
                                         int64_t logz, int t, int top, int *ids, int64_t *tlp,
                                         int tid)
 {
-    for (int i = tid; i < count; i += NT) {
-        const int64_t v = cv[i];
-        const int id = ci[i];
-        int rank = 0;
-        for (int k = 0; k < count; ++k)
-            rank += cv[k] > v || (cv[k] == v && ci[k] < id);
-        if (rank < top) {
-            ids[(size_t)t * top + rank] = id;
-            tlp[(size_t)t * top + rank] = lp_value((uint64_t)m - (uint64_t)v, logz);
-        }
-    }
+    for (int i = tid; i < count; i += NT)
+        lp_place(lp_before(cv, ci, count, cv[i], ci[i]), cv[i], ci[i], m, logz, t, top, ids, tlp);
 }
 
 // The same by top passes over the row, for rows with more candidates: the largest
@@ -374,13 +431,13 @@ __global__ __launch_bounds__(LR_NT) void k_lp_row(const int64_t *__restrict__ X,
     __shared__ int64_t red[2][NW];
     __shared__ uint32_t gmax[LR_NT / 4];
     __shared__ uint64_t sums[NW][4];
-    __shared__ int64_t cv[LP_CAP], slogz;
-    __shared__ int ci[LP_CAP];
+    __shared__ int64_t cv[LP_CAP + 8], slogz, rcps[64], logs[64];
+    __shared__ int ci[LP_CAP + 8];
     __shared__ int count;
     __shared__ uint32_t thr;
     const int tid = threadIdx.x, lane = tid & 63;
     const int whole = V / LR_NT;   // tiles of 512 with every thread in the row
-    lp_table(tab, tid);
+    lp_table(tab, rcps, logs, tid);
     int64_t v[R];
     {
         const LpRow row(X + (size_t)blockIdx.x * V, V);
@@ -415,13 +472,15 @@ __global__ __launch_bounds__(LR_NT) void k_lp_row(const int64_t *__restrict__ X,
         m = block_max64<LR_NT>(m, red[par], false);
         if (top && tid < 64) {
             const uint32_t g[2] = {gmax[tid], gmax[tid + 64]};
-            const uint32_t h = lp_threshold<2>(g, top);
+            const uint32_t h = lp_threshold<2>(
+                g, (uint32_t)__builtin_amdgcn_readfirstlane((int)lp_high(m)), top);
             if (tid == 0)
                 thr = h;
         }
         // (a block's last row: a row of no logits, nothing is read)
         const bool again = t + gridDim.x < (unsigned)T;
         const LpRow next(again ? x + (size_t)gridDim.x * V : x, again ? V : 0);
+        LpToken token(x, V, tokens, logp != nullptr, t);
         uint64_t z64 = 0, w64 = 0;   // R terms below 2^49 each
 #pragma unroll
         for (int k = 0; k < R; k += 4) {
@@ -438,6 +497,7 @@ __global__ __launch_bounds__(LR_NT) void k_lp_row(const int64_t *__restrict__ X,
             lp_terms<4>(u, tab, z64, w64);
             __builtin_amdgcn_sched_barrier(0);   // more terms would not fit the registers
         }
+        asm volatile("" : "+v"(token.y));   // (loaded by now: not after the sums)
         lp_wave_sums<false>(z64, w64, sums[tid >> 6], lane);
         __syncthreads();
         if (tid < 64) {
@@ -446,7 +506,8 @@ __global__ __launch_bounds__(LR_NT) void k_lp_row(const int64_t *__restrict__ X,
                 z += ((q48_u128)sums[i][1] << 64) | sums[i][0];
                 w += ((q48_u128)sums[i][3] << 64) | sums[i][2];
             }
-            const int64_t logz = lp_finish(z, w, m, x, V, t, tokens, logp, entropy, tid == 0);
+            const int64_t logz =
+                lp_finish(z, w, m, token, t, rcps, logs, logp, entropy, tid == 0);
             if (tid == 0)
                 slogz = logz;
         }
@@ -502,8 +563,8 @@ __global__ __launch_bounds__(256) void k_lp_sum(const int64_t *__restrict__ X, i
 {
     q48_round_down();
     __shared__ double tab[64];
-    __shared__ int64_t cv[LP_CAP], bv[4], slogz;
-    __shared__ int ci[LP_CAP], bi[4];
+    __shared__ int64_t cv[LP_CAP + 8], bv[4], slogz, rcps[64], logs[64];
+    __shared__ int ci[LP_CAP + 8], bi[4];
     __shared__ uint32_t thr;
     __shared__ int last;
     const int t = blockIdx.y, c = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
@@ -515,7 +576,8 @@ __global__ __launch_bounds__(256) void k_lp_sum(const int64_t *__restrict__ X, i
         const int k = lane + 64 * i;
         g[i] = k < groups ? p.gmax[(size_t)t * groups + k] : INT64_MIN;
     }
-    lp_table(tab, tid);
+    lp_table(tab, rcps, logs, tid);
+    LpToken token(x, V, tokens, logp != nullptr, t);
     int64_t m = g[0];
 #pragma unroll
     for (int i = 1; i < 4; ++i)
@@ -530,7 +592,8 @@ __global__ __launch_bounds__(256) void k_lp_sum(const int64_t *__restrict__ X, i
             const int k = lane + 64 * i;
             h[i] = k < groups && (k >> 2) * p.ch + 64 * (k & 3) < V ? lp_high(g[i]) : 0;
         }
-        const uint32_t n = lp_threshold<4>(h, top);
+        const uint32_t n = lp_threshold<4>(
+            h, (uint32_t)__builtin_amdgcn_readfirstlane((int)lp_high(m)), top);
         if (tid == 0)
             thr = n;
     }
@@ -550,6 +613,7 @@ __global__ __launch_bounds__(256) void k_lp_sum(const int64_t *__restrict__ X, i
         lp_terms<1>(u, tab, z64, w64);
     }
     uint64_t *sums = p.sums + (size_t)t * groups * 4;
+    asm volatile("" : "+v"(token.y));   // (loaded by now: not after the sums)
     lp_wave_sums<true>(z64, w64, sums + 4 * (4 * c + (tid >> 6)), lane);
     if (top) {
         __syncthreads();   // the threshold
@@ -568,8 +632,12 @@ __global__ __launch_bounds__(256) void k_lp_sum(const int64_t *__restrict__ X, i
     if (!last)
         return;
 
-    // the row's last block.  Wave 0: the row's sums; the others: its candidates
+    // the row's last block.  Wave 0: the row's sums; the others: its candidates, which
+    // wave 1 ranks meanwhile where it holds them all
     const int count = top ? agent_load(p.count + 2 * t) : 0;
+    const bool few = count <= 64;
+    int64_t v = 0;
+    int id = 0, rank = LP_MAX_TOP;
     if (tid < 64) {
         q48_u128 z = 0, w = 0;
 #pragma unroll
@@ -581,19 +649,34 @@ __global__ __launch_bounds__(256) void k_lp_sum(const int64_t *__restrict__ X, i
             }
         z = q48_wave_sum128(z);
         w = q48_wave_sum128(w);
-        const int64_t logz = lp_finish(z, w, m, x, V, t, tokens, logp, entropy, tid == 0);
+        const int64_t logz = lp_finish(z, w, m, token, t, rcps, logs, logp, entropy, tid == 0);
         if (tid == 0)
             slogz = logz;
-    } else {
+    } else if (!few) {
         for (int k = tid - 64; k < min(count, LP_CAP); k += 192) {
             cv[k] = agent_load(p.cv + (size_t)t * LP_CAP + k);
             ci[k] = agent_load(p.ci + (size_t)t * LP_CAP + k);
         }
+    } else if (tid < 128) {
+        if (lane < count) {
+            v = agent_load(p.cv + (size_t)t * LP_CAP + lane);
+            id = agent_load(p.ci + (size_t)t * LP_CAP + lane);
+            cv[lane] = v;
+            ci[lane] = id;
+        }
+        // the wave's own writes before its reads
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (lane < count)
+            rank = lp_before(cv, ci, count, v, id);
     }
     if (!top)
         return;
     __syncthreads();
-    if (count <= LP_CAP)
+    if (few)
+        lp_place(rank, v, id, m, slogz, t, top, ids, tlp);
+    else if (count <= LP_CAP)
         lp_rank<256>(cv, ci, count, m, slogz, t, top, ids, tlp, tid);
     else
         lp_select<256>(x, V, m, slogz, t, top, ids, tlp, tid, bv, bi);
@@ -612,9 +695,9 @@ int q48_logprobs_rows(q48_ctx *c, const int64_t *logits, int T, int vocab, const
         return Q48_EINVAL;
     q48_on_device on(c);
     // A block a row where the row fits its registers and there are rows for most compute
-    // units; else a row over many blocks.  us, a block a row / many: one row of 8000 10.2
-    // / 11.4; 64 rows of 16000 16.2 / 17, of 32000 26.1 / 19.4; 128 of 32000 27.5 / 26.8,
-    // 256 32.4 / 40.4.
+    // units; else a row over many blocks.  us, a block a row / many: one row of 8000 9.7
+    // / 9.8, 16 10.4 / 11.6; 64 rows of 16000 16.0 / 15.6, of 32000 25.6 / 17.9; 128 of
+    // 16000 16.2 / 21.8, of 32000 26.3 / 26.7; 256 of 32000 31.4 / 47.6.
     if (vocab <= 8192 || (vocab <= 16384 && T >= 64) || (vocab <= 32768 && T >= 128)) {
 #define LP_ROW(R, PER)                                                                         \
     hipLaunchKernelGGL(k_lp_row<R>, dim3(T < PER * c->cu_count ? T : PER * c->cu_count),       \
@@ -633,12 +716,14 @@ int q48_logprobs_rows(q48_ctx *c, const int64_t *logits, int T, int vocab, const
         return hipGetLastError() == hipSuccess ? Q48_OK : Q48_EHIP;
     }
     LpWork p = {};
-    // about a block a compute unit (two for long rows), 9 to 64 a row: the blocks of a
-    // row take turns at its ticket (us at 16 rows of 32000: 16 chunks a row 14.2, 32
-    // 16.4, 64 21.9; of 130000: 16 22.7, 32 21.4).  9 leave 8 whole ones, with chunks of
-    // whole 256s, past 8192 logits: 32 wave maxima, which a threshold for 32 tokens needs.
-    int want = (vocab > 65536 ? 2 : 1) * c->cu_count / T;
-    want = want < 9 ? 9 : want > 64 ? 64 : want;
+    // Chunks a row: 16, and up to 64 of long rows that are few: a row's blocks take turns
+    // at its counters.  us with 9 / 16 / 32 / 64: one row of 32000 12.1 / 11.0 / 11.1 /
+    // 10.9, 16 rows 13.8 / 12.6 / 14.9 / 21.6, 64 18.9 / 17.9 / 23.5 / 37.8; of 130000 one
+    // 20.7 / 15.8 / 12.2 / 11.5, 16 22.6 / 20.5 / 18.4 / 24.2, 64 42.8 / 36.0 / 41.1 / 51.8.
+    // (Chunks of whole 256s leave at least 8 past 8192 logits: 32 wave maxima, which a
+    // threshold for 32 tokens needs.)
+    int want = vocab > 65536 ? 2 * c->cu_count / T : 16;
+    want = want < 16 ? 16 : want > 64 ? 64 : want;
     p.ch = ((vocab + want - 1) / want + 255) & ~255;
     p.chunks = (vocab + p.ch - 1) / p.ch;
     size_t o = 0;
