@@ -238,6 +238,23 @@ __device__ __forceinline__ int64_t code_dot(const v4i (&acc)[8], int i, int64_t 
     return (int64_t)((top << 16) | ((uint32_t)u >> 16));
 }
 
+// int64 keys as loaded, 16 dims a lane (dims past the head give digits of zero)
+template <int HD>
+struct WordRow {
+    uint64_t x[HD < 64 ? 16 : HD / 4];
+    __device__ __forceinline__ void load(const RaArgs &a, size_t row, int kq)
+    {
+        const uint64_t *k = reinterpret_cast<const uint64_t *>(a.k) + row * HD;
+#pragma unroll
+        for (int ks = 0; ks < (HD < 64 ? 1 : HD / 64); ++ks)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int d = 64 * ks + 16 * kq;
+                x[16 * ks + e] = d < HD ? k[d + e] : kDig;
+            }
+    }
+};
+
 // Digits of a tile's queries as the A operands of the score products, and C sum_d
 // q_d for int64 keys, by NT threads; qs: rotated queries in LDS, or null.
 template <int BITS, int HD, int NT>
@@ -334,20 +351,20 @@ __device__ __forceinline__ void code_sum(int64_t &c0, int64_t &c1,
 // Operands of 16 int64 key rows (eight digit planes), and C sum_d k_d - HD C^2
 template <int HD>
 __device__ __forceinline__ q48_u128 key_digits(v4i (&B)[HD < 64 ? 1 : HD / 64][8],
-                                               const int64_t *k, int kq)
+                                               const WordRow<HD> &k, int kq)
 {
     constexpr int KS = HD < 64 ? 1 : HD / 64;
     q48_u128 ck = 0;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-        const int d0 = 64 * ks + 16 * kq;
+        const bool in = 64 * ks + 16 * kq < HD;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             uint64_t x4[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                x4[e] = d0 < HD ? (uint64_t)k[d0 + 4 * g + e] : kDig;
-                if (d0 < HD)
+                x4[e] = k.x[16 * ks + 4 * g + e];
+                if (in)
                     ck += (q48_u128)(q48_i128)(int64_t)x4[e];
             }
             uint32_t wd[8];
@@ -435,6 +452,9 @@ __device__ __forceinline__ void word_scores(int64_t (&s)[4], const v4i (*dig)[8]
                              __builtin_amdgcn_alignbit(w2[i], w1[i], 16));
 }
 
+// whether the next rows' keys are loaded ahead (int64: where the registers allow)
+constexpr bool keys_ahead(int bits, int hd, int tb) { return bits != 64 || (hd < 128 && tb == 1); }
+
 // Scores of TB tiles (vectors v0 .. of 16 each) over rows [begin, end), 16 rows a
 // wave at a time (wave w of NW); put(tb, m, j, s) takes vector m's score, and mx
 // and far gather each tile's maxima over the rows seen and far scores.
@@ -444,11 +464,14 @@ __device__ __forceinline__ void score_rows(const RaArgs &a, const v4i (*dig)[HD 
                                            const int *vt, int ntile, int nrow, int kh, int p0,
                                            int begin, int end, const uint8_t *nk, int64_t nst,
                                            int clear, int w, int lane, int64_t (&mx)[TB][4],
-                                           uint32_t (&far)[TB], KeyRow<BITS == 64 ? 8 : BITS, HD> &next,
+                                           uint32_t (&far)[TB],
+                                           std::conditional_t<BITS == 64, WordRow<HD>,
+                                                              KeyRow<BITS == 64 ? 8 : BITS, HD>> &next,
                                            Put put)
 {
     constexpr int KS = HD < 64 ? 1 : HD / 64;
     const int rl = lane & 15, kq = lane >> 4;
+    constexpr bool AHEAD = keys_ahead(BITS, HD, TB);
     for (int j0 = begin + 16 * w; j0 < end; j0 += 16 * NW) {
         const int j = j0 + rl, jc = min(j, end - 1);
         const bool all = j0 + 16 <= clear;   // (clear <= end)
@@ -459,7 +482,11 @@ __device__ __forceinline__ void score_rows(const RaArgs &a, const v4i (*dig)[HD 
         uint64_t step = 0;
         v4i C[KS];
         if constexpr (BITS == 64) {
-            ck = key_digits<HD>(B, reinterpret_cast<const int64_t *>(a.k) + row * HD, kq);
+            if (!AHEAD)
+                next.load(a, row, kq);
+            ck = key_digits<HD>(B, next, kq);
+            if (AHEAD && j0 + 16 * NW < end)
+                next.load(a, (size_t)min(j + 16 * NW, end - 1) * a.n_kv + kh, kq);
         } else {
             KeyRow<BITS, HD> now = next;
             if (j0 + 16 * NW < end)
@@ -835,10 +862,10 @@ __global__ __launch_bounds__(RT_NT) void k_ra_tile(RaArgs a, RaPlan p)
         return;
     const int S = tile_span<DEC>(a, p, v0 + nrow - 1, G, p0);
 
-    KeyRow<BITS == 64 ? 8 : BITS, HD> next;
-    if constexpr (BITS != 64)   // on its way while the queries are split
-        if (16 * w < S)
-            next.load(a, (size_t)min(16 * w + rl, S - 1) * a.n_kv + kh, kq);
+    // the first keys on their way while the queries are split
+    std::conditional_t<BITS == 64, WordRow<HD>, KeyRow<BITS == 64 ? 8 : BITS, HD>> next;
+    if (keys_ahead(BITS, HD, 1) && 16 * w < S)
+        next.load(a, (size_t)min(16 * w + rl, S - 1) * a.n_kv + kh, kq);
     if (tid < 16)
         vt[tid] = p.t0 + min(v0 + tid, NV - 1) / G;
     if (tid == 0)
@@ -995,10 +1022,9 @@ k_ra_score(RaArgs a, RaPlan p)
     if (begin >= end)
         return;
 
-    KeyRow<BITS == 64 ? 8 : BITS, HD> next;
-    if constexpr (BITS != 64)
-        if (begin + 16 * w < end)
-            next.load(a, (size_t)min(begin + 16 * w + rl, end - 1) * a.n_kv + kh, kq);
+    std::conditional_t<BITS == 64, WordRow<HD>, KeyRow<BITS == 64 ? 8 : BITS, HD>> next;
+    if (keys_ahead(BITS, HD, TB) && begin + 16 * w < end)
+        next.load(a, (size_t)min(begin + 16 * w + rl, end - 1) * a.n_kv + kh, kq);
     if (tid < TB * 16)
         vt[tid] = p.t0 + min(16 * tile0 + tid, NV - 1) / G;
     if (tid < TB)
@@ -1330,7 +1356,7 @@ int launch_hd(q48_ctx *c, RaArgs &a)
         if (lds <= rt_lds(HD, 16) &&
             one_launch<BITS, HD>(vb, a.p0 + a.T, (long)a.T * a.n_heads, tiles * a.n_kv,
                                  c->cu_count)) {
-            constexpr bool WIDE = HD == 64 && BITS != 64;
+            constexpr bool WIDE = HD == 64 && BITS != 64 && !DEC;   // (one token: vb is small)
             p.Tn = a.T;
             p.vb = vb;
             const dim3 grid(tiles, a.n_kv);
