@@ -1307,26 +1307,28 @@ bool overlap(const int64_t *a, size_t na, const int64_t *b, size_t nb)
     return (uintptr_t)a < (uintptr_t)(b + nb) && (uintptr_t)b < (uintptr_t)(a + na);
 }
 
-// Estimated times of the two forms, in us, for a span of S rows:
-//   one launch     8 + rounds of blocks * S * (c0 + c1 vb), at one block a compute unit
-//   three launches l + pairs of vectors and rows * c3
-// with (c0, c1, l, c3) measured from 250 to 3000 rows and 8 to 8192 vectors.  us, one
-// / three, 32 heads on 4 of 64, 8 bits: one token at 250 rows 10.1 / 16.0, at 1000
-// 18.0 / 15.0; 16 tokens at 1000 20.8 / 22.9; 64 at 900 30.7 / 42.4, at 2000 54.0 /
-// 74.1; 256 at 700 70.1 / 112.3.  int64: 4 tokens at 500 20.0 / 20.7, 16 at 1000 36.0
-// / 29.6, 64 at 900 44.5 / 62.6.  128-wide heads on 8, 8 bits: one token at 500 17.6 /
-// 16.1, 64 at 2000 114.0 / 91.3.
+// Estimated times of the two forms, in us, for rows that see `most` rows at most and
+// `seen` on average:
+//   one launch     o + (c0 + c1 vb) most, where every block has a compute unit of its own;
+//                  k (a second block's waves fill gaps) a further round, and `seen`
+//   three launches l + c3 vectors seen
+// with the constants fitted to both forms' times from 150 to 2756 rows and 1 to 1000
+// tokens of 8 heads on 2 of 32, 32 on 4 of 64, 32 on 8 of 128: the slower one is chosen by
+// 0.7% on average.  us, one / three, 32 heads on 4 of 64, 8 bits: one token at 300 rows
+// 10.1 / 14.9, at 1000 17.4 / 14.7; 16 tokens at 1000 20.8 / 23.2; 64 at 2000 54.5 / 63.5;
+// 512 at 1500 372 / 320, 256 at 2500 404 / 214.  int64: 4 tokens at 300 16.4 / 20.5, 16 at
+// 1000 38.8 / 28.9, 512 at 1500 556 / 387.
 template <int BITS, int HD>
-bool one_launch(int vb, int S, long vectors, long blocks, int cus)
+bool one_launch(int vb, int most, double seen, long vectors, long blocks, int cus)
 {
-    constexpr int h = HD == 32 ? 0 : HD == 64 ? 1 : 2;
-    constexpr double c0[2][3] = {{7.5e-3, 9e-3, 14e-3}, {33e-3, 22e-3, 43e-3}};
-    constexpr double c1[2][3] = {{1.4e-3, 1.3e-3, 2.4e-3}, {1e-3, 1.5e-3, 2e-3}};
-    constexpr double l[2] = {15, 20};
-    constexpr double c3[2][3] = {{19e-6, 13.7e-6, 17.5e-6}, {31e-6, 23e-6, 37e-6}};
-    constexpr int w = BITS == 64;
-    const double one = 8 + (double)((blocks + cus - 1) / cus) * S * (c0[w][h] + c1[w][h] * vb);
-    return one <= l[w] + (double)vectors * S * c3[w][h];
+    constexpr int h = HD == 32 ? 0 : HD == 64 ? 1 : 2, w = BITS == 64;
+    constexpr double o[2] = {10.8, 14.2}, k[2] = {1.27, 1.31}, l[2] = {16.3, 19.7};
+    constexpr double c0[2][3] = {{3.0e-3, 4.9e-3, 8.3e-3}, {9.9e-3, 11.9e-3, 27.9e-3}};
+    constexpr double c1[2][3] = {{2.27e-3, 2.10e-3, 3.81e-3}, {2.47e-3, 2.78e-3, 4.01e-3}};
+    constexpr double c3[2][3] = {{11.4e-6, 11.6e-6, 18.8e-6}, {15.7e-6, 16.1e-6, 31.5e-6}};
+    const double rounds = (double)blocks / cus;
+    const double rows = rounds <= 1 ? (double)most : seen * (1 + k[w] * (rounds - 1));
+    return o[w] + rows * (c0[w][h] + c1[w][h] * vb) <= l[w] + (double)vectors * seen * c3[w][h];
 }
 
 // Rows of one launch: their scores take at most this much workspace.
@@ -1353,8 +1355,10 @@ int launch_hd(q48_ctx *c, RaArgs &a)
         const long tiles = (a.T * G + vb - 1) / vb;
         const size_t lds = (size_t)vb * (p.spad + 4) * 8;
         // (in step mode the position given says what to expect)
+        const int most = a.p0 + a.T;
+        const double seen = DEC || a.mask ? most : most - 0.5 * a.T;
         if (lds <= rt_lds(HD, 16) &&
-            one_launch<BITS, HD>(vb, a.p0 + a.T, (long)a.T * a.n_heads, tiles * a.n_kv,
+            one_launch<BITS, HD>(vb, most, seen, (long)a.T * a.n_heads, tiles * a.n_kv,
                                  c->cu_count)) {
             constexpr bool WIDE = HD == 64 && BITS != 64 && !DEC;   // (one token: vb is small)
             p.Tn = a.T;
