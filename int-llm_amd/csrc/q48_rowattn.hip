@@ -380,8 +380,9 @@ __device__ __forceinline__ q48_u128 key_digits(v4i (&B)[HD < 64 ? 1 : HD / 64][8
 }
 
 // The 63 digit products by the weight of their sum, 256^d: two chains at a time, and
-// each sum joins the score as soon as it is whole, so that two of the 14 are live
-// instead of all (206 -> 140 registers with HD 64: three waves a SIMD).
+// each sum joins the score as soon as it is whole, under the next pair's products.  All 14
+// at once would take 56 registers for their sums alone, where the operands of both sides
+// leave k_ra_score two waves a SIMD (222 registers) as it is.
 template <int HD>
 __device__ __forceinline__ void word_scores(int64_t (&s)[4], const v4i (*dig)[8][64],
                                             const v4i (&B)[HD < 64 ? 1 : HD / 64][8],
@@ -1381,11 +1382,14 @@ int launch_hd(q48_ctx *c, RaArgs &a)
     constexpr int TB = DEC ? 1 : BITS == 64 && HD < 128 ? 4 : 2;
     // Chunks for about `want` blocks, of 64 rows at least, 128 past 4096: a later launch's
     // blocks read every chunk's maximum or sum, and the values' sums of all chunks meet in
-    // atomics.
-    // us of 48 tokens at 4000 (int64) with 512 / 1024 score blocks 146 / 132, with 512 /
-    // 2048 exponential blocks 146 / 137, with 512 / 1024 value blocks 146 / 147; of 26 at
-    // 2047 (8 bits) 45 / 46, 45 / 43, 45 / 51; of one at 16000 with chunks of 128 / 64
-    // rows 27 / 30 (any of the three).
+    // atomics.  `want` is about what the compute units hold at once (8 exponential blocks
+    // each, 4 score blocks, 2 of int64 keys; 2 value blocks, 1 of 128-wide int64 heads): a
+    // few blocks more are a round more.  us with 512 / 1024 score blocks: 16 tokens at 3000
+    // (8 bits) 40.7 / 37.5, 512 at 1500 319 / 305; int64 48 at 4000 96.7 / 99.9, 200 at 2000
+    // 187 / 197.  1024 / 2048 exponential blocks: 48 at 4000 104 / 100, 512 at 1500 334 /
+    // 319.  256 / 512 / 1024 value blocks: 26 at 2047 (8 bits) 46.8 / 43.1 / 48.8, 48 at
+    // 4000 119 / 100 / 107, 16 at 2000 of 128-wide int64 heads 42.9 / 49.2 / 66.6.  One token
+    // at 16000 with chunks of 128 / 64 rows 27 / 30 (any of the three).
     auto chunk = [&](long blocks, long want, int &ch, int &n) {
         long k = want / blocks, most = p.spad / (S > 4096 ? 128 : 64);
         k = k < most ? k : most;
@@ -1393,9 +1397,9 @@ int launch_hd(q48_ctx *c, RaArgs &a)
         ch = (int)(((S + k - 1) / k + 63) & ~63);
         n = (S + ch - 1) / ch;
     };
-    chunk((tiles + TB - 1) / TB, BITS == 64 ? 1024 : 512, p.ch1, p.n1);
+    chunk((tiles + TB - 1) / TB, BITS == 64 ? 512 : 1024, p.ch1, p.n1);
     chunk(tiles, 2048, p.ch2, p.n2);
-    chunk(tiles, 512, p.ch3, p.n3);
+    chunk(tiles, BITS == 64 && HD == 128 ? 256 : 512, p.ch3, p.n3);
     size_t o = 0;
     auto take = [&](size_t bytes) {
         const size_t at = o;
