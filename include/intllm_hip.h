@@ -475,7 +475,9 @@ int q48_rope_store_rows_qcache(q48_ctx *ctx, int64_t *QKV, const q48_qcache *cac
  * the values the cache stands for.  In step mode pos is read from the
  * device-side state; the kernels are chosen from the pos argument also then, so a
  * graph captured at a short position stays right, and gets slower, as replays move
- * past it.  out shares no words with q, k_new or v_new.  n_heads at most 1024. */
+ * past it.  The context's workspace (scores, for long spans) reaches its size in the
+ * first call of a shape, so call once before capturing.  out shares no words with q,
+ * k_new or v_new.  n_heads at most 1024. */
 int q48_attn_decode_qcache(q48_ctx *ctx, int64_t *out, const int64_t *q, const q48_qcache *cache,
                            const int64_t *k_new, const int64_t *v_new, int layer, int pos,
                            int n_heads);
@@ -494,7 +496,9 @@ int q48_attn_decode_rope_qcache(q48_ctx *ctx, int64_t *out, const int64_t *q,
  * row that attends to nothing (p0 = 0, no bit) gives zeros.  Each row's result
  * is the reference's exact attention (llama_int.c:1502-1529) over the rows it
  * attends to, in cache order, so a token of a tree gets the words that decoding
- * its own path gives.  out [T][n_heads * head_dim] shares no words with QKV.
+ * its own path gives.  Workspace as for q48_attn_decode_qcache (about 1 GiB at
+ * most: more rows take several launches).  out [T][n_heads * head_dim] shares
+ * no words with QKV.
  * head_dim 32, 64 or 128; n_heads at most 1024; p0 + T at most 32767. */
 int q48_attn_tree(q48_ctx *ctx, int64_t *out, const int64_t *QKV, const int64_t *kcache,
                   const int64_t *vcache, int layer, int p0, int T, int n_heads, int n_kv,
@@ -534,7 +538,8 @@ int q48_qcache_keep_rows(q48_ctx *ctx, const q48_qcache *cache, int p0, const in
  *   entropy = logZ + floor(2^48 ((sum (e_i u_i >> 48)) >> b) / z).
  * Unlike fp_safe_exp (fp_math.h:739-744), whose value is 0 below e^-10 and off by
  * up to 0.3% above, e_i is within 4 units of 2^-48 of e^-u: the many improbable
- * tokens of a vocabulary count.  No reference counterpart. */
+ * tokens of a vocabulary count.  Vocabularies past 8192 may use the context's workspace:
+ * call once before capturing.  No reference counterpart. */
 int q48_logprobs_rows(q48_ctx *ctx, const int64_t *logits, int T, int vocab, const int *d_tokens,
                       int64_t *logp, int64_t *entropy, int top_n, int *top_ids,
                       int64_t *top_logp);

