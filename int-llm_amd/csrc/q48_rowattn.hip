@@ -686,29 +686,49 @@ __device__ __forceinline__ bool step_fits(int64_t step)
     return (uint64_t)step <= (uint64_t)1 << (52 - BITS);
 }
 
-// q48_exp_neg with its constants where v_fma_f64 takes them (a multiply-add whose
-// addend is a constant otherwise copies it first: 24 moves in 95 instructions).
+// floor(x^2 / 2^48) for x below 2^56: with h the high word, 2 h and h 2^B fit 32 bits, so
+// that the cross term and the high square are one multiply-add each (B <= 12, x below 2^52;
+// else 8).
+template <int B>
+__device__ __forceinline__ uint64_t square_shr48(uint64_t x)
+{
+    const uint32_t l = (uint32_t)x;
+    uint32_t h = (uint32_t)(x >> 32);
+    asm("" : "+v"(h));   // (shifts of h, not parts of shifts of x)
+    const uint64_t w = (uint64_t)l * (2 * h) + __umulhi(l, l);
+    return (uint64_t)(h << B) * (h << (16 - B)) + (w >> 16);
+}
+
+// q48_exp_neg in fewer operations (95 -> 75).  Its constants stand where v_fma_f64 takes them
+// (a multiply-add whose addend is a constant otherwise copies it first).  The last two
+// squares, of at most e^2.5 and e^5, have small high words.  The reciprocal of r takes one
+// cubic step, y (1 + d + d^2) with d = 1 - r y: y off by 2^-20 becomes 2^-60, and rounding r
+// and y down leaves it within 2^-52 of 1 / r.  Times 2^96 (1 - 2^-50) it is below 2^96 / r <=
+// 2^48 by less than 2^-1, so q1 = floor of it, plus 1, is the quotient or one more; q1 r -
+// 2^96 lies in (-r, r], and the sign of its low 64 bits tells.
 __device__ __forceinline__ uint64_t exp_neg(uint64_t u)
 {
     const uint64_t lim = (uint64_t)10 << 48;
     const bool in = u <= lim;
     double h = __builtin_bit_cast(double, 0x4330000000000000ull + (uint64_t)Q48_ONE +
                                               ((in ? u : lim) >> 14));
-    const double k24 = 0x1p-24, k28 = -0x1p28, k52 = 0x1p52;
+    const double k24 = 0x1p-24, k28 = -0x1p28, k52 = 0x1p52, k96 = 0x1.ffffffffffff8p95;
+    const double one = 0x1p52 + 1;
 #pragma unroll
     for (int k = 0; k < 12; ++k) {
         double y;
         asm("v_fma_f64 %0, %1, %2, %3" : "=v"(y) : "v"(h), "s"(k24), "v"(k28));
         asm("v_fma_f64 %0, %1, %1, %2" : "=v"(h) : "v"(y), "s"(k52));
     }
-    const uint64_t r = (uint64_t)q48_usqr((uint64_t)q48_usqr(q48_word_m52(h)));
+    const uint64_t r = square_shr48<8>(square_shr48<12>(q48_word_m52(h)));
     const double rd = (double)r;
     double y = __builtin_amdgcn_rcp(rd);
-    y = __builtin_fma(y, __builtin_fma(-rd, y, 1.0), y);
-    y = __builtin_fma(y, __builtin_fma(-rd, y, 1.0), y);
-    const uint64_t q0 = q48_word_m52(__builtin_fma(y, 0x1p96, 0x1p52 - 0.5));
-    const uint64_t rem = (uint64_t)0 - q0 * r;
-    return in ? q0 + (rem >= r ? 1 : 0) : 0;
+    const double d = __builtin_fma(-rd, y, 1.0);
+    y = __builtin_fma(y, __builtin_fma(d, d, d), y);
+    double q;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(q) : "v"(y), "s"(k96), "v"(one));
+    const uint64_t q1 = q48_word_m52(q);
+    return in ? q1 - ((int64_t)(q1 * r) > 0 ? 1 : 0) : 0;
 }
 
 // The exponentials of vector t's scores row[j], j = begin + l, + L, ..., in place: 0
@@ -748,25 +768,31 @@ __device__ __forceinline__ uint64_t exp_rows(const RaArgs &a, int p0, int t, int
     return sum;
 }
 
-// 2^48 / d for the quotients of a softmax row (1 <= d < 2^63; 0 for d = 0): as
-// q48_divisor_of, whose bound of 2^62 a row past 16384 positions may pass.  The
-// quotient's bound is the same there: e / d shrinks as d grows.
+// 2^48 (1 - 2^-50) / d for the quotients of a softmax row (1 <= d < 2^63): as
+// q48_divisor_of, whose bound of 2^62 a row past 16384 positions may pass, and always
+// below 2^48 / d, by at most 6 units of 2^-52.
 __device__ __forceinline__ double quotient_factor(uint64_t d)
 {
     const double dd = (double)d;
     double y = __builtin_amdgcn_rcp(dd);
     y = __builtin_fma(y, __builtin_fma(-dd, y, 1.0), y);
     y = __builtin_fma(y, __builtin_fma(-dd, y, 1.0), y);
-    return d ? y * 0x1p48 : 0.0;
+    return y * 0x1.ffffffffffff8p47;
 }
 
-// fp_div(e, den) 2^-48 for 0 <= e <= ONE <= den, or 0 for e = den = 0
+// fp_div(e, den) 2^-48 for 0 <= e <= min(ONE, den), 1 <= den < 2^63, as the reciprocal in
+// exp_neg: t = 2^52 + q1, q1 the quotient (at most 2^48) or one more, q1 den - e 2^48 in
+// (-den, den]; 2^4 + 2^-48 is the double after 2^4.
 __device__ __forceinline__ double quotient_scaled(uint64_t e, uint64_t den, double y48)
 {
     const double ed = __builtin_bit_cast(double, e | 0x4330000000000000ull) - 0x1p52;
-    const uint64_t q0 = q48_word_m52(__builtin_fma(ed, y48, 0x1p52 - 0.5));
-    const uint64_t rem = (e << 48) - q0 * den;
-    return q48_pscaled((int64_t)(q0 + (rem >= den ? 1 : 0)));
+    const double one = 0x1p52 + 1, k48 = 0x1p-48;
+    double t, p;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(t) : "v"(ed), "v"(y48), "v"(one));
+    const int64_t over = (int64_t)(q48_word_m52(t) * den - (e << 48));
+    const double less = __builtin_bit_cast(double, 0x4030000000000000ull | (over > 0 ? 1 : 0));
+    asm("v_fma_f64 %0, %1, %2, -%3" : "=v"(p) : "v"(t), "s"(k48), "v"(less));
+    return p;
 }
 
 // dim d of a vector's sum over rows [begin, end) in integers.  e: exponentials of
@@ -946,7 +972,7 @@ __global__ __launch_bounds__(RT_NT) void k_ra_tile(RaArgs a, RaPlan p)
         ValueRows<BITS, HD> rows(a, kh, lane);
         const int vd = HD == 32 ? lane & 31 : lane, vp = rows.vp;
         for (int r = w / wr; r < nrow; r += RT_NW / wr) {
-            const uint64_t den = total(r);
+            const uint64_t sum = total(r), den = sum ? sum : 1;   // (0: sees nothing)
             const double y48 = quotient_factor(den);
             int64_t *row = sc + r * stride;
 #pragma unroll 2
@@ -1253,6 +1279,7 @@ k_ra_value(RaArgs a, RaPlan p)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             den[i] = dens[4 * i + g];
+            den[i] = den[i] ? den[i] : 1;   // (0: sees nothing)
             y48[i] = quotient_factor(den[i]);
         }
         const int vd = HD == 32 ? lane & 31 : lane, vp = rows.vp;

@@ -605,3 +605,34 @@ def test_verifying_captured(ctx, bits, p0):
             for a, b in zip((*sides[0][:2], *sides[0][2]), (*sides[1][:2], *sides[1][2])):
                 assert (a.download() == b.download()).all()
         intllm.check("drop", lib.q48_graph_drop(c.h))
+
+
+@pytest.mark.parametrize("rows,near", [(64, 64), (64, 3), (4000, 64), (4000, 1000), (32767, 32767)])
+def test_weights_of_chosen_scores(ctx, rows, near):
+    """Scores given directly (q = 8 in one dim of a 64-wide head) and the softmax weights of
+    64 rows read back (a value of ONE in a dim of its own): arguments at the clamp, at the
+    truncation to 2^14ths and down to nothing, sums from one to 32767 times ONE."""
+    hd, lim = 64, 10 << 48
+    rng = np.random.default_rng(rows + near)
+    edges = [0, 1, 2, (1 << 14) - 1, 1 << 14, (1 << 14) + 1, lim - (1 << 14), lim - 1, lim, lim + 1,
+             lim + (1 << 14), 1 << 52, 1 << 61] + [1 << k for k in range(3, 51)]
+    for first in (edges, None):
+        u = np.full(rows, 1 << 60, np.int64)
+        u[:near] = 0 if rows == near and rows > 64 else rng.integers(0, lim, near)
+        n = min(64, near)
+        if first:
+            u[:n] = (first + [0] * 64)[:n] if n == 64 else first[:n]
+        at = rng.permutation(rows)                # the rows read back, anywhere
+        u = u[np.argsort(at)]
+        K, V = np.zeros((rows, 1, hd), np.int64), np.zeros((rows, 1, hd), np.int64)
+        K[:, 0, 5] = -u
+        V[at[:64], 0, np.arange(64)] = P.ONE
+        qkv = np.zeros((1, 3, hd), np.int64)
+        qkv[0, 0, 5] = 8 * P.ONE
+        d, dk, dv = (ctx.to_device(x) for x in (qkv, K, V))
+        out = ctx.buffer(hd)
+        ctx.attn_tree(out.ptr, d.ptr, dk.ptr, dv.ptr, 0, rows - 1, 1, 1, 1, hd, rows)
+        want = P.attend(qkv[:, :1], K, V, np.ones((1, rows), bool))
+        assert (out.download().reshape(1, 1, hd) == want).all()
+        for b in (d, dk, dv, out):
+            b.free()
