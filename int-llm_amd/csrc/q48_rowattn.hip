@@ -214,28 +214,38 @@ struct KeyRow {
 };
 
 // bits 48 .. 111 of step * sum_d q_d c_d from the digit sums: with q = sum_a s_a
-// 256^a + C (q48_digits.hpp), sum_d q_d c_d = sum_a 256^a acc[a] + C cs, below
-// 2^80 (|acc| <= 128 127 128 < 2^21, so two digits join in 32 bits); c0 and c1 are
-// the low and high word of C times cs = sum_d c_d.
+// 256^a + C (q48_digits.hpp), D = sum_d q_d c_d = sum_a 256^a acc[a] + C cs, below
+// 2^80 (|acc| <= 128 127 128 < 2^21).  c0 and c1: the low and high word of C times cs =
+// sum_d c_d, and 2^80 in all, 2^48 of it in c0, so that both halves and D + 2^80 are
+// positive; step 2^32 comes off at the end.  22 operations (38 with signed words).
 __device__ __forceinline__ int64_t code_dot(const v4i (&acc)[8], int i, int64_t c0, int64_t c1,
                                             uint64_t step)
 {
-    int64_t lo = c0 + (acc[0][i] + (acc[1][i] << 8));
-    int64_t hi = c1 + (acc[4][i] + (acc[5][i] << 8));
-    lo = mad_shl<16>(acc[2][i] + (acc[3][i] << 8), lo);
-    hi = mad_shl<16>(acc[6][i] + (acc[7][i] << 8), hi);
-    hi += lo >> 32;
-    // words n0, n1 (unsigned) and n2 (signed) of the sum, s0 and s1 of the step
-    const uint32_t n0 = (uint32_t)lo, n1 = (uint32_t)hi, n2 = (uint32_t)(hi >> 32);
+    int64_t lo = mad_shl<0>(acc[0][i], c0), hi = mad_shl<0>(acc[4][i], c1);
+    lo = mad_shl<8>(acc[1][i], lo);
+    hi = mad_shl<8>(acc[5][i], hi);
+    lo = mad_shl<16>(acc[2][i], lo);
+    hi = mad_shl<16>(acc[6][i], hi);
+    lo = mad_shl<24>(acc[3][i], lo);
+    hi = mad_shl<24>(acc[7][i], hi);
+    hi += (int64_t)(uint32_t)((uint64_t)lo >> 32);
+    // words n0, n1, n2 of the sum, s0 and s1 of the step (below 2^61)
+    const uint32_t n0 = (uint32_t)lo, n1 = (uint32_t)hi, n2 = (uint32_t)((uint64_t)hi >> 32);
     const uint32_t s0 = (uint32_t)step, s1 = (uint32_t)(step >> 32);
-    const uint64_t t = (uint64_t)n0 * s1 + __umulhi(n0, s0);
-    const uint64_t u = (uint64_t)n1 * s0 + (uint32_t)t;
-    const uint64_t v = (uint64_t)n1 * s1 + (t >> 32) + (u >> 32);   // words 2, 3
-    const uint32_t w3 = (uint32_t)(v >> 32) + n2 * s1 + __umulhi(n2, s0) -
-                        ((int32_t)n2 < 0 ? s0 : 0);
-    uint64_t top = ((uint64_t)w3 << 32) | (uint32_t)v;
-    top += (uint64_t)(n2 * s0);
-    return (int64_t)((top << 16) | ((uint32_t)u >> 16));
+    const uint64_t t = (uint64_t)n0 * s1 + __umulhi(n0, s0);   // from bit 32, below 2^62
+    uint64_t u;                                                // n1 s0 + t, and its carry
+    uint32_t carry;
+    asm("v_mad_u64_u32 %0, vcc, %2, %3, %4\n\t"
+        "s_nop 1\n\t"
+        "v_addc_co_u32_e64 %1, vcc, 0, 0, vcc"
+        : "=&v"(u), "=v"(carry)
+        : "v"(n1), "v"(s0), "v"(t)
+        : "vcc");
+    uint64_t w = (uint64_t)n1 * s1 + (((uint64_t)carry << 32) | (uint32_t)(u >> 32));
+    w += (uint64_t)n2 * s0;                                    // from bit 64, 48 bits needed
+    const uint32_t w1 = (uint32_t)(w >> 32) + n2 * s1;
+    return (int64_t)(((uint64_t)(__builtin_amdgcn_alignbit(w1, (uint32_t)w, 16) - s0) << 32) |
+                     __builtin_amdgcn_alignbit((uint32_t)w, (uint32_t)u, 16));
 }
 
 // int64 keys as loaded, 16 dims a lane (dims past the head give digits of zero)
@@ -330,8 +340,8 @@ __device__ __forceinline__ void code_scores(int64_t (&s)[4], const v4i (*dig)[8]
             s[i] = code_dot(acc, i, c0, c1, step);
 }
 
-// C's low and high word times sum_d c_d of the operand's row, on every lane: a
-// product with a row of ones
+// C's low and high word times sum_d c_d of the operand's row (and the bias code_dot wants),
+// on every lane: a product with a row of ones
 template <int HD>
 __device__ __forceinline__ void code_sum(int64_t &c0, int64_t &c1,
                                          const v4i (&B)[HD < 64 ? 1 : HD / 64], int kq)
@@ -342,8 +352,8 @@ __device__ __forceinline__ void code_sum(int64_t &c0, int64_t &c1,
         const int o = 64 * ks + 16 * kq < HD ? 0x01010101 : 0;
         sum = __builtin_amdgcn_mfma_i32_16x16x64_i8((v4i){o, o, o, o}, B[ks], sum, 0, 0, 0);
     }
-    c0 = (int64_t)(uint32_t)kDig * sum[0];
-    c1 = (int64_t)(uint32_t)(kDig >> 32) * sum[0];
+    c0 = (int64_t)(uint32_t)kDig * sum[0] + ((int64_t)1 << 48);
+    c1 = (int64_t)(uint32_t)(kDig >> 32) * sum[0] + ((int64_t)1 << 48) - (1 << 16);
     // the product's other three words are not reused while it may still write them
     asm("" : : "v"(sum), "v"(c0), "v"(c1));
 }
