@@ -447,10 +447,9 @@ __device__ __forceinline__ void word_scores(int64_t (&s)[4], const v4i (*dig)[8]
                         w2[i] = (uint32_t)cur[i];
                     cur[i] = (cur[i] >> 32) + (int64_t)c[i][k / 4];
                 }
-                // |was| <= 8 KS 64 128 128 = 2^24: two join in 64 bits first
-                const int64_t two = mad_shl<8>(was[1][i], (int64_t)was[0][i]);
-                cur[i] = (k & 2) ? (int64_t)((uint64_t)cur[i] + ((uint64_t)two << 16))
-                                 : cur[i] + two;
+                // |was| <= 8 KS 64 128 128 = 2^24: four stay below 2^49
+                cur[i] = (k & 2) ? mad_shl<24>(was[1][i], mad_shl<16>(was[0][i], cur[i]))
+                                 : mad_shl<8>(was[1][i], mad_shl<0>(was[0][i], cur[i]));
             }
         }
         __builtin_amdgcn_sched_barrier(0);
