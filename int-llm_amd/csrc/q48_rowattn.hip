@@ -708,7 +708,7 @@ __device__ __forceinline__ uint64_t square_shr48(uint64_t x)
     return (uint64_t)(h << B) * (h << (16 - B)) + (w >> 16);
 }
 
-// q48_exp_neg in fewer operations (95 -> 75).  Its constants stand where v_fma_f64 takes them
+// q48_exp_neg in fewer operations (98 -> 80, loads and sums of k_ra_exp included).  Its constants stand where v_fma_f64 takes them
 // (a multiply-add whose addend is a constant otherwise copies it first).  The last two
 // squares, of at most e^2.5 and e^5, have small high words.  The reciprocal of r takes one
 // cubic step, y (1 + d + d^2) with d = 1 - r y: y off by 2^-20 becomes 2^-60, and rounding r
@@ -866,12 +866,12 @@ constexpr size_t rt_lds(int hd, int nw) { return 160 * 1024 - rt_static(hd, nw);
 // exponentials, then weights in place.  8 or 16 waves; a wave takes 16 rows at a time for
 // the scores and the values.
 // Bound by vector issue where there are tiles for all compute units: 384 rows at 512 (32
-// heads on 4 of 64, 8 bits), 9.3 M (vector, row) pairs, in 94 us, about 300 instructions
-// per 64 pairs (64 the sums' FP64 operations, 95 the exponential, 25 the quotient) at 88%
+// heads on 4 of 64, 8 bits), 8.7 M (vector, row) pairs, in 88 us, about 280 instructions
+// per 64 pairs (64 the sums' FP64 operations, 80 the exponential, 20 the quotient) at 82%
 // of the rate a SIMD issues FP64 and 64-bit integer operations (one in 4.3 cycles); of a
-// block's 37 us the scores take 8, exponentials 12, quotients 3, values 12.  Few vectors
-// and rows are a chain of latencies: one token at 120 7.4 us, 1.5 of it the query and the
-// new row, 1.3 the scores, 1.1 the exponentials, 0.9 the values.
+// block's 33 us the scores take 7, exponentials 11, quotients 3, values and their sums 12.
+// Few vectors and rows are a chain of latencies: one token at 120 7.2 us, 1.5 of it the query
+// and the new row, 1.3 the scores, 1.0 the exponentials, 0.8 the values.
 template <int BITS, int HD, bool DEC, int RT_NT>
 __global__ __launch_bounds__(RT_NT) void k_ra_tile(RaArgs a, RaPlan p)
 {
@@ -1037,9 +1037,9 @@ __global__ __launch_bounds__(RT_NT) void k_ra_tile(RaArgs a, RaPlan p)
 // The scores of TB tiles of 16 vectors over one chunk, and each vector's maximum
 // over the rows it sees: a row's operand is made once for all TB tiles.  DEC: the
 // store of the new row too (by the blocks that own it).
-// int64 keys: 63 products of 16 cycles for 16 x 16 pairs of 64 dims, and about 250 vector
-// operations to add them up, of two waves a SIMD: 1.7 us a tile for both, 1.0 of it the
-// matrix cores alone.  48 tokens at 4000 (32 heads on 4 of 64; 6.2 M pairs) 44 us, 16 of 8
+// int64 keys: 63 products of 16 cycles for 16 x 16 pairs of 64 dims, and about 200 vector
+// operations to add them up, of two waves a SIMD: 1.5 us a tile for both, 1.0 of it the
+// matrix cores alone.  48 tokens at 4000 (32 heads on 4 of 64; 6.2 M pairs) 41 us, 15 of 8
 // bits (26 at 2047, 1.7 M pairs; 8 products).
 template <int BITS, int HD, int TB, bool DEC>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void
@@ -1135,8 +1135,8 @@ k_ra_score(RaArgs a, RaPlan p)
 }
 
 // Exponentials in place of a chunk's scores (0 for rows a vector does not see,
-// up to the next multiple of 32 rows) and their sums: 95 vector operations each, 24 of
-// them the squarings.  6.2 M in 27 us, 70% of what issue allows; 1.7 M in 13, most of it
+// up to the next multiple of 32 rows) and their sums: 80 vector operations each, 24 of
+// them the squarings.  6.2 M in 25 us, 75% of what issue allows; 1.7 M in 13, most of it
 // the launch, the chunk maxima and the scores on their way from other dies' caches.
 template <bool DEC>
 __global__ __launch_bounds__(256) void k_ra_exp(RaArgs a, RaPlan p)
@@ -1218,7 +1218,7 @@ __global__ __launch_bounds__(256) void k_ra_exp(RaArgs a, RaPlan p)
 // lane l of every row of 16 lanes holds row l % 16's weights.  A chunk with a value
 // outside [-2^51, 2^51), or weights that are no plain softmax, multiplies in
 // integers.
-// Bound by FP64 issue: 16 rows of 16 vectors of 64 dims are 256 sums, 100 operations of
+// Bound by FP64 issue: 16 rows of 16 vectors of 64 dims are 256 sums, 80 operations of
 // quotients and 70 of conversions, 1.9 us for two waves a SIMD and no less.  48 tokens at
 // 4000 over int64 rows 38 us, 25 of it this loop; 26 at 2047 of 8 bits 16 (7 the loop).
 template <int BITS, int HD, bool DEC>
