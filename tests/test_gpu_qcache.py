@@ -636,3 +636,34 @@ def test_weights_of_chosen_scores(ctx, rows, near):
         assert (out.download().reshape(1, 1, hd) == want).all()
         for b in (d, dk, dv, out):
             b.free()
+
+
+def test_workspace_is_not_made_during_a_capture(ctx):
+    """A shape that was never called is refused between begin and end; what was captured
+    replays."""
+    rng = np.random.default_rng(3)
+    lib = intllm.hip_lib()
+    nh, nkv, hd, T, V = 8, 2, 64, 3, 500
+    with intllm.Context(0) as c:
+        p0 = 9000                                # past LDS: scores in the workspace
+        cache = Cache(c, 8, 1, p0 + T, nkv, hd)
+        cache.fill(0, acts(rng, p0 + T, nkv, hd), acts(rng, p0 + T, nkv, hd))
+        x = acts(rng, T, V, sigma=2.0)
+        d, qkv = c.to_device(x), c.to_device(acts(rng, T, nh + 2 * nkv, hd))
+        big = c.to_device(acts(rng, 1, 40000))
+        out, ent = c.to_device(np.full(T * nh * hd, 5, np.int64)), c.buffer(T)
+        intllm.check("begin", lib.q48_graph_begin(c.h))
+        c.logprobs_rows(d.ptr, T, V, None, None, ent.ptr)
+        for call in (lambda: c.attn_rows_qcache(out.ptr, qkv.ptr, cache.c, 0, p0, T, nh),
+                     lambda: c.logprobs_rows(big.ptr, 1, 40000, None, None, ent.ptr)):
+            with pytest.raises(intllm.Q48Error) as e:
+                call()
+            assert e.value.code == intllm.Q48_ESTATE
+        intllm.check("end", lib.q48_graph_end(c.h))
+        for _ in range(3):
+            c.zero(ent.ptr, ent.nbytes)
+            intllm.check("launch", lib.q48_graph_launch(c.h, 1))
+            assert (ent.download() == P.logprobs(x, np.zeros(T, np.int64), 0)[1]).all()
+        assert (out.download() == 5).all()
+        intllm.check("drop", lib.q48_graph_drop(c.h))
+        cache.free()
