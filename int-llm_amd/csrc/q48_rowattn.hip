@@ -1398,9 +1398,11 @@ int launch_hd(q48_ctx *c, RaArgs &a)
     p.spad = (S + 63) & ~63;
     {
         // Tiles of the fewest vectors (a power of two) that still leave about a block a
-        // compute unit, and whose scores fit LDS.  Full tiles of many rows take 16
-        // waves where those keep their registers (128 each; us, 16 / 8 waves: 384 rows
-        // at 512 94 / 104, 256 rows at 0 30.1 / 27.4).
+        // compute unit, and whose scores fit LDS.  16 waves where those keep their
+        // registers (128 each) and a block is alone on its compute unit: by the number
+        // of blocks, or because two of 8 waves do not fit LDS.  us, 16 / 8 waves: 384
+        // rows at 512 87.5 / 100.6, 64 at 900 27.2 / 30.0, 256 at 200 41.7 / 46.7; two
+        // blocks of 8 waves a unit: 256 at 0 29.0 / 25.3, 256 at 192 37.9 / 33.8.
         int vb = 16;
         while (vb > 1 && ((a.T * G + vb - 1) / vb) * a.n_kv < c->cu_count)
             vb >>= 1;
@@ -1414,11 +1416,13 @@ int launch_hd(q48_ctx *c, RaArgs &a)
         if (lds <= rt_lds(HD, 16) &&
             one_launch<BITS, HD>(vb, most, seen, (long)a.T * a.n_heads, tiles * a.n_kv,
                                  c->cu_count)) {
-            constexpr bool WIDE = HD == 64 && BITS != 64 && !DEC;   // (one token: vb is small)
+            constexpr bool WIDE = HD == 64 && BITS != 64 && !DEC;   // (decode: spills)
             p.Tn = a.T;
             p.vb = vb;
             const dim3 grid(tiles, a.n_kv);
-            if (WIDE && vb == 16 && S >= 512)
+            const bool alone = tiles * a.n_kv <= c->cu_count ||
+                               2 * (lds + rt_static(HD, 8)) > 160 * 1024;
+            if (WIDE && vb == 16 && alone)
                 hipLaunchKernelGGL((k_ra_tile<BITS, HD, DEC, WIDE ? 1024 : 512>), grid, dim3(1024),
                                    lds, c->stream, a, p);
             else
