@@ -1397,12 +1397,15 @@ int launch_hd(q48_ctx *c, RaArgs &a)
     RaPlan p = {};
     p.spad = (S + 63) & ~63;
     {
-        // Tiles of the fewest vectors (a power of two) that still leave about a block a
-        // compute unit, and whose scores fit LDS.  16 waves where those keep their
-        // registers (128 each) and a block is alone on its compute unit: by the number
-        // of blocks, or because two of 8 waves do not fit LDS.  us, 16 / 8 waves: 384
-        // rows at 512 87.5 / 100.6, 64 at 900 27.2 / 30.0, 256 at 200 41.7 / 46.7; two
-        // blocks of 8 waves a unit: 256 at 0 29.0 / 25.3, 256 at 192 37.9 / 33.8.
+        // Tiles of the most vectors (a power of two) that still leave about a block a
+        // compute unit, and whose scores fit LDS.  Of the tiles of 16 vectors, those of
+        // 64-wide heads over codes take 16 waves (they keep their 128 registers each)
+        // where a block is alone on its compute unit: there are as many blocks as units,
+        // or two of 8 waves do not fit LDS.  us, 16 / 8 waves, 32 heads on 4, 8 bits: 128
+        // rows (256 blocks) at 0 12.9 / 13.4, at 300 20.9 / 23.1, at 600 30.3 / 34.3; 256
+        // at 200 41.8 / 46.9, 384 at 512 87.3 / 100.8 (4 bits 89.4 / 103.3); two blocks of
+        // 8 waves a unit: 256 at 0 29.0 / 25.3, 256 at 192 37.9 / 33.8.  Tiles of fewer
+        // vectors have 8 waves.
         int vb = 16;
         while (vb > 1 && ((a.T * G + vb - 1) / vb) * a.n_kv < c->cu_count)
             vb >>= 1;

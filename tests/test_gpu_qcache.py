@@ -667,3 +667,36 @@ def test_workspace_is_not_made_during_a_capture(ctx):
         assert (out.download() == 5).all()
         intllm.check("drop", lib.q48_graph_drop(c.h))
         cache.free()
+
+
+def tiles_of_sixteen(cus, nh, nkv, T):
+    """Whether T rows have a block of 16 query vectors for every compute unit (the rule
+    of q48_attn_rows_qcache for its largest tiles), and how many blocks that makes."""
+    blocks = -(-T * (nh // nkv) // 16) * nkv
+    return blocks >= cus, blocks
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("how", ["a block a unit", "scores fill the unit"])
+@pytest.mark.parametrize("kind", ["causal", "tree", "nothing", "big_values", "huge_scores"])
+def test_rows_of_sixteen_waves(ctx, bits, how, kind):
+    """Rows of 64-wide heads whose blocks are alone on a compute unit, which take 16 waves:
+    as many blocks as units, or more where two blocks' scores do not fit one unit (the last
+    tile of them short)."""
+    torch = pytest.importorskip("torch")
+    cus = torch.cuda.get_device_properties(0).multi_processor_count
+    nh, nkv, hd = 32, 4, 64
+    T, p0 = cus // nkv * 16 // (nh // nkv), 0
+    if how == "scores fill the unit":
+        T, p0 = T + 21, 700                    # 16 vectors of 849 scores: more than 80 KB
+    full, blocks = tiles_of_sixteen(cus, nh, nkv, T)
+    assert full and (blocks == cus if p0 == 0 else (p0 + T) * 16 * 8 > 80 << 10)
+    rng = np.random.default_rng(T + bits)
+    sees = None
+    if kind in ("tree", "big_values"):
+        sees, _ = P.tree(rng, T, 3)
+    if kind == "nothing":
+        sees = rng.random((T, T)) < 0.02
+        sees[T // 2:] = False
+    edit = dict(big_values=big_values, huge_scores=huge_scores).get(kind)
+    rows_case(ctx, bits, nh, nkv, hd, T, p0, p0 + T, sees, rng, edit=edit, junk=sees is not None)
