@@ -700,3 +700,48 @@ def test_rows_of_sixteen_waves(ctx, bits, how, kind):
         sees[T // 2:] = False
     edit = dict(big_values=big_values, huge_scores=huge_scores).get(kind)
     rows_case(ctx, bits, nh, nkv, hd, T, p0, p0 + T, sees, rng, edit=edit, junk=sees is not None)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("max_seq,start,nh,nkv,hd", [(900, 2, 8, 2, 64), (3000, 2, 8, 2, 64),
+                                                     (3000, 2990, 8, 2, 64), (20500, 2, 2, 1, 32)])
+def test_one_graph_at_every_position(ctx, bits, max_seq, start, nh, nkv, hd):
+    """One decode captured at a position and replayed at far and near ones, the position
+    set on the device between replays: one launch, three chosen by the position it was
+    captured at, and three because the cache's scores do not fit LDS."""
+    rng = np.random.default_rng(max_seq + bits)
+    lib = intllm.hip_lib()
+    with intllm.Context(0) as c:
+        c.rope_init(hd, max_seq, 10000)
+        cache = Cache(c, bits, 1, max_seq, nkv, hd)
+        cache.fill(0, acts(rng, max_seq, nkv, hd), acts(rng, max_seq, nkv, hd))
+        q, kn, vn = (c.to_device(acts(rng, m, hd)) for m in (nh, nkv, nkv))
+        out, want = c.buffer(nh * hd), c.buffer(nh * hd)
+
+        def step(to, pos):
+            c.attn_decode_rope_qcache(to.ptr, q.ptr, cache.c, kn.ptr, vn.ptr, 0, pos, nh)
+
+        intllm.check("mode", lib.q48_step_mode(c.h, 1))
+        intllm.check("set", lib.q48_step_set(c.h, 0, start))
+        step(out, start)
+        c.sync()
+        intllm.check("begin", lib.q48_graph_begin(c.h))
+        step(out, start)
+        intllm.check("end", lib.q48_graph_end(c.h))
+        for pos in (start, 700, max_seq - 1, 0, 31, max_seq - 2, 2040 % max_seq, start):
+            intllm.check("set", lib.q48_step_set(c.h, 0, pos))
+            intllm.check("launch", lib.q48_graph_launch(c.h, 1))
+            got = out.download()
+            intllm.check("mode", lib.q48_step_mode(c.h, 0))
+            step(want, pos)
+            assert (want.download() == got).all(), pos
+            k, v, ks, vs = cache.read()
+            kv, vv = (P.values(P.unpack(x[0, :pos + 1], bits), s[0, :pos + 1])
+                      for x, s in ((k, ks), (v, vs)))
+            cos_t, sin_t = P.rope_tables(hd, max_seq)
+            qr = P.rope(q.download().reshape(nh, hd), cos_t, sin_t, pos)
+            exp = P.attend(qr[None], kv, vv, np.ones((1, pos + 1), bool))
+            assert (got.reshape(1, nh, hd) == exp).all(), pos
+            intllm.check("mode", lib.q48_step_mode(c.h, 1))
+        intllm.check("drop", lib.q48_graph_drop(c.h))
+        cache.free()
