@@ -197,3 +197,23 @@ def test_captured_over_many_blocks(ctx):
             call(T)
             assert all((b.download() == g).all() for b, g in zip(outs, got))
         intllm.check("drop", lib.q48_graph_drop(c.h))
+
+
+@pytest.mark.parametrize("width", [700, 9000])
+def test_differences_at_multiples_of_ln2(ctx, width):
+    """u = k LN2 and a word to either side, alone and with whole steps of the table, up to
+    where e is 0: the quotient of u by LN2 is settled by a comparison there."""
+    us = {max(0, k * P.LN2 + j * (1 << 42) + d) for k in range(51) for j in (0, 1, 22, 44)
+          for d in (-1, 0, 1)}
+    us = np.array(sorted(us), dtype=np.int64)
+    assert us.size <= width
+    rng = np.random.default_rng(width)
+    x = np.full((4, width), -(60 * P.LN2), dtype=np.int64)
+    for t, m in enumerate((0, 5 * P.ONE + 1, -(1 << 60), I64.max)):
+        x[t] = m - 60 * P.LN2
+        x[t, rng.permutation(width)[:us.size]] = m - us
+    check_rows(ctx, x, rng.integers(0, width, 4), 32)
+    for t in range(4):                         # each alone beside the largest: Z says what e is
+        y = np.full((us.size, 2), x[t].max(), dtype=np.int64)
+        y[:, 1] -= us
+        check_rows(ctx, y, np.ones(us.size, np.int64), 2)
