@@ -496,8 +496,8 @@ int q48_attn_decode_rope_qcache(q48_ctx *ctx, int64_t *out, const int64_t *q,
  * row that attends to nothing (p0 = 0, no bit) gives zeros.  Each row's result
  * is the reference's exact attention (llama_int.c:1502-1529) over the rows it
  * attends to, in cache order, so a token of a tree gets the words that decoding
- * its own path gives.  Workspace as for q48_attn_decode_qcache (about 1 GiB at
- * most: more rows take several launches).  out [T][n_heads * head_dim] shares
+ * its own path gives.  Workspace as for q48_attn_decode_qcache (1 GiB of scores at
+ * most, and a thirtieth of that beside them: more rows take several launches).  out [T][n_heads * head_dim] shares
  * no words with QKV.
  * head_dim 32, 64 or 128; n_heads at most 1024; p0 + T at most 32767. */
 int q48_attn_tree(q48_ctx *ctx, int64_t *out, const int64_t *QKV, const int64_t *kcache,

@@ -101,14 +101,16 @@ __device__ __forceinline__ int64_t row16_max64(int64_t v)
 //    sum before the first quotient, and its truncations leave no way to rescale
 //    later, so each of the two is a launch boundary.
 struct RaPlan {
-    int64_t *sc;     // [n_kv][16 tiles][spad]: scores, then exponentials
-    int64_t *cm;     // [n_kv][16 tiles][n1]: a chunk's maximum
-    uint64_t *cs;    // [n_kv][16 tiles][n2]: a chunk's sum of exponentials
+    int64_t *sc;     // [n_kv][tv tiles][spad]: scores, then exponentials
+    int64_t *cm;     // [n_kv][tv tiles][n1]: a chunk's maximum
+    uint64_t *cs;    // [n_kv][tv tiles][n2]: a chunk's sum of exponentials
     int *far;        // [n_kv][tiles][n1]: a visible score outside [-2^62, 2^62)
     int *odd;        // [n_kv][tiles][n2]: an exponential outside [0, ONE]
     int ch1, n1, ch2, n2, ch3, n3;   // rows a chunk, and chunks, of each launch
     int spad, tiles, t0, Tn;         // rows t0 .. t0 + Tn - 1 of the T
-    int vb;                          // vectors a tile
+    int vb;                          // vectors a tile (one launch)
+    int tv;                          // vectors a tile has room for: 16, or those of a single
+                                     // tile of fewer
 };
 
 // rows [0, span) hold all that vectors up to vlast may see
@@ -1103,12 +1105,12 @@ k_ra_score(RaArgs a, RaPlan p)
         for (int i = 0; i < 4; ++i)
             mx[tb][i] = INT64_MIN;
     }
-    int64_t *sc = p.sc + ((size_t)kh * p.tiles + tile0) * 16 * p.spad;
+    int64_t *sc = p.sc + ((size_t)kh * p.tiles + tile0) * p.tv * p.spad;
     score_rows<BITS, HD, TB, 4, DEC>(a, dig, cq, vt, ntile, min(16, NV - 16 * tile0), kh, p0,
                                      begin, end, nk[0], DEC && BITS != 64 ? nst[0] : 0,
                                      rows_clear<DEC>(a, p0, p.t0 + 16 * tile0 / G), w, lane, mx,
                                      far, next, [&](int tb, int m, int j, int64_t s) {
-                                         if (!DEC || m < NV - 16 * tile0)
+                                         if (m < NV - 16 * tile0)   // (tv rows)
                                              sc[(size_t)(16 * tb + m) * p.spad + j] = s;
                                      });
 #pragma unroll
@@ -1123,12 +1125,12 @@ k_ra_score(RaArgs a, RaPlan p)
             atomicOr(&farw[tb], 1);
     }
     __syncthreads();
-    if (tid < ntile * 16) {
+    if (tid < ntile * p.tv) {   // (tv < 16: one tile)
         int64_t m = mxs[0][tid];
 #pragma unroll
         for (int u = 1; u < 4; ++u)
             m = mxs[u][tid] > m ? mxs[u][tid] : m;
-        p.cm[(((size_t)kh * p.tiles + tile0) * 16 + tid) * p.n1 + blockIdx.x] = m;
+        p.cm[(((size_t)kh * p.tiles + tile0) * p.tv + tid) * p.n1 + blockIdx.x] = m;
     }
     if (tid < ntile)
         p.far[((size_t)kh * p.tiles + tile0 + tid) * p.n1 + blockIdx.x] = farw[tid];
@@ -1158,7 +1160,7 @@ __global__ __launch_bounds__(256) void k_ra_exp(RaArgs a, RaPlan p)
     // lanes of a vector: 16, or 32 or 64 where the tile has few vectors
     const int lg = nrow > 8 ? 4 : nrow > 4 ? 5 : 6, L = 1 << lg;
     const int r = tid >> lg, l = tid & (L - 1);
-    const size_t vec = ((size_t)kh * p.tiles + tile) * 16 + min(r, nrow - 1);
+    const size_t vec = ((size_t)kh * p.tiles + tile) * p.tv + min(r, nrow - 1);
     const int *farp = p.far + ((size_t)kh * p.tiles + tile) * p.n1;
     const int64_t *cm = p.cm + vec * p.n1;
     int64_t *sc = p.sc + vec * p.spad;
@@ -1242,7 +1244,7 @@ k_ra_value(RaArgs a, RaPlan p)
     if (begin >= end)
         return;
     const int chunks = (span + p.ch2 - 1) / p.ch2;
-    const size_t vec0 = ((size_t)kh * p.tiles + tile) * 16;
+    const size_t vec0 = ((size_t)kh * p.tiles + tile) * p.tv;
     const int64_t *sc = p.sc + vec0 * p.spad;
     // the wave's first exponentials and values on their way while the sums are joined
     ValueRows<BITS, HD> rows(a, kh, lane);
@@ -1253,7 +1255,8 @@ k_ra_value(RaArgs a, RaPlan p)
             if (4 * i < nrow)
 #pragma unroll
                 for (int u = 0; u < PG; ++u)
-                    er[PG * i + u] = (uint64_t)sc[(size_t)(4 * i + g) * p.spad + j0 + 16 * u + rl];
+                    er[PG * i + u] =
+                        (uint64_t)sc[(size_t)min(4 * i + g, nrow - 1) * p.spad + j0 + 16 * u + rl];
     };
     constexpr bool AHEAD = BITS != 64;   // (registers)
     if (begin + CP * w < end) {
@@ -1385,7 +1388,8 @@ bool one_launch(int vb, int most, double seen, long vectors, long blocks, int cu
     return o[w] + rows * (c0[w][h] + c1[w][h] * vb) <= l[w] + (double)vectors * seen * c3[w][h];
 }
 
-// Rows of one launch: their scores take at most this much workspace.
+// Rows of one launch: their scores, in whole tiles of every KV head, take at most this
+// much workspace.  (A single row's 1024 vectors of 32767 scores always fit.)
 constexpr size_t RA_WS_MAX = (size_t)1 << 30;
 
 template <int BITS, int HD, bool DEC>
@@ -1434,10 +1438,13 @@ int launch_hd(q48_ctx *c, RaArgs &a)
             return hipGetLastError() == hipSuccess ? Q48_OK : Q48_EHIP;
         }
     }
-    const size_t row_bytes = (size_t)a.n_heads * p.spad * 8;
-    int Tn = (int)(RA_WS_MAX / row_bytes);
+    long fit = (long)(RA_WS_MAX / ((size_t)a.n_kv * p.spad * 8));   // vectors a KV head
+    if (fit > 16)
+        fit &= ~15L;
+    long Tn = fit / G;
     Tn = Tn < 1 ? 1 : Tn < a.T ? Tn : a.T;
-    p.tiles = (Tn * G + 15) / 16;
+    p.tiles = (int)((Tn * G + 15) / 16);
+    p.tv = Tn * G < 16 ? (int)(Tn * G) : 16;
     const long tiles = (long)p.tiles * a.n_kv;
     constexpr int TB = DEC ? 1 : BITS == 64 && HD < 128 ? 4 : 2;
     // Chunks for about `want` blocks, of 64 rows at least, 128 past 4096: a later launch's
@@ -1466,7 +1473,7 @@ int launch_hd(q48_ctx *c, RaArgs &a)
         o += (bytes + 255) & ~(size_t)255;
         return at;
     };
-    const size_t vecs = (size_t)a.n_kv * p.tiles * 16;
+    const size_t vecs = (size_t)a.n_kv * p.tiles * p.tv;
     const size_t o_sc = take(vecs * p.spad * 8), o_cm = take(vecs * p.n1 * 8);
     const size_t o_cs = take(vecs * p.n2 * 8);
     const size_t o_far = take(tiles * p.n1 * 4), o_odd = take(tiles * p.n2 * 4);
@@ -1480,7 +1487,7 @@ int launch_hd(q48_ctx *c, RaArgs &a)
     p.far = (int *)(ws + o_far);
     p.odd = (int *)(ws + o_odd);
     for (p.t0 = 0; p.t0 < a.T; p.t0 += Tn) {
-        p.Tn = Tn < a.T - p.t0 ? Tn : a.T - p.t0;
+        p.Tn = Tn < a.T - p.t0 ? (int)Tn : a.T - p.t0;
         const int nt = (p.Tn * G + 15) / 16;
         hipLaunchKernelGGL((k_ra_score<BITS, HD, TB, DEC>),
                            dim3(p.n1, (nt + TB - 1) / TB, a.n_kv), dim3(256), 0, c->stream, a, p);

@@ -745,3 +745,32 @@ def test_one_graph_at_every_position(ctx, bits, max_seq, start, nh, nkv, hd):
             intllm.check("mode", lib.q48_step_mode(c.h, 1))
         intllm.check("drop", lib.q48_graph_drop(c.h))
         cache.free()
+
+
+@pytest.mark.parametrize("nkv,T,p0", [(240, 40, 32700), (1024, 1, 12000), (960, 20, 8100)])
+def test_workspace_of_many_key_heads(ctx, nkv, T, p0):
+    """One query head a KV head, so that a tile of 16 vectors is 16 rows: the scores stay
+    within a GiB (and 2 / 64 of it for the maxima and sums of chunks of 64 rows), however
+    the rows divide by 16.  Some heads against the plain form."""
+    torch = pytest.importorskip("torch")
+    hd, S, dev = 32, p0 + T, "cuda:0"
+    g = torch.Generator(device=dev).manual_seed(nkv)
+    codes = [torch.randint(-128, 128, (S, nkv, hd // 2), generator=g, device=dev, dtype=torch.int8)
+             for _ in range(2)]
+    steps = [torch.randint(1, 1 << 45, (S, nkv), generator=g, device=dev) for _ in range(2)]
+    x = torch.randint(-P.ONE, P.ONE, (T, 3 * nkv, hd), generator=g, device=dev)
+    out = torch.zeros(T, nkv, hd, dtype=torch.int64, device=dev)
+    torch.cuda.synchronize()
+    with intllm.Context(0) as c:
+        cache = c.qcache(*(t.data_ptr() for t in (*codes, *steps)), 4, 1, S, nkv, hd)
+        before = torch.cuda.mem_get_info()[0]
+        c.attn_rows_qcache(out.data_ptr(), x.data_ptr(), cache, 0, p0, T, nkv)
+        c.sync()
+        used = before - torch.cuda.mem_get_info()[0]
+        assert used <= (1 << 30) * 67 // 64, used
+    see = np.concatenate([np.ones((T, p0), bool), np.tri(T, dtype=bool)], 1)
+    for h in (0, nkv // 2 + 1, nkv - 1):
+        kv, vv = (P.values(P.unpack(b[:, h].cpu().numpy().view(np.uint8), 4),
+                           s[:, h].cpu().numpy())[:, None] for b, s in zip(codes, steps))
+        want = P.attend(x[:, h:h + 1].cpu().numpy(), kv, vv, see)
+        assert (out[:, h:h + 1].cpu().numpy() == want).all(), h
