@@ -11,6 +11,7 @@ namespace {
 
 constexpr int64_t LP_LN2 = 195103586505167LL;   // fp_log's ln 2 (fp_math.h:752-773)
 constexpr int LP_MAX_TOP = 32;
+constexpr int LP_MAX_ROWS = 1 << 30;   // a row's number and a grid's stride add up in 31 bits
 constexpr int LP_CAP = 512;   // candidates of a row; past that (ties) the slow selection
 
 // round(2^48 e^(-j/64)), round(2^48 / k!), floor(2^54 / (64 + j)),
@@ -696,7 +697,7 @@ extern "C" {
 int q48_logprobs_rows(q48_ctx *c, const int64_t *logits, int T, int vocab, const int *d_tokens,
                       int64_t *logp, int64_t *entropy, int top_n, int *top_ids, int64_t *top_logp)
 {
-    if (!c || !logits || T <= 0 || vocab <= 0 || vocab > (1 << 22) || top_n < 0 ||
+    if (!c || !logits || T <= 0 || T > LP_MAX_ROWS || vocab <= 0 || vocab > (1 << 22) || top_n < 0 ||
         top_n > LP_MAX_TOP || top_n > vocab || (logp && !d_tokens) ||
         (top_n > 0 && (!top_ids || !top_logp)) || (!logp && !entropy && top_n == 0))
         return Q48_EINVAL;

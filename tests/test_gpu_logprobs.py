@@ -217,3 +217,16 @@ def test_differences_at_multiples_of_ln2(ctx, width):
         y = np.full((us.size, 2), x[t].max(), dtype=np.int64)
         y[:, 1] -= us
         check_rows(ctx, y, np.ones(us.size, np.int64), 2)
+
+
+def test_sizes_out_of_range_are_refused(ctx):
+    """Nothing is launched: the buffers are of one row."""
+    d, e, ids, lp = ctx.to_device(np.full(64, 3)), ctx.to_device(np.full(2, 5)), *(
+        ctx.buffer(64) for _ in range(2))
+    big = (1 << 30) + 1
+    for T, V, top in ((0, 1, 0), (-1, 1, 0), (big, 1, 0), ((1 << 31) - 1, 1, 0), (1, 0, 0),
+                      (1, (1 << 22) + 1, 0), (1, 8, -1), (1, 8, 9), (1, 64, 33)):
+        with pytest.raises(intllm.Q48Error) as err:
+            ctx.logprobs_rows(d.ptr, T, V, None, None, e.ptr, top, ids.ptr, lp.ptr)
+        assert err.value.code == intllm.Q48_EINVAL, (T, V, top)
+    assert (e.download() == 5).all()
