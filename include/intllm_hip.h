@@ -526,7 +526,8 @@ int q48_qcache_keep_rows(q48_ctx *ctx, const q48_qcache *cache, int p0, const in
  * vocab) most probable tokens, ties to the lowest id, with their log
  * probabilities.  logp (with d_tokens) and entropy may be NULL, top_ids and
  * top_logp [T][top_n] where top_n is 0, but not all of them.  vocab at most
- * 2^22, T at most 2^30.  All in Q16.48: with m = max x, u_i = m - x_i (64 bits, unsigned),
+ * 2^22, T at most 2^30.  The outputs share no words with the logits or the
+ * tokens (but top_ids may be d_tokens where top_n is 1).  All in Q16.48: with m = max x, u_i = m - x_i (64 bits, unsigned),
  *   e_i = floor(floor(T_j h 2^-48) 2^-n), u_i = n LN2 + j 2^42 + s, 0 <= s < 2^42,
  *         j <= 44, LN2 = 195103586505167, T_j = round(2^48 e^(-j/64)),
  *         h = C_0 - (s (C_1 - (s (... C_6) >> 48)) >> 48), C_k = round(2^48 / k!)

@@ -690,6 +690,12 @@ __global__ __launch_bounds__(256) void k_lp_sum(const int64_t *__restrict__ X, i
         lp_select<256>(x, V, m, slogz, t, top, ids, tlp, tid, bv, bi);
 }
 
+// whether two arrays (or a null one) have bytes in common
+bool lp_share(const void *a, size_t na, const void *b, size_t nb)
+{
+    return a && b && na && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
 } // namespace
 
 extern "C" {
@@ -700,6 +706,16 @@ int q48_logprobs_rows(q48_ctx *c, const int64_t *logits, int T, int vocab, const
     if (!c || !logits || T <= 0 || T > LP_MAX_ROWS || vocab <= 0 || vocab > (1 << 22) || top_n < 0 ||
         top_n > LP_MAX_TOP || top_n > vocab || (logp && !d_tokens) ||
         (top_n > 0 && (!top_ids || !top_logp)) || (!logp && !entropy && top_n == 0))
+        return Q48_EINVAL;
+    const size_t n = T, nt = n * top_n;
+    auto over = [&](const void *in, size_t bytes) {   // an output that shares words with it
+        return lp_share(logp, 8 * n, in, bytes) || lp_share(entropy, 8 * n, in, bytes) ||
+               lp_share(top_logp, 8 * nt, in, bytes);
+    };
+    // (one id a row may replace the row's token: it is read first)
+    const bool same = top_n == 1 && top_ids == d_tokens;
+    if (over(logits, 8 * n * vocab) || lp_share(top_ids, 4 * nt, logits, 8 * n * vocab) ||
+        (logp && (over(d_tokens, 4 * n) || (!same && lp_share(top_ids, 4 * nt, d_tokens, 4 * n)))))
         return Q48_EINVAL;
     q48_on_device on(c);
     // A block a row where the row fits its registers and there are rows for most compute

@@ -230,3 +230,34 @@ def test_sizes_out_of_range_are_refused(ctx):
             ctx.logprobs_rows(d.ptr, T, V, None, None, e.ptr, top, ids.ptr, lp.ptr)
         assert err.value.code == intllm.Q48_EINVAL, (T, V, top)
     assert (e.download() == 5).all()
+
+
+def test_outputs_over_the_inputs_are_refused(ctx):
+    """A row's results are written while other rows are still read."""
+    rng = np.random.default_rng(3)
+    T, V, top = 600, 300, 2
+    x, tokens = logits(rng, T, V), rng.integers(0, V, T)
+    d, tk = ctx.to_device(x), ints(ctx, tokens)
+    a, b, i, l = (ctx.to_device(np.full(T * top, 5)) for _ in range(4))
+    inner = d.at(T * V - 1)
+    for logp, ent, ids, tlp in ((d.ptr, b.ptr, i.ptr, l.ptr), (a.ptr, inner, i.ptr, l.ptr),
+                                (a.ptr, b.ptr, d.ptr, l.ptr), (a.ptr, b.ptr, i.ptr, d.at(3)),
+                                (tk.ptr, b.ptr, i.ptr, l.ptr), (a.ptr, b.ptr, tk.ptr, l.ptr),
+                                (d.ptr - 8 * (T - 1), b.ptr, i.ptr, l.ptr)):
+        with pytest.raises(intllm.Q48Error) as err:
+            ctx.logprobs_rows(d.ptr, T, V, tk.ptr, logp, ent, top, ids, tlp)
+        assert err.value.code == intllm.Q48_EINVAL
+    assert (d.download() == x.ravel()).all() and (a.download() == 5).all()
+    assert (tk.download().view(np.int32)[:T] == tokens).all()
+
+
+@pytest.mark.parametrize("T,V", [(600, 300), (3, 20000)])
+def test_the_most_probable_token_in_place_of_the_scored_one(ctx, T, V):
+    rng = np.random.default_rng(V)
+    x, tokens = logits(rng, T, V), rng.integers(0, V, T)
+    d, tk, apart = ctx.to_device(x), ints(ctx, tokens), ints(ctx, tokens)
+    a, b, l, ids = (ctx.buffer(T) for _ in range(4))
+    ctx.logprobs_rows(d.ptr, T, V, apart.ptr, b.ptr, None, 1, ids.ptr, l.ptr)
+    ctx.logprobs_rows(d.ptr, T, V, tk.ptr, a.ptr, None, 1, tk.ptr, l.ptr)
+    assert (tk.download().view(np.int32)[:T] == x.argmax(1)).all()
+    assert (a.download() == b.download()).all()
