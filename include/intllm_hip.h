@@ -46,6 +46,15 @@ typedef struct q48_ctx q48_ctx;
  * the fp_math constants (FP_PI, CORDIC angles and gain) computed on the
  * device exactly as fp_math_init does (fp_math.h:833-858). */
 int q48_ctx_create(q48_ctx **out, int device);
+/* The same with ops enqueued on the caller's stream (a hipStream_t of that
+ * device, NULL for the default stream) instead of one of the context's own,
+ * so that they are ordered with what the caller enqueues there: a context's
+ * own stream is ordered with no other, the default stream included, and only
+ * synchronising both sides makes data pass.  The stream outlives the context.
+ * Capture it with q48_graph_* (not the default stream: Q48_ESTATE).  While
+ * the caller captures it by other means, ops that use a workspace or the
+ * one-launch split attention return Q48_ESTATE, and so does this call. */
+int q48_ctx_create_on(q48_ctx **out, int device, void *stream);
 int q48_ctx_destroy(q48_ctx *ctx);
 
 int q48_malloc(q48_ctx *ctx, void **dptr, size_t bytes);

@@ -55,8 +55,18 @@ void free_retired(q48_ctx *c)
 }
 } // namespace
 
+bool q48_foreign_capture(q48_ctx *c)
+{
+    if (!c->lent || !c->stream || c->capturing)
+        return false;
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    return hipStreamIsCapturing(c->stream, &st) != hipSuccess || st != hipStreamCaptureStatusNone;
+}
+
 int q48_ws_reserve(q48_ctx *c, size_t bytes)
 {
+    if (q48_foreign_capture(c))
+        return Q48_ESTATE;
     if (bytes <= c->ws_bytes)
         return Q48_OK;
     if (c->capturing)
@@ -80,6 +90,8 @@ int q48_ws_reserve(q48_ctx *c, size_t bytes)
 
 int q48_rms_reserve(q48_ctx *c, int blocks)
 {
+    if (q48_foreign_capture(c))
+        return Q48_ESTATE;
     if (blocks <= c->rms_blocks)
         return Q48_OK;
     if (c->capturing)
@@ -118,7 +130,7 @@ const char *q48_strerror(int code)
     }
 }
 
-int q48_ctx_create(q48_ctx **out, int device)
+static int ctx_create(q48_ctx **out, int device, bool lent, hipStream_t stream)
 {
     if (!out)
         return Q48_EINVAL;
@@ -128,6 +140,18 @@ int q48_ctx_create(q48_ctx **out, int device)
         return Q48_EINVAL;
     if (hipSetDevice(device) != hipSuccess)
         return Q48_EHIP;
+    if (lent) {
+        hipDevice_t at = device;
+        hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+        if (stream && (hipStreamGetDevice(stream, &at) != hipSuccess || at != device)) {
+            (void)hipGetLastError();
+            return Q48_EINVAL;
+        }
+        if (hipStreamIsCapturing(stream, &st) != hipSuccess || st != hipStreamCaptureStatusNone) {
+            (void)hipGetLastError();
+            return Q48_ESTATE;   // (creating synchronises the stream)
+        }
+    }
     q48_ctx *c = new (std::nothrow) q48_ctx();
     if (!c)
         return Q48_ENOMEM;
@@ -137,7 +161,9 @@ int q48_ctx_create(q48_ctx **out, int device)
             hipSuccess ||
         c->cu_count <= 0)
         c->cu_count = 1;
-    if (hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking) != hipSuccess) {
+    c->lent = lent;
+    c->stream = stream;
+    if (!lent && hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking) != hipSuccess) {
         delete c;
         return Q48_EHIP;
     }
@@ -179,11 +205,18 @@ int q48_ctx_create(q48_ctx **out, int device)
     return Q48_OK;
 }
 
+int q48_ctx_create(q48_ctx **out, int device) { return ctx_create(out, device, false, nullptr); }
+
+int q48_ctx_create_on(q48_ctx **out, int device, void *stream)
+{
+    return ctx_create(out, device, true, (hipStream_t)stream);
+}
+
 int q48_ctx_destroy(q48_ctx *c)
 {
     if (!c)
         return Q48_EINVAL;
-    if (c->stream)
+    if (c->stream || c->lent)
         (void)hipStreamSynchronize(c->stream);
     (void)hipFree(c->consts);
     (void)hipFree(c->rope_cos);
@@ -213,7 +246,7 @@ int q48_ctx_destroy(q48_ctx *c)
         (void)hipEventDestroy(c->span_a);
     if (c->span_b)
         (void)hipEventDestroy(c->span_b);
-    if (c->stream)
+    if (c->stream && !c->lent)
         (void)hipStreamDestroy(c->stream);
     delete c;
     return Q48_OK;
@@ -615,6 +648,8 @@ int q48_fp_eval(q48_ctx *c, int func, const int64_t *x, const int64_t *y, int64_
 namespace {
 int tmp_reserve(q48_ctx *c, size_t bytes)
 {
+    if (q48_foreign_capture(c))
+        return Q48_ESTATE;
     if (bytes <= c->tmp_bytes)
         return Q48_OK;
     if (c->capturing)
@@ -1227,6 +1262,8 @@ int q48_sample_reserve(q48_ctx *c, int vocab)
     if (!c || vocab <= 0)
         return Q48_EINVAL;
     const size_t words = q48_sample_ws_words(vocab);
+    if (q48_foreign_capture(c))
+        return Q48_ESTATE;
     if (words <= c->smp_words)
         return Q48_OK;
     if (c->capturing)
@@ -1367,6 +1404,8 @@ int q48_graph_capture(q48_ctx *c)
 {
     if (!c || c->capturing)
         return Q48_EINVAL;
+    if (!c->stream || q48_foreign_capture(c))   // the null stream cannot be captured
+        return Q48_ESTATE;
     if (hipStreamBeginCapture(c->stream, hipStreamCaptureModeThreadLocal) != hipSuccess)
         return Q48_EHIP;
     c->capturing = 1;

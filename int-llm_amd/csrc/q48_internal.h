@@ -14,6 +14,7 @@ struct q48_ctx {
     int cu_count;                // compute units of the device
     int gemv_persistent;         // long normed GEMVs take k_gemv_p6 (default on)
     hipStream_t stream;
+    int lent;                    // the stream is the caller's (q48_ctx_create_on)
     q48_consts *consts;          // device: fp_math_init constants
     int64_t *rope_cos, *rope_sin; // device: [max_seq][head_dim/2]
     int rope_head_dim, rope_max_seq, rope_theta;
@@ -91,6 +92,10 @@ struct q48_on_device {
     q48_on_device &operator=(const q48_on_device &) = delete;
 };
 
+// Whether the caller captures the stream it lent: a graph the context knows nothing of,
+// which may hold no workspace (it could be replaced) and no k_attn_g launch (replays
+// would not be counted).
+bool q48_foreign_capture(q48_ctx *c);
 // Grow the context workspace to at least `bytes` (stream-synchronising).
 int q48_ws_reserve(q48_ctx *c, size_t bytes);
 // Give back a device buffer the context owns (stream-synchronising): freed

@@ -1622,6 +1622,8 @@ uint64_t q48_attg_default_wait() { return ATTG_TIMEOUT; }
 int q48_attg_account(q48_ctx *c, const unsigned *sync, uint64_t n)
 {
     constexpr uint64_t kLimit = (uint64_t)1 << 31;
+    if (q48_foreign_capture(c))
+        return Q48_ESTATE;
     uint64_t *count = sync == c->attx_sync ? &c->attg_count : q48_scratch_attg_count(c->device);
     if (!count)
         return Q48_EINVAL;

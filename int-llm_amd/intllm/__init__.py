@@ -34,6 +34,7 @@ GEMM_AUTO, GEMM_VALU, GEMM_I8, GEMM_I8_FUSED, GEMM_I8_PLANES = 0, 1, 2, 3, 4
 _P, _I, _SZ = C.c_void_p, C.c_int, C.c_size_t
 ABI_SIGNATURES = {
     "q48_ctx_create": [C.POINTER(C.c_void_p), _I],
+    "q48_ctx_create_on": [C.POINTER(C.c_void_p), _I, _P],
     "q48_ctx_destroy": [_P],
     "q48_malloc": [_P, C.POINTER(C.c_void_p), _SZ],
     "q48_free": [_P, _P],
@@ -240,11 +241,18 @@ class Buffer:
 
 
 class Context:
-    """q48_ctx: one HIP stream plus the device fp_math constants."""
+    """q48_ctx: one HIP stream plus the device fp_math constants.
 
-    def __init__(self, device: int = 0):
+    The stream is the context's own, ordered with no other; or the caller's, given as
+    its handle (torch.cuda.current_stream().cuda_stream, 0 for the default stream): then
+    the ops take their turn among what the caller enqueues there."""
+
+    def __init__(self, device: int = 0, stream: int | None = None):
         h = C.c_void_p()
-        check("q48_ctx_create", hip_lib().q48_ctx_create(C.byref(h), device))
+        if stream is None:
+            check("q48_ctx_create", hip_lib().q48_ctx_create(C.byref(h), device))
+        else:
+            check("q48_ctx_create_on", hip_lib().q48_ctx_create_on(C.byref(h), device, stream))
         self.h = h.value
         self._bufs: list[Buffer] = []
 

@@ -134,3 +134,11 @@ def test_reference_mgw_load_accepts_written_file():
             assert rc == 0 and np.array_equal(lg, want)
         lib.q48r_model_free_mgw(m)
     om.free()
+
+
+def test_a_context_on_a_stream_is_refused_without_device_work():
+    lib = intllm.hip_lib()
+    assert lib.q48_ctx_create_on(None, 0, None) == intllm.Q48_EINVAL
+    h = C.c_void_p(5)
+    assert lib.q48_ctx_create_on(C.byref(h), -1, None) == intllm.Q48_EINVAL
+    assert h.value is None
