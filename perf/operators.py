@@ -102,7 +102,8 @@ _context = None
 
 
 def _ctx():
-    """A program's one context."""
+    """A program's one context, on the stream that its torch operations use: calls take
+    their turn among them."""
     global _context
     if _context is None:
         pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
@@ -110,7 +111,7 @@ def _ctx():
         if pkg not in sys.path:
             sys.path.insert(0, pkg)
         import intllm
-        _context = intllm.Context(0)
+        _context = intllm.Context(0, stream=torch.cuda.current_stream(DEV).cuda_stream)
     return _context
 
 
