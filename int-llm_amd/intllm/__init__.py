@@ -483,12 +483,22 @@ class Context:
         return QCache(k, v, k_step, v_step, bits, layers, max_seq, n_kv, head_dim)
 
     def new_qcache(self, bits, layers, max_seq, n_kv, head_dim) -> QCache:
-        """A zeroed quantised cache in buffers of this context."""
+        """A zeroed quantised cache in buffers of this context (free_qcache gives them back)."""
         codes, steps = qcache_bytes(bits, layers, max_seq, n_kv, head_dim)
         bufs = [self.buffer(n // 8) for n in (codes, codes, steps, steps)]
         for b in bufs:
             self.zero(b.ptr, b.nbytes)
-        return QCache(*(b.ptr for b in bufs), bits, layers, max_seq, n_kv, head_dim)
+        cache = QCache(*(b.ptr for b in bufs), bits, layers, max_seq, n_kv, head_dim)
+        cache.bufs = bufs
+        return cache
+
+    def free_qcache(self, cache: QCache) -> None:
+        """Give back a cache from new_qcache (which is refused from then on); one that only
+        describes the caller's memory has nothing to give back."""
+        for b in cache.__dict__.pop("bufs", ()):
+            b.free()
+            self._bufs.remove(b)
+            cache.k = cache.v = cache.k_step = cache.v_step = None
 
     def qcache_store_rows(self, cache, layer, p0, T, K, V, ld):
         """Quantise T rows of rotated keys K and values V (rows ld words apart) at row p0."""

@@ -774,3 +774,32 @@ def test_workspace_of_many_key_heads(ctx, nkv, T, p0):
                            s[:, h].cpu().numpy())[:, None] for b, s in zip(codes, steps))
         want = P.attend(x[:, h:h + 1].cpu().numpy(), kv, vv, see)
         assert (out[:, h:h + 1].cpu().numpy() == want).all(), h
+
+
+def test_a_cache_is_given_back(ctx):
+    """A program that makes a cache for each conversation does not grow; a freed cache is
+    refused."""
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(1)
+    with intllm.Context(0) as c:
+        x, out = c.to_device(acts(rng, 1, 12, 64)), c.buffer(4 * 64)
+
+        def conversation():
+            q = c.new_qcache(8, 22, 32767, 4, 64)          # 2 x 185 and 2 x 23 MB
+            c.attn_rows_qcache(out.ptr, x.ptr, q, 21, 0, 1, 4)
+            return q
+
+        c.free_qcache(conversation())
+        held, bufs = torch.cuda.mem_get_info()[0], len(c._bufs)
+        for _ in range(6):
+            q = conversation()
+            assert held - torch.cuda.mem_get_info()[0] < 512 << 20
+            c.free_qcache(q)
+        assert len(c._bufs) == bufs and torch.cuda.mem_get_info()[0] >= held
+        with pytest.raises(intllm.Q48Error) as e:
+            c.attn_rows_qcache(out.ptr, x.ptr, q, 21, 0, 1, 4)
+        assert e.value.code == intllm.Q48_EINVAL
+        c.free_qcache(q)                                    # nothing left to give back
+        mine = c.to_device(np.arange(4))
+        c.free_qcache(c.qcache(mine.ptr, mine.ptr, mine.ptr, mine.ptr, 8, 1, 1, 1, 32))
+        assert (mine.download() == np.arange(4)).all()
