@@ -10,6 +10,8 @@
  * Conventions
  *   - Every int64_t* / int* argument of an op is a DEVICE pointer owned
  *     by the caller (allocate with q48_malloc or any HIP allocator).
+ *     Arguments off the boundary of their type are refused (Q48_EINVAL) by the
+ *     ops that could fault on them.
  *   - Values are Q16.48 fixed point (`fixed_t`, fp_math.h:175).
  *   - Ops are enqueued on the context's stream, in call order; q48_sync
  *     waits for them.  Results are visible after q48_sync or a

@@ -960,7 +960,8 @@ int q48_rope_store_rows_at(q48_ctx *c, int64_t *QKV, int64_t *kcache, int64_t *v
                            int p0, int T, const int *d_pos, int n_heads, int n_kv, int head_dim,
                            int max_seq)
 {
-    if (!c || !QKV || !kcache || !vcache || !d_pos || T <= 0 || layer < 0 || max_seq <= 0 ||
+    if (!c || !QKV || !kcache || !vcache || !d_pos || q48_off_words<8>(QKV, kcache, vcache) ||
+        q48_off_words<4>(d_pos) || T <= 0 || layer < 0 || max_seq <= 0 ||
         !heads_ok(n_heads, n_kv, head_dim))
         return Q48_EINVAL;
     if (!c->rope_cos || head_dim != c->rope_head_dim)

@@ -235,6 +235,13 @@ int q48_launch_pf_attn_mfma(q48_ctx *c, int64_t *out, const int64_t *QKV, int64_
 int q48_launch_pf_attn(q48_ctx *c, int64_t *out, const int64_t *QKV, int64_t *kcache,
                        int64_t *vcache, int layer, int p0, int T, int n_heads, int n_kv, int hd,
                        int max_seq);
+// Whether an argument of words (W: or ints) lies off their boundary: 64-bit atomics and
+// loads of a lane's own words there are not defined.
+template <int W, typename... P>
+inline bool q48_off_words(const P *...p)
+{
+    return (((uintptr_t)p | ...) & (W - 1)) != 0;
+}
 // Whether a q48_qcache describes a cache the kernels can read (pointers, sizes).
 bool q48_qcache_ok(const q48_qcache *qc);
 int q48_launch_pf_silu(q48_ctx *c, int64_t *out, const int64_t *GU, int T, int ffn);

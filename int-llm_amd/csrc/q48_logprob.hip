@@ -705,7 +705,8 @@ int q48_logprobs_rows(q48_ctx *c, const int64_t *logits, int T, int vocab, const
 {
     if (!c || !logits || T <= 0 || T > LP_MAX_ROWS || vocab <= 0 || vocab > (1 << 22) || top_n < 0 ||
         top_n > LP_MAX_TOP || top_n > vocab || (logp && !d_tokens) ||
-        (top_n > 0 && (!top_ids || !top_logp)) || (!logp && !entropy && top_n == 0))
+        (top_n > 0 && (!top_ids || !top_logp)) || (!logp && !entropy && top_n == 0) ||
+        q48_off_words<8>(logits, logp, entropy, top_logp) || q48_off_words<4>(d_tokens, top_ids))
         return Q48_EINVAL;
     const size_t n = T, nt = n * top_n;
     auto over = [&](const void *in, size_t bytes) {   // an output that shares words with it

@@ -199,8 +199,8 @@ int q48_qcache_bytes(int bits, int layers, int max_seq, int n_kv, int head_dim, 
 int q48_qcache_store_rows(q48_ctx *c, const q48_qcache *qc, int layer, int p0, int T,
                           const int64_t *K, const int64_t *V, int ld)
 {
-    if (!c || !K || !V || !q48_qcache_ok(qc) || layer < 0 || layer >= qc->layers || T <= 0 ||
-        ld < qc->n_kv * qc->head_dim)
+    if (!c || !K || !V || q48_off_words<8>(K, V) || !q48_qcache_ok(qc) || layer < 0 ||
+        layer >= qc->layers || T <= 0 || ld < qc->n_kv * qc->head_dim)
         return Q48_EINVAL;
     if (p0 < 0 || p0 >= qc->max_seq || T > qc->max_seq - p0)
         return Q48_ERANGE;
@@ -213,8 +213,8 @@ int q48_qcache_store_rows(q48_ctx *c, const q48_qcache *qc, int layer, int p0, i
 int q48_qcache_load_rows(q48_ctx *c, int64_t *K, int64_t *V, const q48_qcache *qc, int layer,
                          int p0, int T, int ld)
 {
-    if (!c || !K || !V || !q48_qcache_ok(qc) || layer < 0 || layer >= qc->layers || T <= 0 ||
-        ld < qc->n_kv * qc->head_dim)
+    if (!c || !K || !V || q48_off_words<8>(K, V) || !q48_qcache_ok(qc) || layer < 0 ||
+        layer >= qc->layers || T <= 0 || ld < qc->n_kv * qc->head_dim)
         return Q48_EINVAL;
     if (p0 < 0 || p0 >= qc->max_seq || T > qc->max_seq - p0)
         return Q48_ERANGE;
@@ -233,8 +233,9 @@ int q48_qcache_load_rows(q48_ctx *c, int64_t *K, int64_t *V, const q48_qcache *q
 int q48_rope_store_rows_qcache(q48_ctx *c, int64_t *QKV, const q48_qcache *qc, int layer, int p0,
                                int T, const int *d_pos, int n_heads)
 {
-    if (!c || !QKV || !q48_qcache_ok(qc) || layer < 0 || layer >= qc->layers || T <= 0 ||
-        n_heads <= 0 || n_heads > 1024 || n_heads % qc->n_kv)
+    if (!c || !QKV || q48_off_words<8>(QKV) || q48_off_words<4>(d_pos) || !q48_qcache_ok(qc) ||
+        layer < 0 || layer >= qc->layers || T <= 0 || n_heads <= 0 || n_heads > 1024 ||
+        n_heads % qc->n_kv)
         return Q48_EINVAL;
     if (!c->rope_cos || qc->head_dim != c->rope_head_dim || qc->max_seq > c->rope_max_seq)
         return Q48_ESTATE;
@@ -251,7 +252,8 @@ int q48_rope_store_rows_qcache(q48_ctx *c, int64_t *QKV, const q48_qcache *qc, i
 int q48_cache_keep_rows(q48_ctx *c, int64_t *kcache, int64_t *vcache, int layers, int p0,
                         const int *d_rows, int n, int n_kv, int head_dim, int max_seq)
 {
-    if (!c || !kcache || !vcache || !d_rows || layers <= 0 || layers > 65535 || n <= 0 ||
+    if (!c || !kcache || !vcache || q48_off_words<8>(kcache, vcache) || !d_rows ||
+        q48_off_words<4>(d_rows) || layers <= 0 || layers > 65535 || n <= 0 ||
         n_kv <= 0 || n_kv > 65535 || head_dim <= 0 || head_dim > 256 || max_seq <= 0)
         return Q48_EINVAL;
     if (p0 < 0 || p0 >= max_seq || n > max_seq - p0)
@@ -266,7 +268,7 @@ int q48_cache_keep_rows(q48_ctx *c, int64_t *kcache, int64_t *vcache, int layers
 
 int q48_qcache_keep_rows(q48_ctx *c, const q48_qcache *qc, int p0, const int *d_rows, int n)
 {
-    if (!c || !d_rows || !q48_qcache_ok(qc) || n <= 0)
+    if (!c || !d_rows || q48_off_words<4>(d_rows) || !q48_qcache_ok(qc) || n <= 0)
         return Q48_EINVAL;
     if (p0 < 0 || p0 >= qc->max_seq || n > qc->max_seq - p0)
         return Q48_ERANGE;

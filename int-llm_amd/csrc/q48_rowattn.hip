@@ -1511,7 +1511,8 @@ int decode_qcache(q48_ctx *c, int64_t *out, const int64_t *q, const q48_qcache *
                   const int64_t *k_new, const int64_t *v_new, int layer, int pos, int n_heads,
                   bool rope)
 {
-    if (!c || !out || !q || !k_new || !v_new || !q48_qcache_ok(qc) || layer < 0 ||
+    if (!c || !out || !q || !k_new || !v_new || q48_off_words<8>(out, q, k_new, v_new) ||
+        !q48_qcache_ok(qc) || layer < 0 ||
         layer >= qc->layers || n_heads <= 0 || n_heads > RA_MAX_HEADS || n_heads % qc->n_kv)
         return Q48_EINVAL;
     const size_t hd = qc->head_dim, qn = n_heads * hd, kn = qc->n_kv * hd;
@@ -1565,7 +1566,8 @@ int q48_attn_decode_rope_qcache(q48_ctx *c, int64_t *out, const int64_t *q, cons
 int q48_attn_rows_qcache(q48_ctx *c, int64_t *out, const int64_t *QKV, const q48_qcache *qc,
                          int layer, int p0, int T, int n_heads, const uint64_t *mask)
 {
-    if (!c || !out || !QKV || !q48_qcache_ok(qc) || layer < 0 || layer >= qc->layers || T <= 0 ||
+    if (!c || !out || !QKV || q48_off_words<8>(out, QKV, mask) || !q48_qcache_ok(qc) ||
+        layer < 0 || layer >= qc->layers || T <= 0 ||
         n_heads <= 0 || n_heads > RA_MAX_HEADS || n_heads % qc->n_kv)
         return Q48_EINVAL;
     if (p0 < 0 || p0 >= qc->max_seq || T > qc->max_seq - p0)
@@ -1598,7 +1600,8 @@ int q48_attn_tree(q48_ctx *c, int64_t *out, const int64_t *QKV, const int64_t *k
                   const int64_t *vcache, int layer, int p0, int T, int n_heads, int n_kv,
                   int head_dim, int max_seq, const uint64_t *mask)
 {
-    if (!c || !out || !QKV || !kcache || !vcache || layer < 0 || T <= 0 || n_heads <= 0 ||
+    if (!c || !out || !QKV || !kcache || !vcache ||
+        q48_off_words<8>(out, QKV, kcache, vcache, mask) || layer < 0 || T <= 0 || n_heads <= 0 ||
         n_heads > RA_MAX_HEADS || n_kv <= 0 || n_heads % n_kv || max_seq <= 0 ||
         (head_dim != 32 && head_dim != 64 && head_dim != 128))
         return Q48_EINVAL;

@@ -1,6 +1,8 @@
 """The quantised key/value cache on the GPU: what is written and read back, and
 attention over it, word for word against the plain forms.
 """
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -803,3 +805,42 @@ def test_a_cache_is_given_back(ctx):
         mine = c.to_device(np.arange(4))
         c.free_qcache(c.qcache(mine.ptr, mine.ptr, mine.ptr, mine.ptr, 8, 1, 1, 1, 32))
         assert (mine.download() == np.arange(4)).all()
+
+
+def test_arguments_off_their_boundary_are_refused(ctx):
+    """Words at odd halves and ints at odd bytes, one argument at a time; nothing is
+    launched."""
+    rng = np.random.default_rng(1)
+    nh, nkv, hd, S, T = 4, 2, 64, 12, 3
+    ctx.rope_init(hd, S, 10000)
+    cache = Cache(ctx, 8, 1, S, nkv, hd)
+    before = cache.read()
+    n = S * (nh + 2 * nkv) * hd
+    bufs = [ctx.to_device(np.full(n, 5)) for _ in range(6)]
+    w = [b.ptr for b in bufs]
+    q, f = cache.c, intllm.hip_lib()
+    calls = {        # the call, its words and its ints (places among the arguments)
+        "q48_qcache_store_rows": ([q, 0, 0, T, w[0], w[1], nkv * hd], (4, 5), ()),
+        "q48_qcache_load_rows": ([w[0], w[1], q, 0, 0, T, nkv * hd], (0, 1), ()),
+        "q48_rope_store_rows_qcache": ([w[0], q, 0, 0, T, w[1], nh], (0,), (5,)),
+        "q48_attn_decode_qcache": ([w[0], w[1], q, w[2], w[3], 0, 2, nh], (0, 1, 3, 4), ()),
+        "q48_attn_decode_rope_qcache": ([w[0], w[1], q, w[2], w[3], 0, 2, nh], (0, 1, 3, 4), ()),
+        "q48_attn_rows_qcache": ([w[0], w[1], q, 0, 0, T, nh, w[2]], (0, 1, 7), ()),
+        "q48_attn_tree": ([w[0], w[1], w[2], w[3], 0, 0, T, nh, nkv, hd, S, w[4]], (0, 1, 2, 3, 11),
+                          ()),
+        "q48_rope_store_rows_at": ([w[0], w[1], w[2], 0, 0, T, w[3], nh, nkv, hd, S], (0, 1, 2),
+                                   (6,)),
+        "q48_cache_keep_rows": ([w[0], w[1], 1, 0, w[2], 2, nkv, hd, S], (0, 1), (4,)),
+        "q48_qcache_keep_rows": ([q, 0, w[0], 2], (), (2,)),
+        "q48_logprobs_rows": ([w[0], T, 100, w[1], w[2], w[3], 2, w[4], w[5]], (0, 4, 5, 8),
+                              (3, 7)),
+    }
+    for name, (args, words, ints) in calls.items():
+        for at, off in [(i, 4) for i in words] + [(i, 1) for i in words] + [(i, 2) for i in ints]:
+            a = list(args)
+            a[at] += off
+            a = [C.byref(x) if isinstance(x, intllm.QCache) else x for x in a]
+            assert getattr(f, name)(ctx.h, *a) == intllm.Q48_EINVAL, (name, at, off)
+    assert all((a == b).all() for a, b in zip(before, cache.read()))
+    assert all((b.download() == 5).all() for b in bufs)
+    cache.free()
