@@ -420,7 +420,7 @@ constexpr int LR_NT = 512;
 // which wave 0 finds before its exponentials; the few threads with a candidate read
 // their logits again.
 // Bound by vector issue: 500 rows of 32000, 16 M terms of about 60 operations, in 51 us
-// (2.5 TB/s of logits), 60% of what issue allows; two rows a block, and a row's 4 us of
+// (2.5 TB/s of logits), 70% of what issue allows; two rows a block, and a row's 4 us of
 // maximum, threshold, logarithm and candidates are not covered by another's terms.
 template <int R>
 __global__ __launch_bounds__(LR_NT) void k_lp_row(const int64_t *__restrict__ X, int T, int V,
@@ -536,6 +536,10 @@ __global__ __launch_bounds__(LR_NT) void k_lp_row(const int64_t *__restrict__ X,
 // second launch 1.0 the maxima, 1.6 the threshold, 0.6 the terms, 1.5 the candidates on
 // their way out, 0.5 the ticket, 2.3 the sums of all waves (1.3 to fetch them from other
 // dies) and the logarithm.
+// A chunk is one stretch of the row: where the largest logits sit in few chunks (a row in
+// order, or all but a block of ids masked), more candidates come than LP_CAP and the last
+// block passes over the row for each token asked for: 545 us with a top 20, 64 rows of 130000
+// 4.4 ms instead of 41 us.
 
 struct LpWork {
     int64_t *gmax;     // [T][4 chunks]: a wave's maximum

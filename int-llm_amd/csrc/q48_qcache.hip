@@ -24,7 +24,8 @@ QcLayer qc_layer(const q48_qcache *qc, int layer)
 
 // 16 lanes a head vector, 16 vectors a block, each read and written once; with ROPE the
 // query heads too, in place.  Bound by HBM where there are rows: 1999 rows of 8 heads of
-// 128 at 4 bits, 35 MB, in 8.4 us (4.2 TB/s; a large copy reaches 4.4).  One row is a
+// 128 at 4 bits, 35 MB, in 8.4 us (4.2 TB/s; a large copy reaches 4.4); with RoPE 2000 rows
+// of 32 heads on 4 of 64, 79 MB of them in cache, in 16.7 us, 512 in 5.6.  One row is a
 // launch: 2 us.
 template <int BITS, int HD, bool ROPE>
 __global__ __launch_bounds__(256) void k_qc_store(QcLayer L, int64_t *K, int64_t *V, size_t ld,
@@ -112,7 +113,8 @@ struct KeepArrays {
 // One thread a word of a row: the n moves in turn, so that a row that is both
 // source and target is read before it is written (every later source lies past
 // the rows written so far).  The moves of a word wait for one another: a path of a
-// drafted tree is a few rows, and all layers move at once.
+// drafted tree is a few rows, and all layers move at once (22 layers of 4 heads of 64: 1 to
+// 5 rows 3.2 us a call, a launch; 16 rows 4.2).
 __global__ __launch_bounds__(256) void k_keep_rows(KeepArrays a, int max_seq, int p0,
                                                   const int *__restrict__ rows, int n)
 {
