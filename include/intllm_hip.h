@@ -53,9 +53,10 @@ int q48_ctx_create(q48_ctx **out, int device);
  * so that they are ordered with what the caller enqueues there: a context's
  * own stream is ordered with no other, the default stream included, and only
  * synchronising both sides makes data pass.  The stream outlives the context.
- * Capture it with q48_graph_* (not the default stream: Q48_ESTATE).  While
- * the caller captures it by other means, ops that use a workspace or the
- * one-launch split attention return Q48_ESTATE, and so does this call. */
+ * Capture it with q48_graph_* (not the default stream: Q48_ESTATE, from the
+ * host's q48h_decode_graph too).  While the caller captures it by other means,
+ * ops that use a workspace or the one-launch split attention return
+ * Q48_ESTATE, and so does this call. */
 int q48_ctx_create_on(q48_ctx **out, int device, void *stream);
 int q48_ctx_destroy(q48_ctx *ctx);
 
@@ -508,8 +509,8 @@ int q48_attn_decode_rope_qcache(q48_ctx *ctx, int64_t *out, const int64_t *q,
  * is the reference's exact attention (llama_int.c:1502-1529) over the rows it
  * attends to, in cache order, so a token of a tree gets the words that decoding
  * its own path gives.  Workspace as for q48_attn_decode_qcache (1 GiB of scores at
- * most, and a thirtieth of that beside them: more rows take several launches).  out [T][n_heads * head_dim] shares
- * no words with QKV.
+ * most, and a thirtieth of that beside them: more rows take several launches).
+ * out [T][n_heads * head_dim] shares no words with QKV.
  * head_dim 32, 64 or 128; n_heads at most 1024; p0 + T at most 32767. */
 int q48_attn_tree(q48_ctx *ctx, int64_t *out, const int64_t *QKV, const int64_t *kcache,
                   const int64_t *vcache, int layer, int p0, int T, int n_heads, int n_kv,
@@ -538,7 +539,8 @@ int q48_qcache_keep_rows(q48_ctx *ctx, const q48_qcache *cache, int p0, const in
  * probabilities.  logp (with d_tokens) and entropy may be NULL, top_ids and
  * top_logp [T][top_n] where top_n is 0, but not all of them.  vocab at most
  * 2^22, T at most 2^30.  The outputs share no words with the logits or the
- * tokens (but top_ids may be d_tokens where top_n is 1).  All in Q16.48: with m = max x, u_i = m - x_i (64 bits, unsigned),
+ * tokens (but top_ids may be d_tokens where top_n is 1).  All in Q16.48: with
+ * m = max x, u_i = m - x_i (64 bits, unsigned),
  *   e_i = floor(floor(T_j h 2^-48) 2^-n), u_i = n LN2 + j 2^42 + s, 0 <= s < 2^42,
  *         j <= 44, LN2 = 195103586505167, T_j = round(2^48 e^(-j/64)),
  *         h = C_0 - (s (C_1 - (s (... C_6) >> 48)) >> 48), C_k = round(2^48 / k!)

@@ -6,6 +6,7 @@ import pytest
 
 import intllm
 import serve_plain as P
+import spec
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -145,3 +146,28 @@ def test_the_caller_s_capture_takes_what_needs_no_workspace():
             ent.zero_()
             graph.replay()
             assert (ent.cpu().numpy() == P.logprobs(x, np.zeros(T, np.int64), 0)[1]).all()
+
+
+def test_the_host_s_decode_on_a_lent_stream():
+    """Generation through the C host: the same tokens and hashes on the context's own
+    stream, on the caller's, and on the default one, which has no graphs."""
+    cfg = intllm.Config(*spec.TINY)
+    prompt = spec.prompt(spec.SEED_TINY, 16, spec.TINY[6])
+    ran = []
+    for stream in (None, torch.cuda.Stream(0).cuda_stream, 0):
+        with intllm.Context(0, stream=stream) as c:
+            m = intllm.HostModel(c, cfg)
+            m.synth(spec.SEED_TINY, 8)
+            if stream == 0:
+                with pytest.raises(intllm.Q48Error) as e:
+                    m.decode_graph_hashed(5, 0, 8)
+                assert e.value.code == intllm.Q48_ESTATE
+                m.kv_reset()
+            toks, hs, _ = m.generate(prompt, 8)
+            graph = None
+            if stream != 0:
+                m.kv_reset()
+                graph = m.decode_graph_hashed(5, 0, 8)[:3]
+            ran.append((toks, hs, graph))
+            m.free()
+    assert ran[0] == ran[1] and ran[0][:2] == ran[2][:2]
