@@ -558,6 +558,81 @@ int q48_logprobs_rows(q48_ctx *ctx, const int64_t *logits, int T, int vocab, con
                       int64_t *logp, int64_t *entropy, int top_n, int *top_ids,
                       int64_t *top_logp);
 
+/* ---- weights in 8 bits ----------------------------------------------------- */
+/* `count` matrices [N][K] (more than one: a layer's experts) as 8-bit codes with one
+ * Q16.48 step per row: a byte a weight instead of 8, or of the bfloat16 section's 2.
+ * Rows are put into 8 bits by the quantised cache's rule: with a = max |x_k|,
+ *   step   = min(ceil(a / 127), floor((2^63 - 1) / 127))
+ *   code_k = sign(x_k) min(127, floor((|x_k| + floor(step / 2)) / step)), 0 where
+ *            step is 0,
+ * and stand for code_k * step.
+ *
+ * The arrays are device memory of the caller, of the sizes q48_w8_bytes gives.  codes
+ * (16-byte aligned): for each matrix in turn, tiles of 16 rows x 64 columns in row-major
+ * order, ceil(N / 16) x ceil(K / 64) of 1024 bytes, in which byte 256 (k / 16) + 16 n +
+ * k % 16 is row n, column k; rows past N and columns past K are zero.  step [count][N].
+ * N at most 2^24, K at most 131072, count at most 1024.  The struct itself is read
+ * during the call only.  No reference counterpart: its weights are words. */
+typedef struct {
+    void *codes;
+    int64_t *step;
+    int count, N, K;
+} q48_w8;
+int q48_w8_bytes(int count, int N, int K, size_t *codes, size_t *steps);
+/* Fill matrix `index` from words W [N][K], by the rule above. */
+int q48_w8_pack(q48_ctx *ctx, const q48_w8 *w, int index, const int64_t *W);
+/* Fill matrix `index` from codes [N][K] and steps [N] as a checkpoint has them (device
+ * memory; -128 is a code, a negative step counts as 0). */
+int q48_w8_put(q48_ctx *ctx, const q48_w8 *w, int index, const int8_t *codes,
+               const int64_t *steps);
+/* The words that matrix `index` stands for, code * step mod 2^64: out [N][K]. */
+int q48_w8_values(q48_ctx *ctx, int64_t *out, const q48_w8 *w, int index);
+
+/* The product of T rows X [T][K] with weights in 8 bits (count 1), T = 1 for a decoded
+ * token: each row of X, after rmsnorm(x, norm_w) (llama_int.c:1048-1058) where norm_w is
+ * given, is put into 8 bits by the rule above, with codes a and the step sa; then with
+ * S = sum_k a_k code_nk
+ *   Y[t][n] = base[t][n] + floor(S sa step_n / 2^48) mod 2^64
+ * (base NULL: no addend).  base may be Y itself, as a residual is.  Y [T][N] shares no
+ * other words with what the call reads.  T at most 2^20.
+ * The rows' codes go through a buffer of the context, which reaches its size in the first
+ * call of a shape: call once before capturing.  The counterpart of q48_gemv and q48_gemm
+ * for such weights. */
+int q48_gemm_w8(q48_ctx *ctx, int64_t *Y, const int64_t *base, const q48_w8 *w,
+                const int64_t *X, const int64_t *norm_w, int T);
+/* out[t][i] = fp_mul(fp_silu(g_i), u_i) (llama_int.c:1549-1552) with g and u the products
+ * of the same row with gate and up (both [ffn][K]), out [T][ffn].  The counterpart of
+ * q48_rmsnorm_gemv_swiglu. */
+int q48_gemm_w8_swiglu(q48_ctx *ctx, int64_t *out, const q48_w8 *gate, const q48_w8 *up,
+                       const int64_t *X, const int64_t *norm_w, int T);
+
+/* ---- a mixture of experts ---------------------------------------------------- */
+/* A feed-forward layer of gate.count experts, of which every token goes to top_k (at
+ * most 64): router [experts][dim] words; gate and up of experts matrices [ffn][dim], down
+ * of [dim][ffn]. */
+typedef struct {
+    const int64_t *router;
+    q48_w8 gate, up, down;
+    int top_k;
+    int renorm;   /* the weights sum to one over the chosen experts (else over all) */
+} q48_moe;
+/* The whole layer for T rows X [T][dim] (T at most 2^20).  For each row, with x = the row, or
+ * rmsnorm(row, norm_w) where norm_w is given:
+ *   l_e     = matmul_vec(router, x)_e (llama_int.c:1014-1046)
+ *   chosen  = the top_k experts of largest l, ties to the lowest expert, largest first
+ *   weight  = floor(2^48 e / Z), e of the log probabilities' rule (q48_logprobs_rows) with
+ *             u = max l - l_e, Z the sum of e over the chosen (renorm) or over all
+ *   h       = q48_gemm_w8_swiglu of x with the expert's gate and up
+ *   out[t]  = base[t] + sum over the chosen of fp_mul(weight, q48_gemm_w8 of h with down)
+ * mod 2^64 (base NULL: no addend).  base may be out itself, and X too where base is.
+ * chosen and weight [T][top_k] receive the choice; either may be NULL.  Outputs share no
+ * other words with what the call reads, nor with one another.  Buffers of the context
+ * (of hidden words a GiB at most, of long inputs more passes) reach their size in the
+ * first call of a shape: call once before capturing.  No reference counterpart: its
+ * models are dense. */
+int q48_moe_w8(q48_ctx *ctx, int64_t *out, const int64_t *base, const q48_moe *moe,
+               const int64_t *X, const int64_t *norm_w, int T, int *chosen, int64_t *weight);
+
 /* ---- sampling (sample_token, llama_int.c:2958-3039) --------------------- */
 /* rng_seed (llama_int.c:2909-2920): the xoroshiro128+ state of a seed
  * (SplitMix64), computed on the host.  Upload it to a device buffer of two

@@ -230,6 +230,7 @@ int q48_ctx_destroy(q48_ctx *c)
     (void)hipFree(c->rms_part);
     (void)hipFree(c->smp);
     (void)hipFree(c->tmp);
+    (void)hipFree(c->w8);
     (void)hipFree(c->attx_sync);
     graph_destroy(c, c->cur);
     c->cur = nullptr;

@@ -1,0 +1,43 @@
+// q48_expn.hpp — e^-u of Q16.48 words over the whole range: u = n LN2 + j / 64 + s
+// splits the exponent into a shift, a table and a six-step Horner row on s < 2^-6.
+// Included by the HIP sources of libintllm_hip only.
+#pragma once
+
+#include "q48_device.hpp"
+
+namespace {
+
+constexpr int64_t EXPN_LN2 = 195103586505167LL;   // fp_log's ln 2 (fp_math.h:752-773)
+
+// round(2^48 e^(-j/64)), round(2^48 / k!)
+static __constant__ int64_t kExp[45] = {
+    281474976710656LL, 277111111677821LL, 272814902101423LL, 268585299080830LL, 264421269977109LL,
+    260321798160909LL, 256285882764256LL, 252312538436196LL, 248400795102225LL, 244549697727451LL,
+    240758306083425LL, 237025694518590LL, 233350951732284LL, 229733180552255LL, 226171497715615LL,
+    222665033653200LL, 219212932277264LL, 215814350772475LL, 212468459390137LL, 209174441245618LL,
+    205931492118908LL, 202738820258272LL, 199595646186949LL, 196501202512843LL, 193454733741172LL,
+    190455496090014LL, 187502757308717LL, 184595796499121LL, 181733903939560LL, 178916380911580LL,
+    176142539529353LL, 173411702571733LL, 170723203316912LL, 168076385379650LL, 165470602551013LL,
+    162905218640611LL, 160379607321268LL, 157893151976115LL, 155445245548039LL, 153035290391475LL,
+    150662698126495LL, 148326889495156LL, 146027294220076LL, 143763350865205LL, 141534506698753LL};
+constexpr int64_t kFactK[7] = {
+    281474976710656LL, 281474976710656LL, 140737488355328LL, 46912496118443LL, 11728124029611LL,
+    2345624805922LL, 390937467654LL};
+
+// floor(floor(T_j h 2^-48) 2^-n) of one u, by integers: for the few exponentials of a
+// row of expert logits (q48_logprob.hip's lp_terms has the FP64 form for many).
+__device__ __forceinline__ int64_t q48_expn(uint64_t u)
+{
+    if (u >= 49 * (uint64_t)EXPN_LN2)
+        return 0;
+    const uint32_t n = (uint32_t)(u / (uint64_t)EXPN_LN2);
+    const uint64_t r = u - n * (uint64_t)EXPN_LN2;
+    const int64_t s = (int64_t)(r & (((uint64_t)1 << 42) - 1));
+    int64_t h = kFactK[6];
+#pragma unroll
+    for (int k = 5; k >= 0; --k)
+        h = kFactK[k] - q48_mul(s, h);
+    return q48_mul(kExp[r >> 42], h) >> n;
+}
+
+} // namespace

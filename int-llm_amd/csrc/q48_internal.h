@@ -20,6 +20,8 @@ struct q48_ctx {
     int rope_head_dim, rope_max_seq, rope_theta;
     void *ws;                    // device workspace (scores, row sums, partials)
     size_t ws_bytes;
+    void *w8;                    // device: what the 8-bit ops keep between their launches
+    size_t w8_bytes;
     int *d_scalar;               // device: small outputs (norm scalar, bf16_pack's flag)
     int *h_token;                // host memory that kernels write: a call's chosen token
     int *d_step;                 // device: decode-step state {token, pos, count}

@@ -6,29 +6,16 @@
 // shift, a table and a six-step Horner row on s < 2^-6 (s^7 / 5040 < 2^-54), a
 // third of fp_exp's squarings and division, and 4 units of 2^-48 from e^-u.
 #include "q48_attn.hpp"
+#include "q48_expn.hpp"
 
 namespace {
 
-constexpr int64_t LP_LN2 = 195103586505167LL;   // fp_log's ln 2 (fp_math.h:752-773)
+constexpr int64_t LP_LN2 = EXPN_LN2;
 constexpr int LP_MAX_TOP = 32;
 constexpr int LP_MAX_ROWS = 1 << 30;   // a row's number and a grid's stride add up in 31 bits
 constexpr int LP_CAP = 512;   // candidates of a row; past that (ties) the slow selection
 
-// round(2^48 e^(-j/64)), round(2^48 / k!), floor(2^54 / (64 + j)),
-// round(2^48 log(1 + j/64)), round(2^48 / (k + 1))
-static __constant__ int64_t kExp[45] = {
-    281474976710656LL, 277111111677821LL, 272814902101423LL, 268585299080830LL, 264421269977109LL,
-    260321798160909LL, 256285882764256LL, 252312538436196LL, 248400795102225LL, 244549697727451LL,
-    240758306083425LL, 237025694518590LL, 233350951732284LL, 229733180552255LL, 226171497715615LL,
-    222665033653200LL, 219212932277264LL, 215814350772475LL, 212468459390137LL, 209174441245618LL,
-    205931492118908LL, 202738820258272LL, 199595646186949LL, 196501202512843LL, 193454733741172LL,
-    190455496090014LL, 187502757308717LL, 184595796499121LL, 181733903939560LL, 178916380911580LL,
-    176142539529353LL, 173411702571733LL, 170723203316912LL, 168076385379650LL, 165470602551013LL,
-    162905218640611LL, 160379607321268LL, 157893151976115LL, 155445245548039LL, 153035290391475LL,
-    150662698126495LL, 148326889495156LL, 146027294220076LL, 143763350865205LL, 141534506698753LL};
-constexpr int64_t kFactK[7] = {
-    281474976710656LL, 281474976710656LL, 140737488355328LL, 46912496118443LL, 11728124029611LL,
-    2345624805922LL, 390937467654LL};
+// floor(2^54 / (64 + j)), round(2^48 log(1 + j/64)), round(2^48 / (k + 1))
 static __constant__ int64_t kRcp[64] = {
     281474976710656LL, 277144592453568LL, 272945431961848LL, 268871619544507LL, 264917625139440LL,
     261078239267854LL, 257348550135456LL, 253723922668760LL, 250199979298360LL, 246772582321671LL,

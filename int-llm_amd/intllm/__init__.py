@@ -119,6 +119,13 @@ ABI_SIGNATURES = {
     "q48_cache_keep_rows": [_P, _P, _P, _I, _I, _P, _I, _I, _I, _I],
     "q48_qcache_keep_rows": [_P, _P, _I, _P, _I],
     "q48_logprobs_rows": [_P, _P, _I, _I, _P, _P, _P, _I, _P, _P],
+    "q48_w8_bytes": [_I, _I, _I, C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)],
+    "q48_w8_pack": [_P, _P, _I, _P],
+    "q48_w8_put": [_P, _P, _I, _P, _P],
+    "q48_w8_values": [_P, _P, _P, _I],
+    "q48_gemm_w8": [_P, _P, _P, _P, _P, _P, _I],
+    "q48_gemm_w8_swiglu": [_P, _P, _P, _P, _P, _P, _I],
+    "q48_moe_w8": [_P, _P, _P, _P, _P, _P, _I, _P, _P],
     "q48_set_attn_wait": [_P, C.c_int64],
     "q48_prof_enable": [_P, _I],
     "q48_timer_start": [_P],
@@ -144,6 +151,25 @@ def qcache_bytes(bits, layers, max_seq, n_kv, head_dim) -> tuple[int, int]:
     c, s = C.c_size_t(), C.c_size_t()
     check("q48_qcache_bytes", hip_lib().q48_qcache_bytes(bits, layers, max_seq, n_kv, head_dim,
                                                          C.byref(c), C.byref(s)))
+    return c.value, s.value
+
+
+class W8(C.Structure):
+    """q48_w8: matrices of 8-bit codes with a step a row."""
+    _fields_ = [("codes", C.c_void_p), ("step", C.c_void_p), ("count", C.c_int), ("N", C.c_int),
+                ("K", C.c_int)]
+
+
+class Moe(C.Structure):
+    """q48_moe: a mixture-of-experts layer's router and experts."""
+    _fields_ = [("router", C.c_void_p), ("gate", W8), ("up", W8), ("down", W8),
+                ("top_k", C.c_int), ("renorm", C.c_int)]
+
+
+def w8_bytes(count, N, K) -> tuple[int, int]:
+    """Bytes of the codes and steps of `count` matrices [N][K] in 8 bits."""
+    c, s = C.c_size_t(), C.c_size_t()
+    check("q48_w8_bytes", hip_lib().q48_w8_bytes(count, N, K, C.byref(c), C.byref(s)))
     return c.value, s.value
 
 
@@ -547,6 +573,58 @@ class Context:
                       top_logp=None):
         return check("q48_logprobs_rows", hip_lib().q48_logprobs_rows(
             self.h, logits, T, vocab, tokens, logp, entropy, top_n, top_ids, top_logp))
+
+    # weights in 8 bits, mixture of experts
+    @staticmethod
+    def w8(codes, step, count, N, K) -> W8:
+        """Describe weights in 8 bits in device memory the caller owns."""
+        return W8(codes, step, count, N, K)
+
+    def new_w8(self, count, N, K) -> W8:
+        """Room for `count` matrices [N][K] in 8 bits in buffers of this context (free_w8
+        gives them back); w8_pack or w8_put fills each."""
+        codes, steps = w8_bytes(count, N, K)
+        bufs = [self.buffer(codes // 8), self.buffer(steps // 8)]
+        w = W8(bufs[0].ptr, bufs[1].ptr, count, N, K)
+        w.bufs = bufs
+        return w
+
+    def free_w8(self, w: W8) -> None:
+        """Give back weights from new_w8 (which are refused from then on); those that only
+        describe the caller's memory have nothing to give back."""
+        for b in w.__dict__.pop("bufs", ()):
+            b.free()
+            self._bufs.remove(b)
+            w.codes = w.step = None
+
+    def w8_pack(self, w, index, W):
+        """Put matrix `index` into 8 bits from words W [N][K]."""
+        return check("q48_w8_pack", hip_lib().q48_w8_pack(self.h, C.byref(w), index, W))
+
+    def w8_put(self, w, index, codes, steps):
+        """Lay out matrix `index` from row-major codes [N][K] and steps [N]."""
+        return check("q48_w8_put", hip_lib().q48_w8_put(self.h, C.byref(w), index, codes, steps))
+
+    def w8_values(self, out, w, index):
+        return check("q48_w8_values", hip_lib().q48_w8_values(self.h, out, C.byref(w), index))
+
+    def gemm_w8(self, Y, base, w, X, norm_w, T):
+        """Y = base + rows X (rmsnorm'ed with norm_w) in 8 bits times w; base, norm_w: or None."""
+        return check("q48_gemm_w8", hip_lib().q48_gemm_w8(self.h, Y, base, C.byref(w), X, norm_w,
+                                                          T))
+
+    def gemm_w8_swiglu(self, out, gate, up, X, norm_w, T):
+        return check("q48_gemm_w8_swiglu", hip_lib().q48_gemm_w8_swiglu(
+            self.h, out, C.byref(gate), C.byref(up), X, norm_w, T))
+
+    @staticmethod
+    def moe(router, gate, up, down, top_k, renorm) -> Moe:
+        """Describe a mixture-of-experts layer (the weights' buffers stay the caller's)."""
+        return Moe(router, gate, up, down, top_k, int(renorm))
+
+    def moe_w8(self, out, base, moe, X, norm_w, T, chosen=None, weight=None):
+        return check("q48_moe_w8", hip_lib().q48_moe_w8(self.h, out, base, C.byref(moe), X, norm_w,
+                                                        T, chosen, weight))
 
     def prof_enable(self, on: bool = True):
         check("q48_prof_enable", hip_lib().q48_prof_enable(self.h, int(on)))

@@ -1,0 +1,241 @@
+"""Weights in 8 bits and their products on the GPU, word for word against the plain form
+in Python integers.
+"""
+import numpy as np
+import pytest
+
+import intllm
+import w8_plain as W
+
+pytestmark = pytest.mark.gpu
+I64 = np.iinfo(np.int64)
+
+
+def words(rng, *shape, sigma=1.0):
+    return (rng.standard_normal(shape) * (sigma * W.ONE)).astype(np.int64)
+
+
+def weights(rng, *shape, sigma=0.02):
+    c = np.clip(np.rint(rng.standard_normal(shape) * 32), -127, 127).astype(np.int8)
+    return c, (rng.uniform(0.7, 1.3, shape[:-1]) * (sigma / 32 * W.ONE)).astype(np.int64)
+
+
+def raw(ctx, a):
+    """Any array's bytes on the device."""
+    b = np.ascontiguousarray(a).view(np.uint8).ravel()
+    return ctx.to_device(np.concatenate([b, np.zeros(-b.size % 8, np.uint8)]).view(np.int64))
+
+
+def put(ctx, w, i, codes, steps):
+    ctx.w8_put(w, i, raw(ctx, codes).ptr, ctx.to_device(steps).ptr)
+    ctx.sync()
+
+
+def loaded(ctx, codes, steps):
+    """A matrix (or a stack of them) on the device."""
+    c, s = (codes, steps) if codes.ndim == 3 else (codes[None], steps[None])
+    w = ctx.new_w8(*c.shape)
+    for i in range(c.shape[0]):
+        put(ctx, w, i, c[i], s[i])
+    return w
+
+
+@pytest.fixture
+def own():
+    """A context whose buffers go with the test."""
+    with intllm.Context(0) as c:
+        yield c
+
+
+SIZES = [(1, 1), (1, 64), (16, 64), (15, 63), (17, 65), (3, 1000), (33, 129), (100, 2048), (7, 5633)]
+
+
+@pytest.mark.parametrize("N,K", SIZES)
+def test_weights_from_words(own, N, K):
+    rng = np.random.default_rng(N * 10007 + K)
+    x = words(rng, N, K, sigma=0.02)
+    x[N // 2] = 0
+    x[0, K // 2] = I64.min
+    if N > 2:
+        x[2] = rng.integers(-3, 4, K)          # steps of a word or two
+    c, s = W.quantise(x)
+    w = own.new_w8(1, N, K)
+    bufs = w.bufs
+    for b in bufs:
+        b.upload(np.full(b.n, -1))
+    own.w8_pack(w, 0, own.to_device(x).ptr)
+    assert (bufs[1].download() == s).all()
+    assert (bufs[0].download().view(np.int8) == W.tiles(c)).all()
+    out = own.to_device(np.full(N * K + 1, 5))
+    own.w8_values(out.ptr, w, 0)
+    got = out.download()
+    assert (got[:-1].reshape(N, K) == W.values(c, s)).all() and got[-1] == 5
+
+
+def test_one_of_several_matrices(own):
+    """The others stay as they are."""
+    rng = np.random.default_rng(1)
+    N, K, n = 21, 70, 3
+    w = own.new_w8(n, N, K)
+    codes, steps = weights(rng, n, N, K)
+    steps[1, 3] = -5                           # counts as 0
+    codes[1, 4, 5] = -128
+    for i in (2, 0, 1):
+        put(own, w, i, codes[i], steps[i])
+    for i in range(n):
+        out = own.buffer(N * K)
+        own.w8_values(out.ptr, w, i)
+        assert (out.download().reshape(N, K) == W.values(codes[i], steps[i].clip(0))).all()
+    x = words(rng, N, K)
+    own.w8_pack(w, 1, own.to_device(x).ptr)
+    tiles = w.bufs[0].download().view(np.int8).reshape(n, -1)
+    for i in range(n):
+        assert (tiles[i] == W.tiles(W.quantise(x)[0] if i == 1 else codes[i])).all()
+
+
+def check(ctx, T, N, K, norm, base, rng, X=None, codes=None, steps=None):
+    X = words(rng, T, K) if X is None else X
+    if codes is None:
+        codes, steps = weights(rng, N, K)
+    nw = W.ONE + words(rng, K, sigma=0.1) if norm else None
+    b = words(rng, T, N) if base else None
+    w = loaded(ctx, codes, steps)
+    dX, dn = ctx.to_device(X), ctx.to_device(nw) if norm else None
+    want = W.product(X, nw, codes, steps.clip(0), b)
+    y = ctx.to_device(np.full(T * N + 1, 5))
+    db = ctx.to_device(b) if base else None
+    ctx.gemm_w8(y.ptr, db and db.ptr, w, dX.ptr, dn and dn.ptr, T)
+    got = y.download()
+    assert (got[:-1].reshape(T, N) == want).all() and got[-1] == 5
+    assert (dX.download() == X.ravel()).all()
+    if base:                                   # onto the base itself
+        assert (db.download() == b.ravel()).all()
+        ctx.gemm_w8(db.ptr, db.ptr, w, dX.ptr, dn and dn.ptr, T)
+        assert (db.download().reshape(T, N) == want).all()
+
+
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("N,K", SIZES)
+@pytest.mark.parametrize("T", [1, 3])
+def test_products_of_few_rows(own, T, N, K, norm):
+    check(own, T, N, K, norm, norm, np.random.default_rng(T * N + K))
+
+
+@pytest.mark.parametrize("T,N,K", [(2, 40, 300), (15, 33, 130), (16, 64, 64), (17, 31, 257), (31, 48, 100),
+                                   (32, 130, 64), (33, 100, 640), (63, 70, 65), (64, 64, 512),
+                                   (65, 17, 700), (127, 129, 130), (128, 128, 128), (129, 255, 300),
+                                   (200, 300, 200), (257, 257, 257), (300, 128, 1030)])
+@pytest.mark.parametrize("norm,base", [(False, True), (True, False)])
+def test_products_of_many_rows(own, T, N, K, norm, base):
+    check(own, T, N, K, norm, base, np.random.default_rng(T * N + K))
+
+
+@pytest.mark.parametrize("T", [1, 40])
+def test_products_of_decode_shapes(own, T):
+    check(own, T, 2048, 5632, False, True, np.random.default_rng(T))
+    check(own, T, 2560, 2048, True, False, np.random.default_rng(T + 1))
+
+
+@pytest.mark.parametrize("T", [1, 20, 150])
+def test_the_longest_rows(own, T):
+    """K = 131072 with every code at the end of its range: sums near 2^31."""
+    rng = np.random.default_rng(5)
+    K, N = 1 << 17, 5
+    X = np.full((T, K), W.ONE)
+    X[T // 2] = -W.ONE
+    codes = np.full((N, K), 127, dtype=np.int8)
+    codes[1] = -128
+    codes[2, ::2] = -127
+    steps = np.array([W.ONE // 5, W.ONE // 3, 7, (1 << 63) - 1, -1])
+    check(own, T, N, K, False, False, rng, X, codes, steps)
+    with pytest.raises(intllm.Q48Error):
+        own.new_w8(1, N, K + 1)
+
+
+@pytest.mark.parametrize("T", [1, 20, 150])
+def test_extreme_words(own, T):
+    """Rows of the ends of the words' range, of zeros, of single units; steps of 0, 1 and
+    the largest: results mod 2^64."""
+    rng = np.random.default_rng(T)
+    N, K = 40, 200
+    X = words(rng, T, K)
+    X[0] = rng.choice([I64.min, I64.max, 0, 1, -1], K)
+    if T > 5:
+        X[1], X[2], X[3] = 0, I64.min, rng.integers(-2, 3, K)
+        X[4] = rng.integers(I64.min, I64.max, K)
+    codes, steps = weights(rng, N, K)
+    steps[:6] = [0, 1, I64.max, I64.max // 127, W.ONE, W.ONE // 127]
+    codes[7] = 0
+    for norm in (False, True):
+        check(own, T, N, K, norm, True, rng, X, codes, steps)
+
+
+@pytest.mark.parametrize("T,N,K,norm", [(1, 5, 9, True), (1, 688, 256, True), (1, 1408, 2048, False),
+                                        (1, 5632, 2048, True), (4, 33, 65, False), (16, 100, 300, True),
+                                        (17, 50, 64, True), (65, 130, 128, True), (130, 200, 257, False),
+                                        (300, 129, 256, True)])
+def test_swiglu(own, T, N, K, norm):
+    rng = np.random.default_rng(T + N)
+    X = words(rng, T, K, sigma=2.0)
+    gate, up = weights(rng, N, K, sigma=0.1), weights(rng, N, K, sigma=0.1)
+    gate[1][N // 2] *= 40                       # past the sigmoid's 10 on both sides
+    up[1][N // 3] = 0
+    nw = W.ONE + words(rng, K, sigma=0.1) if norm else None
+    g, u = loaded(own, *gate), loaded(own, *up)
+    out = own.to_device(np.full(T * N + 1, 5))
+    own.gemm_w8_swiglu(out.ptr, g, u, own.to_device(X).ptr, own.to_device(nw).ptr if norm else None,
+                       T)
+    got = out.download()
+    assert (got[:-1].reshape(T, N) == W.swiglu(X, nw, gate, up)).all() and got[-1] == 5
+
+
+def test_rows_off_sixteen_bytes(own):
+    """Words on the boundary of a word and no more."""
+    rng = np.random.default_rng(9)
+    for T, N, K in ((1, 65, 64), (3, 40, 2048), (1, 31, 5632), (70, 64, 128)):
+        X, b = words(rng, T, K), words(rng, T, N)
+        codes, steps = weights(rng, N, K)
+        nw = W.ONE + words(rng, K, sigma=0.1)
+        w = loaded(own, codes, steps)
+        dX, dn = own.to_device(np.append(0, X)), own.to_device(np.append(0, nw))
+        db, y = own.to_device(np.append(0, b)), own.buffer(T * N + 1)
+        own.gemm_w8(y.at(1), db.at(1), w, dX.at(1), dn.at(1), T)
+        assert (y.download()[1:].reshape(T, N) == W.product(X, nw, codes, steps, b)).all()
+
+
+def test_captured_and_replayed(own):
+    """Products of one shape as a graph, its inputs changed between replays, eager calls
+    of other shapes among them; a shape that was never called is refused in a capture."""
+    rng = np.random.default_rng(2)
+    lib, c = intllm.hip_lib(), own
+    T, N, K = 3, 96, 300
+    gate, up, down = weights(rng, N, K), weights(rng, N, K), weights(rng, K, N)
+    g, u, d = (loaded(c, *w) for w in (gate, up, down))
+    nw = W.ONE + words(rng, K, sigma=0.1)
+    dn, dX, h = c.to_device(nw), c.buffer(T * K), c.buffer(T * N)
+
+    def step():
+        c.gemm_w8_swiglu(h.ptr, g, u, dX.ptr, dn.ptr, T)
+        c.gemm_w8(dX.ptr, dX.ptr, d, h.ptr, None, T)
+
+    step()
+    c.sync()
+    many, into = c.buffer(3990 * K), c.buffer(3990 * N)
+    intllm.check("begin", lib.q48_graph_begin(c.h))
+    step()
+    with pytest.raises(intllm.Q48Error) as err:
+        c.gemm_w8(into.ptr, None, g, many.ptr, None, 3990)
+    assert err.value.code == intllm.Q48_ESTATE
+    intllm.check("end", lib.q48_graph_end(c.h))
+    x = words(rng, T, K)
+    dX.upload(x)
+    other = words(rng, 200, K)
+    do, oo = c.to_device(other), c.buffer(200 * N)
+    for i in range(4):
+        intllm.check("launch", lib.q48_graph_launch(c.h, 1))
+        x = W.product(W.swiglu(x, nw, gate, up), None, *down, x)
+        assert (dX.download().reshape(T, K) == x).all(), i
+        if i < 2:
+            c.gemm_w8(oo.ptr, None, g, do.ptr, dn.ptr, 200)   # grows the context's buffer once
+            assert (oo.download().reshape(200, N) == W.product(other, nw, *gate)).all()
+    intllm.check("drop", lib.q48_graph_drop(c.h))
