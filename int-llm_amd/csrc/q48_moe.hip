@@ -13,8 +13,130 @@ namespace {
 
 constexpr int MOE_MAX_TOP = 64;
 
-// A wave a token: k times the largest logit not yet taken, the lowest expert of equal
-// ones; then the weights.
+// Words that other blocks of the launch read behind a ticket: coherent stores and loads.
+template <class V>
+__device__ __forceinline__ void out_to_all(V *p, V v)
+{
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <class V>
+__device__ __forceinline__ V from_all(const V *p)
+{
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// A wave chooses a token's experts: lane l holds the logits of experts l + 64 i in v, and
+// gets the l-th choice and its weight (l < top).  top times the largest logit not yet
+// taken, of equal ones the lowest expert.
+template <int PER>
+__device__ __forceinline__ void moe_choose(const int64_t (&v)[PER], int E, int top, bool renorm,
+                                           int &id, int64_t &weight)
+{
+    const int lane = threadIdx.x & 63;
+    uint32_t left = 0;   // bit i: expert lane + 64 i, not taken
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        left |= lane + 64 * i < E ? 1u << i : 0u;
+    int64_t m = 0, mine = 0;
+    id = 0;
+    for (int j = 0; j < top; ++j) {
+        int64_t best = INT64_MIN;
+        int at = E;   // none left: past every expert
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            if (((left >> i) & 1) && (at == E || v[i] > best)) {
+                best = v[i];
+                at = lane + 64 * i;
+            }
+        const int64_t most = q48_wave_max64(best);
+        uint64_t who = __ballot(at < E && best == most);
+        int won;
+        if constexpr (PER == 1) {
+            won = (int)__builtin_ctzll(who);
+        } else {
+            won = E;   // the lowest expert of the lanes that hold it
+            while (who) {
+                const int o = __builtin_amdgcn_readlane(at, (int)__builtin_ctzll(who));
+                won = o < won ? o : won;
+                who &= who - 1;
+            }
+        }
+        if (at == won)
+            left &= ~(1u << (won >> 6));
+        if (j == 0)
+            m = most;
+        if (lane == j) {
+            mine = most;
+            id = won;
+        }
+    }
+    const int64_t e = q48_expn((uint64_t)m - (uint64_t)mine);
+    int64_t sum = lane < top ? e : 0;
+    if (!renorm) {
+        sum = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            sum += lane + 64 * i < E ? q48_expn((uint64_t)m - (uint64_t)v[i]) : 0;
+    }
+    sum = q48_wave_sum64(sum);
+    weight = q48_div(e, sum);
+}
+
+// The pairs counted by expert, each expert's first slot, the items of 16 slots, and every
+// pair into its slot: one block of NT threads.
+struct MoeSlots {
+    int4 *items;
+    int *tok;
+    int64_t *w;
+    int slots, n_items;
+};
+template <int NT>
+__device__ __forceinline__ void moe_slots(const MoeSlots &s, const int *chosen,
+                                          const int64_t *weight, int pairs, int top, int E)
+{
+    __shared__ int count[W8_MAX_COUNT], first[W8_MAX_COUNT];
+    const int tid = threadIdx.x, lane = tid & 63;
+    for (int i = tid; i < E; i += NT)
+        count[i] = 0;
+    for (int i = tid; i < s.slots; i += NT)
+        s.tok[i] = -1;
+    for (int i = tid; i < s.n_items; i += NT)
+        s.items[i] = make_int4(0, 0, 0, 0);
+    __syncthreads();
+    for (int i = tid; i < pairs; i += NT)
+        atomicAdd(&count[from_all(chosen + i)], 1);
+    __syncthreads();
+    if (tid < 64) {   // sixteens before each expert: sums over the lanes of a wave
+        int before = 0;
+        for (int e0 = 0; e0 < E; e0 += 64) {
+            const int n = e0 + lane < E ? (count[e0 + lane] + 15) & ~15 : 0;
+            int sum = n;
+            for (int d = 1; d < 64; d <<= 1) {
+                const int o = __shfl_up(sum, d);
+                sum += lane >= d ? o : 0;
+            }
+            if (e0 + lane < E)
+                first[e0 + lane] = before + sum - n;
+            before += __builtin_amdgcn_readlane(sum, 63);
+        }
+    }
+    __syncthreads();
+    for (int e = tid; e < E; e += NT) {
+        const int n = count[e];
+        for (int i = 0; i < n; i += 16)
+            s.items[(first[e] + i) >> 4] = make_int4(e, first[e] + i, min(16, n - i), 0);
+        count[e] = first[e];
+    }
+    __syncthreads();
+    for (int i = tid; i < pairs; i += NT) {
+        const int at = atomicAdd(&count[from_all(chosen + i)], 1);
+        s.tok[at] = i / top;
+        s.w[at] = from_all(weight + i);
+    }
+}
+
+// A wave a token.
+template <int PER>
 __global__ __launch_bounds__(256) void k_moe_choose(const int64_t *__restrict__ logits, int T,
                                                    int E, int top, int renorm,
                                                    int *__restrict__ chosen,
@@ -24,95 +146,201 @@ __global__ __launch_bounds__(256) void k_moe_choose(const int64_t *__restrict__ 
     const int lane = threadIdx.x & 63, t = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (t >= T)
         return;
-    const int64_t *l = logits + (size_t)t * E;
-    uint32_t taken = 0;   // bit i: expert lane + 64 i
-    int64_t m = 0, sum = 0, mine = 0;
-    int my_id = 0;
-    for (int j = 0; j < top; ++j) {
-        int64_t best = INT64_MIN;
-        int id = E;   // none left: past every id
-        for (int i = 0; lane + 64 * i < E; ++i) {
-            const int64_t v = l[lane + 64 * i];
-            if (!((taken >> i) & 1) && (id == E || v > best)) {
-                best = v;
-                id = lane + 64 * i;
-            }
-        }
-        const int64_t at = q48_wave_max64(best);
-        const int won = (int)-q48_wave_max64(best == at && id < E ? -(int64_t)id : -(int64_t)E);
-        if (id == won)
-            taken |= 1u << (won >> 6);
-        if (j == 0)
-            m = at;
-        const int64_t e = q48_expn((uint64_t)m - (uint64_t)at);
-        if (renorm)
-            sum += e;
-        if (lane == j) {
-            mine = e;
-            my_id = won;
-        }
-    }
-    if (!renorm) {
-        for (int i = lane; i < E; i += 64)
-            sum += q48_expn((uint64_t)m - (uint64_t)l[i]);
-        sum = q48_wave_sum64(sum);
-    }
+    int64_t v[PER], w;
+    int id;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+        v[i] = lane + 64 * i < E ? logits[(size_t)t * E + lane + 64 * i] : 0;
+    moe_choose<PER>(v, E, top, renorm != 0, id, w);
     if (lane < top) {
-        chosen[(size_t)t * top + lane] = my_id;
-        weight[(size_t)t * top + lane] = q48_div(mine, sum);
+        chosen[(size_t)t * top + lane] = id;
+        weight[(size_t)t * top + lane] = w;
     }
 }
 
-// One block: the pairs counted by expert, each expert's first slot, the items of 16
-// slots, and every pair into its slot.
 __global__ __launch_bounds__(1024) void k_moe_slots(const int *__restrict__ chosen,
                                                    const int64_t *__restrict__ weight, int pairs,
-                                                   int top, int E, int slots, int n_items,
-                                                   int4 *__restrict__ items,
-                                                   int *__restrict__ slot_tok,
-                                                   int64_t *__restrict__ slot_w)
+                                                   int top, int E, MoeSlots s)
 {
-    __shared__ int count[W8_MAX_COUNT], first[W8_MAX_COUNT + 1];
-    const int tid = threadIdx.x;
-    count[tid] = 0;
-    for (int i = tid; i < slots; i += 1024)
-        slot_tok[i] = -1;
-    for (int i = tid; i < n_items; i += 1024)
-        items[i] = make_int4(0, 0, 0, 0);
-    __syncthreads();
-    for (int i = tid; i < pairs; i += 1024)
-        atomicAdd(&count[chosen[i]], 1);
-    __syncthreads();
-    if (tid == 0) {
-        int s = 0;
-        for (int e = 0; e < E; ++e) {
-            first[e] = s;
-            s += (count[e] + 15) & ~15;
+    moe_slots<1024>(s, chosen, weight, pairs, top, E);
+}
+
+// Everything before the experts in one launch, for few tokens: block (g, t) norms row t
+// and makes the logits of experts g per + 0 .. per - 1; one block more a token its codes.
+// The last block of a token to finish chooses, the last of those makes the slots (tickets;
+// no block waits for another).
+constexpr int ROUTE_PER = 16;    // experts a block at most
+constexpr int ROUTE_T = 1024;    // tokens at most
+struct MoeRoute {
+    W8Rows rows;
+    const int64_t *router;
+    int64_t *logits;
+    int E, per, sl, top, renorm;
+    int *chosen;
+    int64_t *weight;
+    int *ticket;                 // [0]: tokens, [1 + t]: blocks of token t; zeros between launches
+    MoeSlots s;
+};
+template <int NT, int J, bool NORM, int PER>
+__global__ __launch_bounds__(1024) void k_moe_route(MoeRoute a)
+{
+    q48_round_down();
+    constexpr int NW = 16;
+    extern __shared__ __align__(16) int64_t xs[];   // the row, normed
+    __shared__ uint64_t red[NT / 64][2], peak[NT / 64], part[NW][2];
+    __shared__ int last;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int t = blockIdx.y, K = a.rows.K, T = a.rows.T, E = a.E, G = gridDim.x - 1;
+    const int e0 = blockIdx.x * a.per, n = min(a.per, E - e0);
+    if (tid < NT) {
+        RowWords<NT, 2, J> x;
+        x.load(a.rows.X + (size_t)t * K, K);
+        if constexpr (NORM) {
+            RowWords<NT, 2, J> nw;
+            nw.load(a.rows.norm_w, K);
+            x.norm(nw, K, red);
         }
-        first[E] = s;
+        if ((int)blockIdx.x == G) {
+            const int KT = (K + 63) / 64;
+            const int64_t step = x.quantise(K, KT, peak, [&](int i, uint32_t q) {
+                *(uint16_t *)(a.rows.codes + w8_at(t, i, KT)) = (uint16_t)q;
+            });
+            if (tid == 0)
+                a.rows.step[t] = step;
+            return;
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+            if (x.at(j) < K) {
+                xs[x.at(j)] = x.v[j][0];
+                xs[x.at(j) + 1] = x.v[j][1];
+            }
+    } else {
+        if constexpr (NORM)
+            lds_barrier();
+        if ((int)blockIdx.x == G) {
+            if (a.rows.out)
+                for (int i = tid - NT; i < K; i += 1024 - NT)
+                    a.rows.out[(size_t)t * K + i] = a.rows.base ? a.rows.base[(size_t)t * K + i] : 0;
+            lds_barrier();
+            return;
+        }
+    }
+    lds_barrier();
+    // S = 2^sl waves an expert, each its share of the row
+    const int sl = a.sl, S = 1 << sl, e = w >> sl, seg = ((K + S - 1) >> sl);
+    q48_u128 sum = 0;
+    if (e < n) {
+        const int from = (w & (S - 1)) * seg, to = min(from + seg, K);
+        const int64_t *r = a.router + (size_t)(e0 + e) * K;
+        for (int i = from + lane; i < to; i += 64 * 8) {
+            int64_t v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                v[u] = i + 64 * u < to ? r[i + 64 * u] : 0;
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (i - lane + 64 * u < to)
+                    sum += (q48_u128)q48_smul128(xs[min(i + 64 * u, K - 1)], v[u]);
+        }
+        sum = q48_wave_sum128(sum);
+    }
+    if (lane == 0) {
+        part[w][0] = (uint64_t)sum;
+        part[w][1] = (uint64_t)(sum >> 64);
+    }
+    lds_barrier();
+    if (tid < n) {
+        sum = 0;
+        for (int i = 0; i < S; ++i)
+            sum += ((q48_u128)part[(tid << sl) + i][1] << 64) | part[(tid << sl) + i][0];
+        out_to_all(a.logits + (size_t)t * E + e0 + tid, (int64_t)(uint64_t)(sum >> 48));
+        __builtin_amdgcn_s_waitcnt(0);   // out before the ticket (n <= 16: one wave's stores)
+    }
+    if (tid == 0) {
+        const int at = __hip_atomic_fetch_add(a.ticket + 1 + t, 1, __ATOMIC_RELAXED,
+                                              __HIP_MEMORY_SCOPE_AGENT);
+        last = at == G - 1;
+        if (at == G - 1)
+            out_to_all(a.ticket + 1 + t, 0);
     }
     __syncthreads();
-    if (tid < E)
-        for (int s = 0; s < count[tid]; s += 16)
-            items[(first[tid] + s) >> 4] =
-                make_int4(tid, first[tid] + s, min(16, count[tid] - s), 0);
-    __syncthreads();
-    if (tid < E)
-        count[tid] = 0;
-    __syncthreads();
-    for (int i = tid; i < pairs; i += 1024) {
-        const int e = chosen[i], s = first[e] + atomicAdd(&count[e], 1);
-        slot_tok[s] = i / top;
-        slot_w[s] = weight[i];
+    if (!last)
+        return;
+    if (tid < 64) {
+        int64_t v[PER], wt;
+        int id;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+            v[i] = lane + 64 * i < E ? from_all(a.logits + (size_t)t * E + lane + 64 * i) : 0;
+        moe_choose<PER>(v, E, a.top, a.renorm != 0, id, wt);
+        if (lane < a.top) {
+            out_to_all(a.chosen + (size_t)t * a.top + lane, id);
+            out_to_all(a.weight + (size_t)t * a.top + lane, wt);
+            if (T == 1) {   // every choice an item of one slot
+                a.s.items[lane] = make_int4(id, 16 * lane, 1, 0);
+                a.s.tok[16 * lane] = 0;
+                a.s.w[16 * lane] = wt;
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(0);
+        if (lane == 0 && T > 1) {
+            const int at = __hip_atomic_fetch_add(a.ticket, 1, __ATOMIC_RELAXED,
+                                                  __HIP_MEMORY_SCOPE_AGENT);
+            last = at == T - 1;
+            if (at == T - 1)
+                out_to_all(a.ticket, 0);
+        }
     }
+    if (T == 1)
+        return;
+    __syncthreads();
+    if (last)
+        moe_slots<1024>(a.s, a.chosen, a.weight, T * a.top, a.top, E);
 }
 
 int launch_rc(int e) { return e == (int)hipSuccess ? Q48_OK : Q48_EHIP; }
 
 // slots that n pairs of at most E experts can take, in sixteens
-size_t moe_slots(size_t pairs, int E)
+size_t slots_of(size_t pairs, int E)
 {
     return (pairs + 15 * (pairs < (size_t)E ? pairs : (size_t)E) + 15) & ~(size_t)15;
+}
+
+// experts a block of k_moe_route, 0 for the separate launches (a row of words in LDS)
+int route_per(const q48_ctx *c, int T, int E, int dim)
+{
+    const int per = ((long)E * T + c->cu_count - 1) / c->cu_count;
+    return dim <= 6144 && T <= ROUTE_T && per <= ROUTE_PER ? per : 0;
+}
+
+int launch_route(q48_ctx *c, const MoeRoute &a)
+{
+    const dim3 grid((a.E + a.per - 1) / a.per + 1, a.rows.T);
+    const size_t lds = 8 * (size_t)((a.rows.K + 1) & ~1);
+#define ROUTE(NT, J, NORM, PER)                                                                \
+    hipLaunchKernelGGL((k_moe_route<NT, J, NORM, PER>), grid, dim3(1024), lds, c->stream, a)
+#define ROUTE_P(NT, J, NORM)                                                                   \
+    do {                                                                                       \
+        if (a.E <= 64)                                                                         \
+            ROUTE(NT, J, NORM, 1);                                                                 \
+        else if (a.E <= 128)                                                                   \
+            ROUTE(NT, J, NORM, 2);                                                                 \
+        else                                                                                   \
+            ROUTE(NT, J, NORM, 16);                                                                \
+    } while (0)
+    if (a.rows.K <= 2048 && a.rows.norm_w)
+        ROUTE_P(256, 4, true);
+    else if (a.rows.K <= 2048)
+        ROUTE_P(256, 4, false);
+    else if (a.rows.norm_w)
+        ROUTE_P(512, 8, true);
+    else
+        ROUTE_P(512, 8, false);
+#undef ROUTE_P
+#undef ROUTE
+    return (int)hipGetLastError();
 }
 
 } // namespace
@@ -152,7 +380,8 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
     if (q48_share(chosen, np * 4, weight, np * 8))
         return Q48_EINVAL;
     q48_on_device on(c);
-    size_t o = 0;
+    static_assert(sizeof(int) * (1 + ROUTE_T) <= W8_TICKETS, "tickets");
+    size_t o = W8_TICKETS;
     auto take = [&](size_t bytes) {
         const size_t at = o;
         o += (bytes + 255) & ~(size_t)255;
@@ -162,7 +391,7 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
     size_t Tc = ((size_t)1 << 30) / ((size_t)16 * top * ffn);
     Tc = Tc < ((size_t)1 << 19) / top ? Tc : ((size_t)1 << 19) / top;
     Tc = Tc < 16 ? 16 : Tc < (size_t)T ? Tc : (size_t)T;
-    const size_t slots = moe_slots(Tc * top, E), n_items = slots / 16;
+    const size_t slots = slots_of(Tc * top, E), n_items = slots / 16;
     const size_t o_x = take(w8_tiles((int)Tc, dim)), o_xs = take(Tc * 8);
     const size_t o_xn = take(norm_w ? Tc * row : 0), o_l = take(Tc * E * 8);
     const size_t o_c = take(Tc * top * 4), o_w = take(Tc * top * 8);
@@ -175,7 +404,7 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
     uint8_t *ws = (uint8_t *)c->w8;
     for (size_t t0 = 0; t0 < (size_t)T; t0 += Tc) {
         const int n = (int)(Tc < T - t0 ? Tc : T - t0);
-        const int sl = (int)moe_slots((size_t)n * top, E), it = sl / 16;
+        const int sl = (int)slots_of((size_t)n * top, E), it = sl / 16;
         W8Rows r = {};
         r.codes = ws + o_x;
         r.step = (int64_t *)(ws + o_xs);
@@ -188,23 +417,46 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
         }
         r.T = n;
         r.K = dim;
-        if ((rc = q48_launch_w8_rows(c, r)))
-            return launch_rc(rc);
-        const int64_t *xr = norm_w ? r.xn : r.X;
-        int64_t *lg = (int64_t *)(ws + o_l);
-        rc = n == 1 ? launch_rc(q48_launch_gemv(c, lg, moe->router, xr, E, dim))
-                    : q48_launch_gemm_i8(c, lg, moe->router, xr, n, E, dim, Q48_GEMM_AUTO, nullptr);
-        if (rc)
-            return rc < 0 ? rc : launch_rc(rc);
         int *ch = chosen ? chosen + t0 * top : (int *)(ws + o_c);
         int64_t *wt = weight ? weight + t0 * top : (int64_t *)(ws + o_w);
-        hipLaunchKernelGGL(k_moe_choose, dim3((n + 3) / 4), dim3(256), 0, c->stream, lg, n, E, top,
-                           moe->renorm, ch, wt);
+        int64_t *lg = (int64_t *)(ws + o_l);
         int4 *items = (int4 *)(ws + o_i);
         int *tok = (int *)(ws + o_t);
         int64_t *sw = (int64_t *)(ws + o_sw);
-        hipLaunchKernelGGL(k_moe_slots, dim3(1), dim3(1024), 0, c->stream, ch, wt, n * top, top, E,
-                           sl, it, items, tok, sw);
+        const MoeSlots s = {items, tok, sw, sl, it};
+        const int per = route_per(c, n, E, dim);
+        if (per) {
+            int spl = 4;
+            while ((per << spl) > 16)
+                --spl;
+            const MoeRoute a = {r, moe->router, lg, E, per, spl, top, moe->renorm, ch, wt,
+                                (int *)ws, s};
+            rc = launch_route(c, a);
+        } else {
+            if ((rc = q48_launch_w8_rows(c, r)))
+                return launch_rc(rc);
+            const int64_t *xr = norm_w ? r.xn : r.X;
+            rc = n == 1 ? launch_rc(q48_launch_gemv(c, lg, moe->router, xr, E, dim))
+                        : q48_launch_gemm_i8(c, lg, moe->router, xr, n, E, dim, Q48_GEMM_AUTO,
+                                             nullptr);
+            if (rc)
+                return rc < 0 ? rc : launch_rc(rc);
+#define MOE_CHOOSE(PER)                                                                        \
+    hipLaunchKernelGGL(k_moe_choose<PER>, dim3((n + 3) / 4), dim3(256), 0, c->stream, lg, n, E, \
+                       top, moe->renorm, ch, wt)
+            if (E <= 64)
+                MOE_CHOOSE(1);
+            else if (E <= 128)
+                MOE_CHOOSE(2);
+            else
+                MOE_CHOOSE(16);
+#undef MOE_CHOOSE
+            hipLaunchKernelGGL(k_moe_slots, dim3(1), dim3(1024), 0, c->stream, ch, wt, n * top, top,
+                               E, s);
+            rc = (int)hipGetLastError();
+        }
+        if (rc)
+            return launch_rc(rc);
         W8Mul m = {};
         m.A = (const uint8_t *)g.codes;
         m.A2 = (const uint8_t *)u.codes;
@@ -220,7 +472,9 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
         m.items = items;
         m.slot_tok = tok;
         m.slot_w = sw;
-        if ((rc = q48_launch_w8_mul(c, m, 1, true, it)))
+        const bool one = n == 1 && q48_w8_one_ok(ffn);   // every item a slot
+        if ((rc = one ? q48_launch_w8_one(c, m, 1, nullptr, nullptr, dim, top)
+                      : q48_launch_w8_mul(c, m, 1, true, it)))
             return launch_rc(rc);
         W8Rows h = {};
         h.codes = ws + o_hc;
@@ -229,7 +483,7 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
         h.tok = tok;
         h.T = sl;
         h.K = ffn;
-        if ((rc = q48_launch_w8_rows(c, h)))
+        if (!one && (rc = q48_launch_w8_rows(c, h)))
             return launch_rc(rc);
         m.A = (const uint8_t *)d.codes;
         m.A2 = nullptr;
@@ -241,7 +495,8 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
         m.B = h.codes;
         m.sb = h.step;
         m.Y = out + t0 * dim;
-        if ((rc = q48_launch_w8_mul(c, m, 2, true, it)))
+        if ((rc = one ? q48_launch_w8_one(c, m, 2, h.X, nullptr, ffn, top)
+                      : q48_launch_w8_mul(c, m, 2, true, it)))
             return launch_rc(rc);
     }
     return Q48_OK;

@@ -4,26 +4,6 @@
 
 namespace {
 
-// floor(S sa sw / 2^48) mod 2^64 for steps in [0, 2^63): the product of the three mod
-// 2^128 holds the bits 48 .. 111 that are asked for.
-__device__ __forceinline__ int64_t w8_scaled(int S, int64_t sa, int64_t sw)
-{
-    const q48_u128 p = (q48_u128)(uint64_t)sa * (uint64_t)sw;
-    const q48_u128 v = p * (uint32_t)(S < 0 ? 0u - (uint32_t)S : (uint32_t)S);
-    return (int64_t)(uint64_t)((q48_i128)(S < 0 ? 0 - v : v) >> 48);
-}
-
-// the step of a row whose largest magnitude is a, and its reciprocal
-__device__ __forceinline__ uint64_t w8_step(uint64_t a, double &r)
-{
-    const uint64_t cap = (uint64_t)INT64_MAX / 127, s = (a + 126) / 127;
-    const uint64_t step = s < cap ? s : cap;
-    const double d = (double)step;
-    r = __builtin_amdgcn_rcp(d);
-    r = __builtin_fma(r, __builtin_fma(-d, r, 1.0), r);
-    return step;
-}
-
 __device__ __forceinline__ uint64_t block_umax(uint64_t v, uint64_t *red)
 {
     // magnitudes are at most 2^63: as signed words, less one, in order
@@ -36,12 +16,6 @@ __device__ __forceinline__ uint64_t block_umax(uint64_t v, uint64_t *red)
         t = red[w] > t ? red[w] : t;
     __syncthreads();
     return t;
-}
-
-__device__ __forceinline__ size_t w8_at(int row, int col, int KT)
-{
-    return ((size_t)(row >> 4) * KT + (col >> 6)) * 1024 + ((col & 63) >> 4) * 256 +
-           (row & 15) * 16 + (col & 15);
 }
 
 // A block a row: sum of squares, largest magnitude, codes, each a pass over the row.
@@ -83,6 +57,43 @@ __global__ __launch_bounds__(256) void k_w8_rows(W8Rows a)
         a.step[t] = (int64_t)step;
     for (int i = tid; i < KT * 64; i += 256)
         a.codes[w8_at(t, i, KT)] = i < K && step ? (uint8_t)q48_code<127>(at(i), step, rc) : 0;
+}
+
+// The same with the row in registers, read once.
+template <int NT, int C, int J, bool NORM>
+__global__ __launch_bounds__(NT) void k_w8_rows_r(W8Rows a)
+{
+    q48_round_down();
+    __shared__ uint64_t red[NT / 64][2], top[NT / 64];
+    const int t = blockIdx.x, K = a.K, KT = (K + 63) / 64;
+    if (a.tok && a.tok[t] < 0)
+        return;
+    RowWords<NT, C, J> x;
+    x.load(a.X + (size_t)t * K, K);
+    if constexpr (NORM) {
+        RowWords<NT, C, J> nw;
+        nw.load(a.norm_w, K);
+        x.norm(nw, K, red);
+    }
+    if (a.xn)
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+                if (x.at(j) + c < K)
+                    a.xn[(size_t)t * K + x.at(j) + c] = x.v[j][c];
+    if (a.out)
+        for (int i = threadIdx.x; i < K; i += NT)
+            a.out[(size_t)t * K + i] = a.base ? a.base[(size_t)t * K + i] : 0;
+    const int64_t step = x.quantise(K, KT, top, [&](int i, uint32_t q) {
+        uint8_t *to = a.codes + w8_at(t, i, KT);
+        if constexpr (C == 4)
+            *(uint32_t *)to = q;
+        else
+            *(uint16_t *)to = (uint16_t)q;
+    });
+    if (threadIdx.x == 0)
+        a.step[t] = step;
 }
 
 // A block a row of weights: step and codes, or codes and steps as they come.
@@ -165,20 +176,28 @@ __global__ __launch_bounds__(256) void k_w8_mul(W8Mul m)
         }
     }
     v4i acc[M][NB] = {};
-#pragma unroll 4
-    for (int k = w; k < KT; k += 4) {
-        v4i a[M], b[NB];
+    constexpr int P = NB == 1 ? 4 : 2;
+    for (int k0 = w; k0 < KT; k0 += 4 * P) {
+        v4i a[M][P], b[NB][P];
 #pragma unroll
-        for (int j = 0; j < M; ++j)
-            a[j] = *(const v4i *)(A[j] + (size_t)k * 1024);
-#pragma unroll
-        for (int g = 0; g < NB; ++g)
-            b[g] = *(const v4i *)(B[g] + (size_t)k * 1024);
-#pragma unroll
-        for (int g = 0; g < NB; ++g)
+        for (int p = 0; p < P; ++p) {
+            const size_t k = min(k0 + 4 * p, KT - 1);
 #pragma unroll
             for (int j = 0; j < M; ++j)
-                acc[j][g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[j], b[g], acc[j][g], 0, 0, 0);
+                a[j][p] = *(const v4i *)(A[j] + k * 1024);
+#pragma unroll
+            for (int g = 0; g < NB; ++g)
+                b[g][p] = *(const v4i *)(B[g] + k * 1024);
+        }
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+            if (k0 + 4 * p < KT)
+#pragma unroll
+                for (int g = 0; g < NB; ++g)
+#pragma unroll
+                    for (int j = 0; j < M; ++j)
+                        acc[j][g] =
+                            __builtin_amdgcn_mfma_i32_16x16x64_i8(a[j][p], b[g][p], acc[j][g], 0, 0, 0);
     }
     // lane l, register i: weight row 4 (l / 16) + i, row l % 16
     const int n = n0 + (tid & 15);
@@ -217,6 +236,163 @@ __global__ __launch_bounds__(256) void k_w8_mul(W8Mul m)
     }
 }
 
+// ---- one row ------------------------------------------------------------------
+
+constexpr int ONE_NT = 1024;   // threads of a k_w8_one block
+
+// One row times weights: S = 2^sl of the block's sixteen waves share a tile of 16 weight
+// rows, each every S-th of its 64-column tiles; the row stands in all 16 columns of the
+// matrix instruction's other operand.  SRC 1: the row from words, 2: rmsnorm'ed, both
+// quantised by every block while its first weight tiles are on their way; 0: from codes.
+template <int EPI, bool EXPERTS, int SRC, int NT, int J>
+__global__ __launch_bounds__(ONE_NT) void k_w8_one(W8Mul m, const int64_t *__restrict__ X,
+                                                  const int64_t *__restrict__ norm_w, int K, int sl)
+{
+    q48_round_down();
+    constexpr int M = EPI == 1 ? 2 : 1, NW = ONE_NT / 64, P = 8 / M;
+    __shared__ __align__(16) uint8_t codes[SRC ? 2 * NT * J : 16];
+    __shared__ uint64_t red[NW][2], top[NW];
+    __shared__ int64_t step;
+    __shared__ __align__(16) int sums[M][NW][16];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int S = 1 << sl, TB = NW >> sl, ks = w & (S - 1);
+    int expert = 0, slot = 0, tok = 0;
+    int64_t wt = 0;
+    if constexpr (EXPERTS) {
+        const int4 it = m.items[blockIdx.y];
+        expert = it.x;
+        slot = it.y;
+        if (it.z <= 0)
+            return;
+        tok = m.slot_tok[slot];
+        if constexpr (EPI == 2)
+            wt = m.slot_w[slot];
+    }
+    const int KT = m.KT, NTILE = (m.N + 15) / 16, groups = (NTILE + TB - 1) / TB;
+    const size_t ex = (size_t)expert * m.a_stride + lane * 16;
+    const uint8_t *A0 = m.A + ex, *A1 = M == 2 ? m.A2 + ex : nullptr;
+    auto tile_at = [&](int g) { return (size_t)min(g * TB + (w >> sl), NTILE - 1) * KT; };
+    v4i pre[M][P];
+    auto load = [&](size_t t, int k0) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            const int k = k0 + p * S;
+            if (k >= KT)
+                break;
+            pre[0][p] = *(const v4i *)(A0 + (t + k) * 1024);
+            if constexpr (M == 2)
+                pre[1][p] = *(const v4i *)(A1 + (t + k) * 1024);
+        }
+    };
+    int g = blockIdx.x;
+    load(tile_at(g), ks);
+    int64_t sb;
+    const uint8_t *B = nullptr;
+    if constexpr (SRC) {
+        if (tid < NT) {
+            RowWords<NT, 2, J> x;
+            x.load(X + (EXPERTS ? (size_t)slot * K : 0), K);
+            if constexpr (SRC == 2) {
+                RowWords<NT, 2, J> nw;
+                nw.load(norm_w, K);
+                x.norm(nw, K, red);
+            }
+            sb = x.quantise(K, KT, top,
+                            [&](int i, uint32_t q) { *(uint16_t *)&codes[i] = (uint16_t)q; });
+            if (tid == 0)
+                step = sb;
+        } else {
+            lds_barrier();
+            if constexpr (SRC == 2)
+                lds_barrier();
+        }
+        lds_barrier();
+        sb = step;
+    } else {
+        sb = m.sb[tok];
+        B = m.B + (size_t)(tok >> 4) * KT * 1024 + (tok & 15) * 16 + (lane >> 4) * 256;
+    }
+    auto row = [&](int k) {
+        if constexpr (SRC)
+            return *(const v4i *)&codes[k * 64 + (lane >> 4) * 16];
+        else
+            return *(const v4i *)(B + (size_t)k * 1024);
+    };
+    const int64_t *sw = m.sw + (size_t)expert * m.N, *sw2 = m.sw2 + (size_t)expert * m.N;
+    for (; g < groups; g += gridDim.x) {
+        const size_t t = tile_at(g);
+        // what the epilogue needs, ahead of the products
+        int64_t s1 = 0, s2 = 0, add = 0;
+        const int at = min((g * TB + (tid >> (sl + 4))) * 16 + ((tid >> sl) & 15), m.N - 1);
+        if (tid < 256) {
+            s1 = sw[at];
+            if constexpr (EPI == 1)
+                s2 = sw2[at];
+            if (EPI == 0 && m.base)
+                add = m.base[at];
+        }
+        v4i acc[M] = {};
+        for (int k0 = ks; k0 < KT; k0 += P * S) {
+            v4i now[M][P];
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+#pragma unroll
+                for (int j = 0; j < M; ++j)
+                    now[j][p] = pre[j][p];
+            // the next tiles: of this row block, or of the block's next one
+            if (k0 + P * S < KT)
+                load(t, k0 + P * S);
+            else if (g + (int)gridDim.x < groups)
+                load(tile_at(g + gridDim.x), ks);
+#pragma unroll
+            for (int p = 0; p < P; ++p)
+                if (k0 + p * S < KT) {
+                    const v4i b = row(k0 + p * S);
+#pragma unroll
+                    for (int j = 0; j < M; ++j)
+                        acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(now[j][p], b, acc[j], 0, 0, 0);
+                }
+        }
+        // every column holds the sums of weight rows 4 (l / 16) + i
+        if ((lane & 15) == 0)
+#pragma unroll
+            for (int j = 0; j < M; ++j)
+                *(v4i *)&sums[j][w][4 * (lane >> 4)] = acc[j];
+        lds_barrier();
+        // lane i of every S: the i-th wave's sum of one weight row
+        if (tid < 256) {
+            const int i = tid & (S - 1), ch = (tid >> sl) & 15, tl = tid >> (sl + 4);
+            int sum[M];
+#pragma unroll
+            for (int j = 0; j < M; ++j) {
+                sum[j] = sums[j][(tl << sl) + i][ch];
+                if (sl > 0)
+                    sum[j] += q48_dpp32<Q48_DPP_XOR1>(sum[j]);
+                if (sl > 1)
+                    sum[j] += q48_dpp32<Q48_DPP_XOR2>(sum[j]);
+                if (sl > 2)
+                    sum[j] += q48_dpp32<Q48_DPP_HALF_MIRROR>(sum[j]);
+                if (sl > 3)
+                    sum[j] += q48_dpp32<Q48_DPP_MIRROR>(sum[j]);
+            }
+            const int n = (g * TB + tl) * 16 + ch;
+            if (i == 0 && n < m.N) {
+                int64_t y = w8_scaled(sum[0], sb, s1);
+                if constexpr (EPI == 1)
+                    y = q48_mul(q48_silu(y), w8_scaled(sum[1], sb, s2));
+                if constexpr (EPI == 2)
+                    atomicAdd((unsigned long long *)m.Y + (size_t)tok * m.N + n,
+                              (unsigned long long)q48_mul(wt, y));
+                else
+                    m.Y[(size_t)slot * m.N + n] = (int64_t)((uint64_t)y + (uint64_t)add);
+            }
+        }
+        if (g + (int)gridDim.x < groups)
+            lds_barrier();
+    }
+}
+
 int launch_rc(int e) { return e == (int)hipSuccess ? Q48_OK : Q48_EHIP; }
 
 // Y and what a product reads, and the product itself: gate and up, or one matrix.
@@ -238,20 +414,6 @@ int w8_product(q48_ctx *c, int64_t *Y, const int64_t *base, const q48_w8 *w, con
                   q48_share(Y, out, m->step, (size_t)N * 8)))
             return Q48_EINVAL;
     q48_on_device on(c);
-    const size_t codes = w8_tiles(T, K);
-    int rc = q48_w8_reserve(c, codes + (size_t)T * 8);
-    if (rc)
-        return rc;
-    uint8_t *ws = (uint8_t *)c->w8;
-    W8Rows r = {};
-    r.codes = ws;
-    r.step = (int64_t *)(ws + codes);
-    r.X = X;
-    r.norm_w = norm_w;
-    r.T = T;
-    r.K = K;
-    if ((rc = q48_launch_w8_rows(c, r)))
-        return launch_rc(rc);
     W8Mul m = {};
     m.A = (const uint8_t *)w->codes;
     m.sw = w->step;
@@ -261,11 +423,27 @@ int w8_product(q48_ctx *c, int64_t *Y, const int64_t *base, const q48_w8 *w, con
     }
     m.N = N;
     m.KT = w8_kt(K);
-    m.B = r.codes;
-    m.sb = r.step;
     m.T = T;
     m.Y = Y;
     m.base = base;
+    if (T == 1 && q48_w8_one_ok(K))
+        return launch_rc(q48_launch_w8_one(c, m, w2 ? 1 : 0, X, norm_w, K, 0));
+    const size_t codes = w8_tiles(T, K);
+    int rc = q48_w8_reserve(c, W8_TICKETS + codes + (size_t)T * 8);
+    if (rc)
+        return rc;
+    uint8_t *ws = (uint8_t *)c->w8 + W8_TICKETS;
+    W8Rows r = {};
+    r.codes = ws;
+    r.step = (int64_t *)(ws + codes);
+    r.X = X;
+    r.norm_w = norm_w;
+    r.T = T;
+    r.K = K;
+    if ((rc = q48_launch_w8_rows(c, r)))
+        return launch_rc(rc);
+    m.B = r.codes;
+    m.sb = r.step;
     return launch_rc(q48_launch_w8_mul(c, m, w2 ? 1 : 0, false, 0));
 }
 
@@ -300,12 +478,70 @@ int q48_w8_reserve(q48_ctx *c, size_t bytes)
         return Q48_ENOMEM;
     }
     c->w8_bytes = sz;
-    return Q48_OK;
+    // tickets at its start are zeros between launches
+    return launch_rc(q48_launch_zero(c, c->w8, W8_TICKETS));
 }
 
 int q48_launch_w8_rows(q48_ctx *c, const W8Rows &r)
 {
-    hipLaunchKernelGGL(k_w8_rows, dim3(r.T), dim3(256), 0, c->stream, r);
+#define W8_ROWS(NT, C, J)                                                                      \
+    do {                                                                                       \
+        if (r.norm_w)                                                                          \
+            hipLaunchKernelGGL((k_w8_rows_r<NT, C, J, true>), dim3(r.T), dim3(NT), 0, c->stream, r);  \
+        else                                                                                   \
+            hipLaunchKernelGGL((k_w8_rows_r<NT, C, J, false>), dim3(r.T), dim3(NT), 0, c->stream, r); \
+    } while (0)
+    if (r.K > 8192)
+        hipLaunchKernelGGL(k_w8_rows, dim3(r.T), dim3(256), 0, c->stream, r);
+    else if (r.T <= c->cu_count && r.K > 2048)
+        W8_ROWS(512, 2, 8);
+    else if (r.K <= 1024)
+        W8_ROWS(256, 4, 1);
+    else if (r.K <= 2048)
+        W8_ROWS(256, 4, 2);
+    else if (r.K <= 6144)
+        W8_ROWS(256, 4, 6);
+    else
+        W8_ROWS(256, 4, 8);
+#undef W8_ROWS
+    return (int)hipGetLastError();
+}
+
+int q48_launch_w8_one(q48_ctx *c, const W8Mul &m, int epi, const int64_t *X,
+                      const int64_t *norm_w, int K, int n_items)
+{
+    const int nt = (m.N + 15) / 16, per = n_items ? n_items : 1;
+    // the most waves a tile with which every block is resident at once
+    int sl = 4;
+    auto groups_of = [&](int l) { return (nt + (16 >> l) - 1) / (16 >> l); };
+    while (sl > 0 && groups_of(sl) * per > c->cu_count)
+        --sl;
+    const int groups = groups_of(sl), most = c->cu_count;
+    const dim3 grid(groups < most ? groups : most, per);
+#define W8_ONE(EPI, EX, SRC, NT, J)                                                                  \
+    hipLaunchKernelGGL((k_w8_one<EPI, EX, SRC, NT, J>), grid, dim3(ONE_NT), 0, c->stream, m, X, norm_w, \
+                       K, sl)
+#define W8_ONE_J(EPI, EX, SRC)                                                                   \
+    do {                                                                                         \
+        if (K <= 2048)                                                                     \
+            W8_ONE(EPI, EX, SRC, 256, 4);                                                             \
+        else                                                                                     \
+            W8_ONE(EPI, EX, SRC, 512, 8);                                                             \
+    } while (0)
+    if (n_items && epi == 1)
+        W8_ONE(1, true, 0, 64, 1);
+    else if (n_items)
+        W8_ONE_J(2, true, 1);
+    else if (epi == 1 && norm_w)
+        W8_ONE_J(1, false, 2);
+    else if (epi == 1)
+        W8_ONE_J(1, false, 1);
+    else if (norm_w)
+        W8_ONE_J(0, false, 2);
+    else
+        W8_ONE_J(0, false, 1);
+#undef W8_ONE_J
+#undef W8_ONE
     return (int)hipGetLastError();
 }
 
