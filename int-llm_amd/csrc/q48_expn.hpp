@@ -24,20 +24,29 @@ constexpr int64_t kFactK[7] = {
     281474976710656LL, 281474976710656LL, 140737488355328LL, 46912496118443LL, 11728124029611LL,
     2345624805922LL, 390937467654LL};
 
-// floor(floor(T_j h 2^-48) 2^-n) of one u, by integers: for the few exponentials of a
-// row of expert logits (q48_logprob.hip's lp_terms has the FP64 form for many).
+// floor(floor(T_j h 2^-48) 2^-n) of one u, for the few exponentials of a row of expert
+// logits (q48_logprob.hip's lp_terms has the form for many).  FP64 rounds down
+// (q48_round_down): a truncated product of integers below 2^49 is one fused operation,
+// fma(a, b 2^-48, 2^52) = 2^52 + floor(a b / 2^48).
 __device__ __forceinline__ int64_t q48_expn(uint64_t u)
 {
-    if (u >= 49 * (uint64_t)EXPN_LN2)
-        return 0;
-    const uint32_t n = (uint32_t)(u / (uint64_t)EXPN_LN2);
-    const uint64_t r = u - n * (uint64_t)EXPN_LN2;
-    const int64_t s = (int64_t)(r & (((uint64_t)1 << 42) - 1));
-    int64_t h = kFactK[6];
+    constexpr uint64_t L = (uint64_t)EXPN_LN2;
+    const bool in = u < 49 * L;
+    const uint64_t v = in ? u : 0;
+    // the quotient or one less: both factors are rounded down
+    uint32_t n = (uint32_t)((double)(v >> 8) * (0x1.7154765200000p-48 * 256));
+    uint64_t r = v - n * L;
+    if (r >= L) {
+        r -= L;
+        ++n;
+    }
+    const double s = (double)(int64_t)(r & (((uint64_t)1 << 42) - 1)) * 0x1p-48;
+    double h = (double)kFactK[6];
 #pragma unroll
     for (int k = 5; k >= 0; --k)
-        h = kFactK[k] - q48_mul(s, h);
-    return q48_mul(kExp[r >> 42], h) >> n;
+        h = ((double)kFactK[k] + 0x1p52) - __builtin_fma(s, h, 0x1p52);
+    const double e = __builtin_fma((double)kExp[r >> 42] * 0x1p-48, h, 0x1p52);
+    return in ? (int64_t)(q48_word_m52(e) >> n) : 0;
 }
 
 } // namespace

@@ -175,18 +175,18 @@ struct MoeRoute {
     W8Rows rows;
     const int64_t *router;
     int64_t *logits;
-    int E, per, sl, top, renorm;
+    int E, per, sl, p2, top, renorm;   // p2: 2^p2 >= E, at least 64
     int *chosen;
     int64_t *weight;
     int *ticket;                 // [0]: tokens, [1 + t]: blocks of token t; zeros between launches
     MoeSlots s;
 };
-template <int NT, int J, bool NORM, int PER>
-__global__ __launch_bounds__(1024) void k_moe_route(MoeRoute a)
+template <int NT, int J, bool NORM>
+__global__ __launch_bounds__(1024, J == 8 ? 4 : 8) void k_moe_route(MoeRoute a)
 {
     q48_round_down();
     constexpr int NW = 16;
-    extern __shared__ __align__(16) int64_t xs[];   // the row, normed
+    extern __shared__ __align__(16) int64_t xs[];   // the row, normed; then logits and ranks
     __shared__ uint64_t red[NT / 64][2], peak[NT / 64], part[NW][2];
     __shared__ int last;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -213,8 +213,8 @@ __global__ __launch_bounds__(1024) void k_moe_route(MoeRoute a)
 #pragma unroll
         for (int j = 0; j < J; ++j)
             if (x.at(j) < K) {
-                xs[x.at(j)] = x.v[j][0];
-                xs[x.at(j) + 1] = x.v[j][1];
+                xs[x.at(j)] = x.word(j, 0);
+                xs[x.at(j) + 1] = x.word(j, 1);
             }
     } else {
         if constexpr (NORM)
@@ -228,12 +228,17 @@ __global__ __launch_bounds__(1024) void k_moe_route(MoeRoute a)
         }
     }
     lds_barrier();
-    // S = 2^sl waves an expert, each its share of the row
+    // S = 2^sl waves an expert, each its share of the row.  Words below 2^54 as halves of 27
+    // bits: four multiply-adds into three sums without a carry (the four products of a
+    // signed 64 x 64 multiplication with its carries and signs take twice as long); a share
+    // with larger words again in 128 bits.
     const int sl = a.sl, S = 1 << sl, e = w >> sl, seg = ((K + S - 1) >> sl);
     q48_u128 sum = 0;
     if (e < n) {
         const int from = (w & (S - 1)) * seg, to = min(from + seg, K);
         const int64_t *r = a.router + (size_t)(e0 + e) * K;
+        int64_t hh = 0, hl = 0, ll = 0;
+        uint32_t big = 0;
         for (int i = from + lane; i < to; i += 64 * 8) {
             int64_t v[8];
 #pragma unroll
@@ -241,8 +246,23 @@ __global__ __launch_bounds__(1024) void k_moe_route(MoeRoute a)
                 v[u] = i + 64 * u < to ? r[i + 64 * u] : 0;
 #pragma unroll
             for (int u = 0; u < 8; ++u)
-                if (i - lane + 64 * u < to)
-                    sum += (q48_u128)q48_smul128(xs[min(i + 64 * u, K - 1)], v[u]);
+                if (i - lane + 64 * u < to) {
+                    const int64_t x = xs[min(i + 64 * u, K - 1)];
+                    const int xh = (int)(x >> 27), xl = (int)((uint32_t)x & 0x7ffffffu);
+                    const int vh = (int)(v[u] >> 27), vl = (int)((uint32_t)v[u] & 0x7ffffffu);
+                    const int xt = (int)(x >> 32), vt = (int)(v[u] >> 32);
+                    big |= (uint32_t)(xt ^ (xt >> 31)) | (uint32_t)(vt ^ (vt >> 31));
+                    hh += (int64_t)xh * vh;
+                    hl += (int64_t)xh * vl;
+                    hl += (int64_t)xl * vh;
+                    ll += (int64_t)xl * vl;
+                }
+        }
+        sum = ((q48_u128)(q48_i128)hh << 54) + ((q48_u128)(q48_i128)hl << 27) + (uint64_t)ll;
+        if (__any(big >= 1u << 22)) {
+            sum = 0;
+            for (int i = from + lane; i < to; i += 64)
+                sum += (q48_u128)q48_smul128(xs[i], r[i]);
         }
         sum = q48_wave_sum128(sum);
     }
@@ -268,33 +288,61 @@ __global__ __launch_bounds__(1024) void k_moe_route(MoeRoute a)
     __syncthreads();
     if (!last)
         return;
-    if (tid < 64) {
-        int64_t v[PER], wt;
-        int id;
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-            v[i] = lane + 64 * i < E ? from_all(a.logits + (size_t)t * E + lane + 64 * i) : 0;
-        moe_choose<PER>(v, E, a.top, a.renorm != 0, id, wt);
-        if (lane < a.top) {
-            out_to_all(a.chosen + (size_t)t * a.top + lane, id);
-            out_to_all(a.weight + (size_t)t * a.top + lane, wt);
-            if (T == 1) {   // every choice an item of one slot
-                a.s.items[lane] = make_int4(id, 16 * lane, 1, 0);
-                a.s.tok[16 * lane] = 0;
-                a.s.w[16 * lane] = wt;
-            }
+    // The token's choice by all threads: an expert's rank is the number of larger logits
+    // and of equal ones before it, counted by 1024 / P threads an expert (P: experts to a
+    // power of two), and each chosen expert makes its own weight.
+    {
+        __shared__ int64_t most;
+        __shared__ uint64_t z;
+        int64_t *lg = xs;   // (the row is done with)
+        int *rank = (int *)(xs + E);
+        const int P = 1 << a.p2, ex = tid & (P - 1), parts = 1024 >> a.p2, part_ = tid >> a.p2;
+        if (tid < E) {
+            lg[tid] = from_all(a.logits + (size_t)t * E + tid);
+            rank[tid] = 0;
         }
-        __builtin_amdgcn_s_waitcnt(0);
-        if (lane == 0 && T > 1) {
-            const int at = __hip_atomic_fetch_add(a.ticket, 1, __ATOMIC_RELAXED,
-                                                  __HIP_MEMORY_SCOPE_AGENT);
-            last = at == T - 1;
-            if (at == T - 1)
-                out_to_all(a.ticket, 0);
+        if (tid == 0)
+            z = 0;
+        lds_barrier();
+        const int64_t mine = lg[min(ex, E - 1)];
+        int before = 0;
+        for (int i = part_; i < E; i += parts)
+            before += lg[i] > mine || (lg[i] == mine && i < ex) ? 1 : 0;
+        if (ex < E && before)
+            atomicAdd(&rank[ex], before);
+        lds_barrier();
+        const int my = tid < E ? rank[tid] : E;
+        if (my == 0)
+            most = mine;
+        lds_barrier();
+        int64_t ew = 0;
+        if (my < (a.renorm ? a.top : E)) {
+            ew = q48_expn((uint64_t)most - (uint64_t)mine);
+            atomicAdd((unsigned long long *)&z, (unsigned long long)ew);
+        }
+        lds_barrier();
+        if (my < a.top) {
+            const int64_t wt = q48_div(ew, (int64_t)z);
+            out_to_all(a.chosen + (size_t)t * a.top + my, tid);
+            out_to_all(a.weight + (size_t)t * a.top + my, wt);
+            if (T == 1) {   // every choice an item of one slot
+                a.s.items[my] = make_int4(tid, 16 * my, 1, 0);
+                a.s.tok[16 * my] = 0;
+                a.s.w[16 * my] = wt;
+            }
         }
     }
     if (T == 1)
         return;
+    __builtin_amdgcn_s_waitcnt(0);   // every wave's stores are out before the ticket
+    __syncthreads();
+    if (tid == 0) {
+        const int at = __hip_atomic_fetch_add(a.ticket, 1, __ATOMIC_RELAXED,
+                                              __HIP_MEMORY_SCOPE_AGENT);
+        last = at == T - 1;
+        if (at == T - 1)
+            out_to_all(a.ticket, 0);
+    }
     __syncthreads();
     if (last)
         moe_slots<1024>(a.s, a.chosen, a.weight, T * a.top, a.top, E);
@@ -311,34 +359,26 @@ size_t slots_of(size_t pairs, int E)
 // experts a block of k_moe_route, 0 for the separate launches (a row of words in LDS)
 int route_per(const q48_ctx *c, int T, int E, int dim)
 {
-    const int per = ((long)E * T + c->cu_count - 1) / c->cu_count;
+    // the fewest with which every block, the codes' among them, is resident at once
+    const int G = T <= c->cu_count ? (dim <= 2048 ? 2 : 1) * c->cu_count / T - 1 : 0;
+    const int per = G > 0 ? (E + G - 1) / G : ROUTE_PER + 1;
     return dim <= 6144 && T <= ROUTE_T && per <= ROUTE_PER ? per : 0;
 }
 
 int launch_route(q48_ctx *c, const MoeRoute &a)
 {
     const dim3 grid((a.E + a.per - 1) / a.per + 1, a.rows.T);
-    const size_t lds = 8 * (size_t)((a.rows.K + 1) & ~1);
-#define ROUTE(NT, J, NORM, PER)                                                                \
-    hipLaunchKernelGGL((k_moe_route<NT, J, NORM, PER>), grid, dim3(1024), lds, c->stream, a)
-#define ROUTE_P(NT, J, NORM)                                                                   \
-    do {                                                                                       \
-        if (a.E <= 64)                                                                         \
-            ROUTE(NT, J, NORM, 1);                                                                 \
-        else if (a.E <= 128)                                                                   \
-            ROUTE(NT, J, NORM, 2);                                                                 \
-        else                                                                                   \
-            ROUTE(NT, J, NORM, 16);                                                                \
-    } while (0)
+    const size_t lds = max(8 * ((a.rows.K + 1) & ~1), 12 * a.E);
+#define ROUTE(NT, J, NORM)                                                                   \
+    hipLaunchKernelGGL((k_moe_route<NT, J, NORM>), grid, dim3(1024), lds, c->stream, a)
     if (a.rows.K <= 2048 && a.rows.norm_w)
-        ROUTE_P(256, 4, true);
+        ROUTE(256, 4, true);
     else if (a.rows.K <= 2048)
-        ROUTE_P(256, 4, false);
+        ROUTE(256, 4, false);
     else if (a.rows.norm_w)
-        ROUTE_P(512, 8, true);
+        ROUTE(512, 8, true);
     else
-        ROUTE_P(512, 8, false);
-#undef ROUTE_P
+        ROUTE(512, 8, false);
 #undef ROUTE
     return (int)hipGetLastError();
 }
@@ -429,7 +469,10 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
             int spl = 4;
             while ((per << spl) > 16)
                 --spl;
-            const MoeRoute a = {r, moe->router, lg, E, per, spl, top, moe->renorm, ch, wt,
+            int p2 = 6;
+            while ((1 << p2) < E)
+                ++p2;
+            const MoeRoute a = {r, moe->router, lg, E, per, spl, p2, top, moe->renorm, ch, wt,
                                 (int *)ws, s};
             rc = launch_route(c, a);
         } else {

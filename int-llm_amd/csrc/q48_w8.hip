@@ -81,7 +81,7 @@ __global__ __launch_bounds__(NT) void k_w8_rows_r(W8Rows a)
 #pragma unroll
             for (int c = 0; c < C; ++c)
                 if (x.at(j) + c < K)
-                    a.xn[(size_t)t * K + x.at(j) + c] = x.v[j][c];
+                    a.xn[(size_t)t * K + x.at(j) + c] = x.word(j, c);
     if (a.out)
         for (int i = threadIdx.x; i < K; i += NT)
             a.out[(size_t)t * K + i] = a.base ? a.base[(size_t)t * K + i] : 0;
