@@ -393,6 +393,247 @@ __global__ __launch_bounds__(ONE_NT) void k_w8_one(W8Mul m, const int64_t *__res
     }
 }
 
+// ---- many rows ------------------------------------------------------------------
+
+typedef int v16i __attribute__((ext_vector_type(16)));
+
+// s_waitcnt vmcnt(n) with the other counters left alone (gfx9 encoding)
+template <int N>
+__device__ __forceinline__ void wait_vm()
+{
+    static_assert(N >= 0 && N < 64, "vmcnt");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
+}
+
+constexpr int GT = 128;                  // weight rows (EPI 1: half of each matrix) and rows a block
+constexpr int GSTAGE = 2 * GT * 64;      // bytes of a stage: 64 columns of both
+
+// A block 128 weight rows x 128 rows, four waves of 64 x 64.  Tiles of both operands go to a
+// ring of four LDS stages by DMA, 1 KB a wave and instruction, three stages ahead; the
+// matrix instruction's first operand is the rows, so that a lane holds one weight row and
+// stores of a wave are 256 contiguous bytes.  The sums leave the registers through LDS, so
+// that one loop of the epilogue's code serves all of them.
+template <int EPI, bool EXPERTS>
+__global__ __launch_bounds__(256, 2) void k_w8_gemm(W8Mul m, int nx, int ny)
+{
+    q48_round_down();
+    constexpr int CH = EPI == 1 ? GT / 2 : GT;   // weight rows of one matrix
+    // four arrays, so that the compiler sees that a stage's reads do not wait for another's DMA
+    __shared__ __align__(16) uint8_t r0[GSTAGE], r1[GSTAGE], r2[GSTAGE], r3[GSTAGE];
+    __shared__ double sd[GT];
+    __shared__ int toks[EXPERTS ? GT : 1];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wc = w & 1, wr = w >> 1;
+    // blocks of one die (every eighth) take neighbouring tiles, the rows' fastest
+    const int per = (nx * ny + 7) >> 3, at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || at >= nx * ny)
+        return;
+    const int bx = at / ny, by = at % ny;
+    int expert = 0, row0 = by * GT, rows = m.T - row0;
+    if constexpr (EXPERTS) {
+        const int4 it = m.items[by];
+        expert = it.x;
+        row0 = it.y;
+        rows = it.z;
+        if (rows <= 0)
+            return;
+    }
+    rows = min(rows, GT);
+    const int KT = m.KT, n0 = bx * CH, ntile = (m.N + 15) / 16;
+    if (tid < GT) {
+        const int r = min(tid, rows - 1);
+        int64_t step;
+        if constexpr (EXPERTS) {
+            const int tok = m.slot_tok[row0 + r];
+            toks[tid] = tok;
+            step = m.sb[EPI == 1 ? max(tok, 0) : row0 + r];
+        } else {
+            step = m.sb[row0 + r];
+        }
+        sd[tid] = w8_step_double(step);
+    }
+    auto row_of = [&](int t) {   // of the wave's rows, in sb
+        if constexpr (EXPERTS && EPI == 1)
+            return max(toks[64 * wr + t], 0);
+        else
+            return row0 + 64 * wr + t;
+    };
+    // this wave's tiles of a stage: two of the weights, two of the rows
+    const uint8_t *src[4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const int a = 2 * w + j;   // EPI 1: tiles 0 .. 3 of gate, 4 .. 7 of up
+        const bool second = EPI == 1 && a >= 4;
+        const int t = min((n0 >> 4) + (second ? a - 4 : a), ntile - 1);
+        src[j] = (second ? m.A2 : m.A) + (size_t)expert * m.a_stride + (size_t)t * KT * 1024 + lane * 16;
+        const int r = min(16 * (2 * w + j), (rows - 1) & ~15) + row0;
+        if constexpr (EXPERTS && EPI == 1) {
+            const int tok = max(m.slot_tok[r + (lane & 15)], 0);
+            src[2 + j] = m.B + (size_t)(tok >> 4) * KT * 1024 + (lane >> 4) * 256 + (tok & 15) * 16;
+        } else {
+            src[2 + j] = m.B + (size_t)(r >> 4) * KT * 1024 + lane * 16;
+        }
+    }
+    auto dma = [&](int k, uint8_t(&st)[GSTAGE]) {
+        uint8_t *to = st + 2 * w * 1024;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            __builtin_amdgcn_global_load_lds(src[j] + (size_t)k * 1024,
+                                             to + (j >> 1) * (GT * 64) + (j & 1) * 1024, 16, 0, 0);
+    };
+    v16i acc[2][2] = {};
+    // rows l % 32 of a pair of tiles, columns 16 (l / 32) on
+    const int mine = ((lane & 31) >> 4) * 1024 + (lane >> 5) * 256 + (lane & 15) * 16;
+    auto step = [&](const uint8_t(&stage)[GSTAGE]) {
+        const uint8_t *st = stage + mine;
+        v4i a[2][2], b[2][2];   // [pair][half of the columns]
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int f = 0; f < 2; ++f) {
+                const int ta = EPI == 1 ? 4 * f + 2 * wc : 4 * wc + 2 * f;
+                a[f][h] = *(const v4i *)(st + ta * 1024 + h * 512);
+                b[f][h] = *(const v4i *)(st + GT * 64 + (4 * wr + 2 * f) * 1024 + h * 512);
+            }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int f = 0; f < 2; ++f)
+                    acc[f][g] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[g][h], a[f][h], acc[f][g], 0, 0, 0);
+    };
+    dma(0, r0);
+    if (KT > 1)
+        dma(1, r1);
+    if (KT > 2)
+        dma(2, r2);
+    int k = 0;
+    // of the stages under way the oldest has arrived; the next DMA goes where the last
+    // step's was
+    auto turn = [&](const uint8_t(&now)[GSTAGE], uint8_t(&next)[GSTAGE]) {
+        wait_vm<8>();
+        lds_barrier();
+        dma(k + 3, next);
+        step(now);
+        ++k;
+    };
+    while (k + 7 <= KT) {
+        turn(r0, r3);
+        turn(r1, r0);
+        turn(r2, r1);
+        turn(r3, r2);
+    }
+    // three to six stages left, three of them under way
+    auto tail = [&](const uint8_t(&now)[GSTAGE], uint8_t(&next)[GSTAGE]) {
+        if (k >= KT)
+            return;
+        wait_vm<0>();
+        lds_barrier();
+        if (k + 3 < KT)
+            dma(k + 3, next);
+        step(now);
+        ++k;
+    };
+    tail(r0, r3);
+    tail(r1, r0);
+    tail(r2, r1);
+    tail(r3, r2);
+    tail(r0, r3);
+    tail(r1, r0);
+    lds_barrier();
+    // [pair of weight rows][pair of rows][row][weight row] of the wave
+    int *sums = (int *)(w == 0 ? r0 : w == 1 ? r1 : w == 2 ? r2 : r3);
+#pragma unroll
+    for (int f = 0; f < 2; ++f)
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                sums[((f * 2 + g) * 32 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3)) * 32 + (lane & 31)] =
+                    acc[f][g][i];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own words
+    const int64_t *sw = m.sw + (size_t)expert * m.N, *sw2 = m.sw2 + (size_t)expert * m.N;
+    const int n = n0 + (EPI == 1 ? 32 * wc + (lane & 31) : 64 * wc + lane);
+    const bool in = n < m.N;
+    const int64_t s1 = in ? sw[n] : 0, s2 = in && EPI == 1 ? sw2[n] : 0;
+    const double d1 = w8_step_double(s1) * 0x1p-48, d2 = w8_step_double(s2) * 0x1p-48;
+    const int last = min(64, rows - 64 * wr);
+    // U outputs a turn: chains of FP64 operations side by side
+    constexpr int U = 4, PER = EPI == 1 ? 2 : 1;   // rows of a wave at once
+    const int first = EPI == 1 ? lane >> 5 : 0;
+    // the base a turn ahead of the sums
+    int64_t add[U] = {};
+    auto base = [&](int t0) {
+        if constexpr (EPI == 0)
+            if (m.base && in)
+#pragma unroll
+                for (int j = 0; j < U; ++j)
+                    add[j] = m.base[(size_t)row_of(min(t0 + j, last - 1)) * m.N + n];
+    };
+    base(0);
+    for (int t0 = 0; t0 < last; t0 += U * PER) {
+        double y[U];
+        bool ok = true;
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int t = t0 + PER * j + first;   // (rows past the last: sums of other rows)
+            const double sa = sd[64 * wr + t];
+            bool sure;
+            if constexpr (EPI == 1) {
+                const int o = t * 32 + (lane & 31);
+                const double g = w8_scaled_double(sums[o], sa, d1, sure);
+                ok = ok && sure;
+                const double u = w8_scaled_double(sums[2048 + o], sa, d2, sure);
+                ok = ok && sure;
+                y[j] = w8_silu_mul(g, u, sure);
+                ok = ok && __builtin_fabs(y[j]) < 0x1p53;
+            } else {
+                y[j] = w8_scaled_double(sums[(lane >> 5) * 2048 + t * 32 + (lane & 31)], sa, d1, sure);
+            }
+            ok = ok && sure;
+        }
+        int64_t v[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+            v[j] = (int64_t)y[j];
+        if (__any(!ok))
+            for (int j = 0; j < U; ++j) {
+                const int t = t0 + PER * j + first;
+                const int64_t sa = m.sb[row_of(min(t, last - 1))];
+                int64_t z;
+                if constexpr (EPI == 1) {
+                    const int o = t * 32 + (lane & 31);
+                    z = q48_mul(q48_silu(w8_scaled(sums[o], sa, s1)), w8_scaled(sums[2048 + o], sa, s2));
+                } else {
+                    z = w8_scaled(sums[(lane >> 5) * 2048 + t * 32 + (lane & 31)], sa, s1);
+                }
+#pragma unroll
+                for (int i = 0; i < U; ++i)
+                    v[i] = i == j ? z : v[i];
+            }
+        if constexpr (EPI == 0) {
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+                v[j] = (int64_t)((uint64_t)v[j] + (uint64_t)add[j]);
+            if (t0 + U < last)
+                base(t0 + U);
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int t = t0 + PER * j + first;
+            const size_t row = (size_t)(row0 + 64 * wr + t);
+            if (!in || t >= last || (EXPERTS && toks[64 * wr + t] < 0))
+                continue;
+            if constexpr (EPI == 2)
+                atomicAdd((unsigned long long *)m.Y + (size_t)toks[64 * wr + t] * m.N + n,
+                          (unsigned long long)q48_mul(m.slot_w[row], v[j]));
+            else
+                m.Y[row * m.N + n] = v[j];
+        }
+    }
+}
+
 int launch_rc(int e) { return e == (int)hipSuccess ? Q48_OK : Q48_EHIP; }
 
 // Y and what a product reads, and the product itself: gate and up, or one matrix.
@@ -548,6 +789,16 @@ int q48_launch_w8_one(q48_ctx *c, const W8Mul &m, int epi, const int64_t *X,
 int q48_launch_w8_mul(q48_ctx *c, const W8Mul &m, int epi, bool experts, int n_items)
 {
     const unsigned nx = (m.N + 15) / 16;
+    if (!experts && m.T > 64) {
+        const int gx = (m.N + (epi == 1 ? GT / 2 : GT) - 1) / (epi == 1 ? GT / 2 : GT);
+        const int gy = (m.T + GT - 1) / GT;
+        const dim3 grid((unsigned)((gx * gy + 7) / 8 * 8));
+        if (epi == 1)
+            hipLaunchKernelGGL((k_w8_gemm<1, false>), grid, dim3(256), 0, c->stream, m, gx, gy);
+        else
+            hipLaunchKernelGGL((k_w8_gemm<0, false>), grid, dim3(256), 0, c->stream, m, gx, gy);
+        return (int)hipGetLastError();
+    }
 #define W8_MUL(NB, EPI, EX)                                                            \
     hipLaunchKernelGGL((k_w8_mul<NB, EPI, EX>), dim3(nx, EX ? n_items : (m.T + 16 * NB - 1) / (16 * NB)), \
                        dim3(256), 0, c->stream, m)

@@ -24,6 +24,84 @@ __device__ __forceinline__ int64_t w8_scaled(int S, int64_t sa, int64_t sw)
     return (int64_t)(uint64_t)((q48_i128)(S < 0 ? 0 - v : v) >> 48);
 }
 
+// The same in FP64 rounding down (q48_round_down), as a double: sa and sw = step 2^-48 (inf
+// for steps of 2^53 and more, w8_step_double).  P = sa sw and S P as rounded products and
+// their exact remainders: the floor of the first, and of what the others add to its
+// fraction.  Rounding down makes that sum too small by less than 2^-50, so only a fraction
+// next to 1 may hide a whole number: `sure` is false there and where the value passes 2^52
+// (about one product in 2^40; w8_scaled then).
+__device__ __forceinline__ double w8_scaled_double(int S, double sa, double sw, bool &sure)
+{
+#pragma clang fp contract(off)   // h as rounded
+    const double p = sa * sw, pl = __builtin_fma(sa, sw, -p), s = (double)S;
+    const double h = s * p, hl = __builtin_fma(s, p, -h), f = __builtin_floor(h);
+    const double t = (h - f) + __builtin_fma(s, pl, hl), g = __builtin_floor(t);
+    sure = __builtin_fabs(h) < 0x1p52 && t - g < 1.0 - 0x1p-40;
+    return f + g;
+}
+__device__ __forceinline__ double w8_step_double(int64_t step)
+{
+    return (uint64_t)step < (uint64_t)1 << 53 ? (double)step : __builtin_inf();
+}
+
+// floor(2^96 / r), 2^48 <= r < 2^53, FP64 rounding down: the estimate from above the quotient
+// or one less (q48_recip), its remainder exact
+__device__ __forceinline__ double w8_recip(double r)
+{
+    double y = __builtin_amdgcn_rcp(r);
+    y = __builtin_fma(y, __builtin_fma(-r, y, 1.0), y);
+    y = __builtin_fma(y, __builtin_fma(-r, y, 1.0), y);
+    const double q = __builtin_fma(y, 0x1p96, 0x1p52 - 0.5) - 0x1p52;
+    return __builtin_fma(-q, r, 0x1p96) >= r ? q + 1.0 : q;
+}
+
+// fp_mul(fp_silu(g), u) (fp_math.h:911-921) of whole numbers below 2^53, in FP64 rounding
+// down alone.  The squares of fp_exp: the first 12 stay below 2^52 (two operations each,
+// q48_exp_small), the last two, of at most e^10 2^48, are a rounded product and its exact
+// remainder each, r = A + T with A a double and T < 2^13.  Rounding down makes the sums
+// behind T too small by less than 2^-39: `sure` is false where that may hide a whole number
+// (q48_silu then).  A quotient by A + T: an estimate as in q48_recip, its remainder 2^96 -
+// q A exact (a multiple of A's last place, below 2^53 of them) and compared with A +
+// (q + 1) T, whose product is below 2^53.  About 85 operations; with 64-bit integers for
+// the last squares and the quotients 160, a third of them of quarter rate.
+__device__ __forceinline__ double w8_silu_mul(double g, double u, bool &sure)
+{
+#pragma clang fp contract(off)   // products as rounded
+    const double ten = 10 * 0x1p48, m = __builtin_fmin(__builtin_fabs(g), ten);
+    // 1 + floor(m / 2^14)
+    double h = __builtin_fma(m, 0x1p-14, 0x1p52 + 0x1p48);
+#pragma unroll
+    for (int k = 0; k < 12; ++k) {
+        const double y = __builtin_fma(h, 0x1p-24, -0x1p28);
+        h = __builtin_fma(y, y, 0x1p52);
+    }
+    const double y = __builtin_fma(h, 0x1p-24, -0x1p28);
+    const double p = y * y, pi = __builtin_floor(p);
+    const double l = __builtin_floor((p - pi) + __builtin_fma(y, y, -p));   // square 13: pi + l
+    const double H = pi * 0x1p-24, L = l * 0x1p-24;
+    const double A0 = H * H, t0 = __builtin_fma(2 * H, L, __builtin_fma(H, H, -A0));
+    double A = __builtin_floor(A0);
+    const double t = (A0 - A) + __builtin_fma(L, L, t0);
+    double T = __builtin_floor(t);
+    sure = t - T < 1.0 - 0x1p-30;
+    const bool pos = g > 0;
+    // what is divided by: e^g where g > 0, else 1 + e^-g
+    const double c = pos ? 0.0 : 0x1p48, B = A + c;
+    T += c - (B - A);
+    A = B;
+    double r = __builtin_amdgcn_rcp(A);
+    r = __builtin_fma(r, __builtin_fma(-A, r, 1.0), r);
+    r = __builtin_fma(r, __builtin_fma(-A, r, 1.0), r);
+    r = __builtin_fma(-(r * T), r, r);
+    double q = __builtin_fma(r, 0x1p96, 0x1p52 - 0.5) - 0x1p52;
+    const double rem = __builtin_fma(-q, A, 0x1p96);
+    q += rem - A >= (q + 1.0) * T ? 1.0 : 0.0;
+    double s = pos ? w8_recip(q + 0x1p48) : q;
+    s = g > ten ? 0x1p48 : g < -ten ? 0.0 : s;
+    const double v = __builtin_floor(g * (s * 0x1p-48));
+    return __builtin_floor(v * (u * 0x1p-48));
+}
+
 // the step of a row whose largest magnitude is a, and its reciprocal
 __device__ __forceinline__ uint64_t w8_step(uint64_t a, double &r)
 {
