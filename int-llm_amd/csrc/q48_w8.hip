@@ -405,25 +405,40 @@ __device__ __forceinline__ void wait_vm()
     __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | (15 << 8) | ((N >> 4) << 14));
 }
 
+// 16 bytes a lane from `from` to the wave's 1 KB at `to`
+__device__ __forceinline__ void dma_tile(const uint8_t *from, uint8_t *to)
+{
+    __builtin_amdgcn_global_load_lds(from, to, 16, 0, 0);
+}
+
 constexpr int GT = 128;                  // weight rows (EPI 1: half of each matrix) and rows a block
 constexpr int GSTAGE = 2 * GT * 64;      // bytes of a stage: 64 columns of both
 
-// A block 128 weight rows x 128 rows, four waves of 64 x 64.  Tiles of both operands go to a
-// ring of four LDS stages by DMA, 1 KB a wave and instruction, three stages ahead; the
-// matrix instruction's first operand is the rows, so that a lane holds one weight row and
-// stores of a wave are 256 contiguous bytes.  The sums leave the registers through LDS, so
-// that one loop of the epilogue's code serves all of them.
-template <int EPI, bool EXPERTS>
-__global__ __launch_bounds__(256, 2) void k_w8_gemm(W8Mul m, int nx, int ny)
+// A block 128 weight rows x 128 rows, eight waves.  Tiles of both operands go to a ring of
+// four LDS stages by DMA, 1 KB a wave and instruction, three stages ahead; the matrix
+// instruction's first operand is the rows, so that a lane holds one weight row and stores of
+// a wave are 256 contiguous bytes.  The sums leave the registers through LDS, so that one
+// loop of the epilogue's code serves all of them.
+// KS 1: waves of 64 x 32, two blocks and four waves a SIMD: a wave alone there issues every
+// other turn at most, and the epilogue is more work than the products.  KS 2, where there is
+// at most a block a compute unit: two groups of four waves of 64 x 64, each over half of the
+// columns with a ring of its own, that share the epilogue.
+template <int EPI, bool EXPERTS, int KS>
+__global__ __launch_bounds__(512, KS == 1 ? 4 : 2) void k_w8_gemm(W8Mul m, int nx, int ny)
 {
     q48_round_down();
     constexpr int CH = EPI == 1 ? GT / 2 : GT;   // weight rows of one matrix
-    // four arrays, so that the compiler sees that a stage's reads do not wait for another's DMA
-    __shared__ __align__(16) uint8_t r0[GSTAGE], r1[GSTAGE], r2[GSTAGE], r3[GSTAGE];
+    constexpr int WPG = 8 / KS;                  // waves of a group
+    constexpr int RB = 4 / (WPG / 2);            // blocks of 32 rows a wave
+    constexpr int TPW = 16 / WPG;                // tiles of a stage a wave moves
+    // apart, so that the compiler sees that a stage's reads do not wait for another's DMA
+    __shared__ __align__(16) uint8_t r0[KS * GSTAGE], r1[KS * GSTAGE], r2[KS * GSTAGE],
+        r3[KS * GSTAGE];
     __shared__ double sd[GT];
     __shared__ int toks[EXPERTS ? GT : 1];
     const int tid = threadIdx.x, lane = tid & 63;
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wc = w & 1, wr = w >> 1;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int q = wave / WPG, w = wave % WPG, wc = w & 1, r_w = (w >> 1) * 32 * RB;   // its rows
     // blocks of one die (every eighth) take neighbouring tiles, the rows' fastest
     const int per = (nx * ny + 7) >> 3, at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per || at >= nx * ny)
@@ -439,7 +454,9 @@ __global__ __launch_bounds__(256, 2) void k_w8_gemm(W8Mul m, int nx, int ny)
             return;
     }
     rows = min(rows, GT);
-    const int KT = m.KT, n0 = bx * CH, ntile = (m.N + 15) / 16;
+    const int KT = (m.KT + KS - 1) / KS;        // steps of a group; of the last one, its own
+    const int kt0 = q * KT, mine_kt = KS == 1 ? KT : min(KT, m.KT - kt0);
+    const int n0 = bx * CH, ntile = (m.N + 15) / 16;
     if (tid < GT) {
         const int r = min(tid, rows - 1);
         int64_t step;
@@ -452,115 +469,153 @@ __global__ __launch_bounds__(256, 2) void k_w8_gemm(W8Mul m, int nx, int ny)
         }
         sd[tid] = w8_step_double(step);
     }
-    auto row_of = [&](int t) {   // of the wave's rows, in sb
+    // row t of the wave's, in sb and base; rows past the block's last: that one
+    auto row_of = [&](int t) {
+        const int i = min(r_w + t, rows - 1);
         if constexpr (EXPERTS && EPI == 1)
-            return max(toks[64 * wr + t], 0);
+            return max(toks[i], 0);
         else
-            return row0 + 64 * wr + t;
+            return row0 + i;
     };
-    // this wave's tiles of a stage: two of the weights, two of the rows
-    const uint8_t *src[4];
+    // this wave's tiles of a stage, of 8 of the weights and then 8 of the rows
+    const uint8_t *src[TPW];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        const int a = 2 * w + j;   // EPI 1: tiles 0 .. 3 of gate, 4 .. 7 of up
-        const bool second = EPI == 1 && a >= 4;
-        const int t = min((n0 >> 4) + (second ? a - 4 : a), ntile - 1);
-        src[j] = (second ? m.A2 : m.A) + (size_t)expert * m.a_stride + (size_t)t * KT * 1024 + lane * 16;
-        const int r = min(16 * (2 * w + j), (rows - 1) & ~15) + row0;
-        if constexpr (EXPERTS && EPI == 1) {
-            const int tok = max(m.slot_tok[r + (lane & 15)], 0);
-            src[2 + j] = m.B + (size_t)(tok >> 4) * KT * 1024 + (lane >> 4) * 256 + (tok & 15) * 16;
+    for (int j = 0; j < TPW; ++j) {
+        const int a = TPW * w + j;
+        if (a < 8) {   // EPI 1: tiles 0 .. 3 of gate, 4 .. 7 of up
+            const bool second = EPI == 1 && a >= 4;
+            const int t = min((n0 >> 4) + (second ? a - 4 : a), ntile - 1);
+            src[j] = (second ? m.A2 : m.A) + (size_t)expert * m.a_stride +
+                     ((size_t)t * m.KT + kt0) * 1024 + lane * 16;
         } else {
-            src[2 + j] = m.B + (size_t)(r >> 4) * KT * 1024 + lane * 16;
+            const int r = min(16 * (a - 8), (rows - 1) & ~15) + row0;
+            if constexpr (EXPERTS && EPI == 1) {
+                const int tok = max(m.slot_tok[r + (lane & 15)], 0);
+                src[j] = m.B + ((size_t)(tok >> 4) * m.KT + kt0) * 1024 + (lane >> 4) * 256 +
+                         (tok & 15) * 16;
+            } else {
+                src[j] = m.B + ((size_t)(r >> 4) * m.KT + kt0) * 1024 + lane * 16;
+            }
         }
     }
-    auto dma = [&](int k, uint8_t(&st)[GSTAGE]) {
-        uint8_t *to = st + 2 * w * 1024;
+    auto dma = [&](int k, uint8_t(&st)[KS * GSTAGE]) {
+        uint8_t *to = st + q * GSTAGE + TPW * w * 1024;
+        if constexpr (KS > 1)   // (past a shorter group's end: a stage that is not multiplied)
+            k = min(k, mine_kt - 1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            __builtin_amdgcn_global_load_lds(src[j] + (size_t)k * 1024,
-                                             to + (j >> 1) * (GT * 64) + (j & 1) * 1024, 16, 0, 0);
+        for (int j = 0; j < TPW; ++j)
+            dma_tile(src[j] + (size_t)k * 1024, to + j * 1024);
     };
-    v16i acc[2][2] = {};
+    v16i acc[2][RB] = {};
     // rows l % 32 of a pair of tiles, columns 16 (l / 32) on
     const int mine = ((lane & 31) >> 4) * 1024 + (lane >> 5) * 256 + (lane & 15) * 16;
-    auto step = [&](const uint8_t(&stage)[GSTAGE]) {
-        const uint8_t *st = stage + mine;
-        v4i a[2][2], b[2][2];   // [pair][half of the columns]
+    // a stage's operands: [pair][half of the columns], of the weights and of the rows
+    struct Opnd {
+        v4i a[2][2], b[RB][2];
+    };
+    auto read = [&](const uint8_t(&stage)[KS * GSTAGE], Opnd &o) {
+        const uint8_t *st = stage + q * GSTAGE + mine;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int g = 0; g < RB; ++g)
+                o.b[g][h] = *(const v4i *)(st + (8 + r_w / 16 + 2 * g) * 1024 + h * 512);
 #pragma unroll
             for (int f = 0; f < 2; ++f) {
                 const int ta = EPI == 1 ? 4 * f + 2 * wc : 4 * wc + 2 * f;
-                a[f][h] = *(const v4i *)(st + ta * 1024 + h * 512);
-                b[f][h] = *(const v4i *)(st + GT * 64 + (4 * wr + 2 * f) * 1024 + h * 512);
+                o.a[f][h] = *(const v4i *)(st + ta * 1024 + h * 512);
             }
+        }
+    };
+    auto multiply = [&](const Opnd &o) {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int g = 0; g < 2; ++g)
+            for (int g = 0; g < RB; ++g)
 #pragma unroll
                 for (int f = 0; f < 2; ++f)
-                    acc[f][g] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[g][h], a[f][h], acc[f][g], 0, 0, 0);
+                    acc[f][g] =
+                        __builtin_amdgcn_mfma_i32_32x32x32_i8(o.b[g][h], o.a[f][h], acc[f][g], 0, 0, 0);
     };
     dma(0, r0);
     if (KT > 1)
         dma(1, r1);
     if (KT > 2)
         dma(2, r2);
+    Opnd even, odd;
+    wait_vm<0>();
+    lds_barrier();
+    read(r0, even);
     int k = 0;
-    // of the stages under way the oldest has arrived; the next DMA goes where the last
-    // step's was
-    auto turn = [&](const uint8_t(&now)[GSTAGE], uint8_t(&next)[GSTAGE]) {
-        wait_vm<8>();
+    // Step k: stage k + 1 has arrived, and stage k - 1 is in every wave's registers; the DMA
+    // of k + 3 goes there, and k + 1 is read under the products of k.
+    auto turn = [&](const Opnd &now, const uint8_t(&next)[KS * GSTAGE], Opnd &then,
+                    uint8_t(&free)[KS * GSTAGE]) {
+        wait_vm<TPW>();
         lds_barrier();
-        dma(k + 3, next);
-        step(now);
+        dma(k + 3, free);
+        read(next, then);
+        multiply(now);
         ++k;
     };
-    while (k + 7 <= KT) {
-        turn(r0, r3);
-        turn(r1, r0);
-        turn(r2, r1);
-        turn(r3, r2);
-    }
-    // three to six stages left, three of them under way
-    auto tail = [&](const uint8_t(&now)[GSTAGE], uint8_t(&next)[GSTAGE]) {
+    // the last ones
+    auto tail = [&](const Opnd &now, const uint8_t(&next)[KS * GSTAGE], Opnd &then,
+                    uint8_t(&free)[KS * GSTAGE]) {
         if (k >= KT)
             return;
         wait_vm<0>();
         lds_barrier();
         if (k + 3 < KT)
-            dma(k + 3, next);
-        step(now);
+            dma(k + 3, free);
+        if (k + 1 < KT)
+            read(next, then);
+        if (KS == 1 || k < mine_kt)
+            multiply(now);
         ++k;
     };
-    tail(r0, r3);
-    tail(r1, r0);
-    tail(r2, r1);
-    tail(r3, r2);
-    tail(r0, r3);
-    tail(r1, r0);
+    while (k + 6 < KT) {
+        turn(even, r1, odd, r3);
+        turn(odd, r2, even, r0);
+        turn(even, r3, odd, r1);
+        turn(odd, r0, even, r2);
+    }
+    tail(even, r1, odd, r3);
+    tail(odd, r2, even, r0);
+    tail(even, r3, odd, r1);
+    tail(odd, r0, even, r2);
+    tail(even, r1, odd, r3);
+    tail(odd, r2, even, r0);
     lds_barrier();
-    // [pair of weight rows][pair of rows][row][weight row] of the wave
-    int *sums = (int *)(w == 0 ? r0 : w == 1 ? r1 : w == 2 ? r2 : r3);
+    // of wave i: [pair of weight rows][row][weight row]
+    constexpr int ROWS = 32 * RB, WORDS = 2 * ROWS * 32;
+    auto sums_of = [&](int i) {
+        uint8_t *r = i < 2 ? r0 : i < 4 ? r1 : i < 6 ? r2 : r3;
+        return (int *)r + (i & 1) * WORDS;
+    };
+    static_assert(2 * 4 * WORDS == KS * GSTAGE, "two waves' sums a stage");
+    int *own = sums_of(wave);
+    // lane l, register i: row 8 (i / 4) + 4 (l / 32) + i % 4, weight row l % 32
 #pragma unroll
     for (int f = 0; f < 2; ++f)
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+        for (int g = 0; g < RB; ++g)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                sums[((f * 2 + g) * 32 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3)) * 32 + (lane & 31)] =
+                own[(f * ROWS + 32 * g + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3)) * 32 + (lane & 31)] =
                     acc[f][g][i];
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own words
+    if constexpr (KS > 1)
+        lds_barrier();
+    else
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own words
+    const int *part0 = sums_of(w), *part1 = sums_of(KS > 1 ? WPG + w : w);
+    auto sum = [&](int o) { return KS > 1 ? part0[o] + part1[o] : part0[o]; };
     const int64_t *sw = m.sw + (size_t)expert * m.N, *sw2 = m.sw2 + (size_t)expert * m.N;
     const int n = n0 + (EPI == 1 ? 32 * wc + (lane & 31) : 64 * wc + lane);
     const bool in = n < m.N;
     const int64_t s1 = in ? sw[n] : 0, s2 = in && EPI == 1 ? sw2[n] : 0;
     const double d1 = w8_step_double(s1) * 0x1p-48, d2 = w8_step_double(s2) * 0x1p-48;
-    const int last = min(64, rows - 64 * wr);
     // U outputs a turn: chains of FP64 operations side by side
-    constexpr int U = 4, PER = EPI == 1 ? 2 : 1;   // rows of a wave at once
+    constexpr int U = EPI == 1 ? 2 : 8, PER = EPI == 1 ? 2 : 1;   // rows of a wave at once
     const int first = EPI == 1 ? lane >> 5 : 0;
     // the base a turn ahead of the sums
     int64_t add[U] = {};
@@ -569,69 +624,72 @@ __global__ __launch_bounds__(256, 2) void k_w8_gemm(W8Mul m, int nx, int ny)
             if (m.base && in)
 #pragma unroll
                 for (int j = 0; j < U; ++j)
-                    add[j] = m.base[(size_t)row_of(min(t0 + j, last - 1)) * m.N + n];
+                    add[j] = m.base[(size_t)row_of(t0 + j) * m.N + n];
     };
-    base(0);
-    for (int t0 = 0; t0 < last; t0 += U * PER) {
-        double y[U];
-        bool ok = true;
+    const int begin = 32 * q, last = min(begin + 32, rows - r_w);
+    base(begin);
+#pragma nounroll
+        for (int t0 = begin; t0 < last; t0 += U * PER) {
+            double y[U], up[EPI == 1 ? U : 1];
+            bool ok = true;
+            // output j's sum (up's lies 32 ROWS words on)
+            auto at_of = [&](int j) {
+                const int t = t0 + PER * j + first;   // (past the last: of other rows)
+                return t * 32 + (lane & 31) + (EPI == 1 ? 0 : (lane >> 5) * 32 * ROWS);
+            };
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const int t = t0 + PER * j + first;   // (rows past the last: sums of other rows)
-            const double sa = sd[64 * wr + t];
-            bool sure;
-            if constexpr (EPI == 1) {
-                const int o = t * 32 + (lane & 31);
-                const double g = w8_scaled_double(sums[o], sa, d1, sure);
-                ok = ok && sure;
-                const double u = w8_scaled_double(sums[2048 + o], sa, d2, sure);
-                ok = ok && sure;
-                y[j] = w8_silu_mul(g, u, sure);
-                ok = ok && __builtin_fabs(y[j]) < 0x1p53;
-            } else {
-                y[j] = w8_scaled_double(sums[(lane >> 5) * 2048 + t * 32 + (lane & 31)], sa, d1, sure);
-            }
-            ok = ok && sure;
-        }
-        int64_t v[U];
-#pragma unroll
-        for (int j = 0; j < U; ++j)
-            v[j] = (int64_t)y[j];
-        if (__any(!ok))
             for (int j = 0; j < U; ++j) {
-                const int t = t0 + PER * j + first;
-                const int64_t sa = m.sb[row_of(min(t, last - 1))];
-                int64_t z;
+                const double sa = sd[r_w + t0 + PER * j + first];
+                bool sure;
+                y[j] = w8_scaled_double(sum(at_of(j)), sa, d1, sure);
+                ok &= sure;
                 if constexpr (EPI == 1) {
-                    const int o = t * 32 + (lane & 31);
-                    z = q48_mul(q48_silu(w8_scaled(sums[o], sa, s1)), w8_scaled(sums[2048 + o], sa, s2));
-                } else {
-                    z = w8_scaled(sums[(lane >> 5) * 2048 + t * 32 + (lane & 31)], sa, s1);
+                    up[j] = w8_scaled_double(sum(32 * ROWS + at_of(j)), sa, d2, sure);
+                    ok &= sure;
                 }
-#pragma unroll
-                for (int i = 0; i < U; ++i)
-                    v[i] = i == j ? z : v[i];
             }
-        if constexpr (EPI == 0) {
+            if constexpr (EPI == 1) {
+                double z[U];
+                ok &= w8_silu_mul<U>(y, up, z);
+#pragma unroll
+                for (int j = 0; j < U; ++j)
+                    y[j] = z[j];
+            }
+            int64_t v[U];
 #pragma unroll
             for (int j = 0; j < U; ++j)
-                v[j] = (int64_t)((uint64_t)v[j] + (uint64_t)add[j]);
-            if (t0 + U < last)
-                base(t0 + U);
-        }
+                v[j] = (int64_t)y[j];
+            if (__any(!ok))
+#pragma nounroll
+                for (int j = 0; j < U; ++j) {
+                    const int64_t sa = m.sb[row_of(t0 + PER * j + first)];
+                    int64_t z = w8_scaled(sum(at_of(j)), sa, s1);
+                    if constexpr (EPI == 1)
+                        z = q48_mul(q48_silu(z), w8_scaled(sum(32 * ROWS + at_of(j)), sa, s2));
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const int t = t0 + PER * j + first;
-            const size_t row = (size_t)(row0 + 64 * wr + t);
-            if (!in || t >= last || (EXPERTS && toks[64 * wr + t] < 0))
-                continue;
-            if constexpr (EPI == 2)
-                atomicAdd((unsigned long long *)m.Y + (size_t)toks[64 * wr + t] * m.N + n,
-                          (unsigned long long)q48_mul(m.slot_w[row], v[j]));
-            else
-                m.Y[row * m.N + n] = v[j];
+                    for (int i = 0; i < U; ++i)
+                        v[i] = i == j ? z : v[i];
+                }
+            if constexpr (EPI == 0) {
+#pragma unroll
+                for (int j = 0; j < U; ++j)
+                    v[j] = (int64_t)((uint64_t)v[j] + (uint64_t)add[j]);
+                if (t0 + U < last)
+                    base(t0 + U);
+            }
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const int t = t0 + PER * j + first;
+                const size_t row = (size_t)(row0 + r_w + t);
+                if (!in || t >= last || (EXPERTS && toks[r_w + t] < 0))
+                    continue;
+                if constexpr (EPI == 2)
+                    atomicAdd((unsigned long long *)m.Y + (size_t)toks[r_w + t] * m.N + n,
+                              (unsigned long long)q48_mul(m.slot_w[row], v[j]));
+                else
+                    m.Y[row * m.N + n] = v[j];
+            }
         }
-    }
 }
 
 int launch_rc(int e) { return e == (int)hipSuccess ? Q48_OK : Q48_EHIP; }
@@ -793,10 +851,18 @@ int q48_launch_w8_mul(q48_ctx *c, const W8Mul &m, int epi, bool experts, int n_i
         const int gx = (m.N + (epi == 1 ? GT / 2 : GT) - 1) / (epi == 1 ? GT / 2 : GT);
         const int gy = (m.T + GT - 1) / GT;
         const dim3 grid((unsigned)((gx * gy + 7) / 8 * 8));
-        if (epi == 1)
-            hipLaunchKernelGGL((k_w8_gemm<1, false>), grid, dim3(256), 0, c->stream, m, gx, gy);
+        const bool halves = gx * gy <= c->cu_count && m.KT >= 8;
+#define W8_GEMM(EPI, KS)                                                                  \
+    hipLaunchKernelGGL((k_w8_gemm<EPI, false, KS>), grid, dim3(512), 0, c->stream, m, gx, gy)
+        if (epi == 1 && halves)
+            W8_GEMM(1, 2);
+        else if (epi == 1)
+            W8_GEMM(1, 1);
+        else if (halves)
+            W8_GEMM(0, 2);
         else
-            hipLaunchKernelGGL((k_w8_gemm<0, false>), grid, dim3(256), 0, c->stream, m, gx, gy);
+            W8_GEMM(0, 1);
+#undef W8_GEMM
         return (int)hipGetLastError();
     }
 #define W8_MUL(NB, EPI, EX)                                                            \

@@ -36,7 +36,7 @@ __device__ __forceinline__ double w8_scaled_double(int S, double sa, double sw, 
     const double p = sa * sw, pl = __builtin_fma(sa, sw, -p), s = (double)S;
     const double h = s * p, hl = __builtin_fma(s, p, -h), f = __builtin_floor(h);
     const double t = (h - f) + __builtin_fma(s, pl, hl), g = __builtin_floor(t);
-    sure = __builtin_fabs(h) < 0x1p52 && t - g < 1.0 - 0x1p-40;
+    sure = (__builtin_fabs(h) < 0x1p52) & (t - g < 1.0 - 0x1p-40);
     return f + g;
 }
 __device__ __forceinline__ double w8_step_double(int64_t step)
@@ -44,62 +44,105 @@ __device__ __forceinline__ double w8_step_double(int64_t step)
     return (uint64_t)step < (uint64_t)1 << 53 ? (double)step : __builtin_inf();
 }
 
-// floor(2^96 / r), 2^48 <= r < 2^53, FP64 rounding down: the estimate from above the quotient
-// or one less (q48_recip), its remainder exact
-__device__ __forceinline__ double w8_recip(double r)
+// A constant that stays in a register: as a literal every fused operation that adds it
+// would copy it into its result first.
+__device__ __forceinline__ double w8_kept(double c)
 {
-    double y = __builtin_amdgcn_rcp(r);
-    y = __builtin_fma(y, __builtin_fma(-r, y, 1.0), y);
-    y = __builtin_fma(y, __builtin_fma(-r, y, 1.0), y);
-    const double q = __builtin_fma(y, 0x1p96, 0x1p52 - 0.5) - 0x1p52;
-    return __builtin_fma(-q, r, 0x1p96) >= r ? q + 1.0 : q;
+    asm("" : "+v"(c));
+    return c;
 }
 
-// fp_mul(fp_silu(g), u) (fp_math.h:911-921) of whole numbers below 2^53, in FP64 rounding
-// down alone.  The squares of fp_exp: the first 12 stay below 2^52 (two operations each,
-// q48_exp_small), the last two, of at most e^10 2^48, are a rounded product and its exact
-// remainder each, r = A + T with A a double and T < 2^13.  Rounding down makes the sums
-// behind T too small by less than 2^-39: `sure` is false where that may hide a whole number
-// (q48_silu then).  A quotient by A + T: an estimate as in q48_recip, its remainder 2^96 -
-// q A exact (a multiple of A's last place, below 2^53 of them) and compared with A +
-// (q + 1) T, whose product is below 2^53.  About 85 operations; with 64-bit integers for
-// the last squares and the quotients 160, a third of them of quarter rate.
-__device__ __forceinline__ double w8_silu_mul(double g, double u, bool &sure)
+// All of v before anything behind: chains of operations that would else be scheduled one
+// after the other.
+__device__ __forceinline__ void w8_together(double (&v)[4])
+{
+    asm volatile("" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
+}
+__device__ __forceinline__ void w8_together(double (&v)[2])
+{
+    asm volatile("" : "+v"(v[0]), "+v"(v[1]));
+}
+__device__ __forceinline__ void w8_together(double (&v)[1]) {}
+
+// fp_mul(fp_silu(g), u) (fp_math.h:911-921) of U pairs of whole numbers below 2^53, |g| at
+// most 10 (false else), in FP64 rounding down alone.  The squares of fp_exp: the first 12 stay below 2^52 (two operations
+// each, q48_exp_small), the last two, of at most e^10 2^48, are a rounded product and its
+// exact remainder each, r = A + T with A a double and T < 2^13.  Rounding down makes the
+// sums behind T too small by less than 2^-39: false is returned where that may hide a whole
+// number (q48_silu then).  A quotient by A + T: an estimate as in q48_recip, its remainder
+// 2^96 - q A exact (a multiple of A's last place, below 2^53 of them) and compared with A +
+// (q + 1) T, whose product is below 2^53.  About 90 operations (with 64-bit integers for the
+// last squares and the quotients 160, a third of them of quarter rate), step by step for all
+// pairs: one is a chain, and a wave alone on its SIMD waits for each of its links.
+template <int U>
+__device__ __forceinline__ bool w8_silu_mul(const double (&g)[U], const double (&u)[U], double (&out)[U])
 {
 #pragma clang fp contract(off)   // products as rounded
-    const double ten = 10 * 0x1p48, m = __builtin_fmin(__builtin_fabs(g), ten);
-    // 1 + floor(m / 2^14)
-    double h = __builtin_fma(m, 0x1p-14, 0x1p52 + 0x1p48);
+#define W8_EACH _Pragma("unroll") for (int j = 0; j < U; ++j)
+    constexpr double ten = 10 * 0x1p48, unit = 0x1p-48;
+    const double m28 = w8_kept(-0x1p28), p52 = w8_kept(0x1p52), r24 = w8_kept(0x1p-24);
+    double h[U], y[U], A[U], T[U], r[U], q[U], c[U];
+    bool sure = true;
+    W8_EACH sure &= __builtin_fabs(g[j]) <= ten;
+    W8_EACH h[j] = __builtin_fma(__builtin_fabs(g[j]), 0x1p-14, p52 + 0x1p48);
 #pragma unroll
     for (int k = 0; k < 12; ++k) {
-        const double y = __builtin_fma(h, 0x1p-24, -0x1p28);
-        h = __builtin_fma(y, y, 0x1p52);
+        W8_EACH y[j] = __builtin_fma(h[j], r24, m28);
+        W8_EACH h[j] = __builtin_fma(y[j], y[j], p52);
+        w8_together(h);
     }
-    const double y = __builtin_fma(h, 0x1p-24, -0x1p28);
-    const double p = y * y, pi = __builtin_floor(p);
-    const double l = __builtin_floor((p - pi) + __builtin_fma(y, y, -p));   // square 13: pi + l
-    const double H = pi * 0x1p-24, L = l * 0x1p-24;
-    const double A0 = H * H, t0 = __builtin_fma(2 * H, L, __builtin_fma(H, H, -A0));
-    double A = __builtin_floor(A0);
-    const double t = (A0 - A) + __builtin_fma(L, L, t0);
-    double T = __builtin_floor(t);
-    sure = t - T < 1.0 - 0x1p-30;
-    const bool pos = g > 0;
+    W8_EACH y[j] = __builtin_fma(h[j], r24, m28);
+    W8_EACH r[j] = y[j] * y[j];   // square 13: A + T
+    W8_EACH A[j] = __builtin_floor(r[j]);
+    W8_EACH T[j] = __builtin_fma(y[j], y[j], -r[j]);
+    W8_EACH T[j] = __builtin_floor((r[j] - A[j]) + T[j]);
+    w8_together(T);
+    W8_EACH A[j] *= r24;          // square 14
+    W8_EACH T[j] *= r24;
+    W8_EACH r[j] = A[j] * A[j];
+    W8_EACH q[j] = __builtin_fma(A[j], A[j], -r[j]);
+    W8_EACH q[j] = __builtin_fma(2 * A[j], T[j], q[j]);
+    W8_EACH q[j] = __builtin_fma(T[j], T[j], q[j]);
+    W8_EACH A[j] = __builtin_floor(r[j]);
+    W8_EACH q[j] = (r[j] - A[j]) + q[j];
+    W8_EACH T[j] = __builtin_floor(q[j]);
+    W8_EACH sure &= q[j] - T[j] < 1.0 - 0x1p-30;
+    w8_together(T);
     // what is divided by: e^g where g > 0, else 1 + e^-g
-    const double c = pos ? 0.0 : 0x1p48, B = A + c;
-    T += c - (B - A);
-    A = B;
-    double r = __builtin_amdgcn_rcp(A);
-    r = __builtin_fma(r, __builtin_fma(-A, r, 1.0), r);
-    r = __builtin_fma(r, __builtin_fma(-A, r, 1.0), r);
-    r = __builtin_fma(-(r * T), r, r);
-    double q = __builtin_fma(r, 0x1p96, 0x1p52 - 0.5) - 0x1p52;
-    const double rem = __builtin_fma(-q, A, 0x1p96);
-    q += rem - A >= (q + 1.0) * T ? 1.0 : 0.0;
-    double s = pos ? w8_recip(q + 0x1p48) : q;
-    s = g > ten ? 0x1p48 : g < -ten ? 0.0 : s;
-    const double v = __builtin_floor(g * (s * 0x1p-48));
-    return __builtin_floor(v * (u * 0x1p-48));
+    W8_EACH c[j] = g[j] > 0 ? 0.0 : 0x1p48;
+    W8_EACH r[j] = A[j] + c[j];
+    W8_EACH T[j] += c[j] - (r[j] - A[j]);
+    W8_EACH A[j] = r[j];
+    W8_EACH r[j] = __builtin_amdgcn_rcp(A[j]);
+    W8_EACH y[j] = __builtin_fma(-A[j], r[j], 1.0);
+    W8_EACH y[j] = __builtin_fma(y[j], y[j], y[j]);
+    W8_EACH r[j] = __builtin_fma(r[j], y[j], r[j]);
+    w8_together(r);
+    W8_EACH r[j] = __builtin_fma(-(r[j] * T[j]), r[j], r[j]);
+    // the quotient in units of 2^-48, or a unit less
+    const double p48 = w8_kept(0x1p48), low = w8_kept(16.0 - 0.5 * unit);
+    W8_EACH q[j] = __builtin_fma(r[j], p48, low) - 16.0;
+    W8_EACH y[j] = __builtin_fma(-q[j], A[j], p48);
+    W8_EACH h[j] = q[j] + unit;
+    W8_EACH y[j] = y[j] - A[j] * unit;
+    W8_EACH q[j] = y[j] >= h[j] * T[j] ? h[j] : q[j];
+    w8_together(q);
+    // floor(2^96 / (1 + e^-g)) where g > 0: below 2^53, so the remainder is one operation
+    W8_EACH A[j] = q[j] + 1.0;
+    W8_EACH r[j] = __builtin_amdgcn_rcp(A[j]);
+    W8_EACH y[j] = __builtin_fma(-A[j], r[j], 1.0);
+    W8_EACH y[j] = __builtin_fma(y[j], y[j], y[j]);
+    W8_EACH r[j] = __builtin_fma(r[j], y[j], r[j]);
+    w8_together(r);
+    W8_EACH r[j] = (r[j] + low) - 16.0;
+    W8_EACH h[j] = r[j] + unit;
+    W8_EACH r[j] = __builtin_fma(-h[j], A[j], 1.0) >= 0 ? h[j] : r[j];
+    W8_EACH r[j] = c[j] == 0 ? w8_kept(r[j]) : q[j];   // (kept: else a branch around its making)
+    W8_EACH y[j] = __builtin_floor(g[j] * r[j]);
+    W8_EACH out[j] = __builtin_floor(y[j] * (u[j] * unit));
+    W8_EACH sure &= __builtin_fabs(out[j]) < 0x1p53;
+#undef W8_EACH
+    return sure;
 }
 
 // the step of a row whose largest magnitude is a, and its reciprocal
