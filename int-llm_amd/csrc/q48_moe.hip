@@ -82,19 +82,19 @@ __device__ __forceinline__ void moe_choose(const int64_t (&v)[PER], int E, int t
     weight = q48_div(e, sum);
 }
 
-// The pairs counted by expert, each expert's first slot, the items of 16 slots, and every
+// The pairs counted by expert, each expert's first slot, the items of `rows` slots, and every
 // pair into its slot: one block of NT threads.
 struct MoeSlots {
     int4 *items;
     int *tok;
     int64_t *w;
-    int slots, n_items;
+    int slots, n_items, rows;
 };
 template <int NT>
 __device__ __forceinline__ void moe_slots(const MoeSlots &s, const int *chosen,
                                           const int64_t *weight, int pairs, int top, int E)
 {
-    __shared__ int count[W8_MAX_COUNT], first[W8_MAX_COUNT];
+    __shared__ int count[W8_MAX_COUNT], first[W8_MAX_COUNT], item[W8_MAX_COUNT];
     const int tid = threadIdx.x, lane = tid & 63;
     for (int i = tid; i < E; i += NT)
         count[i] = 0;
@@ -106,25 +106,30 @@ __device__ __forceinline__ void moe_slots(const MoeSlots &s, const int *chosen,
     for (int i = tid; i < pairs; i += NT)
         atomicAdd(&count[from_all(chosen + i)], 1);
     __syncthreads();
-    if (tid < 64) {   // sixteens before each expert: sums over the lanes of a wave
-        int before = 0;
+    if (tid < 64) {   // slots (in sixteens) and items before each expert: sums over a wave
+        int slots = 0, items = 0;
         for (int e0 = 0; e0 < E; e0 += 64) {
-            const int n = e0 + lane < E ? (count[e0 + lane] + 15) & ~15 : 0;
-            int sum = n;
+            const int c = e0 + lane < E ? count[e0 + lane] : 0;
+            const int n = (c + 15) & ~15, k = (c + s.rows - 1) / s.rows;
+            int sn = n, sk = k;
             for (int d = 1; d < 64; d <<= 1) {
-                const int o = __shfl_up(sum, d);
-                sum += lane >= d ? o : 0;
+                const int on = __shfl_up(sn, d), ok = __shfl_up(sk, d);
+                sn += lane >= d ? on : 0;
+                sk += lane >= d ? ok : 0;
             }
-            if (e0 + lane < E)
-                first[e0 + lane] = before + sum - n;
-            before += __builtin_amdgcn_readlane(sum, 63);
+            if (e0 + lane < E) {
+                first[e0 + lane] = slots + sn - n;
+                item[e0 + lane] = items + sk - k;
+            }
+            slots += __builtin_amdgcn_readlane(sn, 63);
+            items += __builtin_amdgcn_readlane(sk, 63);
         }
     }
     __syncthreads();
     for (int e = tid; e < E; e += NT) {
         const int n = count[e];
-        for (int i = 0; i < n; i += 16)
-            s.items[(first[e] + i) >> 4] = make_int4(e, first[e] + i, min(16, n - i), 0);
+        for (int i = 0; i < n; i += s.rows)
+            s.items[item[e] + i / s.rows] = make_int4(e, first[e] + i, min(s.rows, n - i), 0);
         count[e] = first[e];
     }
     __syncthreads();
@@ -383,6 +388,12 @@ int launch_route(q48_ctx *c, const MoeRoute &a)
     return (int)hipGetLastError();
 }
 
+// items of `rows` slots that they can take
+size_t items_of(size_t pairs, int E, int rows)
+{
+    return pairs / rows + (pairs < (size_t)E ? pairs : (size_t)E);
+}
+
 } // namespace
 
 extern "C" {
@@ -431,7 +442,7 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
     size_t Tc = ((size_t)1 << 30) / ((size_t)16 * top * ffn);
     Tc = Tc < ((size_t)1 << 19) / top ? Tc : ((size_t)1 << 19) / top;
     Tc = Tc < 16 ? 16 : Tc < (size_t)T ? Tc : (size_t)T;
-    const size_t slots = slots_of(Tc * top, E), n_items = slots / 16;
+    const size_t slots = slots_of(Tc * top, E), n_items = items_of(Tc * top, E, 16);
     const size_t o_x = take(w8_tiles((int)Tc, dim)), o_xs = take(Tc * 8);
     const size_t o_xn = take(norm_w ? Tc * row : 0), o_l = take(Tc * E * 8);
     const size_t o_c = take(Tc * top * 4), o_w = take(Tc * top * 8);
@@ -444,7 +455,11 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
     uint8_t *ws = (uint8_t *)c->w8;
     for (size_t t0 = 0; t0 < (size_t)T; t0 += Tc) {
         const int n = (int)(Tc < T - t0 ? Tc : T - t0);
-        const int sl = (int)slots_of((size_t)n * top, E), it = sl / 16;
+        const int sl = (int)slots_of((size_t)n * top, E);
+        // Slots an item, by an expert's average: weights are read once an item.
+        const size_t mean = (size_t)n * top / E;
+        const int rows = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 256 ? 64 : 128;
+        const int it = (int)items_of((size_t)n * top, E, rows);
         W8Rows r = {};
         r.codes = ws + o_x;
         r.step = (int64_t *)(ws + o_xs);
@@ -463,7 +478,7 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
         int4 *items = (int4 *)(ws + o_i);
         int *tok = (int *)(ws + o_t);
         int64_t *sw = (int64_t *)(ws + o_sw);
-        const MoeSlots s = {items, tok, sw, sl, it};
+        const MoeSlots s = {items, tok, sw, sl, it, rows};
         const int per = route_per(c, n, E, dim);
         if (per) {
             int spl = 4;
@@ -511,6 +526,7 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
         m.B = r.codes;
         m.sb = r.step;
         m.T = n;
+        m.rows = rows;
         m.Y = (int64_t *)(ws + o_h);
         m.items = items;
         m.slot_tok = tok;

@@ -131,25 +131,78 @@ __global__ __launch_bounds__(256) void k_w8_pack(uint8_t *__restrict__ codes,
     }
 }
 
-__global__ __launch_bounds__(256) void k_w8_values(int64_t *__restrict__ out,
+// Eight rows of weights a block, a wave each, read once; their codes through LDS, so that
+// words and tiles (128 bytes of each) are whole lines.
+template <int J>
+__global__ __launch_bounds__(512, J <= 16 ? 4 : 2) void k_w8_pack_r(uint8_t *__restrict__ codes,
+                                                  int64_t *__restrict__ steps,
+                                                  const int64_t *__restrict__ W, int N, int K)
+{
+    q48_round_down();
+    constexpr int LD = 128 * J + 16;
+    __shared__ __align__(16) uint8_t rows[8][LD];
+    const int tid = threadIdx.x, w = tid >> 6, n = blockIdx.x * 8 + w, KT = (K + 63) / 64;
+    if (n < N) {
+        RowWords<64, 2, J> x;
+        x.load(W + (size_t)n * K, K);
+        const int64_t step = x.quantise(K, KT, nullptr, [&](int i, uint32_t q) {
+            *(uint16_t *)&rows[w][i] = (uint16_t)q;
+        });
+        if ((tid & 63) == 0)
+            steps[n] = step;
+    } else {
+        for (int i = (tid & 63) * 16; i < KT * 64; i += 1024)
+            *(v4i *)&rows[w][i] = v4i{0, 0, 0, 0};
+    }
+    __syncthreads();
+    uint8_t *to = codes + (size_t)(blockIdx.x >> 1) * KT * 1024 + (blockIdx.x & 1) * 128;
+    for (int i = tid; i < KT * 32; i += 512)   // 16 bytes: row i % 8, columns 16 (i / 8) on
+        *(v4i *)(to + (i >> 3) * 256 + (i & 7) * 16) = *(const v4i *)&rows[i & 7][(i >> 3) * 16];
+}
+
+// The way back: eight rows x 2048 columns a block.
+__global__ __launch_bounds__(512) void k_w8_values(int64_t *__restrict__ out,
                                                   const uint8_t *__restrict__ codes,
                                                   const int64_t *__restrict__ steps, int N, int K)
 {
-    const int n = blockIdx.x, KT = (K + 63) / 64;
+    constexpr int LD = 2048 + 16;
+    __shared__ __align__(16) uint8_t rows[8][LD];
+    const int tid = threadIdx.x, w = tid >> 6, n = blockIdx.x * 8 + w, KT = (K + 63) / 64;
+    const int k0 = blockIdx.y * 2048, nk = min(K - k0, 2048);
+    const uint8_t *from = codes + ((size_t)(blockIdx.x >> 1) * KT + (k0 >> 6)) * 1024 +
+                          (blockIdx.x & 1) * 128;
+    for (int i = tid; i < (nk + 15) / 16 * 8; i += 512)
+        *(v4i *)&rows[i & 7][(i >> 3) * 16] = *(const v4i *)(from + (i >> 3) * 256 + (i & 7) * 16);
+    __syncthreads();
+    if (n >= N)
+        return;
     const uint64_t step = (uint64_t)steps[n];
-    for (int i = threadIdx.x; i < K; i += 256)
-        out[(size_t)n * K + i] = (int64_t)((uint64_t)(int64_t)(int8_t)codes[w8_at(n, i, KT)] * step);
+    int64_t *to = out + (size_t)n * K + k0;
+    typedef int64_t words __attribute__((ext_vector_type(2), aligned(8)));
+    for (int i = 2 * (tid & 63); i < nk; i += 128) {
+        const uint16_t c = *(const uint16_t *)&rows[w][i];
+        const words v = {(int64_t)((uint64_t)(int64_t)(int8_t)c * step),
+                         (int64_t)((uint64_t)(int64_t)(int8_t)(c >> 8) * step)};
+        if (i + 1 < nk)
+            *(words *)(to + i) = v;
+        else
+            to[i] = v.x;
+    }
 }
 
-// A block 16 weight rows x 16 NB rows: its four waves take every fourth tile of 64
-// columns and add up in LDS.
-template <int NB, int EPI, bool EXPERTS>
-__global__ __launch_bounds__(256) void k_w8_mul(W8Mul m)
+// A block 16 weight rows x 16 NB rows: its NW waves take every NW-th tile of 64 columns,
+// straight from memory into the matrix instruction's operands, and add up in LDS.  What
+// bounds it is the loads under way, and for many rows the weights read again for every 64.
+template <int NB, int EPI, bool EXPERTS, int NW>
+__global__ __launch_bounds__(64 * NW) void k_w8_mul(W8Mul m)
 {
     q48_round_down();
-    constexpr int M = EPI == 1 ? 2 : 1;
-    __shared__ __align__(16) int red[M][4][256];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    constexpr int M = EPI == 1 ? 2 : 1, NT = 64 * NW;
+    constexpr int P = 12 / (M + NB) > 4 ? 4 : 12 / (M + NB);    // tiles a turn
+    constexpr int IT = (NB * 256 + NT - 1) / NT;                // outputs a thread
+    __shared__ __align__(16) int red[M * NB * NW][256];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     int expert = 0, row0 = blockIdx.y * 16 * NB, rows = m.T - row0;
     if constexpr (EXPERTS) {
         const int4 it = m.items[blockIdx.y];
@@ -159,29 +212,47 @@ __global__ __launch_bounds__(256) void k_w8_mul(W8Mul m)
         if (rows <= 0)
             return;
     }
+    rows = min(rows, 16 * NB);
     const int KT = m.KT, n0 = blockIdx.x * 16;
     const size_t tile = (size_t)expert * m.a_stride + (size_t)blockIdx.x * KT * 1024 + lane * 16;
     const uint8_t *A[2] = {m.A + tile, M == 2 ? m.A2 + tile : nullptr};
     const uint8_t *B[NB];
 #pragma unroll
     for (int g = 0; g < NB; ++g) {
-        const int last = (rows + 15) / 16 - 1;
-        const int r = row0 + 16 * (g < last ? g : last);
+        const int r = row0 + 16 * min(g, (rows - 1) >> 4);
         if constexpr (EXPERTS && EPI == 1) {
-            int tok = m.slot_tok[r + (lane & 15)];
-            tok = tok < 0 ? 0 : tok;
+            const int tok = max(m.slot_tok[r + (lane & 15)], 0);
             B[g] = m.B + (size_t)(tok >> 4) * KT * 1024 + (lane >> 4) * 256 + (tok & 15) * 16;
         } else {
             B[g] = m.B + (size_t)(r >> 4) * KT * 1024 + lane * 16;
         }
     }
+    // what the epilogue needs, ahead of the products
+    const int n = n0 + (tid & 15);
+    const bool in = n < m.N;
+    const size_t at_n = (size_t)expert * m.N + min(n, m.N - 1);
+    const int64_t s1 = m.sw[at_n], s2 = M == 2 ? m.sw2[at_n] : 0;
+    int64_t sb[IT], more[IT];   // more: the base, or the slot's weight
+    int tok[IT];
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        const int r = min((tid + NT * i) >> 4, rows - 1);
+        tok[i] = EXPERTS ? m.slot_tok[row0 + r] : 0;
+        sb[i] = m.sb[EXPERTS && EPI == 1 ? max(tok[i], 0) : row0 + r];
+        more[i] = 0;
+        if constexpr (EPI == 2)
+            more[i] = m.slot_w[row0 + r];
+        if (EPI == 0 && m.base)
+            more[i] = m.base[(size_t)(row0 + r) * m.N + min(n, m.N - 1)];
+    }
     v4i acc[M][NB] = {};
-    constexpr int P = NB == 1 ? 4 : 2;
-    for (int k0 = w; k0 < KT; k0 += 4 * P) {
+    for (int k0 = w; k0 < KT; k0 += NW * P) {
         v4i a[M][P], b[NB][P];
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const size_t k = min(k0 + 4 * p, KT - 1);
+            const size_t k = k0 + NW * p;
+            if ((int)k >= KT)
+                break;
 #pragma unroll
             for (int j = 0; j < M; ++j)
                 a[j][p] = *(const v4i *)(A[j] + k * 1024);
@@ -191,7 +262,7 @@ __global__ __launch_bounds__(256) void k_w8_mul(W8Mul m)
         }
 #pragma unroll
         for (int p = 0; p < P; ++p)
-            if (k0 + 4 * p < KT)
+            if (k0 + NW * p < KT)
 #pragma unroll
                 for (int g = 0; g < NB; ++g)
 #pragma unroll
@@ -200,39 +271,34 @@ __global__ __launch_bounds__(256) void k_w8_mul(W8Mul m)
                             __builtin_amdgcn_mfma_i32_16x16x64_i8(a[j][p], b[g][p], acc[j][g], 0, 0, 0);
     }
     // lane l, register i: weight row 4 (l / 16) + i, row l % 16
-    const int n = n0 + (tid & 15);
-    const int64_t *sw = m.sw + (size_t)expert * m.N, *sw2 = m.sw2 + (size_t)expert * m.N;
-    const bool in = n < m.N;
-    const int64_t s1 = in ? sw[n] : 0, s2 = in && M == 2 ? sw2[n] : 0;
 #pragma unroll
-    for (int g = 0; g < NB; ++g) {
+    for (int j = 0; j < M; ++j)
+#pragma unroll
+        for (int g = 0; g < NB; ++g)
+            *(v4i *)&red[(j * NB + g) * NW + w][(lane & 15) * 16 + 4 * (lane >> 4)] = acc[j][g];
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < IT; ++i) {
+        const int o = tid + NT * i, g = o >> 8, r = o >> 4;
+        if (!in || r >= rows || tok[i] < 0)
+            continue;
+        int S[2] = {};
 #pragma unroll
         for (int j = 0; j < M; ++j)
-            *(v4i *)&red[j][w][(lane & 15) * 16 + 4 * (lane >> 4)] = acc[j][g];
-        __syncthreads();
-        const int r = 16 * g + (tid >> 4);
-        if (in && r < rows) {
-            int S[2] = {};
 #pragma unroll
-            for (int j = 0; j < M; ++j)
-                S[j] = red[j][0][tid] + red[j][1][tid] + red[j][2][tid] + red[j][3][tid];
-            const size_t row = (size_t)row0 + r;
-            const int tok = EXPERTS ? m.slot_tok[row] : 0;
-            if (tok >= 0) {
-                const int64_t sb = m.sb[EXPERTS && EPI == 1 ? (size_t)tok : row];
-                int64_t y = w8_scaled(S[0], sb, s1);
-                if constexpr (EPI == 1)
-                    y = q48_mul(q48_silu(y), w8_scaled(S[1], sb, s2));
-                if constexpr (EPI == 2)
-                    atomicAdd((unsigned long long *)m.Y + (size_t)tok * m.N + n,
-                              (unsigned long long)q48_mul(m.slot_w[row], y));
-                else
-                    m.Y[row * m.N + n] =
-                        (int64_t)((uint64_t)y +
-                                  (EPI == 0 && m.base ? (uint64_t)m.base[row * m.N + n] : 0));
-            }
+            for (int u = 0; u < NW; ++u)
+                S[j] += red[(j * NB + g) * NW + u][o & 255];
+        const size_t row = (size_t)row0 + r;
+        if constexpr (EPI == 1) {
+            m.Y[row * m.N + n] = w8_swiglu(S[0], S[1], sb[i], s1, s2);
+        } else {
+            const int64_t y = w8_times(S[0], sb[i], s1);
+            if constexpr (EPI == 2)
+                atomicAdd((unsigned long long *)m.Y + (size_t)tok[i] * m.N + n,
+                          (unsigned long long)q48_mul(more[i], y));
+            else
+                m.Y[row * m.N + n] = (int64_t)((uint64_t)y + (uint64_t)more[i]);
         }
-        __syncthreads();
     }
 }
 
@@ -378,9 +444,11 @@ __global__ __launch_bounds__(ONE_NT) void k_w8_one(W8Mul m, const int64_t *__res
             }
             const int n = (g * TB + tl) * 16 + ch;
             if (i == 0 && n < m.N) {
-                int64_t y = w8_scaled(sum[0], sb, s1);
+                int64_t y;
                 if constexpr (EPI == 1)
-                    y = q48_mul(q48_silu(y), w8_scaled(sum[1], sb, s2));
+                    y = w8_swiglu(sum[0], sum[1], sb, s1, s2);
+                else
+                    y = w8_times(sum[0], sb, s1);
                 if constexpr (EPI == 2)
                     atomicAdd((unsigned long long *)m.Y + (size_t)tok * m.N + n,
                               (unsigned long long)q48_mul(wt, y));
@@ -847,42 +915,65 @@ int q48_launch_w8_one(q48_ctx *c, const W8Mul &m, int epi, const int64_t *X,
 int q48_launch_w8_mul(q48_ctx *c, const W8Mul &m, int epi, bool experts, int n_items)
 {
     const unsigned nx = (m.N + 15) / 16;
-    if (!experts && m.T > 64) {
-        const int gx = (m.N + (epi == 1 ? GT / 2 : GT) - 1) / (epi == 1 ? GT / 2 : GT);
-        const int gy = (m.T + GT - 1) / GT;
+    // Tiles of 128 x 128 where there are outputs to fill the chip with them.  us, k_w8_mul /
+    // k_w8_gemm: 2560 x 2048 512 rows 18.5 / 22.1, 1024 28.8 / 26.7; 2048 x 5632 512 30.0 /
+    // 37.9, 1024 48.9 / 43.0; 1031 x 2047 1024 22.4 / 26.1; SwiGLU of 5632 x 2048 512 38.8 /
+    // 39.9, 1024 69.9 / 60.9.
+    const bool tiles = experts ? m.rows > 64 : (size_t)m.T * m.N >= (epi == 1 ? 3u : 2u) << 20;
+    if (tiles) {
+        const int ch = epi == 1 ? GT / 2 : GT, gx = (m.N + ch - 1) / ch;
+        const int gy = experts ? n_items : (m.T + GT - 1) / GT;
         const dim3 grid((unsigned)((gx * gy + 7) / 8 * 8));
         const bool halves = gx * gy <= c->cu_count && m.KT >= 8;
-#define W8_GEMM(EPI, KS)                                                                  \
-    hipLaunchKernelGGL((k_w8_gemm<EPI, false, KS>), grid, dim3(512), 0, c->stream, m, gx, gy)
-        if (epi == 1 && halves)
-            W8_GEMM(1, 2);
+#define W8_GEMM(EPI, EX, KS)                                                              \
+    hipLaunchKernelGGL((k_w8_gemm<EPI, EX, KS>), grid, dim3(512), 0, c->stream, m, gx, gy)
+        if (experts && epi == 1)
+            W8_GEMM(1, true, 1);
+        else if (experts)
+            W8_GEMM(2, true, 1);
+        else if (epi == 1 && halves)
+            W8_GEMM(1, false, 2);
         else if (epi == 1)
-            W8_GEMM(1, 1);
+            W8_GEMM(1, false, 1);
         else if (halves)
-            W8_GEMM(0, 2);
+            W8_GEMM(0, false, 2);
         else
-            W8_GEMM(0, 1);
+            W8_GEMM(0, false, 1);
 #undef W8_GEMM
         return (int)hipGetLastError();
     }
-#define W8_MUL(NB, EPI, EX)                                                            \
-    hipLaunchKernelGGL((k_w8_mul<NB, EPI, EX>), dim3(nx, EX ? n_items : (m.T + 16 * NB - 1) / (16 * NB)), \
-                       dim3(256), 0, c->stream, m)
-    if (experts) {
-        if (epi == 1)
-            W8_MUL(1, 1, true);
-        else
-            W8_MUL(1, 2, true);
-    } else if (epi == 1) {
-        if (m.T <= 16)
-            W8_MUL(1, 1, false);
-        else
-            W8_MUL(4, 1, false);
-    } else if (m.T <= 16) {
-        W8_MUL(1, 0, false);
-    } else {
-        W8_MUL(4, 0, false);
-    }
+    // Eight waves a block where that is two blocks a compute unit at most.  us, four / eight /
+    // sixteen: 26 rows x 2048 x 5632 11.8 / 9.9 / 10.1, 64 14.3 / 12.1 / 12.2; x 2560 x 2048
+    // 26 rows 7.4 / 7.1 / 7.3, 256 12.6 / 12.9 / 14.5; SwiGLU of 5632 x 2048 2 rows 7.7 / 7.6
+    // / 8.6, 256 24.5 / 24.3 / 24.6.
+    const int rows = experts ? m.rows : m.T <= 16 ? 16 : m.T <= 32 ? 32 : 64;
+    const int ny = experts ? n_items : (m.T + rows - 1) / rows;
+    const bool eight = (size_t)nx * ny <= 2 * (size_t)c->cu_count;
+#define W8_MUL(NB, EPI, EX)                                                                      \
+    do {                                                                                         \
+        if (eight)                                                                               \
+            hipLaunchKernelGGL((k_w8_mul<NB, EPI, EX, 8>), dim3(nx, ny), dim3(512), 0, c->stream, m); \
+        else                                                                                     \
+            hipLaunchKernelGGL((k_w8_mul<NB, EPI, EX, 4>), dim3(nx, ny), dim3(256), 0, c->stream, m); \
+    } while (0)
+#define W8_MUL_NB(EPI, EX)                                                                       \
+    do {                                                                                         \
+        if (rows == 16)                                                                          \
+            W8_MUL(1, EPI, EX);                                                                  \
+        else if (rows == 32)                                                                     \
+            W8_MUL(2, EPI, EX);                                                                  \
+        else                                                                                     \
+            W8_MUL(4, EPI, EX);                                                                  \
+    } while (0)
+    if (experts && epi == 1)
+        W8_MUL_NB(1, true);
+    else if (experts)
+        W8_MUL_NB(2, true);
+    else if (epi == 1)
+        W8_MUL_NB(1, false);
+    else
+        W8_MUL_NB(0, false);
+#undef W8_MUL_NB
 #undef W8_MUL
     return (int)hipGetLastError();
 }
@@ -915,8 +1006,14 @@ static int w8_fill(q48_ctx *c, const q48_w8 *w, int index, const int64_t *W, con
     if (over(W, n * 8) || over(codes, n) || over(steps, (size_t)N * 8))
         return Q48_EINVAL;
     q48_on_device on(c);
-    hipLaunchKernelGGL(k_w8_pack, dim3((N + 15) / 16 * 16), dim3(256), 0, c->stream, to, st, W,
-                       codes, steps, N, K);
+    const dim3 eights((N + 15) / 16 * 2);
+    if (W && K <= 2048)
+        hipLaunchKernelGGL(k_w8_pack_r<16>, eights, dim3(512), 0, c->stream, to, st, W, N, K);
+    else if (W && K <= 4096)
+        hipLaunchKernelGGL(k_w8_pack_r<32>, eights, dim3(512), 0, c->stream, to, st, W, N, K);
+    else
+        hipLaunchKernelGGL(k_w8_pack, dim3((N + 15) / 16 * 16), dim3(256), 0, c->stream, to, st, W,
+                           codes, steps, N, K);
     return launch_rc((int)hipGetLastError());
 }
 
@@ -945,7 +1042,7 @@ int q48_w8_values(q48_ctx *c, int64_t *out, const q48_w8 *w, int index)
     if (q48_share(out, n, from, bytes) || q48_share(out, n, st, (size_t)N * 8))
         return Q48_EINVAL;
     q48_on_device on(c);
-    hipLaunchKernelGGL(k_w8_values, dim3(N), dim3(256), 0, c->stream, out, from, st, N, K);
+    hipLaunchKernelGGL(k_w8_values, dim3((N + 7) / 8, (K + 2047) / 2048), dim3(512), 0, c->stream, out, from, st, N, K);
     return launch_rc((int)hipGetLastError());
 }
 

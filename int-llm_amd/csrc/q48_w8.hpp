@@ -145,6 +145,25 @@ __device__ __forceinline__ bool w8_silu_mul(const double (&g)[U], const double (
     return sure;
 }
 
+// One product, and one SwiGLU of two, of steps in words
+__device__ __forceinline__ int64_t w8_times(int S, int64_t sa, int64_t sw)
+{
+    bool sure;
+    const double y = w8_scaled_double(S, w8_step_double(sa), w8_step_double(sw) * 0x1p-48, sure);
+    return sure ? (int64_t)y : w8_scaled(S, sa, sw);
+}
+__device__ __forceinline__ int64_t w8_swiglu(int Sg, int Su, int64_t sa, int64_t sg, int64_t su)
+{
+    const double a = w8_step_double(sa);
+    bool s1, s2;
+    const double g[1] = {w8_scaled_double(Sg, a, w8_step_double(sg) * 0x1p-48, s1)};
+    const double u[1] = {w8_scaled_double(Su, a, w8_step_double(su) * 0x1p-48, s2)};
+    double y[1];
+    if (w8_silu_mul<1>(g, u, y) & s1 & s2)
+        return (int64_t)y[0];
+    return q48_mul(q48_silu(w8_scaled(Sg, sa, sg)), w8_scaled(Su, sa, su));
+}
+
 // the step of a row whose largest magnitude is a, and its reciprocal
 __device__ __forceinline__ uint64_t w8_step(uint64_t a, double &r)
 {
@@ -181,7 +200,8 @@ __device__ __forceinline__ int q48_dpp32(int v)
 // C (i + NT j) + 0 .. C - 1 for j < J, zeros past K (at most NT C J).  Four waves, one a
 // SIMD, for rows of up to 2048: what every wave does alike (its sums, the row's scalar, the
 // step) was half of the work with sixteen.  norm and quantise have a barrier each: the
-// block's other waves call lds_barrier for them.
+// block's other waves call lds_barrier for them.  With NT 64 every wave has a row of its
+// own, and quantise no barrier.
 //
 // The arithmetic is FP64 rounding down (q48_round_down) where a wave's words allow it,
 // integer elsewhere, per wave.  For integers below LIM: floor(x r / 2^48) is the floor of
@@ -203,7 +223,11 @@ struct RowWords {
     Word v[J][C];
     bool dbl = false;   // the wave's words are doubles (uniform)
 
-    __device__ __forceinline__ static int at(int j) { return C * ((int)threadIdx.x + NT * j); }
+    static_assert((NT & (NT - 1)) == 0, "whole waves");
+    __device__ __forceinline__ static int at(int j)
+    {
+        return C * (((int)threadIdx.x & (NT - 1)) + NT * j);
+    }
 
     // x is on the boundary of its words only
     __device__ __forceinline__ void load(const int64_t *x, int K)
@@ -239,15 +263,15 @@ struct RowWords {
     // words to doubles if all of the wave's are below LIM
     __device__ __forceinline__ void to_doubles(int K)
     {
-        double m = 0;
-        double d[J][C];
+        uint32_t m = 0;   // of the high halves
         each(K, [&](int j, int c) {
-            d[j][c] = (double)v[j][c].i;
-            m = __builtin_fmax(m, __builtin_fabs(d[j][c]));
+            const int hi = (int)(v[j][c].i >> 32);
+            m = max(m, (uint32_t)(hi ^ (hi >> 31)));
         });
-        dbl = !__any(m >= LIM);
+        static_assert(LIM == (double)(((uint64_t)1 << 53) - ((uint64_t)1 << 47)), "by halves");
+        dbl = !__any(m >= (1u << 21) - (1u << 15));
         if (dbl)
-            each(K, [&](int j, int c) { v[j][c].d = d[j][c]; });
+            each(K, [&](int j, int c) { v[j][c].d = (double)v[j][c].i; });
     }
     __device__ __forceinline__ void to_words(int K)
     {
@@ -332,12 +356,14 @@ struct RowWords {
             });
             m = (uint64_t)q48_wave_max64((int64_t)(m - 1)) + 1;   // at most 2^63: in order less one
         }
-        if ((threadIdx.x & 63) == 0)
-            red[threadIdx.x >> 6] = m;
-        lds_barrier();
+        if constexpr (NT > 64) {
+            if ((threadIdx.x & 63) == 0)
+                red[threadIdx.x >> 6] = m;
+            lds_barrier();
 #pragma unroll 4
-        for (int i = 0; i < NT / 64; ++i)
-            m = red[i] > m ? red[i] : m;
+            for (int i = 0; i < NT / 64; ++i)
+                m = red[i] > m ? red[i] : m;
+        }
         double rc;
         const uint64_t step = w8_step(m, rc);
         if (step > STEP_LIM)   // another wave's words
@@ -385,7 +411,9 @@ struct W8Mul {
     int T;                        // rows
     int64_t *Y;
     const int64_t *base;
-    // experts: items {expert, first slot, slots, 0}, a slot's token (-1: none) and weight
+    // experts: items {expert, first slot, slots (at most rows), 0}, a slot's token (-1: none)
+    // and weight
+    int rows;   // 16, 32, 64 or 128
     const int4 *items;
     const int *slot_tok;
     const int64_t *slot_w;

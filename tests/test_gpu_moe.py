@@ -88,6 +88,12 @@ def test_ties_go_to_the_lowest_expert(own, T):  # noqa: F811
     check(own, layer, X, 12, False)
 
 
+@pytest.mark.parametrize("T,E,top", [(300, 1, 1), (150, 2, 2), (700, 4, 2), (1100, 3, 1)])
+def test_many_rows_an_expert(own, T, E, top):  # noqa: F811
+    rng = np.random.default_rng(T)
+    check(own, Layer(rng, E, 70, 130), words(rng, T, 70), top, True)
+
+
 def test_all_tokens_to_one_expert(own):  # noqa: F811
     rng = np.random.default_rng(4)
     layer = Layer(rng, 6, 64, 48)
