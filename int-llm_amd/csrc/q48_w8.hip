@@ -482,31 +482,29 @@ __device__ __forceinline__ void dma_tile(const uint8_t *from, uint8_t *to)
 constexpr int GT = 128;                  // weight rows (EPI 1: half of each matrix) and rows a block
 constexpr int GSTAGE = 2 * GT * 64;      // bytes of a stage: 64 columns of both
 
-// A block 128 weight rows x 128 rows, eight waves.  Tiles of both operands go to a ring of
-// four LDS stages by DMA, 1 KB a wave and instruction, three stages ahead; the matrix
+// A block 128 weight rows x 128 rows, four waves of 64 x 64.  Tiles of both operands go to a
+// ring of three LDS stages by DMA, 1 KB a wave and instruction, two stages ahead; the matrix
 // instruction's first operand is the rows, so that a lane holds one weight row and stores of
-// a wave are 256 contiguous bytes.  The sums leave the registers through LDS, so that one
-// loop of the epilogue's code serves all of them.
-// KS 1: waves of 64 x 32, two blocks and four waves a SIMD: a wave alone there issues every
-// other turn at most, and the epilogue is more work than the products.  KS 2, where there is
-// at most a block a compute unit: two groups of four waves of 64 x 64, each over half of the
-// columns with a ring of its own, that share the epilogue.
+// a wave are 256 contiguous bytes.  The sums leave the registers through LDS, half of the
+// rows at a time, so that one loop of the epilogue's code serves all of them.
+// KS 1: three blocks a compute unit; a wave alone on its SIMD issues every other turn at
+// most, and the epilogue is as much work as the products.  KS 2, where there is at most a
+// block a compute unit: two groups of four waves, each over half of the columns with a ring
+// of its own, that share the epilogue.
 template <int EPI, bool EXPERTS, int KS>
-__global__ __launch_bounds__(512, KS == 1 ? 4 : 2) void k_w8_gemm(W8Mul m, int nx, int ny)
+__global__ __launch_bounds__(256 * KS, KS == 1 ? 3 : 2) void k_w8_gemm(W8Mul m, int nx, int ny)
 {
     q48_round_down();
     constexpr int CH = EPI == 1 ? GT / 2 : GT;   // weight rows of one matrix
-    constexpr int WPG = 8 / KS;                  // waves of a group
-    constexpr int RB = 4 / (WPG / 2);            // blocks of 32 rows a wave
-    constexpr int TPW = 16 / WPG;                // tiles of a stage a wave moves
+    constexpr int WPG = 4;                       // waves of a group
+    constexpr int TPW = GSTAGE / 1024 / WPG;     // tiles of it a wave moves
     // apart, so that the compiler sees that a stage's reads do not wait for another's DMA
-    __shared__ __align__(16) uint8_t r0[KS * GSTAGE], r1[KS * GSTAGE], r2[KS * GSTAGE],
-        r3[KS * GSTAGE];
+    __shared__ __align__(16) uint8_t r0[KS * GSTAGE], r1[KS * GSTAGE], r2[KS * GSTAGE];
     __shared__ double sd[GT];
     __shared__ int toks[EXPERTS ? GT : 1];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int q = wave / WPG, w = wave % WPG, wc = w & 1, r_w = (w >> 1) * 32 * RB;   // its rows
+    const int q = wave / WPG, w = wave % WPG, wc = w & 1, r_w = (w >> 1) * 64;   // its rows
     // blocks of one die (every eighth) take neighbouring tiles, the rows' fastest
     const int per = (nx * ny + 7) >> 3, at = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
     if ((int)(blockIdx.x >> 3) >= per || at >= nx * ny)
@@ -525,6 +523,7 @@ __global__ __launch_bounds__(512, KS == 1 ? 4 : 2) void k_w8_gemm(W8Mul m, int n
     const int KT = (m.KT + KS - 1) / KS;        // steps of a group; of the last one, its own
     const int kt0 = q * KT, mine_kt = KS == 1 ? KT : min(KT, m.KT - kt0);
     const int n0 = bx * CH, ntile = (m.N + 15) / 16;
+    int64_t mine_step = 0;   // in LDS behind the first DMA
     if (tid < GT) {
         const int r = min(tid, rows - 1);
         int64_t step;
@@ -535,7 +534,7 @@ __global__ __launch_bounds__(512, KS == 1 ? 4 : 2) void k_w8_gemm(W8Mul m, int n
         } else {
             step = m.sb[row0 + r];
         }
-        sd[tid] = w8_step_double(step);
+        mine_step = step;
     }
     // row t of the wave's, in sb and base; rows past the block's last: that one
     auto row_of = [&](int t) {
@@ -574,113 +573,73 @@ __global__ __launch_bounds__(512, KS == 1 ? 4 : 2) void k_w8_gemm(W8Mul m, int n
         for (int j = 0; j < TPW; ++j)
             dma_tile(src[j] + (size_t)k * 1024, to + j * 1024);
     };
-    v16i acc[2][RB] = {};
+    v16i acc[2][2] = {};
     // rows l % 32 of a pair of tiles, columns 16 (l / 32) on
     const int mine = ((lane & 31) >> 4) * 1024 + (lane >> 5) * 256 + (lane & 15) * 16;
-    // a stage's operands: [pair][half of the columns], of the weights and of the rows
-    struct Opnd {
-        v4i a[2][2], b[RB][2];
-    };
-    auto read = [&](const uint8_t(&stage)[KS * GSTAGE], Opnd &o) {
+    auto step = [&](const uint8_t(&stage)[KS * GSTAGE]) {
         const uint8_t *st = stage + q * GSTAGE + mine;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int g = 0; g < RB; ++g)
-                o.b[g][h] = *(const v4i *)(st + (8 + r_w / 16 + 2 * g) * 1024 + h * 512);
-#pragma unroll
-            for (int f = 0; f < 2; ++f) {
-                const int ta = EPI == 1 ? 4 * f + 2 * wc : 4 * wc + 2 * f;
-                o.a[f][h] = *(const v4i *)(st + ta * 1024 + h * 512);
-            }
-        }
-    };
-    auto multiply = [&](const Opnd &o) {
+        v4i a[2][2], b[2][2];   // [pair][half of the columns], of the weights and of the rows
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int g = 0; g < RB; ++g)
+            for (int f = 0; f < 2; ++f) {
+                const int ta = EPI == 1 ? 4 * f + 2 * wc : 4 * wc + 2 * f;
+                a[f][h] = *(const v4i *)(st + ta * 1024 + h * 512);
+                b[f][h] = *(const v4i *)(st + (8 + r_w / 16 + 2 * f) * 1024 + h * 512);
+            }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
 #pragma unroll
                 for (int f = 0; f < 2; ++f)
-                    acc[f][g] =
-                        __builtin_amdgcn_mfma_i32_32x32x32_i8(o.b[g][h], o.a[f][h], acc[f][g], 0, 0, 0);
+                    acc[f][g] = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[g][h], a[f][h], acc[f][g], 0, 0, 0);
     };
     dma(0, r0);
     if (KT > 1)
         dma(1, r1);
-    if (KT > 2)
-        dma(2, r2);
-    Opnd even, odd;
-    wait_vm<0>();
-    lds_barrier();
-    read(r0, even);
-    int k = 0;
-    // Step k: stage k + 1 has arrived, and stage k - 1 is in every wave's registers; the DMA
-    // of k + 3 goes there, and k + 1 is read under the products of k.
-    auto turn = [&](const Opnd &now, const uint8_t(&next)[KS * GSTAGE], Opnd &then,
-                    uint8_t(&free)[KS * GSTAGE]) {
-        wait_vm<TPW>();
-        lds_barrier();
-        dma(k + 3, free);
-        read(next, then);
-        multiply(now);
-        ++k;
-    };
-    // the last ones
-    auto tail = [&](const Opnd &now, const uint8_t(&next)[KS * GSTAGE], Opnd &then,
-                    uint8_t(&free)[KS * GSTAGE]) {
-        if (k >= KT)
-            return;
-        wait_vm<0>();
-        lds_barrier();
-        if (k + 3 < KT)
-            dma(k + 3, free);
-        if (k + 1 < KT)
-            read(next, then);
-        if (KS == 1 || k < mine_kt)
-            multiply(now);
-        ++k;
-    };
-    while (k + 6 < KT) {
-        turn(even, r1, odd, r3);
-        turn(odd, r2, even, r0);
-        turn(even, r3, odd, r1);
-        turn(odd, r0, even, r2);
-    }
-    tail(even, r1, odd, r3);
-    tail(odd, r2, even, r0);
-    tail(even, r3, odd, r1);
-    tail(odd, r0, even, r2);
-    tail(even, r1, odd, r3);
-    tail(odd, r2, even, r0);
-    lds_barrier();
-    // of wave i: [pair of weight rows][row][weight row]
-    constexpr int ROWS = 32 * RB, WORDS = 2 * ROWS * 32;
-    auto sums_of = [&](int i) {
-        uint8_t *r = i < 2 ? r0 : i < 4 ? r1 : i < 6 ? r2 : r3;
-        return (int *)r + (i & 1) * WORDS;
-    };
-    static_assert(2 * 4 * WORDS == KS * GSTAGE, "two waves' sums a stage");
-    int *own = sums_of(wave);
-    // lane l, register i: row 8 (i / 4) + 4 (l / 32) + i % 4, weight row l % 32
-#pragma unroll
-    for (int f = 0; f < 2; ++f)
-#pragma unroll
-        for (int g = 0; g < RB; ++g)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                own[(f * ROWS + 32 * g + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3)) * 32 + (lane & 31)] =
-                    acc[f][g][i];
-    if constexpr (KS > 1)
-        lds_barrier();
-    else
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own words
-    const int *part0 = sums_of(w), *part1 = sums_of(KS > 1 ? WPG + w : w);
-    auto sum = [&](int o) { return KS > 1 ? part0[o] + part1[o] : part0[o]; };
     const int64_t *sw = m.sw + (size_t)expert * m.N, *sw2 = m.sw2 + (size_t)expert * m.N;
     const int n = n0 + (EPI == 1 ? 32 * wc + (lane & 31) : 64 * wc + lane);
     const bool in = n < m.N;
     const int64_t s1 = in ? sw[n] : 0, s2 = in && EPI == 1 ? sw2[n] : 0;
+    if (tid < GT)
+        sd[tid] = w8_step_double(mine_step);
+    int k = 0;
+    // Step k: its stage has arrived, and every wave is done with the last one's, which the
+    // DMA of k + 2 takes.
+    auto turn = [&](const uint8_t(&now)[KS * GSTAGE], uint8_t(&free)[KS * GSTAGE]) {
+        wait_vm<TPW>();
+        lds_barrier();
+        dma(k + 2, free);
+        step(now);
+        ++k;
+    };
+    // the last ones
+    auto tail = [&](const uint8_t(&now)[KS * GSTAGE], uint8_t(&free)[KS * GSTAGE]) {
+        if (k >= KT)
+            return;
+        wait_vm<0>();
+        lds_barrier();
+        if (k + 2 < KT)
+            dma(k + 2, free);
+        if (KS == 1 || k < mine_kt)
+            step(now);
+        ++k;
+    };
+    while (k + 4 < KT) {
+        turn(r0, r2);
+        turn(r1, r0);
+        turn(r2, r1);
+    }
+    tail(r0, r2);
+    tail(r1, r0);
+    tail(r2, r1);
+    tail(r0, r2);
+    // of wave i: [pair of weight rows][row][weight row]
+    auto sums_of = [&](int i) { return (int *)((i < 2 * KS ? r0 : r1) + i % (2 * KS) * 8192); };
+    int *own = sums_of(wave);
+    const int *part0 = sums_of(w), *part1 = sums_of(KS > 1 ? WPG + w : w);
+    auto sum = [&](int o) { return KS > 1 ? part0[o] + part1[o] : part0[o]; };
     const double d1 = w8_step_double(s1) * 0x1p-48, d2 = w8_step_double(s2) * 0x1p-48;
     // U outputs a turn: chains of FP64 operations side by side
     constexpr int U = EPI == 1 ? 2 : 8, PER = EPI == 1 ? 2 : 1;   // rows of a wave at once
@@ -694,16 +653,36 @@ __global__ __launch_bounds__(512, KS == 1 ? 4 : 2) void k_w8_gemm(W8Mul m, int n
                 for (int j = 0; j < U; ++j)
                     add[j] = m.base[(size_t)row_of(t0 + j) * m.N + n];
     };
-    const int begin = 32 * q, last = min(begin + 32, rows - r_w);
-    base(begin);
+#pragma nounroll
+    for (int half = 0; half < 2; ++half) {
+        lds_barrier();   // the ring, or the other half's sums, are done with
+        // lane l, register i: row 8 (i / 4) + 4 (l / 32) + i % 4, weight row l % 32
+        auto put = [&](const v16i(&s)[2][2], int g) {
+#pragma unroll
+            for (int f = 0; f < 2; ++f)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    own[(f * 32 + 8 * (i >> 2) + 4 * (lane >> 5) + (i & 3)) * 32 + (lane & 31)] = s[f][g][i];
+        };
+        if (half)
+            put(acc, 1);
+        else
+            put(acc, 0);
+        // (a group's share of the rows)
+        const int begin = 32 * half + 32 / KS * q, last = min(begin + 32 / KS, rows - r_w);
+        base(begin);
+        if constexpr (KS > 1)
+            lds_barrier();
+        else
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the wave's own words
 #pragma nounroll
         for (int t0 = begin; t0 < last; t0 += U * PER) {
             double y[U], up[EPI == 1 ? U : 1];
             bool ok = true;
-            // output j's sum (up's lies 32 ROWS words on)
+            // output j's sum (up's lies 1024 words on)
             auto at_of = [&](int j) {
-                const int t = t0 + PER * j + first;   // (past the last: of other rows)
-                return t * 32 + (lane & 31) + (EPI == 1 ? 0 : (lane >> 5) * 32 * ROWS);
+                const int t = t0 - 32 * half + PER * j + first;   // (past the last: of other rows)
+                return t * 32 + (lane & 31) + (EPI == 1 ? 0 : (lane >> 5) * 1024);
             };
 #pragma unroll
             for (int j = 0; j < U; ++j) {
@@ -712,7 +691,7 @@ __global__ __launch_bounds__(512, KS == 1 ? 4 : 2) void k_w8_gemm(W8Mul m, int n
                 y[j] = w8_scaled_double(sum(at_of(j)), sa, d1, sure);
                 ok &= sure;
                 if constexpr (EPI == 1) {
-                    up[j] = w8_scaled_double(sum(32 * ROWS + at_of(j)), sa, d2, sure);
+                    up[j] = w8_scaled_double(sum(1024 + at_of(j)), sa, d2, sure);
                     ok &= sure;
                 }
             }
@@ -733,7 +712,7 @@ __global__ __launch_bounds__(512, KS == 1 ? 4 : 2) void k_w8_gemm(W8Mul m, int n
                     const int64_t sa = m.sb[row_of(t0 + PER * j + first)];
                     int64_t z = w8_scaled(sum(at_of(j)), sa, s1);
                     if constexpr (EPI == 1)
-                        z = q48_mul(q48_silu(z), w8_scaled(sum(32 * ROWS + at_of(j)), sa, s2));
+                        z = q48_mul(q48_silu(z), w8_scaled(sum(1024 + at_of(j)), sa, s2));
 #pragma unroll
                     for (int i = 0; i < U; ++i)
                         v[i] = i == j ? z : v[i];
@@ -758,6 +737,7 @@ __global__ __launch_bounds__(512, KS == 1 ? 4 : 2) void k_w8_gemm(W8Mul m, int n
                     m.Y[row * m.N + n] = v[j];
             }
         }
+    }
 }
 
 int launch_rc(int e) { return e == (int)hipSuccess ? Q48_OK : Q48_EHIP; }
@@ -926,7 +906,7 @@ int q48_launch_w8_mul(q48_ctx *c, const W8Mul &m, int epi, bool experts, int n_i
         const dim3 grid((unsigned)((gx * gy + 7) / 8 * 8));
         const bool halves = gx * gy <= c->cu_count && m.KT >= 8;
 #define W8_GEMM(EPI, EX, KS)                                                              \
-    hipLaunchKernelGGL((k_w8_gemm<EPI, EX, KS>), grid, dim3(512), 0, c->stream, m, gx, gy)
+    hipLaunchKernelGGL((k_w8_gemm<EPI, EX, KS>), grid, dim3(256 * KS), 0, c->stream, m, gx, gy)
         if (experts && epi == 1)
             W8_GEMM(1, true, 1);
         else if (experts)
