@@ -96,6 +96,9 @@ __device__ __forceinline__ void moe_slots(const MoeSlots &s, const int *chosen,
 {
     __shared__ int count[W8_MAX_COUNT], first[W8_MAX_COUNT], item[W8_MAX_COUNT];
     const int tid = threadIdx.x, lane = tid & 63;
+    // a thread's first pair, fetched once
+    const int e0 = tid < pairs ? from_all(chosen + tid) : 0;
+    const int64_t w0 = tid < pairs ? from_all(weight + tid) : 0;
     for (int i = tid; i < E; i += NT)
         count[i] = 0;
     for (int i = tid; i < s.slots; i += NT)
@@ -103,13 +106,15 @@ __device__ __forceinline__ void moe_slots(const MoeSlots &s, const int *chosen,
     for (int i = tid; i < s.n_items; i += NT)
         s.items[i] = make_int4(0, 0, 0, 0);
     __syncthreads();
-    for (int i = tid; i < pairs; i += NT)
-        atomicAdd(&count[from_all(chosen + i)], 1);
+    for (int i = tid; i < pairs; i += NT) {
+        const int e = i == tid ? e0 : from_all(chosen + i);
+        atomicAdd(&count[e], 1);
+    }
     __syncthreads();
     if (tid < 64) {   // slots (in sixteens) and items before each expert: sums over a wave
         int slots = 0, items = 0;
-        for (int e0 = 0; e0 < E; e0 += 64) {
-            const int c = e0 + lane < E ? count[e0 + lane] : 0;
+        for (int b = 0; b < E; b += 64) {
+            const int c = b + lane < E ? count[b + lane] : 0;
             const int n = (c + 15) & ~15, k = (c + s.rows - 1) / s.rows;
             int sn = n, sk = k;
             for (int d = 1; d < 64; d <<= 1) {
@@ -117,9 +122,9 @@ __device__ __forceinline__ void moe_slots(const MoeSlots &s, const int *chosen,
                 sn += lane >= d ? on : 0;
                 sk += lane >= d ? ok : 0;
             }
-            if (e0 + lane < E) {
-                first[e0 + lane] = slots + sn - n;
-                item[e0 + lane] = items + sk - k;
+            if (b + lane < E) {
+                first[b + lane] = slots + sn - n;
+                item[b + lane] = items + sk - k;
             }
             slots += __builtin_amdgcn_readlane(sn, 63);
             items += __builtin_amdgcn_readlane(sk, 63);
@@ -134,9 +139,9 @@ __device__ __forceinline__ void moe_slots(const MoeSlots &s, const int *chosen,
     }
     __syncthreads();
     for (int i = tid; i < pairs; i += NT) {
-        const int at = atomicAdd(&count[from_all(chosen + i)], 1);
+        const int at = atomicAdd(&count[i == tid ? e0 : from_all(chosen + i)], 1);
         s.tok[at] = i / top;
-        s.w[at] = from_all(weight + i);
+        s.w[at] = i == tid ? w0 : from_all(weight + i);
     }
 }
 
@@ -275,35 +280,43 @@ __global__ __launch_bounds__(1024, J == 8 ? 4 : 8) void k_moe_route(MoeRoute a)
         part[w][0] = (uint64_t)sum;
         part[w][1] = (uint64_t)(sum >> 64);
     }
-    lds_barrier();
+    lds_barrier();   // (the row is done with)
+    int64_t *lg = xs;
+    int *rank = (int *)(xs + E);
+    int64_t mine_l = 0;
     if (tid < n) {
         sum = 0;
         for (int i = 0; i < S; ++i)
             sum += ((q48_u128)part[(tid << sl) + i][1] << 64) | part[(tid << sl) + i][0];
-        out_to_all(a.logits + (size_t)t * E + e0 + tid, (int64_t)(uint64_t)(sum >> 48));
-        __builtin_amdgcn_s_waitcnt(0);   // out before the ticket (n <= 16: one wave's stores)
+        mine_l = (int64_t)(uint64_t)(sum >> 48);
     }
-    if (tid == 0) {
-        const int at = __hip_atomic_fetch_add(a.ticket + 1 + t, 1, __ATOMIC_RELAXED,
-                                              __HIP_MEMORY_SCOPE_AGENT);
-        last = at == G - 1;
-        if (at == G - 1)
-            out_to_all(a.ticket + 1 + t, 0);
+    if (G > 1) {
+        if (tid < n) {
+            out_to_all(a.logits + (size_t)t * E + e0 + tid, mine_l);
+            __builtin_amdgcn_s_waitcnt(0);   // out before the ticket (n <= 16: one wave's stores)
+        }
+        if (tid == 0) {
+            const int at = __hip_atomic_fetch_add(a.ticket + 1 + t, 1, __ATOMIC_RELAXED,
+                                                  __HIP_MEMORY_SCOPE_AGENT);
+            last = at == G - 1;
+            if (at == G - 1)
+                out_to_all(a.ticket + 1 + t, 0);
+        }
+        __syncthreads();
+        if (!last)
+            return;
+        if (tid < E)
+            mine_l = from_all(a.logits + (size_t)t * E + tid);
     }
-    __syncthreads();
-    if (!last)
-        return;
     // The token's choice by all threads: an expert's rank is the number of larger logits
     // and of equal ones before it, counted by 1024 / P threads an expert (P: experts to a
     // power of two), and each chosen expert makes its own weight.
     {
         __shared__ int64_t most;
         __shared__ uint64_t z;
-        int64_t *lg = xs;   // (the row is done with)
-        int *rank = (int *)(xs + E);
         const int P = 1 << a.p2, ex = tid & (P - 1), parts = 1024 >> a.p2, part_ = tid >> a.p2;
         if (tid < E) {
-            lg[tid] = from_all(a.logits + (size_t)t * E + tid);
+            lg[tid] = mine_l;
             rank[tid] = 0;
         }
         if (tid == 0)
@@ -361,10 +374,10 @@ size_t slots_of(size_t pairs, int E)
     return (pairs + 15 * (pairs < (size_t)E ? pairs : (size_t)E) + 15) & ~(size_t)15;
 }
 
-// experts a block of k_moe_route, 0 for the separate launches (a row of words in LDS)
+// Experts a block of k_moe_route, 0 for the separate launches (a row of words in LDS): the
+// fewest with which every block, the codes' among them, is resident at once.
 int route_per(const q48_ctx *c, int T, int E, int dim)
 {
-    // the fewest with which every block, the codes' among them, is resident at once
     const int G = T <= c->cu_count ? (dim <= 2048 ? 2 : 1) * c->cu_count / T - 1 : 0;
     const int per = G > 0 ? (E + G - 1) / G : ROUTE_PER + 1;
     return dim <= 6144 && T <= ROUTE_T && per <= ROUTE_PER ? per : 0;

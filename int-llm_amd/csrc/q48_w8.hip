@@ -842,6 +842,8 @@ int q48_launch_w8_rows(q48_ctx *c, const W8Rows &r)
         hipLaunchKernelGGL(k_w8_rows, dim3(r.T), dim3(256), 0, c->stream, r);
     else if (r.T <= c->cu_count && r.K > 2048)
         W8_ROWS(512, 2, 8);
+    else if (r.T <= c->cu_count && r.K > 1024)
+        W8_ROWS(512, 2, 2);
     else if (r.K <= 1024)
         W8_ROWS(256, 4, 1);
     else if (r.K <= 2048)
