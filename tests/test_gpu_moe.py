@@ -68,6 +68,22 @@ def test_sizes(own, dim, ffn, T):  # noqa: F811
     check(own, Layer(rng, 4, dim, ffn), words(rng, T, dim), 2, True)
 
 
+@pytest.mark.parametrize("dim,ffn", [(2049, 40), (4000, 9000), (6144, 33), (6145, 33), (8300, 20)])
+@pytest.mark.parametrize("T", [1, 3])
+def test_long_rows(own, dim, ffn, T):  # noqa: F811
+    rng = np.random.default_rng(dim)
+    X = words(rng, T, dim)
+    X[T - 1, dim // 2] = 40 * W.ONE
+    check(own, Layer(rng, 3, dim, ffn), X, 2, T == 1)
+
+
+@pytest.mark.parametrize("T,E", [(60, 40), (200, 15), (256, 16), (257, 16), (300, 64)])
+def test_where_the_routing_changes(own, T, E):  # noqa: F811
+    """A token's experts in one block, in several, and the separate launches."""
+    rng = np.random.default_rng(E)
+    check(own, Layer(rng, E, 100, 40), words(rng, T, 100), 3, False)
+
+
 @pytest.mark.parametrize("T", [1, 33])
 def test_every_expert_and_many(own, T):  # noqa: F811
     """top_k of all experts; 64 of 1024."""

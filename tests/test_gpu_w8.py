@@ -203,6 +203,107 @@ def test_rows_off_sixteen_bytes(own):
         assert (y.download()[1:].reshape(T, N) == W.product(X, nw, codes, steps, b)).all()
 
 
+def test_weights_off_sixteen_bytes(own):
+    rng = np.random.default_rng(10)
+    for N, K in ((21, 300), (9, 2047), (17, 3001), (3, 4097)):
+        x = words(rng, N, K)
+        c, s = W.quantise(x)
+        w = own.new_w8(1, N, K)
+        own.w8_pack(w, 0, own.to_device(np.append(0, x)).at(1))
+        out = own.to_device(np.full(N * K + 2, 5))
+        own.w8_values(out.at(1), w, 0)
+        got = out.download()
+        assert got[0] == 5 and got[-1] == 5
+        assert (got[1:-1].reshape(N, K) == W.values(c, s)).all()
+
+
+@pytest.mark.parametrize("K", [2049, 4096, 4097, 6145, 8192, 8193, 9000])
+@pytest.mark.parametrize("T", [1, 5, 300])
+def test_long_rows(own, T, K):
+    """Every form that a row's length selects, with an outlier past 32 in some rows."""
+    rng = np.random.default_rng(K)
+    X = words(rng, T, K)
+    X[T // 2, K // 3] = 40 * W.ONE
+    X[T - 1, K - 1] = -(1 << 60)
+    codes, steps = weights(rng, 20, K)
+    check(own, T, 20, K, K % 2 == 0, True, rng, X, codes, steps)
+    w = own.new_w8(1, 20, K)
+    x = words(rng, 20, K, sigma=0.02)
+    own.w8_pack(w, 0, own.to_device(x).ptr)
+    out = own.buffer(20 * K)
+    own.w8_values(out.ptr, w, 0)
+    assert (out.download().reshape(20, K) == W.values(*W.quantise(x))).all()
+
+
+@pytest.mark.parametrize("N,T", [(1, 1100), (17, 2100), (2100, 1000), (4100, 700)])
+def test_tiles_of_many_outputs(own, N, T):
+    """Both forms for many rows, on either side of where they change."""
+    rng = np.random.default_rng(N)
+    check(own, T, N, 90, False, True, rng)
+    X = words(rng, T, 600)
+    gate, up = weights(rng, N, 600), weights(rng, N, 600)
+    out = own.buffer(T * N)
+    own.gemm_w8_swiglu(out.ptr, loaded(own, *gate), loaded(own, *up), own.to_device(X).ptr, None, T)
+    assert (out.download().reshape(T, N) == W.swiglu(X, None, gate, up)).all()
+
+
+def test_on_the_callers_stream():
+    """Rows that torch is still making when the product is enqueued, results that torch
+    reads and rows that it overwrites right behind it."""
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(3)
+    T, N, K = 40, 96, 700
+    codes, steps = weights(rng, N, K)
+    X = words(rng, T, K)
+    want = W.product(X, None, codes, steps)
+    for s in (torch.cuda.default_stream(0), torch.cuda.Stream(0)):
+        with torch.cuda.stream(s), intllm.Context(0, stream=s.cuda_stream) as c:
+            w = loaded(c, codes, steps)
+            y = torch.zeros(T, N, dtype=torch.int64, device="cuda:0")
+            d = torch.zeros(T, K, dtype=torch.int64, device="cuda:0")
+            c.gemm_w8(y.data_ptr(), None, w, d.data_ptr(), None, T)
+            host = torch.from_numpy(X).pin_memory()
+            big = torch.randn(4096, 4096, device="cuda:0")
+            for _ in range(3):
+                for _ in range(4):
+                    big = torch.mm(big, big) * 1e-4
+                d.copy_(host, non_blocking=True)
+                c.gemm_w8(y.data_ptr(), None, w, d.data_ptr(), None, T)
+                got = y + 1
+                d.zero_()
+                y.zero_()
+                assert (got.cpu().numpy() == want + 1).all()
+
+
+def test_two_graphs_share_a_buffer(own):
+    """Two captured products of one context, replayed in turns."""
+    rng = np.random.default_rng(4)
+    lib, c = intllm.hip_lib(), own
+    import ctypes as C
+    codes, steps = weights(rng, 50, 256)
+    w = loaded(c, codes, steps)
+    graphs = []
+    for T in (3, 40):
+        X = words(rng, T, 256)
+        dX, y = c.to_device(X), c.buffer(T * 50)
+        c.gemm_w8(y.ptr, None, w, dX.ptr, None, T)
+        c.sync()
+        intllm.check("capture", lib.q48_graph_capture(c.h))
+        c.gemm_w8(y.ptr, None, w, dX.ptr, None, T)
+        g = C.c_void_p()
+        intllm.check("instantiate", lib.q48_graph_instantiate(c.h, C.byref(g)))
+        graphs.append((g, X, dX, y))
+    for i in range(3):
+        for g, X, dX, y in graphs:
+            dX.upload(X + i)
+            y.upload(np.zeros(y.n, np.int64))
+            intllm.check("replay", lib.q48_graph_replay(c.h, g, 1))
+        for g, X, dX, y in graphs:
+            assert (y.download().reshape(-1, 50) == W.product(X + i, None, codes, steps)).all()
+    for g, *_ in graphs:
+        intllm.check("destroy", lib.q48_graph_destroy(c.h, g))
+
+
 def test_captured_and_replayed(own):
     """Products of one shape as a graph, its inputs changed between replays, eager calls
     of other shapes among them; a shape that was never called is refused in a capture."""
