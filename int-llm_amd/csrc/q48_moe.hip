@@ -206,11 +206,8 @@ __global__ __launch_bounds__(1024, J == 8 ? 4 : 8) void k_moe_route(MoeRoute a)
     if (tid < NT) {
         RowWords<NT, 2, J> x;
         x.load(a.rows.X + (size_t)t * K, K);
-        if constexpr (NORM) {
-            RowWords<NT, 2, J> nw;
-            nw.load(a.rows.norm_w, K);
-            x.norm(nw, K, red);
-        }
+        if constexpr (NORM)
+            x.norm(a.rows.X + (size_t)t * K, a.rows.norm_w, K, red);
         if ((int)blockIdx.x == G) {
             const int KT = (K + 63) / 64;
             const int64_t step = x.quantise(K, KT, peak, [&](int i, uint32_t q) {

@@ -70,11 +70,8 @@ __global__ __launch_bounds__(NT) void k_w8_rows_r(W8Rows a)
         return;
     RowWords<NT, C, J> x;
     x.load(a.X + (size_t)t * K, K);
-    if constexpr (NORM) {
-        RowWords<NT, C, J> nw;
-        nw.load(a.norm_w, K);
-        x.norm(nw, K, red);
-    }
+    if constexpr (NORM)
+        x.norm(a.X + (size_t)t * K, a.norm_w, K, red);
     if (a.xn)
 #pragma unroll
         for (int j = 0; j < J; ++j)
@@ -359,11 +356,8 @@ __global__ __launch_bounds__(ONE_NT) void k_w8_one(W8Mul m, const int64_t *__res
         if (tid < NT) {
             RowWords<NT, 2, J> x;
             x.load(X + (EXPERTS ? (size_t)slot * K : 0), K);
-            if constexpr (SRC == 2) {
-                RowWords<NT, 2, J> nw;
-                nw.load(norm_w, K);
-                x.norm(nw, K, red);
-            }
+            if constexpr (SRC == 2)
+                x.norm(X, norm_w, K, red);
             sb = x.quantise(K, KT, top,
                             [&](int i, uint32_t q) { *(uint16_t *)&codes[i] = (uint16_t)q; });
             if (tid == 0)
@@ -705,7 +699,7 @@ __global__ __launch_bounds__(256 * KS, KS == 1 ? 3 : 2) void k_w8_gemm(W8Mul m, 
             int64_t v[U];
 #pragma unroll
             for (int j = 0; j < U; ++j)
-                v[j] = (int64_t)y[j];
+                v[j] = EPI == 1 ? w8_word51(y[j]) : (int64_t)y[j];
             if (__any(!ok))
 #pragma nounroll
                 for (int j = 0; j < U; ++j) {

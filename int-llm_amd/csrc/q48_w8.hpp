@@ -65,7 +65,7 @@ __device__ __forceinline__ void w8_together(double (&v)[2])
 __device__ __forceinline__ void w8_together(double (&v)[1]) {}
 
 // fp_mul(fp_silu(g), u) (fp_math.h:911-921) of U pairs of whole numbers below 2^53, |g| at
-// most 10 (false else), in FP64 rounding down alone.  The squares of fp_exp: the first 12 stay below 2^52 (two operations
+// most 10 (false else, and where the result passes 2^51), in FP64 rounding down alone.  The squares of fp_exp: the first 12 stay below 2^52 (two operations
 // each, q48_exp_small), the last two, of at most e^10 2^48, are a rounded product and its
 // exact remainder each, r = A + T with A a double and T < 2^13.  Rounding down makes the
 // sums behind T too small by less than 2^-39: false is returned where that may hide a whole
@@ -140,9 +140,15 @@ __device__ __forceinline__ bool w8_silu_mul(const double (&g)[U], const double (
     W8_EACH r[j] = c[j] == 0 ? w8_kept(r[j]) : q[j];   // (kept: else a branch around its making)
     W8_EACH y[j] = __builtin_floor(g[j] * r[j]);
     W8_EACH out[j] = __builtin_floor(y[j] * (u[j] * unit));
-    W8_EACH sure &= __builtin_fabs(out[j]) < 0x1p53;
+    W8_EACH sure &= __builtin_fabs(out[j]) < 0x1p51;   // (for w8_word51)
 #undef W8_EACH
     return sure;
+}
+
+// the word of a whole number below 2^51
+__device__ __forceinline__ int64_t w8_word51(double v)
+{
+    return (int64_t)(__builtin_bit_cast(uint64_t, v + 0x1.8p52) - 0x4338000000000000ull);
 }
 
 // One product, and one SwiGLU of two, of steps in words
@@ -160,7 +166,7 @@ __device__ __forceinline__ int64_t w8_swiglu(int Sg, int Su, int64_t sa, int64_t
     const double u[1] = {w8_scaled_double(Su, a, w8_step_double(su) * 0x1p-48, s2)};
     double y[1];
     if (w8_silu_mul<1>(g, u, y) & s1 & s2)
-        return (int64_t)y[0];
+        return w8_word51(y[0]);
     return q48_mul(q48_silu(w8_scaled(Sg, sa, sg)), w8_scaled(Su, sa, su));
 }
 
@@ -285,9 +291,12 @@ struct RowWords {
         return dbl ? (int64_t)v[j][c].d : v[j][c].i;
     }
 
-    // rmsnorm (llama_int.c:1048-1058) of the row by weights g; red: two words a wave
-    __device__ __forceinline__ void norm(const RowWords &g, int K, uint64_t (*red)[2])
+    // rmsnorm (llama_int.c:1048-1058) of the row x that was loaded, by weights w; red: two
+    // words a wave
+    __device__ __forceinline__ void norm(const int64_t *x, const int64_t *w, int K, uint64_t (*red)[2])
     {
+        RowWords g;
+        g.load(w, K);
         // squares of halves of 27 and 26 bits, three sums without a carry; of any words in
         // 128 bits
         uint32_t big = 0;
@@ -322,19 +331,18 @@ struct RowWords {
         const int64_t rl = low > 0 ? r & (((int64_t)1 << low) - 1) : 0;
         const double rh = (double)(r - rl) * 0x1p-48, rd = (double)rl * 0x1p-48;
         double m = 0;
-        double d[J][C];
         each(K, [&](int j, int c) {
-            const double x = (double)v[j][c].i, w = (double)g.v[j][c].i;
-            const double y = __builtin_floor(__builtin_fma(x, rh, x * rd));
-            d[j][c] = __builtin_floor(y * (w * 0x1p-48));
+            const double a = (double)v[j][c].i, b = (double)g.v[j][c].i;
+            const double y = __builtin_floor(__builtin_fma(a, rh, a * rd));
+            v[j][c].d = __builtin_floor(y * (b * 0x1p-48));
             m = __builtin_fmax(__builtin_fmax(m, __builtin_fabs(y)),
-                               __builtin_fmax(__builtin_fabs(w), __builtin_fabs(d[j][c])));
+                               __builtin_fmax(__builtin_fabs(b), __builtin_fabs(v[j][c].d)));
         });
         dbl = fits && !__any(m >= LIM);
-        if (dbl)
-            each(K, [&](int j, int c) { v[j][c].d = d[j][c]; });
-        else
+        if (!dbl) {   // the words once more
+            load(x, K);
             each(K, [&](int j, int c) { v[j][c].i = q48_mul(q48_mul(v[j][c].i, r), g.v[j][c].i); });
+        }
     }
 
     // The row's step; store(i, codes) gets C codes from column i on, bytes of an integer,
