@@ -186,6 +186,7 @@ struct MoeRoute {
     const int64_t *router;
     int64_t *logits;
     int E, per, sl, p2, top, renorm;   // p2: 2^p2 >= E, at least 64
+    int one;                     // T = 1 and k_w8_one behind it: every choice an item of one slot
     int *chosen;
     int64_t *weight;
     int *ticket;                 // [0]: tokens, [1 + t]: blocks of token t; zeros between launches
@@ -340,14 +341,14 @@ __global__ __launch_bounds__(1024, J == 8 ? 4 : 8) void k_moe_route(MoeRoute a)
             const int64_t wt = q48_div(ew, (int64_t)z);
             out_to_all(a.chosen + (size_t)t * a.top + my, tid);
             out_to_all(a.weight + (size_t)t * a.top + my, wt);
-            if (T == 1) {   // every choice an item of one slot
+            if (a.one) {
                 a.s.items[my] = make_int4(tid, 16 * my, 1, 0);
                 a.s.tok[16 * my] = 0;
                 a.s.w[16 * my] = wt;
             }
         }
     }
-    if (T == 1)
+    if (a.one)
         return;
     __builtin_amdgcn_s_waitcnt(0);   // every wave's stores are out before the ticket
     __syncthreads();
@@ -489,6 +490,7 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
         int *tok = (int *)(ws + o_t);
         int64_t *sw = (int64_t *)(ws + o_sw);
         const MoeSlots s = {items, tok, sw, sl, it, rows};
+        const bool one = n == 1 && q48_w8_one_ok(ffn);   // every item a slot
         const int per = route_per(c, n, E, dim);
         if (per) {
             int spl = 4;
@@ -497,8 +499,8 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
             int p2 = 6;
             while ((1 << p2) < E)
                 ++p2;
-            const MoeRoute a = {r, moe->router, lg, E, per, spl, p2, top, moe->renorm, ch, wt,
-                                (int *)ws, s};
+            const MoeRoute a = {r, moe->router, lg, E, per, spl, p2, top, moe->renorm, one, ch,
+                                wt, (int *)ws, s};
             rc = launch_route(c, a);
         } else {
             if ((rc = q48_launch_w8_rows(c, r)))
@@ -541,7 +543,6 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
         m.items = items;
         m.slot_tok = tok;
         m.slot_w = sw;
-        const bool one = n == 1 && q48_w8_one_ok(ffn);   // every item a slot
         if ((rc = one ? q48_launch_w8_one(c, m, 1, nullptr, nullptr, dim, top)
                       : q48_launch_w8_mul(c, m, 1, true, it)))
             return launch_rc(rc);

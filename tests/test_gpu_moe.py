@@ -77,6 +77,18 @@ def test_long_rows(own, dim, ffn, T):  # noqa: F811
     check(own, Layer(rng, 3, dim, ffn), X, 2, T == 1)
 
 
+@pytest.mark.parametrize("top", [2, 16])
+def test_a_token_of_long_hidden_rows_in_a_used_buffer(own, top):  # noqa: F811
+    """Hidden rows too long for the form of one token, where an earlier call left the
+    buffer full of other words: no slot and no item of it may be taken for one of now."""
+    rng = np.random.default_rng(top)
+    big = loaded(own, *weights(rng, 16, 2048))
+    X = rng.integers(-2 ** 62, 2 ** 62, (12000, 2048))
+    Y = own.buffer(12000 * 16)
+    own.gemm_w8(Y.ptr, None, big, own.to_device(X).ptr, None, 12000)
+    check(own, Layer(rng, 16, 48, 8300), words(rng, 1, 48), top, True)
+
+
 @pytest.mark.parametrize("T,E", [(60, 40), (200, 15), (256, 16), (257, 16), (300, 64)])
 def test_where_the_routing_changes(own, T, E):  # noqa: F811
     """A token's experts in one block, in several, and the separate launches."""
