@@ -93,7 +93,7 @@ __global__ __launch_bounds__(NT) void k_w8_rows_r(W8Rows a)
         a.step[t] = step;
 }
 
-// A block a row of weights: step and codes, or codes and steps as they come.
+// A row of weights at a time: step and codes, or codes and steps as they come.
 __global__ __launch_bounds__(256) void k_w8_pack(uint8_t *__restrict__ codes,
                                                 int64_t *__restrict__ steps,
                                                 const int64_t *__restrict__ W,
@@ -103,28 +103,30 @@ __global__ __launch_bounds__(256) void k_w8_pack(uint8_t *__restrict__ codes,
 {
     q48_round_down();
     __shared__ uint64_t red[4];
-    const int n = blockIdx.x, tid = threadIdx.x, KT = (K + 63) / 64;
-    uint64_t m = 0, step = 0;
-    double rc = 0;
-    if (n < N) {
-        if (W) {
-            for (int i = tid; i < K; i += 256) {
-                const uint64_t g = q48_magnitude(W[(size_t)n * K + i]);
-                m = g > m ? g : m;
+    const int tid = threadIdx.x, KT = (K + 63) / 64;
+    for (int n = blockIdx.x; n < ((N + 15) & ~15); n += gridDim.x) {
+        uint64_t m = 0, step = 0;
+        double rc = 0;
+        if (n < N) {
+            if (W) {
+                for (int i = tid; i < K; i += 256) {
+                    const uint64_t g = q48_magnitude(W[(size_t)n * K + i]);
+                    m = g > m ? g : m;
+                }
+                step = w8_step(block_umax(m, red), rc);
+            } else {
+                step = from_step[n] < 0 ? 0 : (uint64_t)from_step[n];
             }
-            step = w8_step(block_umax(m, red), rc);
-        } else {
-            step = from_step[n] < 0 ? 0 : (uint64_t)from_step[n];
+            if (tid == 0)
+                steps[n] = (int64_t)step;
         }
-        if (tid == 0)
-            steps[n] = (int64_t)step;
-    }
-    for (int i = tid; i < KT * 64; i += 256) {
-        int q = 0;
-        if (n < N && i < K)
-            q = W ? step ? q48_code<127>(W[(size_t)n * K + i], step, rc) : 0
-                  : from[(size_t)n * K + i];
-        codes[w8_at(n, i, KT)] = (uint8_t)q;
+        for (int i = tid; i < KT * 64; i += 256) {
+            int q = 0;
+            if (n < N && i < K)
+                q = W ? step ? q48_code<127>(W[(size_t)n * K + i], step, rc) : 0
+                      : from[(size_t)n * K + i];
+            codes[w8_at(n, i, KT)] = (uint8_t)q;
+        }
     }
 }
 
@@ -987,9 +989,9 @@ static int w8_fill(q48_ctx *c, const q48_w8 *w, int index, const int64_t *W, con
         hipLaunchKernelGGL(k_w8_pack_r<16>, eights, dim3(512), 0, c->stream, to, st, W, N, K);
     else if (W && K <= 4096)
         hipLaunchKernelGGL(k_w8_pack_r<32>, eights, dim3(512), 0, c->stream, to, st, W, N, K);
-    else
-        hipLaunchKernelGGL(k_w8_pack, dim3((N + 15) / 16 * 16), dim3(256), 0, c->stream, to, st, W,
-                           codes, steps, N, K);
+    else   // (a launch holds fewer than 2^32 threads: N may be 2^24)
+        hipLaunchKernelGGL(k_w8_pack, dim3(min((N + 15) / 16 * 16, 1 << 20)), dim3(256), 0, c->stream,
+                           to, st, W, codes, steps, N, K);
     return launch_rc((int)hipGetLastError());
 }
 

@@ -72,6 +72,20 @@ def test_weights_from_words(own, N, K):
     assert (got[:-1].reshape(N, K) == W.values(c, s)).all() and got[-1] == 5
 
 
+@pytest.mark.parametrize("N", [1 << 24, (1 << 20) + 5])
+def test_the_most_rows(own, N):
+    """Codes put and read back, and a token's product, with as many rows as there may be."""
+    rng = np.random.default_rng(7)
+    codes, steps = rng.integers(-128, 128, (N, 1)).astype(np.int8), rng.integers(0, 1 << 40, N)
+    w = loaded(own, codes, steps)
+    out = own.buffer(N)
+    own.w8_values(out.ptr, w, 0)
+    assert (out.download() == codes[:, 0].astype(np.int64) * steps).all()
+    own.gemm_w8(out.ptr, None, w, own.to_device(np.array([127 << 48])).ptr, None, 1)
+    # 127 2^48: the code 127 and the step 2^48
+    assert (out.download() == 127 * codes[:, 0].astype(np.int64) * steps).all()
+
+
 def test_one_of_several_matrices(own):
     """The others stay as they are."""
     rng = np.random.default_rng(1)
