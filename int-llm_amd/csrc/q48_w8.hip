@@ -699,9 +699,13 @@ __global__ __launch_bounds__(256 * KS, KS == 1 ? 3 : 2) void k_w8_gemm(W8Mul m, 
                     y[j] = z[j];
             }
             int64_t v[U];
+            if constexpr (EPI == 1) {
+                w8_words<U>(y, v);
+            } else {
 #pragma unroll
-            for (int j = 0; j < U; ++j)
-                v[j] = EPI == 1 ? w8_word51(y[j]) : (int64_t)y[j];
+                for (int j = 0; j < U; ++j)
+                    v[j] = (int64_t)y[j];
+            }
             if (__any(!ok))
 #pragma nounroll
                 for (int j = 0; j < U; ++j) {

@@ -64,14 +64,15 @@ __device__ __forceinline__ void w8_together(double (&v)[2])
 }
 __device__ __forceinline__ void w8_together(double (&v)[1]) {}
 
-// fp_mul(fp_silu(g), u) (fp_math.h:911-921) of U pairs of whole numbers below 2^53, |g| at
-// most 10 (false else, and where the result passes 2^51), in FP64 rounding down alone.  The squares of fp_exp: the first 12 stay below 2^52 (two operations
-// each, q48_exp_small), the last two, of at most e^10 2^48, are a rounded product and its
-// exact remainder each, r = A + T with A a double and T < 2^13.  Rounding down makes the
-// sums behind T too small by less than 2^-39: false is returned where that may hide a whole
-// number (q48_silu then).  A quotient by A + T: an estimate as in q48_recip, its remainder
-// 2^96 - q A exact (a multiple of A's last place, below 2^53 of them) and compared with A +
-// (q + 1) T, whose product is below 2^53.  About 90 operations (with 64-bit integers for the
+// fp_mul(fp_silu(g), u) (fp_math.h:911-921) of U pairs of whole numbers below 2^53 in FP64
+// rounding down alone; false where the result passes 2^53.  The squares of fp_exp: the first
+// 12 stay below 2^52 (two operations each, q48_exp_small), the last two, of at most e^10
+// 2^48, are a rounded product and its exact remainder each, r = A + T with A a double and
+// T < 2^13.  Rounding down makes the sums behind T too small by less than 2^-39: false is
+// returned where that may hide a whole number (q48_silu then).  A quotient by A + T: an
+// estimate as in q48_recip, its remainder 2^96 - q A exact (a multiple of A's last place,
+// below 2^53 of them) and compared with A + (q + 1) T, whose product is below 2^53.  Past
+// 10 in magnitude the sigmoid is 0 or 1.  About 90 operations (with 64-bit integers for the
 // last squares and the quotients 160, a third of them of quarter rate), step by step for all
 // pairs: one is a chain, and a wave alone on its SIMD waits for each of its links.
 template <int U>
@@ -82,9 +83,9 @@ __device__ __forceinline__ bool w8_silu_mul(const double (&g)[U], const double (
     constexpr double ten = 10 * 0x1p48, unit = 0x1p-48;
     const double m28 = w8_kept(-0x1p28), p52 = w8_kept(0x1p52), r24 = w8_kept(0x1p-24);
     double h[U], y[U], A[U], T[U], r[U], q[U], c[U];
-    bool sure = true;
-    W8_EACH sure &= __builtin_fabs(g[j]) <= ten;
-    W8_EACH h[j] = __builtin_fma(__builtin_fabs(g[j]), 0x1p-14, p52 + 0x1p48);
+    bool sure = true, far = false;
+    W8_EACH far |= __builtin_fabs(g[j]) > ten;
+    W8_EACH h[j] = __builtin_fma(__builtin_fmin(__builtin_fabs(g[j]), ten), 0x1p-14, p52 + 0x1p48);
 #pragma unroll
     for (int k = 0; k < 12; ++k) {
         W8_EACH y[j] = __builtin_fma(h[j], r24, m28);
@@ -138,17 +139,32 @@ __device__ __forceinline__ bool w8_silu_mul(const double (&g)[U], const double (
     W8_EACH h[j] = r[j] + unit;
     W8_EACH r[j] = __builtin_fma(-h[j], A[j], 1.0) >= 0 ? h[j] : r[j];
     W8_EACH r[j] = c[j] == 0 ? w8_kept(r[j]) : q[j];   // (kept: else a branch around its making)
+    if (__any(far))
+        W8_EACH r[j] = g[j] > ten ? 1.0 : g[j] < -ten ? 0.0 : r[j];
     W8_EACH y[j] = __builtin_floor(g[j] * r[j]);
     W8_EACH out[j] = __builtin_floor(y[j] * (u[j] * unit));
-    W8_EACH sure &= __builtin_fabs(out[j]) < 0x1p51;   // (for w8_word51)
+    W8_EACH sure &= __builtin_fabs(out[j]) < 0x1p53;
 #undef W8_EACH
     return sure;
 }
 
-// the word of a whole number below 2^51
-__device__ __forceinline__ int64_t w8_word51(double v)
+// The words of whole numbers below 2^63: by their bits where a wave's are below 2^51
+template <int U>
+__device__ __forceinline__ void w8_words(const double (&v)[U], int64_t (&w)[U])
 {
-    return (int64_t)(__builtin_bit_cast(uint64_t, v + 0x1.8p52) - 0x4338000000000000ull);
+    bool wide = false;
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+        wide |= __builtin_fabs(v[j]) >= 0x1p51;
+    if (__any(wide)) {
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+            w[j] = (int64_t)v[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+            w[j] = (int64_t)(__builtin_bit_cast(uint64_t, v[j] + 0x1.8p52) - 0x4338000000000000ull);
+    }
 }
 
 // One product, and one SwiGLU of two, of steps in words
@@ -165,8 +181,11 @@ __device__ __forceinline__ int64_t w8_swiglu(int Sg, int Su, int64_t sa, int64_t
     const double g[1] = {w8_scaled_double(Sg, a, w8_step_double(sg) * 0x1p-48, s1)};
     const double u[1] = {w8_scaled_double(Su, a, w8_step_double(su) * 0x1p-48, s2)};
     double y[1];
-    if (w8_silu_mul<1>(g, u, y) & s1 & s2)
-        return w8_word51(y[0]);
+    if (w8_silu_mul<1>(g, u, y) & s1 & s2) {
+        int64_t w[1];
+        w8_words<1>(y, w);
+        return w[0];
+    }
     return q48_mul(q48_silu(w8_scaled(Sg, sa, sg)), w8_scaled(Su, sa, su));
 }
 

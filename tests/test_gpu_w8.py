@@ -203,6 +203,23 @@ def test_swiglu(own, T, N, K, norm):
     assert (got[:-1].reshape(T, N) == W.swiglu(X, nw, gate, up)).all() and got[-1] == 5
 
 
+@pytest.mark.parametrize("T", [1, 40, 1100])
+def test_swiglu_of_large_gates(own, T):
+    """Gates on either side of 10 in magnitude, where the sigmoid ends; results on either
+    side of 2^51, 2^52 and 2^53."""
+    rng = np.random.default_rng(T)
+    N, K = 3000 if T == 1100 else 70, 130
+    gate, up = weights(rng, N, K, sigma=0.5), weights(rng, N, K, sigma=0.5)
+    X = words(rng, T, K)
+    X[1::3] = X[1::3] // 16
+    want = W.swiglu(X, None, gate, up)
+    size = abs(want.ravel())
+    assert (size < 2 ** 51).any() and (size > 2 ** 51).any() and (size > 2 ** 53).any()
+    out = own.buffer(T * N)
+    own.gemm_w8_swiglu(out.ptr, loaded(own, *gate), loaded(own, *up), own.to_device(X).ptr, None, T)
+    assert (out.download().reshape(T, N) == want).all()
+
+
 def test_rows_off_sixteen_bytes(own):
     """Words on the boundary of a word and no more."""
     rng = np.random.default_rng(9)

@@ -3,7 +3,7 @@ device, against integer arithmetic (no GPU):
 
 1. a scaled product (w8_scaled_double): where it is sure it is the floor, and it is
    sure but for fractions next to 1;
-2. SwiGLU (w8_silu_mul): the same, over the whole of |g| <= 10, whatever first
+2. SwiGLU (w8_silu_mul): the same, past |g| = 10 too, whatever first
    approximations of the two reciprocals within 2^-20 the hardware gives;
 3. a normed word and its code (RowWords).
 """
@@ -81,9 +81,9 @@ def rcp(d, rel):
 
 
 def silu_mul(g, u, rel1, rel2):
-    ok = abs(g) <= 10 * ONE
+    ok = True
     p52, m28, r24 = F(1 << 52), F(-(1 << 28)), F(1, 1 << 24)
-    h = fma(abs(g), F(1, 1 << 14), p52 + ONE)
+    h = fma(min(abs(g), 10 * ONE), F(1, 1 << 14), p52 + ONE)
     for _ in range(12):
         y = fma(h, r24, m28)
         h = fma(y, y, p52)
@@ -119,6 +119,7 @@ def silu_mul(g, u, rel1, rel2):
     h = add(r, UNIT)
     r = h if fma(-h, A, 1) >= 0 else r
     r = r if c == 0 else q
+    r = F(1) if g > 10 * ONE else F(0) if g < -10 * ONE else r
     out = F(math.floor(mul(math.floor(mul(g, r)), F(u) * UNIT)))
     return int(out), ok and abs(out) < 1 << 53
 
@@ -142,8 +143,9 @@ def test_swiglu():
         elif abs(want) < (1 << 53) - 1:
             unsure += 1
     assert unsure < 20
-    for g in (10 * ONE + 1, -10 * ONE - 1):
-        assert not silu_mul(g, ONE, rel(), rel())[1]
+    for g in (10 * ONE + 1, -10 * ONE - 1, (1 << 52) - 1, 1 - (1 << 52), 12 * ONE + 5, -15 * ONE):
+        for u in (ONE, -ONE, 1, -1, 0, ONE // 3):
+            assert silu_mul(g, u, rel(), rel()) == (fp_silu(g) * u >> 48, True), (g, u)
 
 
 def test_silu_squares_remainders():
