@@ -467,9 +467,18 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
     for (size_t t0 = 0; t0 < (size_t)T; t0 += Tc) {
         const int n = (int)(Tc < T - t0 ? Tc : T - t0);
         const int sl = (int)slots_of((size_t)n * top, E);
-        // Slots an item, by an expert's average: weights are read once an item.
-        const size_t mean = (size_t)n * top / E;
-        const int rows = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 256 ? 64 : 128;
+        // Slots an item, by an expert's average: weights are read once an item.  128, in
+        // k_w8_gemm, where that leaves blocks for most of the chip in down's launch too.
+        // us, 32 / 64 / 128 slots: 8 experts of 2048 x 5632, 64 pairs each 162 / 163 / 162,
+        // 128 287 / 285 / 253, 512 815 / 766 / 499; 64 of 2048 x 1024, 16 pairs 175 / 192 /
+        // 183 (16 slots: 172), 32 223 / 226 / 215, 256 894 / 855 / 635; 8 of 1024 x 2816, 64
+        // pairs 57 / 60 / 99, 256 165 / 163 / 177, 512 266 / 257 / 238.
+        const size_t pairs = (size_t)n * top, mean = pairs / E;
+        const size_t blocks = (pairs / 128 + E / 2) * ((dim + 127) / 128);   // of down, expected
+        const int rows = mean <= 16                                                  ? 16
+                         : mean >= 32 && blocks >= (size_t)c->cu_count * 3 / 4 ? 128
+                         : mean <= 32                                          ? 32
+                                                                               : 64;
         const int it = (int)items_of((size_t)n * top, E, rows);
         W8Rows r = {};
         r.codes = ws + o_x;

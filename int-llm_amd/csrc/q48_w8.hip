@@ -496,7 +496,7 @@ __global__ __launch_bounds__(256 * KS, KS == 1 ? 3 : 2) void k_w8_gemm(W8Mul m, 
     constexpr int TPW = GSTAGE / 1024 / WPG;     // tiles of it a wave moves
     // apart, so that the compiler sees that a stage's reads do not wait for another's DMA
     __shared__ __align__(16) uint8_t r0[KS * GSTAGE], r1[KS * GSTAGE], r2[KS * GSTAGE];
-    __shared__ double sd[GT];
+    __shared__ double sd[GT], wd[EPI == 2 ? GT : 1];
     __shared__ int toks[EXPERTS ? GT : 1];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -527,6 +527,8 @@ __global__ __launch_bounds__(256 * KS, KS == 1 ? 3 : 2) void k_w8_gemm(W8Mul m, 
             const int tok = m.slot_tok[row0 + r];
             toks[tid] = tok;
             step = m.sb[EPI == 1 ? max(tok, 0) : row0 + r];
+            if constexpr (EPI == 2)
+                wd[tid] = (double)m.slot_w[row0 + r] * 0x1p-48;
         } else {
             step = m.sb[row0 + r];
         }
@@ -698,14 +700,12 @@ __global__ __launch_bounds__(256 * KS, KS == 1 ? 3 : 2) void k_w8_gemm(W8Mul m, 
                 for (int j = 0; j < U; ++j)
                     y[j] = z[j];
             }
-            int64_t v[U];
-            if constexpr (EPI == 1) {
-                w8_words<U>(y, v);
-            } else {
+            if constexpr (EPI == 2)   // fp_mul by the weight, at most 1
 #pragma unroll
                 for (int j = 0; j < U; ++j)
-                    v[j] = (int64_t)y[j];
-            }
+                    y[j] = __builtin_floor(y[j] * wd[r_w + t0 + j]);
+            int64_t v[U];
+            w8_words<U>(y, v);
             if (__any(!ok))
 #pragma nounroll
                 for (int j = 0; j < U; ++j) {
@@ -713,6 +713,8 @@ __global__ __launch_bounds__(256 * KS, KS == 1 ? 3 : 2) void k_w8_gemm(W8Mul m, 
                     int64_t z = w8_scaled(sum(at_of(j)), sa, s1);
                     if constexpr (EPI == 1)
                         z = q48_mul(q48_silu(z), w8_scaled(sum(1024 + at_of(j)), sa, s2));
+                    if constexpr (EPI == 2)
+                        z = q48_mul(z, m.slot_w[row_of(t0 + j)]);
 #pragma unroll
                     for (int i = 0; i < U; ++i)
                         v[i] = i == j ? z : v[i];
@@ -732,7 +734,7 @@ __global__ __launch_bounds__(256 * KS, KS == 1 ? 3 : 2) void k_w8_gemm(W8Mul m, 
                     continue;
                 if constexpr (EPI == 2)
                     atomicAdd((unsigned long long *)m.Y + (size_t)toks[r_w + t] * m.N + n,
-                              (unsigned long long)q48_mul(m.slot_w[row], v[j]));
+                              (unsigned long long)v[j]);
                 else
                     m.Y[row * m.N + n] = v[j];
             }
@@ -898,10 +900,11 @@ int q48_launch_w8_mul(q48_ctx *c, const W8Mul &m, int epi, bool experts, int n_i
 {
     const unsigned nx = (m.N + 15) / 16;
     // Tiles of 128 x 128 where there are outputs to fill the chip with them.  us, k_w8_mul /
-    // k_w8_gemm: 2560 x 2048 512 rows 18.5 / 22.1, 1024 28.8 / 26.7; 2048 x 5632 512 30.0 /
-    // 37.9, 1024 48.9 / 43.0; 1031 x 2047 1024 22.4 / 26.1; SwiGLU of 5632 x 2048 512 38.8 /
-    // 39.9, 1024 69.9 / 60.9.
-    const bool tiles = experts ? m.rows > 64 : (size_t)m.T * m.N >= (epi == 1 ? 3u : 2u) << 20;
+    // k_w8_gemm: 2560 x 2048 512 rows 18.6 / 21.7, 768 24.6 / 24.1, 1024 28.6 / 25.7; 2048 x
+    // 5632 512 30.9 / 35.3, 1024 49.7 / 40.3; 1031 x 2047 1024 21.9 / 25.2, 2048 33.1 / 29.0;
+    // 8000 x 512 256 12.8 / 15.4, 512 19.3 / 16.7; SwiGLU of 5632 x 2048 512 40.3 / 43.8, 768
+    // 57.9 / 58.7, 1024 75.4 / 62.7; of 3001 x 700 1024 32.7 / 35.3.
+    const bool tiles = experts ? m.rows > 64 : (size_t)m.T * m.N >= (epi == 1 ? 4u : 2u) << 20;
     if (tiles) {
         const int ch = epi == 1 ? GT / 2 : GT, gx = (m.N + ch - 1) / ch;
         const int gy = experts ? n_items : (m.T + GT - 1) / GT;
