@@ -18,7 +18,8 @@ __device__ __forceinline__ uint64_t block_umax(uint64_t v, uint64_t *red)
     return t;
 }
 
-// A block a row: sum of squares, largest magnitude, codes, each a pass over the row.
+// A block a row: sum of squares, largest magnitude, codes, each a pass over the row.  Rows
+// past T: zero codes.
 __global__ __launch_bounds__(256) void k_w8_rows(W8Rows a)
 {
     q48_round_down();
@@ -28,6 +29,7 @@ __global__ __launch_bounds__(256) void k_w8_rows(W8Rows a)
     if (a.tok && a.tok[t] < 0)
         return;
     const int64_t *x = a.X + (size_t)t * K;
+    const bool past = t >= a.T;
     int64_t r = 0;
     if (a.norm_w) {
         q48_u128 ss = 0;
@@ -39,7 +41,9 @@ __global__ __launch_bounds__(256) void k_w8_rows(W8Rows a)
         __syncthreads();
         r = r_sh;
     }
-    auto at = [&](int i) { return a.norm_w ? q48_mul(q48_mul(x[i], r), a.norm_w[i]) : x[i]; };
+    auto at = [&](int i) {
+        return past ? 0 : a.norm_w ? q48_mul(q48_mul(x[i], r), a.norm_w[i]) : x[i];
+    };
     uint64_t m = 0;
     for (int i = tid; i < K; i += 256) {
         const int64_t v = at(i);
@@ -53,7 +57,7 @@ __global__ __launch_bounds__(256) void k_w8_rows(W8Rows a)
     m = block_umax(m, red);
     double rc;
     const uint64_t step = w8_step(m, rc);
-    if (tid == 0)
+    if (tid == 0 && !past)
         a.step[t] = (int64_t)step;
     for (int i = tid; i < KT * 64; i += 256)
         a.codes[w8_at(t, i, KT)] = i < K && step ? (uint8_t)q48_code<127>(at(i), step, rc) : 0;
@@ -69,7 +73,7 @@ __global__ __launch_bounds__(NT) void k_w8_rows_r(W8Rows a)
     if (a.tok && a.tok[t] < 0)
         return;
     RowWords<NT, C, J> x;
-    x.load(a.X + (size_t)t * K, K);
+    x.load(a.X + (size_t)t * K, t < a.T ? K : 0);
     if constexpr (NORM)
         x.norm(a.X + (size_t)t * K, a.norm_w, K, red);
     if (a.xn)
@@ -89,44 +93,22 @@ __global__ __launch_bounds__(NT) void k_w8_rows_r(W8Rows a)
         else
             *(uint16_t *)to = (uint16_t)q;
     });
-    if (threadIdx.x == 0)
+    if (threadIdx.x == 0 && t < a.T)
         a.step[t] = step;
 }
 
-// A row of weights at a time: step and codes, or codes and steps as they come.
-__global__ __launch_bounds__(256) void k_w8_pack(uint8_t *__restrict__ codes,
-                                                int64_t *__restrict__ steps,
-                                                const int64_t *__restrict__ W,
-                                                const int8_t *__restrict__ from,
-                                                const int64_t *__restrict__ from_step, int N,
-                                                int K)
+// Codes and steps as they come, a row of weights at a time.
+__global__ __launch_bounds__(256) void k_w8_put(uint8_t *__restrict__ codes,
+                                               int64_t *__restrict__ steps,
+                                               const int8_t *__restrict__ from,
+                                               const int64_t *__restrict__ from_step, int N, int K)
 {
-    q48_round_down();
-    __shared__ uint64_t red[4];
     const int tid = threadIdx.x, KT = (K + 63) / 64;
     for (int n = blockIdx.x; n < ((N + 15) & ~15); n += gridDim.x) {
-        uint64_t m = 0, step = 0;
-        double rc = 0;
-        if (n < N) {
-            if (W) {
-                for (int i = tid; i < K; i += 256) {
-                    const uint64_t g = q48_magnitude(W[(size_t)n * K + i]);
-                    m = g > m ? g : m;
-                }
-                step = w8_step(block_umax(m, red), rc);
-            } else {
-                step = from_step[n] < 0 ? 0 : (uint64_t)from_step[n];
-            }
-            if (tid == 0)
-                steps[n] = (int64_t)step;
-        }
-        for (int i = tid; i < KT * 64; i += 256) {
-            int q = 0;
-            if (n < N && i < K)
-                q = W ? step ? q48_code<127>(W[(size_t)n * K + i], step, rc) : 0
-                      : from[(size_t)n * K + i];
-            codes[w8_at(n, i, KT)] = (uint8_t)q;
-        }
+        if (tid == 0 && n < N)
+            steps[n] = from_step[n] < 0 ? 0 : from_step[n];
+        for (int i = tid; i < KT * 64; i += 256)
+            codes[w8_at(n, i, KT)] = n < N && i < K ? (uint8_t)from[(size_t)n * K + i] : 0;
     }
 }
 
@@ -831,17 +813,20 @@ int q48_w8_reserve(q48_ctx *c, size_t bytes)
     return launch_rc(q48_launch_zero(c, c->w8, W8_TICKETS));
 }
 
-int q48_launch_w8_rows(q48_ctx *c, const W8Rows &r)
+int q48_launch_w8_rows(q48_ctx *c, const W8Rows &r, int blocks)
 {
+    const dim3 grid(blocks ? blocks : r.T);
 #define W8_ROWS(NT, C, J)                                                                      \
     do {                                                                                       \
         if (r.norm_w)                                                                          \
-            hipLaunchKernelGGL((k_w8_rows_r<NT, C, J, true>), dim3(r.T), dim3(NT), 0, c->stream, r);  \
+            hipLaunchKernelGGL((k_w8_rows_r<NT, C, J, true>), grid, dim3(NT), 0, c->stream, r);  \
         else                                                                                   \
-            hipLaunchKernelGGL((k_w8_rows_r<NT, C, J, false>), dim3(r.T), dim3(NT), 0, c->stream, r); \
+            hipLaunchKernelGGL((k_w8_rows_r<NT, C, J, false>), grid, dim3(NT), 0, c->stream, r); \
     } while (0)
-    if (r.K > 8192)
-        hipLaunchKernelGGL(k_w8_rows, dim3(r.T), dim3(256), 0, c->stream, r);
+    if (r.K > 16384)
+        hipLaunchKernelGGL(k_w8_rows, grid, dim3(256), 0, c->stream, r);
+    else if (r.K > 8192)
+        W8_ROWS(1024, 2, 8);
     else if (r.T <= c->cu_count && r.K > 2048)
         W8_ROWS(512, 2, 8);
     else if (r.T <= c->cu_count && r.K > 1024)
@@ -996,9 +981,17 @@ static int w8_fill(q48_ctx *c, const q48_w8 *w, int index, const int64_t *W, con
         hipLaunchKernelGGL(k_w8_pack_r<16>, eights, dim3(512), 0, c->stream, to, st, W, N, K);
     else if (W && K <= 4096)
         hipLaunchKernelGGL(k_w8_pack_r<32>, eights, dim3(512), 0, c->stream, to, st, W, N, K);
-    else   // (a launch holds fewer than 2^32 threads: N may be 2^24)
-        hipLaunchKernelGGL(k_w8_pack, dim3(min((N + 15) / 16 * 16, 1 << 20)), dim3(256), 0, c->stream,
-                           to, st, W, codes, steps, N, K);
+    else if (W) {   // as rows are
+        W8Rows r = {};
+        r.codes = to;
+        r.step = st;
+        r.X = W;
+        r.T = N;
+        r.K = K;
+        return launch_rc(q48_launch_w8_rows(c, r, (N + 15) & ~15));
+    } else   // (a launch holds fewer than 2^32 threads: N may be 2^24)
+        hipLaunchKernelGGL(k_w8_put, dim3(min((N + 15) / 16 * 16, 1 << 20)), dim3(256), 0, c->stream,
+                           to, st, codes, steps, N, K);
     return launch_rc((int)hipGetLastError());
 }
 

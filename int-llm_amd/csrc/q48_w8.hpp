@@ -460,7 +460,8 @@ struct W8Rows {
     int T, K;
 };
 
-int q48_launch_w8_rows(q48_ctx *c, const W8Rows &r);
+// (blocks: 0, or T rounded up to 16: rows past T get zero codes)
+int q48_launch_w8_rows(q48_ctx *c, const W8Rows &r, int blocks = 0);
 // epi: 0 Y = base + product, 1 SwiGLU of two, 2 weighted adds to the tokens' rows of Y
 int q48_launch_w8_mul(q48_ctx *c, const W8Mul &m, int epi, bool experts, int n_items);
 // One row, or one slot an item, in one launch: X the words that are put into 8 bits on the

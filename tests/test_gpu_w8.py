@@ -48,9 +48,10 @@ def own():
 
 
 SIZES = [(1, 1), (1, 64), (16, 64), (15, 63), (17, 65), (3, 1000), (33, 129), (100, 2048), (7, 5633)]
+LONG = [(21, 2049), (5, 4096), (33, 4097), (17, 8193), (3, 16384), (2, 16385)]
 
 
-@pytest.mark.parametrize("N,K", SIZES)
+@pytest.mark.parametrize("N,K", SIZES + LONG)
 def test_weights_from_words(own, N, K):
     rng = np.random.default_rng(N * 10007 + K)
     x = words(rng, N, K, sigma=0.02)
@@ -248,7 +249,7 @@ def test_weights_off_sixteen_bytes(own):
         assert (got[1:-1].reshape(N, K) == W.values(c, s)).all()
 
 
-@pytest.mark.parametrize("K", [2049, 4096, 4097, 6145, 8192, 8193, 9000])
+@pytest.mark.parametrize("K", [2049, 4096, 4097, 6145, 8192, 8193, 9000, 16384, 16385])
 @pytest.mark.parametrize("T", [1, 5, 300])
 def test_long_rows(own, T, K):
     """Every form that a row's length selects, with an outlier past 32 in some rows."""
