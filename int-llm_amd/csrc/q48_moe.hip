@@ -178,7 +178,9 @@ __global__ __launch_bounds__(1024) void k_moe_slots(const int *__restrict__ chos
 // Everything before the experts in one launch, for few tokens: block (g, t) norms row t
 // and makes the logits of experts g per + 0 .. per - 1; one block more a token its codes.
 // The last block of a token to finish chooses, the last of those makes the slots (tickets;
-// no block waits for another).
+// no block waits for another).  It is a chain of latencies: a token and 8 experts of 2048
+// 9.3 us (the separate launches' kernels 18), 26 tokens and 64 experts 20.5 (45), 200 tokens
+// and 15 of 1000 16.3 (30).
 constexpr int ROUTE_PER = 16;    // experts a block at most
 constexpr int ROUTE_T = 1024;    // tokens at most
 struct MoeRoute {
@@ -373,12 +375,19 @@ size_t slots_of(size_t pairs, int E)
 }
 
 // Experts a block of k_moe_route, 0 for the separate launches (a row of words in LDS): the
-// fewest with which every block, the codes' among them, is resident at once.
+// fewest with which every block, the codes' among them, is resident at once, or 16 and up to
+// three rounds of blocks (two of them a compute unit for rows of up to 2048).  us for a whole
+// layer, one launch / separate: 8 experts, 64 tokens 32 / 68, 512 86 / 111, 700 113 / 130; 16,
+// 700 131 / 136, 1024 185 / 174; 64, 128 tokens 71 / 88, 256 123 / 127, 400 161 / 150; 128 of
+// rows of 1024, 128 tokens 62 / 74, 256 90 / 77; 8 of rows of 4096, 512 133 / 141, 700 171 / 160.
 int route_per(const q48_ctx *c, int T, int E, int dim)
 {
-    const int G = T <= c->cu_count ? (dim <= 2048 ? 2 : 1) * c->cu_count / T - 1 : 0;
-    const int per = G > 0 ? (E + G - 1) / G : ROUTE_PER + 1;
-    return dim <= 6144 && T <= ROUTE_T && per <= ROUTE_PER ? per : 0;
+    if (dim > 6144 || T > ROUTE_T)
+        return 0;
+    const int most = (dim <= 2048 ? 2 : 1) * c->cu_count, G = most / T > 1 ? most / T - 1 : 1;
+    const int per = (E + G - 1) / G < ROUTE_PER ? (E + G - 1) / G : ROUTE_PER;
+    const int blocks = T * ((E + per - 1) / per + 1);
+    return blocks <= (dim <= 2048 ? 6 : 4) * c->cu_count ? per : 0;
 }
 
 int launch_route(q48_ctx *c, const MoeRoute &a)

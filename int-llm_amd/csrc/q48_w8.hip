@@ -71,7 +71,10 @@ __global__ __launch_bounds__(256) void k_w8_rows(W8Rows a)
         a.codes[w8_at(t, i, KT)] = i < K && step ? (uint8_t)q48_code<127>(at(i), step, rc) : 0;
 }
 
-// The same with the row in registers, read once.
+// The same with the row in registers, read once, FP64 where the words allow (RowWords).
+// Many rows are bound by memory: 2048 rows of 5632 19.0 us (104 MB, 5.5 TB/s), 2560 rows of
+// weights of 2048 9.6; with the norm by vector issue too: 2048 rows of 2048 15.0 (6.1 M wave
+// instructions, about 10 us of FP64).  Few rows are one block's chain: 26 of 5632 5.0.
 template <int NT, int C, int J, bool NORM>
 __global__ __launch_bounds__(NT) void k_w8_rows_r(W8Rows a)
 {
@@ -122,7 +125,8 @@ __global__ __launch_bounds__(256) void k_w8_put(uint8_t *__restrict__ codes,
     }
 }
 
-// The way back: eight rows x 2048 columns a block.
+// The way back: eight rows x 2048 columns a block, through LDS so that tiles and words are
+// whole lines.  Bound by memory: 2560 x 2048 10.6 us, 47 MB at 4.5 TB/s.
 __global__ __launch_bounds__(512) void k_w8_values(int64_t *__restrict__ out,
                                                   const uint8_t *__restrict__ codes,
                                                   const int64_t *__restrict__ steps, int N, int K)
@@ -154,7 +158,9 @@ __global__ __launch_bounds__(512) void k_w8_values(int64_t *__restrict__ out,
 
 // A block 16 weight rows x 16 NB rows: its NW waves take every NW-th tile of 64 columns,
 // straight from memory into the matrix instruction's operands, and add up in LDS.  What
-// bounds it is the loads under way, and for many rows the weights read again for every 64.
+// bounds it is the loads under way, and for many rows the weights read again for every 64:
+// 26 rows x 2048 x 5632 5.2 us; 208 pairs of 64 experts, gate and up of 1024 x 2048 48 us
+// (5.6 TB/s of codes), down 28.5 (4.7; a block's 16 KB are one turn of loads).
 template <int NB, int EPI, bool EXPERTS, int NW>
 __global__ __launch_bounds__(64 * NW) void k_w8_mul(W8Mul m)
 {
@@ -272,6 +278,8 @@ constexpr int ONE_NT = 1024;   // threads of a k_w8_one block
 // rows, each every S-th of its 64-column tiles; the row stands in all 16 columns of the
 // matrix instruction's other operand.  SRC 1: the row from words, 2: rmsnorm'ed, both
 // quantised by every block while its first weight tiles are on their way; 0: from codes.
+// 32000 x 2048 normed 13.5 us: 65.5 MB at 6 TB/s behind the row's own 4 us (a launch of its
+// own for the row would come on top); 2560 x 2048 7.0, nearly all of it the row's chain.
 template <int EPI, bool EXPERTS, int SRC, int NT, int J>
 __global__ __launch_bounds__(ONE_NT) void k_w8_one(W8Mul m, const int64_t *__restrict__ X,
                                                   const int64_t *__restrict__ norm_w, int K, int sl)
@@ -450,6 +458,10 @@ constexpr int GSTAGE = 2 * GT * 64;      // bytes of a stage: 64 columns of both
 // most, and the epilogue is as much work as the products.  KS 2, where there is at most a
 // block a compute unit: two groups of four waves, each over half of the columns with a ring
 // of its own, that share the epilogue.
+// 2048 x 2048 x 5632 with a residual 36.5 us (1.29 POP/s, epilogue included).  SwiGLU of 2048
+// x 5632 x 2048 100 us: FP64 instructions (28.5 M of all kinds, four cycles each) and matrix
+// instructions (45 k cycles a SIMD) add up to 0.9 of its cycles; they do not overlap on one
+// SIMD, whatever the order of the blocks or the waves a block.
 template <int EPI, bool EXPERTS, int KS>
 __global__ __launch_bounds__(256 * KS, KS == 1 ? 3 : 2) void k_w8_gemm(W8Mul m, int nx, int ny)
 {
@@ -797,6 +809,10 @@ int q48_w8_reserve(q48_ctx *c, size_t bytes)
 int q48_launch_w8_rows(q48_ctx *c, const W8Rows &r, int blocks)
 {
     const dim3 grid(blocks ? blocks : r.T);
+    // Waves for a row by what it holds: one up to 512 words (20000 rows of 100 23.6 to 11.1 us,
+    // 7000 of 300 11.6 to 7.6), sixteen past 8192, else four (eight are no faster where rows are
+    // few either: with a product behind, 26 normed rows of 2048 8.7 / 7.9, 200 of 5632 16.0 /
+    // 15.0, not normed 12.4 / 12.4).
 #define W8_ROWS(NT, C, J)                                                                      \
     do {                                                                                       \
         if (r.norm_w)                                                                          \
@@ -808,10 +824,6 @@ int q48_launch_w8_rows(q48_ctx *c, const W8Rows &r, int blocks)
         hipLaunchKernelGGL(k_w8_rows, grid, dim3(256), 0, c->stream, r);
     else if (r.K > 8192)
         W8_ROWS(1024, 2, 8);
-    else if (r.T <= c->cu_count && r.K > 2048)
-        W8_ROWS(512, 2, 8);
-    else if (r.T <= c->cu_count && r.K > 1024)
-        W8_ROWS(512, 2, 2);
     else if (r.K <= 512)
         W8_ROWS(64, 4, 2);
     else if (r.K <= 1024)

@@ -89,11 +89,19 @@ def test_a_token_of_long_hidden_rows_in_a_used_buffer(own, top):  # noqa: F811
     check(own, Layer(rng, 16, 48, 8300), words(rng, 1, 48), top, True)
 
 
-@pytest.mark.parametrize("T,E", [(60, 40), (200, 15), (256, 16), (257, 16), (300, 64)])
+@pytest.mark.parametrize("T,E", [(60, 40), (200, 15), (256, 16), (257, 16), (300, 64), (307, 64), (308, 64),
+                                 (768, 8), (769, 8), (1025, 4)])
 def test_where_the_routing_changes(own, T, E):  # noqa: F811
-    """A token's experts in one block, in several, and the separate launches."""
+    """A token's experts in one block, in several, in more blocks than are resident, and the
+    separate launches."""
     rng = np.random.default_rng(E)
     check(own, Layer(rng, E, 100, 40), words(rng, T, 100), 3, False)
+
+
+@pytest.mark.parametrize("T", [256, 512, 513])
+def test_routing_of_longer_rows(own, T):  # noqa: F811
+    rng = np.random.default_rng(T)
+    check(own, Layer(rng, 3, 2050, 8), words(rng, T, 2050), 2, True)
 
 
 @pytest.mark.parametrize("T", [1, 33])

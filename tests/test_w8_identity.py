@@ -33,7 +33,7 @@ def scaled(S, sa, sw):
     f = F(math.floor(h))
     t = add(add(h, -f), fma(S, pl, hl))
     g = F(math.floor(t))
-    sure = abs(h) < 1 << 52 and add(t, -g) < 1 - F(1, 1 << 40)
+    sure = abs(h) < 1 << 53 and add(t, -g) < 1 - F(1, 1 << 40)
     return int(add(f, g)), sure
 
 
@@ -54,12 +54,16 @@ def test_scaled_products():
         sa, k = rng.randrange(1 << 30, 1 << 44), rng.randrange(1 << 36, 1 << 50)
         S = rng.randrange(1, 1 << 20)
         cases.append((S, sa, min((k << 48) // (S * sa), (1 << 53) - 1)))
+    for _ in range(2000):   # up to the last that a double holds
+        sa, S = rng.randrange(1 << 40, 1 << 53), rng.choice([-1, 1]) * rng.randrange(1 << 10, 1 << 31)
+        sw = (rng.randrange(1 << 50, 1 << 53) << 48) // (abs(S) * sa)
+        cases.append((S, sa, min(sw, (1 << 53) - 1)))
     for S, sa, sw in cases:
         want = S * sa * sw >> 48
         got, sure = scaled(S, sa, sw)
         if sure:
             assert got == want, (S, sa, sw)
-        elif abs(want) < 1 << 51:
+        elif abs(want) < 1 << 52:
             unsure += 1
             assert S * sa * sw % (1 << 48) > (1 << 48) - (1 << 10), (S, sa, sw)
     assert unsure < 20
