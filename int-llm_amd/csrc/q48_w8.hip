@@ -680,7 +680,13 @@ __global__ __launch_bounds__(256 * KS, KS == 1 ? 3 : 2) void k_w8_gemm(W8Mul m, 
                 for (int j = 0; j < U; ++j)
                     y[j] = __builtin_floor(y[j] * wd[r_w + t0 + j]);
             int64_t v[U];
-            w8_words<U>(y, v);
+            if constexpr (EPI == 0) {   // (w8_words' two forms of eight would spill)
+#pragma unroll
+                for (int j = 0; j < U; ++j)
+                    v[j] = (int64_t)y[j];
+            } else {
+                w8_words<U>(y, v);
+            }
             if (__any(!ok))
 #pragma nounroll
                 for (int j = 0; j < U; ++j) {
