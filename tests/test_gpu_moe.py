@@ -163,6 +163,28 @@ def test_weights_far_apart(own):  # noqa: F811
     check(own, layer, words(rng, 9, 64), 4, True)
 
 
+def test_long_inputs_in_passes(own):  # noqa: F811
+    """More hidden words than a pass holds (a GiB): 70000 tokens of hidden rows of 1500, four
+    passes, a token's words the same in each."""
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(8)
+    distinct, dim, ffn, T = 10, 64, 1500, 70000
+    X = words(rng, distinct, dim)
+    layer = Layer(rng, 6, dim, ffn)
+    with intllm.Context(0, stream=torch.cuda.current_stream(0).cuda_stream) as c:
+        m = layer.load(c, 2, True)
+        want, ids, wt = layer.want(X, True, 2, True, X)
+        d = torch.from_numpy(X).to("cuda:0").repeat(T // distinct, 1)
+        norm = torch.from_numpy(layer.norm).to("cuda:0")
+        ch = torch.full((T, 2), 9, dtype=torch.int32, device="cuda:0")
+        w = torch.full((T, 2), 9, dtype=torch.int64, device="cuda:0")
+        c.moe_w8(d.data_ptr(), d.data_ptr(), m, d.data_ptr(), norm.data_ptr(), T, ch.data_ptr(), w.data_ptr())
+        for got, one in ((d, want), (ch, ids), (w, wt)):
+            one = torch.from_numpy(np.asarray(one).astype(np.int64)).to("cuda:0")
+            assert bool((got.view(-1, *one.shape) == one).all())
+        c.sync()
+
+
 @pytest.mark.parametrize("T,top", [(1, 2), (5, 3), (90, 2)])
 def test_captured_and_replayed(own, T, top):  # noqa: F811
     """A layer onto its own input as a graph, replayed among eager calls: each replay's

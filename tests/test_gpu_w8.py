@@ -279,6 +279,27 @@ def test_tiles_of_many_outputs(own, N, T):
     assert (out.download().reshape(T, N) == W.swiglu(X, None, gate, up)).all()
 
 
+def test_results_past_four_gib():
+    """Offsets that pass 32 bits in the results, of products and of SwiGLU."""
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(5)
+    distinct, N, K = 7, 2048, 70
+    T = distinct * 40000                       # 4.6 GB of results
+    X = words(rng, distinct, K)
+    gate, up = weights(rng, N, K), weights(rng, N, K)
+    with intllm.Context(0, stream=torch.cuda.current_stream(0).cuda_stream) as c:
+        g, u = loaded(c, *gate), loaded(c, *up)
+        d = torch.from_numpy(X).to("cuda:0").repeat(T // distinct, 1)
+        y = torch.full((T, N), 3, dtype=torch.int64, device="cuda:0")
+        c.gemm_w8(y.data_ptr(), y.data_ptr(), g, d.data_ptr(), None, T)
+        want = torch.from_numpy(W.product(X, None, *gate).astype(np.int64) + 3).to("cuda:0")
+        assert bool((y.view(-1, distinct, N) == want).all())
+        c.gemm_w8_swiglu(y.data_ptr(), g, u, d.data_ptr(), None, T)
+        want = torch.from_numpy(W.swiglu(X, None, gate, up).astype(np.int64)).to("cuda:0")
+        assert bool((y.view(-1, distinct, N) == want).all())
+        c.sync()
+
+
 def test_on_the_callers_stream():
     """Rows that torch is still making when the product is enqueued, results that torch
     reads and rows that it overwrites right behind it."""
