@@ -27,16 +27,18 @@ __device__ __forceinline__ int64_t w8_scaled(int S, int64_t sa, int64_t sw)
 // The same in FP64 rounding down (q48_round_down), as a double: sa and sw = step 2^-48 (inf
 // for steps of 2^53 and more, w8_step_double).  P = sa sw and S P as rounded products and
 // their exact remainders: the floor of the first, and of what the others add to its
-// fraction.  Rounding down makes that sum (below 4) too small by less than 2^-49, so only a
-// fraction next to 1 may hide a whole number: `sure` is false there and where the value
-// passes 2^53 (about one product in 2^40; w8_scaled then).
+// fraction.  Rounding down makes that sum (between -2 and 4) too small by less than 2^-49, so
+// only a fraction next to 1 may hide a whole number: `sure` is false there (about one product
+// in 2^40; w8_scaled then), and where h reaches 2^53 - 2^32: below that the sum of both
+// floors is a whole number that a double holds, which next to 2^53 it need not be (2^32, of
+// any margin past 4, for a constant whose low half is zero).
 __device__ __forceinline__ double w8_scaled_double(int S, double sa, double sw, bool &sure)
 {
 #pragma clang fp contract(off)   // h as rounded
     const double p = sa * sw, pl = __builtin_fma(sa, sw, -p), s = (double)S;
     const double h = s * p, hl = __builtin_fma(s, p, -h), f = __builtin_floor(h);
     const double t = (h - f) + __builtin_fma(s, pl, hl), g = __builtin_floor(t);
-    sure = (__builtin_fabs(h) < 0x1p53) & (t - g < 1.0 - 0x1p-40);
+    sure = (__builtin_fabs(h) < 0x1p53 - 0x1p32) & (t - g < 1.0 - 0x1p-40);
     return f + g;
 }
 __device__ __forceinline__ double w8_step_double(int64_t step)
