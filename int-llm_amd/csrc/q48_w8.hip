@@ -977,17 +977,22 @@ static int w8_fill(q48_ctx *c, const q48_w8 *w, int index, const int64_t *W, con
     if (over(W, n * 8) || over(codes, n) || over(steps, (size_t)N * 8))
         return Q48_EINVAL;
     q48_on_device on(c);
+    // a launch holds fewer than 2^32 threads: N may be 2^24
+    constexpr int most = 1 << 20;
     if (W) {   // as rows are
-        W8Rows r = {};
-        r.codes = to;
-        r.step = st;
-        r.X = W;
-        r.T = N;
-        r.K = K;
-        return launch_rc(q48_launch_w8_rows(c, r, (N + 15) & ~15));
+        for (int n0 = 0; n0 < N; n0 += most) {
+            W8Rows r = {};
+            r.codes = to + (size_t)(n0 / 16) * w8_kt(K) * 1024;
+            r.step = st + n0;
+            r.X = W + (size_t)n0 * K;
+            r.T = min(N - n0, most);
+            r.K = K;
+            if (const int rc = q48_launch_w8_rows(c, r, (r.T + 15) & ~15))
+                return launch_rc(rc);
+        }
+        return Q48_OK;
     }
-    // (a launch holds fewer than 2^32 threads: N may be 2^24)
-    hipLaunchKernelGGL(k_w8_put, dim3(min((N + 15) / 16 * 16, 1 << 20)), dim3(256), 0, c->stream, to,
+    hipLaunchKernelGGL(k_w8_put, dim3(min((N + 15) / 16 * 16, most)), dim3(256), 0, c->stream, to,
                        st, codes, steps, N, K);
     return launch_rc((int)hipGetLastError());
 }

@@ -393,3 +393,31 @@ def test_captured_and_replayed(own):
             c.gemm_w8(oo.ptr, None, g, do.ptr, dn.ptr, 200)   # grows the context's buffer once
             assert (oo.download().reshape(200, N) == W.product(other, nw, *gate)).all()
     intllm.check("drop", lib.q48_graph_drop(c.h))
+
+
+@pytest.mark.parametrize("N", [(1 << 24) - 7, (1 << 20) + 5])
+def test_the_most_rows_from_words(N):
+    """As many rows of words as there may be, of a length that takes four waves a row: every
+    row's codes and step, in the layout that the header gives."""
+    torch = pytest.importorskip("torch")
+    K, KT, NT, at = 513, 9, (N + 15) // 16, "cuda:0"
+    with intllm.Context(0, stream=torch.cuda.current_stream(0).cuda_stream) as c:
+        assert intllm.w8_bytes(1, N, K) == (NT * KT * 1024, N * 8)
+        g = torch.Generator(device=at).manual_seed(N)
+        some = torch.randint(-(1 << 44), 1 << 44, (4096, K), generator=g, device=at)
+        x = some.repeat((N + 4095) // 4096, 1)[:N]
+        x[:, 7] = torch.arange(N, device=at) << 22                # every row another step
+        codes = torch.full((NT, KT, 4, 16, 16), -1, dtype=torch.int8, device=at)
+        steps = torch.full((N,), -1, dtype=torch.int64, device=at)
+        c.w8_pack(c.w8(codes.data_ptr(), steps.data_ptr(), 1, N, K), 0, x.data_ptr())
+        for n in range(0, NT * 16, 1 << 20):
+            w, rows = x[n:n + (1 << 20)], codes[n // 16:(n + (1 << 20)) // 16]
+            step = (w.abs().amax(1) + 126) // 127
+            assert bool((steps[n:n + (1 << 20)] == step).all()), n
+            got = rows.permute(0, 3, 1, 2, 4).reshape(-1, KT * 64)
+            want = ((w.abs() + (step >> 1)[:, None]) // step[:, None]).clamp_(max=127) * w.sign()
+            assert bool((got[:w.shape[0], :K] == want).all()), n
+            assert not bool(got[w.shape[0]:].any()) and not bool(got[:, K:].any()), n
+        c.sync()
+    del x, codes, some
+    torch.cuda.empty_cache()
