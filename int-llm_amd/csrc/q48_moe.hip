@@ -458,10 +458,15 @@ int q48_moe_w8(q48_ctx *c, int64_t *out, const int64_t *base, const q48_moe *moe
         o += (bytes + 255) & ~(size_t)255;
         return at;
     };
-    // tokens of one pass: a GiB of hidden words and 2^19 pairs at most
+    // Tokens of one pass: 2^19 pairs and half a GiB of their hidden words at most, and a GiB
+    // with the slots that fill up each expert's sixteens (16 slots a pair while there are no
+    // more pairs than experts: a token's 64 pairs of the longest rows are a GiB).
     size_t Tc = ((size_t)1 << 30) / ((size_t)16 * top * ffn);
     Tc = Tc < ((size_t)1 << 19) / top ? Tc : ((size_t)1 << 19) / top;
-    Tc = Tc < 16 ? 16 : Tc < (size_t)T ? Tc : (size_t)T;
+    const size_t most = ((size_t)1 << 30) / ((size_t)8 * ffn);   // slots
+    const size_t fit = (most / 16 <= (size_t)E ? most / 16 : most - 15 * (size_t)E - 15) / top;
+    Tc = Tc < fit ? Tc : fit;
+    Tc = Tc < 1 ? 1 : Tc < (size_t)T ? Tc : (size_t)T;
     const size_t slots = slots_of(Tc * top, E), n_items = items_of(Tc * top, E, 16);
     const size_t o_x = take(w8_tiles((int)Tc, dim)), o_xs = take(Tc * 8);
     const size_t o_xn = take(norm_w ? Tc * row : 0), o_l = take(Tc * E * 8);

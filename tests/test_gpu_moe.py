@@ -214,3 +214,53 @@ def test_captured_and_replayed(own, T, top):  # noqa: F811
             c.moe_w8(oo.ptr, None, m, do.ptr, None, 300)
             assert (oo.download().reshape(300, 64) == layer.want(other, False, top, True, None)[0]).all()
     intllm.check("drop", lib.q48_graph_drop(c.h))
+
+
+def grown(call):
+    """Bytes of the card that a call keeps."""
+    torch = pytest.importorskip("torch")
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    call()
+    torch.cuda.synchronize()
+    return free - torch.cuda.mem_get_info()[0]
+
+
+def test_the_buffer_of_a_token_with_many_long_rows(own):  # noqa: F811
+    """64 experts of hidden rows past 2^16 words for one token: its own 16 slots each."""
+    rng = np.random.default_rng(12)
+    E, ffn = 64, 66000
+    gate, up, down = weights(rng, ffn, 1, sigma=0.3), weights(rng, ffn, 1, sigma=0.3), weights(rng, 1, ffn)
+    w = []
+    for codes, steps in (gate, up, down):      # the experts all alike
+        a, dc, ds = own.new_w8(E, *codes.shape), raw(own, codes), own.to_device(steps)
+        for e in range(E):
+            own.w8_put(a, e, dc.ptr, ds.ptr)
+        w.append(a)
+    x, router = words(rng, 1, 1), words(rng, E, 1)
+    m = own.moe(own.to_device(router).ptr, *w, E, False)
+    out, dx = own.buffer(1), own.to_device(x)
+    own.sync()
+    most = 16 * E * ffn * 8                    # hidden words; their codes are an eighth
+    assert grown(lambda: own.moe_w8(out.ptr, None, m, dx.ptr, None, 1)) < 1.5 * most < 1 << 30
+    y = int(W.product(W.swiglu(x, None, gate, up), None, *down)[0, 0])
+    _, weight = W.choose(W.logits(x, router)[0], E, False)
+    assert int(out.download()[0]) == sum(a * y >> 48 for a in weight)
+
+
+def test_the_buffer_of_many_experts(own):  # noqa: F811
+    """A GiB of hidden words with every expert's last sixteen slots among them: 1024 experts
+    of hidden rows of 8192, a pass after a pass."""
+    rng = np.random.default_rng(13)
+    E, dim, ffn, top, distinct, T = 1024, 2, 8192, 8, 5, 1000
+    layer = Layer(rng, E, dim, ffn, sigma=0.3)
+    m = layer.load(own, top, True)
+    x = words(rng, distinct, dim)
+    want = layer.want(x, False, top, True, None)
+    dx, out = own.to_device(np.tile(x, (T // distinct, 1))), own.buffer(T * dim)
+    ch, wt = own.buffer(T * top // 2), own.buffer(T * top)
+    own.sync()
+    assert grown(lambda: own.moe_w8(out.ptr, None, m, dx.ptr, None, T, ch.ptr, wt.ptr)) < 1.25 * 2 ** 30
+    assert (out.download().reshape(-1, distinct, dim) == want[0]).all()
+    assert (ch.download().view(np.int32).reshape(-1, distinct, top) == want[1]).all()
+    assert (wt.download().reshape(-1, distinct, top) == want[2]).all()
