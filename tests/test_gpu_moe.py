@@ -264,3 +264,34 @@ def test_the_buffer_of_many_experts(own):  # noqa: F811
     assert (out.download().reshape(-1, distinct, dim) == want[0]).all()
     assert (ch.download().view(np.int32).reshape(-1, distinct, top) == want[1]).all()
     assert (wt.download().reshape(-1, distinct, top) == want[2]).all()
+
+
+@pytest.mark.parametrize("T,top", [(1, 2), (5, 3), (90, 2)])
+def test_graphs_outlive_a_grown_buffer(own, T, top):  # noqa: F811
+    """Eager layers of ever more tokens, past the context's first MiB, between the replays of
+    a graph that holds the buffer's first address."""
+    rng = np.random.default_rng(9)
+    lib, c = intllm.hip_lib(), own
+    layer = Layer(rng, 8, 64, 48, sigma=0.3)
+    m = layer.load(c, top, True)
+    x = words(rng, T, 64)
+    dX = c.to_device(x)
+    c.moe_w8(dX.ptr, dX.ptr, m, dX.ptr, None, T)
+    c.sync()
+    intllm.check("begin", lib.q48_graph_begin(c.h))
+    c.moe_w8(dX.ptr, dX.ptr, m, dX.ptr, None, T)
+    intllm.check("end", lib.q48_graph_end(c.h))
+    dX.upload(x)
+    some = words(rng, 50, 64)
+    want = layer.want(some, False, top, True, None)[0]
+    for i in range(4):
+        intllm.check("launch", lib.q48_graph_launch(c.h, 1))
+        x = layer.want(x, False, top, True, x)[0]
+        assert (dX.download().reshape(T, 64) == x).all(), i
+        n = 50 * (100 << i)                    # 5000 to 40000 tokens: another buffer each time
+        do, oo = c.to_device(np.tile(some, (n // 50, 1))), c.buffer(n * 64)
+        assert grown(lambda: c.moe_w8(oo.ptr, None, m, do.ptr, None, n)) > 0
+        assert (oo.download().reshape(-1, 50, 64) == want).all()
+        c.moe_w8(oo.ptr, None, m, do.ptr, None, 50)          # the new buffer's tickets
+        assert (oo.download().reshape(-1, 50, 64)[0] == want).all()
+    intllm.check("drop", lib.q48_graph_drop(c.h))

@@ -421,3 +421,41 @@ def test_the_most_rows_from_words(N):
         c.sync()
     del x, codes, some
     torch.cuda.empty_cache()
+
+
+def test_graphs_outlive_a_grown_buffer(own):
+    """Eager products of ever more rows, past the context's first MiB, between the replays of
+    a graph that holds the buffer's first address."""
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(12)
+    lib, c = intllm.hip_lib(), own
+    T, N, K = 3, 96, 300
+    gate, up, down = weights(rng, N, K), weights(rng, N, K), weights(rng, K, N)
+    g, u, d = (loaded(c, *w) for w in (gate, up, down))
+    x = words(rng, T, K)
+    dX, h = c.to_device(x), c.buffer(T * N)
+
+    def step():
+        c.gemm_w8_swiglu(h.ptr, g, u, dX.ptr, None, T)
+        c.gemm_w8(dX.ptr, dX.ptr, d, h.ptr, None, T)
+
+    step()
+    c.sync()
+    intllm.check("begin", lib.q48_graph_begin(c.h))
+    step()
+    intllm.check("end", lib.q48_graph_end(c.h))
+    dX.upload(x)
+    some = words(rng, 50, K)
+    want = W.product(some, None, *gate)
+    for i in range(3):
+        intllm.check("launch", lib.q48_graph_launch(c.h, 1))
+        x = W.product(W.swiglu(x, None, gate, up), None, *down, x)
+        assert (dX.download().reshape(T, K) == x).all(), i
+        n = 50 * (400 << i)
+        do, oo = c.to_device(np.tile(some, (n // 50, 1))), c.buffer(n * N)
+        torch.cuda.synchronize()
+        free = torch.cuda.mem_get_info()[0]
+        c.gemm_w8(oo.ptr, None, g, do.ptr, None, n)
+        assert (oo.download().reshape(-1, 50, N) == want).all()
+        assert torch.cuda.mem_get_info()[0] < free            # it has grown
+    intllm.check("drop", lib.q48_graph_drop(c.h))
