@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import weakref
 from pathlib import Path
 
 import numpy as np
@@ -161,9 +162,15 @@ class W8(C.Structure):
 
 
 class Moe(C.Structure):
-    """q48_moe: a mixture-of-experts layer's router and experts."""
+    """q48_moe: a mixture-of-experts layer's router and experts.  The fields are copies of
+    the weights' descriptions: free_w8 empties those of what it gives back."""
     _fields_ = [("router", C.c_void_p), ("gate", W8), ("up", W8), ("down", W8),
                 ("top_k", C.c_int), ("renorm", C.c_int)]
+
+    def __setattr__(self, name, value):
+        super().__setattr__(name, value)
+        if isinstance(value, W8):
+            value.__dict__.setdefault("layers", weakref.WeakValueDictionary())[id(self)] = self
 
 
 def w8_bytes(count, N, K) -> tuple[int, int]:
@@ -590,12 +597,19 @@ class Context:
         return w
 
     def free_w8(self, w: W8) -> None:
-        """Give back weights from new_w8 (which are refused from then on); those that only
-        describe the caller's memory have nothing to give back."""
-        for b in w.__dict__.pop("bufs", ()):
+        """Give back weights from new_w8 (which are refused from then on, with the layers that
+        were described by them); those that only describe the caller's memory have nothing to
+        give back."""
+        bufs = w.__dict__.pop("bufs", ())
+        if bufs:
+            for m in w.__dict__.pop("layers", {}).values():
+                for part in (m.gate, m.up, m.down):
+                    if part.codes == w.codes:
+                        part.codes = part.step = None
+            w.codes = w.step = None
+        for b in bufs:
             b.free()
             self._bufs.remove(b)
-            w.codes = w.step = None
 
     def w8_pack(self, w, index, W):
         """Put matrix `index` into 8 bits from words W [N][K]."""

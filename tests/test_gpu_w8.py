@@ -459,3 +459,26 @@ def test_graphs_outlive_a_grown_buffer(own):
         assert (oo.download().reshape(-1, 50, N) == want).all()
         assert torch.cuda.mem_get_info()[0] < free            # it has grown
     intllm.check("drop", lib.q48_graph_drop(c.h))
+
+
+def test_weights_given_back(own):
+    """The card has their memory again; they are refused, and the context works on."""
+    torch = pytest.importorskip("torch")
+    rng = np.random.default_rng(14)
+    codes, steps = weights(rng, 40, 100)
+    kept = loaded(own, codes, steps)
+    x = words(rng, 3, 100)
+    dx, y = own.to_device(x), own.buffer(3 * 40)
+    own.gemm_w8(y.ptr, None, kept, dx.ptr, None, 3)
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    big = own.new_w8(3, 4096, 8192)
+    put(own, big, 1, *weights(rng, 4096, 8192))
+    assert torch.cuda.mem_get_info()[0] < free - 3 * 4096 * 8192 + 1
+    own.free_w8(big)
+    assert torch.cuda.mem_get_info()[0] > free - 2 * 4096 * 8192      # (the words that were put)
+    with pytest.raises(intllm.Q48Error):
+        own.w8_values(y.ptr, big, 1)
+    own.free_w8(big)
+    own.gemm_w8(y.ptr, None, kept, dx.ptr, None, 3)
+    assert (y.download().reshape(3, 40) == W.product(x, None, codes, steps)).all()

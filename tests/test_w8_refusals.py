@@ -171,3 +171,53 @@ def test_experts():
         no(wt=at)
     no(b=wt)
     no(ch=wt + 8)
+
+
+class Room:
+    """Stands for a buffer of a context."""
+    def __init__(self, ptr):
+        self.ptr = ptr
+
+    def free(self):
+        self.ptr = None
+
+
+def test_layers_of_weights_that_were_given_back():
+    """A layer holds copies of its weights' descriptions: with the weights these are refused
+    too, however the layer came by them; other weights' are left alone."""
+    ctx = object.__new__(intllm.Context)
+    ctx.h, ctx._bufs = C.addressof(CTX), []
+    Y, X = 1 << 44, 1 << 45
+
+    def new(i, E, N, K):
+        at = A + (i << 33)
+        w = ctx.w8(at, at + (1 << 32), E, N, K)
+        w.bufs = [Room(w.codes), Room(w.step)]
+        ctx._bufs += w.bufs
+        return w
+
+    shapes = dict(gate=(4, 64, 128), up=(4, 64, 128), down=(4, 128, 64))
+    for part in shapes:
+        w = {n: new(i, *s) for i, (n, s) in enumerate(shapes.items())}
+        layers = [ctx.moe(1 << 43, *w.values(), 2, True), intllm.Moe(1 << 43, **w, top_k=2, renorm=1),
+                  intllm.Moe(router=1 << 43, top_k=2)]
+        for n, m in w.items():
+            setattr(layers[2], n, m)
+        other = ctx.moe(1 << 43, *w.values(), 2, True)
+        setattr(other, part, new(5, *shapes[part]))
+        kept = getattr(other, part).codes
+        ctx.free_w8(w[part])
+        for m in layers:
+            for n in shapes:
+                assert (getattr(m, n).codes is None) == (getattr(m, n).step is None) == (n == part)
+            refused("q48_moe_w8", CTX, Y, None, m, X, None, 1, None, None)
+            with pytest.raises(intllm.Q48Error) as err:
+                ctx.moe_w8(Y, None, m, X, None, 1)
+            assert err.value.code == intllm.Q48_EINVAL
+        assert getattr(other, part).codes == kept
+        refused("q48_w8_values", CTX, Y, w[part], 0)
+        ctx.free_w8(w[part])                                # nothing is left to give back
+        mine = w8(count=4, N=64, K=128)
+        m = ctx.moe(1 << 43, mine, mine, w["down"], 2, True)
+        ctx.free_w8(mine)                                   # the caller's memory
+        assert mine.codes == m.gate.codes == A
