@@ -902,9 +902,7 @@ int q48_launch_w8_mul(q48_ctx *c, const W8Mul &m, int epi, bool experts, int n_i
             W8_GEMM(1, true, 1);
         else if (experts)
             W8_GEMM(2, true, 1);
-        else if (epi == 1 && halves)
-            W8_GEMM(1, false, 2);
-        else if (epi == 1)
+        else if (epi == 1)   // (512 blocks and more)
             W8_GEMM(1, false, 1);
         else if (halves)
             W8_GEMM(0, false, 2);

@@ -56,10 +56,6 @@ __device__ __forceinline__ double w8_kept(double c)
 
 // All of v before anything behind: chains of operations that would else be scheduled one
 // after the other.
-__device__ __forceinline__ void w8_together(double (&v)[4])
-{
-    asm volatile("" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]));
-}
 __device__ __forceinline__ void w8_together(double (&v)[2])
 {
     asm volatile("" : "+v"(v[0]), "+v"(v[1]));
