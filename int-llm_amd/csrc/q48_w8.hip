@@ -27,7 +27,7 @@ __device__ __forceinline__ int w8_near(int b, int n)
 }
 
 // A block a row: sum of squares, largest magnitude, codes, each a pass over the row.  Rows
-// past T: zero codes.
+// past T: zero codes.  Bound by the one block's passes in integers: a row of 28672 63 us.
 __global__ __launch_bounds__(256) void k_w8_rows(W8Rows a)
 {
     q48_round_down();
@@ -108,7 +108,8 @@ __global__ __launch_bounds__(NT) void k_w8_rows_r(W8Rows a)
         a.step[t] = step;
 }
 
-// Codes and steps as they come, a row of weights at a time.
+// Codes and steps as they come, a row of weights at a time.  A byte a thread: 32000 x 2048
+// 52 us (131 MB, 2.5 TB/s), 2560 x 2048 5.3.
 __global__ __launch_bounds__(256) void k_w8_put(uint8_t *__restrict__ codes,
                                                int64_t *__restrict__ steps,
                                                const int8_t *__restrict__ from,
@@ -280,6 +281,8 @@ constexpr int ONE_NT = 1024;   // threads of a k_w8_one block
 // quantised by every block while its first weight tiles are on their way; 0: from codes.
 // 32000 x 2048 normed 13.5 us: 65.5 MB at 6 TB/s behind the row's own 4 us (a launch of its
 // own for the row would come on top); 2560 x 2048 7.0, nearly all of it the row's chain.
+// Rows of 4096 (512 threads of 16 words): 4096 x 4096 normed 11.3, 128256 x 4096 103.  With a
+// norm that form spills 53 registers, 56 with SwiGLU.
 template <int EPI, bool EXPERTS, int SRC, int NT, int J>
 __global__ __launch_bounds__(ONE_NT) void k_w8_one(W8Mul m, const int64_t *__restrict__ X,
                                                   const int64_t *__restrict__ norm_w, int K, int sl)
@@ -458,10 +461,12 @@ constexpr int GSTAGE = 2 * GT * 64;      // bytes of a stage: 64 columns of both
 // most, and the epilogue is as much work as the products.  KS 2, where there is at most a
 // block a compute unit: two groups of four waves, each over half of the columns with a ring
 // of its own, that share the epilogue.
-// 2048 x 2048 x 5632 with a residual 36.5 us (1.29 POP/s, epilogue included).  SwiGLU of 2048
-// x 5632 x 2048 100 us: FP64 instructions (28.5 M of all kinds, four cycles each) and matrix
-// instructions (45 k cycles a SIMD) add up to 0.9 of its cycles; they do not overlap on one
-// SIMD, whatever the order of the blocks or the waves a block.
+// 2048 x 2048 x 5632 with a residual 36.5 us (1.29 POP/s, epilogue included): one tile a
+// compute unit, so that its residual and results (67 MB) wait for its products; of 66 k cycles
+// 23 k are matrix instructions and 12 k vector instructions.  SwiGLU of 2048 x 5632 x 2048 100
+// us: vector instructions (28.5 M, four cycles each; 158 an output, 112 of them FP64) and
+// matrix instructions (45 k cycles a SIMD) add up to 0.9 of its cycles; they do not overlap on
+// one SIMD, whatever the order of the blocks or the waves a block.
 template <int EPI, bool EXPERTS, int KS>
 __global__ __launch_bounds__(256 * KS, KS == 1 ? 3 : 2) void k_w8_gemm(W8Mul m, int nx, int ny)
 {
@@ -889,7 +894,10 @@ int q48_launch_w8_mul(q48_ctx *c, const W8Mul &m, int epi, bool experts, int n_i
     // k_w8_gemm: 2560 x 2048 512 rows 18.6 / 21.7, 768 24.6 / 24.1, 1024 28.6 / 25.7; 2048 x
     // 5632 512 30.9 / 35.3, 1024 49.7 / 40.3; 1031 x 2047 1024 21.9 / 25.2, 2048 33.1 / 29.0;
     // 8000 x 512 256 12.8 / 15.4, 512 19.3 / 16.7; SwiGLU of 5632 x 2048 512 40.3 / 43.8, 768
-    // 57.9 / 58.7, 1024 75.4 / 62.7; of 3001 x 700 1024 32.7 / 35.3.
+    // 57.9 / 58.7, 1024 75.4 / 62.7; of 3001 x 700 1024 32.7 / 35.3.  Few rows of many outputs:
+    // 128000 x 2048 17 rows 58 / 60, 32 66 / 75, 64 101 / 85; x 4096 17 133 / 118, 64 185 / 134;
+    // 64000 x 2048 32 27 / 39, 33 33 / 41, 64 38 / 44, 65 59 / 45; 32000 x 2048 64 22.7 / 24.2, 65
+    // 33.1 / 24.4; SwiGLU of 64000 x 2048 64 77 / 94, 96 119 / 95; of 14336 x 4096 256 86 / 64.
     const bool tiles = experts ? m.rows > 64 : (size_t)m.T * m.N >= (epi == 1 ? 4u : 2u) << 20;
     if (tiles) {
         const int ch = epi == 1 ? GT / 2 : GT, gx = (m.N + ch - 1) / ch;
